@@ -7,6 +7,7 @@ Everything computes in ``libcvcuda_b200.so`` (hand-written sm_100a kernels); the
 importing the operator functions fails loudly when the library has not been built.
 """
 from . import ops as _ops
+from . import rows as _rows
 from . import cvcuda  # noqa: F401  (the reference-style object surface: cvcuda = nvcv = cvcuda_b200.cvcuda)
 from . import sharding  # noqa: F401
 from .ops import (  # noqa: F401
@@ -45,5 +46,6 @@ from .ops import (  # noqa: F401
     self_test_wait_timeout,
     set_kernel_path,
 )
+from .rows import *  # noqa: F401,F403  (LayerNorm and the embedding lookup, with their gradients)
 
-__all__ = [n for n in dir(_ops) if not n.startswith("_")]
+__all__ = [n for n in dir(_ops) if not n.startswith("_")] + _rows.__all__

@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcvcuda_b200.so")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-SOURCES = ["library.cu", "cvcuda_ops.cpp", "random_crop.cpp"]
+SOURCES = ["library.cu", "row_ops.cu", "cvcuda_ops.cpp", "random_crop.cpp"]
 
 
 def _stale() -> bool:
@@ -32,7 +32,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
     cmd = [
-        NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
+        NVCC, "--threads", "0", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
         # the goldens are defined by un-fused float arithmetic: never contract a*b+c into an FMA
         "--fmad=false", "--ftz=false", "--prec-div=true", "--prec-sqrt=true",
         "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "-shared",

@@ -1,7 +1,8 @@
 // Host side of the plain-C launch layer: argument validation, kernel selection and launch.
-// The single translation unit that contains all device code of the library.
+// The translation unit that contains the device code of the image operators (row_ops.cu: that of the row operators).
 #include "border_kernels.cuh"
 #include "convert_kernels.cuh"
+#include "host_common.h"
 #include "normalize_kernels.cuh"
 #include "plain_resize_kernels.cuh"
 #include "reformat_kernels.cuh"
@@ -36,7 +37,7 @@ int fail(int status, const char *fmt, ...)
 static std::atomic<int>      g_kernelPath{0};
 static std::atomic<uint64_t> g_launchCount{0};
 
-static int check_launch(const char *what)
+int check_launch(const char *what)
 {
     cudaError_t e = cudaPeekAtLastError();
     if (e != cudaSuccess)

@@ -18,7 +18,7 @@ from typing import Optional, Sequence, Tuple, Union
 import numpy as np
 import torch
 
-from . import ops
+from . import ops, rows
 from .ops import Border, ChannelManip, Error, Interp, RectI, Status  # noqa: F401  (re-exported)
 
 
@@ -37,6 +37,8 @@ class Type:
     S32 = np.dtype(np.int32)
     F32 = np.dtype(np.float32)
     F16 = np.dtype(np.float16)
+    BF16 = torch.bfloat16  # numpy has no such type; the row operators (layernorm, embedding) take it
+    S64 = np.dtype(np.int64)  # indices of the row operators
 
 
 class Format(enum.Enum):
@@ -70,7 +72,7 @@ class Format(enum.Enum):
 
 
 _TORCH = {np.dtype(np.uint8): torch.uint8, np.dtype(np.int8): torch.int8, np.dtype(np.int16): torch.int16,
-          np.dtype(np.int32): torch.int32, np.dtype(np.float32): torch.float32, np.dtype(np.float16): torch.float16}
+          np.dtype(np.int32): torch.int32, np.dtype(np.int64): torch.int64, np.dtype(np.float32): torch.float32, np.dtype(np.float16): torch.float16}
 if hasattr(torch, "uint16"):
     _TORCH[np.dtype(np.uint16)] = torch.uint16
 _NUMPY = {v: k for k, v in _TORCH.items()}
@@ -150,7 +152,7 @@ class Tensor:
 
     @property
     def dtype(self):
-        return _NUMPY[self._t.dtype]
+        return _NUMPY.get(self._t.dtype, self._t.dtype)
 
     @property
     def layout(self) -> str:
@@ -444,3 +446,79 @@ def random_resized_crop(src, shape_or_sizes, min_scale: float = 0.08, max_scale:
     s, lay = _src_of(src)
     out = ops.random_resized_crop(s, shape_or_sizes, min_scale, max_scale, min_ratio, max_ratio, interp, seed, stream=_stream_of(stream))
     return out if lay is None else _wrap(out, lay)
+
+
+# ------------------------------------------------------------------------------------------------ row operators
+
+def _axes(t: Tensor, axes) -> int:
+    """Number of trailing dimensions: a number, or the labels that end the tensor's layout ("C", "HWC")."""
+    if isinstance(axes, str):
+        if not axes or not t.layout.endswith(axes):
+            raise Error(Status.ERROR_INVALID_ARGUMENT, f"Layout '{t.layout}' does not end in '{axes}'")
+        return len(axes)
+    return int(axes)
+
+
+def _opt(t):
+    return None if t is None else as_tensor(t)._t
+
+
+def layernorm(src, weight=None, bias=None, epsilon: float = 1e-5, *, axes: Union[int, str] = 1, dtype=None, stats: bool = False,
+              stream=None):
+    """:func:`cvcuda_b200.layernorm` on objects of this module: ``axes`` may name the labels the layout ends in ("C": every
+    pixel's channels, "HWC": whole images). With ``stats``: (result, mean, rstd)."""
+    t = as_tensor(src)
+    out = rows.layernorm(t._t, _opt(weight), _opt(bias), epsilon, axes=_axes(t, axes), stats=stats, stream=_stream_of(stream),
+                         data_type=None if dtype is None else _torch_dtype(dtype))
+    if not stats:
+        return _wrap(out, t.layout)
+    lead = t.layout[:len(t.layout) - _axes(t, axes)] if t.layout else ""
+    return _wrap(out[0], t.layout), _wrap(out[1], lead), _wrap(out[2], lead)
+
+
+def layernorm_into(dst: Tensor, src, weight=None, bias=None, epsilon: float = 1e-5, *, axes: Union[int, str] = 1, mean=None, rstd=None,
+                   stream=None) -> Tensor:
+    t = as_tensor(src)
+    rows.layernorm_into(as_tensor(dst)._t, t._t, _opt(weight), _opt(bias), epsilon, axes=_axes(t, axes), mean=_opt(mean),
+                        rstd=_opt(rstd), stream=_stream_of(stream))
+    return dst
+
+
+def layernorm_backward(grad, src, mean, rstd, weight=None, *, axes: Union[int, str] = 1, dtype=None, src_grad: bool = True,
+                       weight_grad: bool = True, bias_grad: bool = True, stream=None):
+    """:func:`cvcuda_b200.layernorm_backward` on objects of this module: (dsrc, dweight, dbias)."""
+    t = as_tensor(src)
+    n = _axes(t, axes)
+    dx, dw, db = rows.layernorm_backward(as_tensor(grad)._t, t._t, as_tensor(mean)._t, as_tensor(rstd)._t, _opt(weight), axes=n,
+                                         data_type=None if dtype is None else _torch_dtype(dtype), src_grad=src_grad,
+                                         weight_grad=weight_grad, bias_grad=bias_grad, stream=_stream_of(stream))
+    row = t.layout[len(t.layout) - n:] if t.layout else ""
+    return tuple(None if g is None else _wrap(g, lay) for g, lay in ((dx, t.layout), (dw, row), (db, row)))
+
+
+def embedding(indices, table, scale: float = 1.0, *, dtype=None, stream=None) -> Tensor:
+    """:func:`cvcuda_b200.embedding` on objects of this module; indices of layout "NHW" give "NHWC"."""
+    t = as_tensor(indices)
+    out = rows.embedding(t._t, as_tensor(table)._t, scale, data_type=None if dtype is None else _torch_dtype(dtype),
+                         stream=_stream_of(stream))
+    return _wrap(out, t.layout + "C" if t.layout and "C" not in t.layout else "")
+
+
+def embedding_into(dst: Tensor, indices, table, scale: float = 1.0, *, stream=None) -> Tensor:
+    rows.embedding_into(as_tensor(dst)._t, as_tensor(indices)._t, as_tensor(table)._t, scale, stream=_stream_of(stream))
+    return dst
+
+
+def embedding_backward(grad, indices, num_rows: int, scale: float = 1.0, *, padding_index: Optional[int] = None, dtype=Type.F32,
+                       stream=None) -> Tensor:
+    """:func:`cvcuda_b200.embedding_backward` on objects of this module: the gradient of a table of ``num_rows`` rows."""
+    out = rows.embedding_backward(as_tensor(grad)._t, as_tensor(indices)._t, num_rows, scale, padding_index=padding_index,
+                                  data_type=_torch_dtype(dtype), stream=_stream_of(stream))
+    return _wrap(out, "")
+
+
+def embedding_backward_into(dtable: Tensor, grad, indices, scale: float = 1.0, *, padding_index: Optional[int] = None,
+                            accumulate: bool = False, stream=None) -> Tensor:
+    rows.embedding_backward_into(as_tensor(dtable)._t, as_tensor(grad)._t, as_tensor(indices)._t, scale, padding_index=padding_index,
+                                 accumulate=accumulate, stream=_stream_of(stream))
+    return dtable

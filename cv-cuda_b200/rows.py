@@ -1,0 +1,367 @@
+"""Row operators: LayerNorm and the embedding lookup, each with its gradient, on torch CUDA tensors.
+
+They sit between what the image operators produce (normalised batches, patches, label maps and the token ids that come with
+them) and the first activations of a model: :func:`layernorm` is the sibling of :func:`cvcuda_b200.normalize` that takes the
+statistics from the data, :func:`embedding` the sibling of :func:`cvcuda_b200.convertto` that gathers. The reference has no
+counterpart. PyTorch provides memory and streams; every value is computed by ``libcvcuda_b200.so`` through
+``include/cvcuda_b200/row_ops.h``.
+
+The functions do not take part in torch's autograd: gradients are calls of their own (``layernorm_backward``,
+``embedding_backward``). A tensor may be CUDA memory of any device (the call runs there) or page-locked host memory. Outputs and
+workspaces are allocated on the stream the call runs on; on a ``stream`` other than torch's current one, the caller orders the
+two as for every other operator here.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import ops
+from .ops import Error, Status, _check
+
+
+class _Rows(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("dtype", C.c_int32), ("cols", C.c_int64), ("count", C.c_int64 * 3), ("stride", C.c_int64 * 3)]
+
+
+class _LayerNormOp(C.Structure):
+    _fields_ = [("weight", C.c_void_p), ("bias", C.c_void_p), ("weightType", C.c_int32), ("biasType", C.c_int32),
+                ("epsilon", C.c_float), ("mean", C.c_void_p), ("rstd", C.c_void_p)]
+
+
+class _LayerNormGradOp(C.Structure):
+    _fields_ = [("mean", C.c_void_p), ("rstd", C.c_void_p), ("weight", C.c_void_p), ("weightType", C.c_int32),
+                ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("dweightType", C.c_int32), ("dbiasType", C.c_int32)]
+
+
+class _EmbeddingGradOp(C.Structure):
+    _fields_ = [("scale", C.c_float), ("accumulate", C.c_int32), ("paddingIndex", C.c_int64)]
+
+
+_TYPES = {torch.uint8: 0, torch.float32: 6, torch.float16: 7, torch.bfloat16: 8, torch.int32: 5, torch.int64: 9}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+_bound: Optional[C.CDLL] = None
+
+
+def _lib() -> C.CDLL:
+    global _bound
+    L = ops.lib()
+    if _bound is not L:
+        R, S = C.POINTER(_Rows), C.POINTER(C.c_size_t)
+        for name, args in (("LayerNormWorkspace", [R, S]),
+                           ("LayerNorm", [R, R, C.POINTER(_LayerNormOp), C.c_void_p, C.c_size_t, C.c_void_p]),
+                           ("LayerNormBackwardWorkspace", [R, S]),
+                           ("LayerNormBackward", [R, R, R, C.POINTER(_LayerNormGradOp), C.c_void_p, C.c_size_t, C.c_void_p]),
+                           ("Embedding", [R, R, R, C.c_float, C.c_void_p]),
+                           ("EmbeddingBackwardWorkspace", [R, S]),
+                           ("EmbeddingBackward", [R, R, R, C.POINTER(_EmbeddingGradOp), C.c_void_p, C.c_size_t, C.c_void_p])):
+            f = getattr(L, "b200pp" + name)
+            f.restype, f.argtypes = C.c_int, args
+        _bound = L
+    return _bound
+
+
+# ------------------------------------------------------------------------------------------------ arguments
+
+def _invalid(message: str) -> Error:
+    return Error(Status.ERROR_INVALID_ARGUMENT, message)
+
+
+def _device_of(*tensors) -> torch.device:
+    """The device the call runs on: that of the CUDA tensors, which must agree (page-locked host tensors follow)."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors")
+        if t.is_cuda:
+            if dev is None:
+                dev = t.device
+            elif t.device != dev:
+                raise _invalid(f"Tensors are on different devices ({dev} and {t.device})")
+        elif not t.is_pinned():
+            raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors")
+    return dev if dev is not None else torch.device("cuda", torch.cuda.current_device())
+
+
+def _rows(t: torch.Tensor, axes: int, what: str) -> _Rows:
+    """The rows that the last `axes` dimensions of `t` make, in the order of the others."""
+    shape, stride, lead = t.shape, t.stride(), t.dim() - axes
+    cols, es = 1, t.element_size()
+    for k in range(t.dim() - 1, lead - 1, -1):
+        if stride[k] != cols and shape[k] != 1 and t.numel():
+            raise _invalid(f"{what}: the last {axes} dimension(s) must be contiguous")
+        cols *= shape[k]
+    r = _Rows(t.data_ptr(), _TYPES.get(t.dtype, -1), cols)
+    dims = []  # (count, stride in elements), dimensions that continue one another merged
+    for k in range(lead):
+        n, s = shape[k], stride[k]
+        if n == 1:
+            continue
+        if dims and dims[-1][1] == n * s:
+            dims[-1] = (dims[-1][0] * n, s)
+        else:
+            dims.append((n, s))
+    if not t.numel():
+        dims = [(shape[k], 0) for k in range(lead)]
+        n = 1
+        for d in dims:
+            n *= d[0]
+        dims = [(n, cols)]
+    if len(dims) > 3:
+        raise _invalid(f"{what} has more than three independently strided dimensions of rows")
+    for k, (n, s) in enumerate(dims):
+        r.count[k], r.stride[k] = n, s * es
+    for k in range(len(dims), 3):
+        r.count[k] = 1
+    return r
+
+
+def _axes_of(t: torch.Tensor, axes: int) -> int:
+    axes = int(axes)
+    if axes < 1 or axes > t.dim():
+        raise _invalid(f"axes must be 1 to {t.dim()} for a tensor of {t.dim()} dimension(s)")
+    return axes
+
+
+def _param(t: Optional[torch.Tensor], numel: int, what: str, kinds=_FLOATS) -> Tuple[Optional[int], int]:
+    """(address, type code) of a packed tensor of `numel` values, or (None, 0)."""
+    if t is None:
+        return None, 0
+    if t.dtype not in kinds:
+        raise _invalid(f"Invalid DataType of the {what}")
+    if t.numel() != numel or not t.is_contiguous():
+        raise _invalid(f"The {what} must be packed and hold {numel} value(s)")
+    return t.data_ptr(), _TYPES[t.dtype]
+
+
+class _Launch(contextlib.AbstractContextManager):
+    """Makes `device` and the launch stream torch's current ones, so that what the call allocates belongs to that stream;
+    gives the stream's handle. Does nothing where they are current already."""
+
+    def __init__(self, device: torch.device, stream):
+        self._stack = None
+        other = device.index is not None and device.index != torch.cuda.current_device()
+        if stream is None:
+            if other:
+                self._stack = contextlib.ExitStack()
+                self._stack.enter_context(torch.cuda.device(device))
+            self.handle = torch.cuda.current_stream(device).cuda_stream
+            return
+        self.handle = ops._stream_handle(stream)
+        if other or self.handle != torch.cuda.current_stream(device).cuda_stream:
+            self._stack = contextlib.ExitStack()
+            if other:
+                self._stack.enter_context(torch.cuda.device(device))
+            if isinstance(stream, torch.cuda.Stream):
+                if stream.device != device:
+                    raise _invalid(f"The stream belongs to {stream.device}, the tensors to {device}")
+            else:
+                stream = torch.cuda.ExternalStream(self.handle, device=device) if self.handle else torch.cuda.default_stream(device)
+            self._stack.enter_context(torch.cuda.stream(stream))
+
+    def __enter__(self):
+        return self.handle
+
+    def __exit__(self, *exc):
+        return self._stack.__exit__(*exc) if self._stack is not None else None
+
+
+def _workspace(query, rows: _Rows, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    n = C.c_size_t(0)
+    _check(query(C.byref(rows), C.byref(n)))
+    if n.value == 0:
+        return None, None, 0
+    t = torch.empty(n.value, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), n.value
+
+
+# ------------------------------------------------------------------------------------------------ LayerNorm
+
+def _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle):
+    s = _rows(src, axes, "Input")
+    d = _rows(dst, axes, "Output")
+    count = src.numel() // s.cols if s.cols else 0
+    op = _LayerNormOp()
+    op.weight, op.weightType = _param(weight, s.cols, "weight")
+    op.bias, op.biasType = _param(bias, s.cols, "bias")
+    op.epsilon = epsilon
+    op.mean, _ = _param(mean, count, "mean", (torch.float32,))
+    op.rstd, _ = _param(rstd, count, "rstd", (torch.float32,))
+    L = _lib()
+    keep, ws, size = _workspace(L.b200ppLayerNormWorkspace, s, device)
+    _check(L.b200ppLayerNorm(C.byref(s), C.byref(d), C.byref(op), ws, size, handle))
+
+
+def layernorm_into(dst: torch.Tensor, src: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, epsilon: float = 1e-5, *, axes: int = 1,
+                   mean: Optional[torch.Tensor] = None, rstd: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """LayerNorm into ``dst`` (float16, bfloat16 or float32, the shape of ``src``): see :func:`layernorm`. ``mean`` and
+    ``rstd``: packed float32 tensors, one value per row, that receive the statistics. ``dst`` may be ``src``."""
+    device = _device_of(src, dst, weight, bias, mean, rstd)
+    axes = _axes_of(src, axes)
+    if dst.shape != src.shape:
+        raise _invalid("Input and output shapes are different")
+    with _Launch(device, stream) as handle:
+        _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle)
+    return dst
+
+
+def layernorm(src: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+              epsilon: float = 1e-5, *, axes: int = 1, data_type: Optional[torch.dtype] = None, stats: bool = False, stream=None):
+    """``(src - mean) / sqrt(variance + epsilon) * weight + bias`` with the mean and variance of each row, a row being the last
+    ``axes`` dimensions of ``src``: 1 normalises the channels of an NHWC tensor or the features of tokens, 3 whole HWC images
+    (per-image standardisation). ``src``: uint8, float16, bfloat16 or float32; the dimensions of a row must be contiguous, the
+    others may have any strides. ``weight`` / ``bias``: one value per element of a row, or None. The result has
+    ``data_type`` (float16, bfloat16 or float32; default: that of ``src``, float32 for uint8). With ``stats``, returns
+    (result, mean, rstd), the float32 statistics of the rows that :func:`layernorm_backward` takes."""
+    device = _device_of(src, weight, bias)
+    axes = _axes_of(src, axes)
+    kind = data_type or (src.dtype if src.dtype != torch.uint8 else torch.float32)
+    with _Launch(device, stream) as handle:
+        dst = torch.empty(src.shape, dtype=kind, device=device)
+        mean = rstd = None
+        if stats:
+            mean = torch.empty(src.shape[:src.dim() - axes], dtype=torch.float32, device=device)
+            rstd = torch.empty_like(mean)
+        _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle)
+    return (dst, mean, rstd) if stats else dst
+
+
+def _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle):
+    g, s = _rows(grad, axes, "Gradient"), _rows(src, axes, "Input")
+    d = _rows(dsrc, axes, "Input gradient") if dsrc is not None else None
+    count = src.numel() // s.cols if s.cols else 0
+    op = _LayerNormGradOp()
+    op.mean, _ = _param(mean, count, "mean", (torch.float32,))
+    op.rstd, _ = _param(rstd, count, "rstd", (torch.float32,))
+    op.weight, op.weightType = _param(weight, s.cols, "weight")
+    op.dweight, op.dweightType = _param(dweight, s.cols, "weight gradient")
+    op.dbias, op.dbiasType = _param(dbias, s.cols, "bias gradient")
+    L = _lib()
+    keep, ws, size = (None, None, 0)
+    if dweight is not None or dbias is not None:
+        keep, ws, size = _workspace(L.b200ppLayerNormBackwardWorkspace, s, device)
+    _check(L.b200ppLayerNormBackward(C.byref(g), C.byref(s), C.byref(d) if d is not None else None, C.byref(op), ws, size, handle))
+
+
+def layernorm_backward_into(dsrc: Optional[torch.Tensor], dweight: Optional[torch.Tensor], dbias: Optional[torch.Tensor],
+                            grad: torch.Tensor, src: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                            weight: Optional[torch.Tensor] = None, *, axes: int = 1, stream=None):
+    """The gradients of :func:`layernorm` into the tensors given (None: not wanted): see :func:`layernorm_backward`.
+    ``dsrc`` may be ``grad`` or ``src``."""
+    device = _device_of(grad, src, mean, rstd, weight, dsrc, dweight, dbias)
+    axes = _axes_of(src, axes)
+    if grad.shape != src.shape or (dsrc is not None and dsrc.shape != src.shape):
+        raise _invalid("Input and gradient shapes are different")
+    with _Launch(device, stream) as handle:
+        _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle)
+    return dsrc, dweight, dbias
+
+
+def layernorm_backward(grad: torch.Tensor, src: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                       weight: Optional[torch.Tensor] = None, *, axes: int = 1, data_type: Optional[torch.dtype] = None,
+                       src_grad: bool = True, weight_grad: bool = True, bias_grad: bool = True, stream=None):
+    """(dsrc, dweight, dbias): the gradients of :func:`layernorm`, given that of its result and the statistics it returned;
+    None for those switched off. ``dsrc`` has ``data_type`` (default: the type of ``src``, that of ``grad`` for uint8);
+    ``dweight`` and ``dbias`` have the type of ``weight`` (float32 without one) and the shape of a row."""
+    device = _device_of(grad, src, mean, rstd, weight)
+    axes = _axes_of(src, axes)
+    if grad.shape != src.shape:
+        raise _invalid("Input and gradient shapes are different")
+    with _Launch(device, stream) as handle:
+        dsrc = dweight = dbias = None
+        row = src.shape[src.dim() - axes:]
+        if src_grad:
+            dsrc = torch.empty(src.shape, dtype=data_type or (src.dtype if src.dtype != torch.uint8 else grad.dtype), device=device)
+        kind = weight.dtype if weight is not None else torch.float32
+        if weight_grad:
+            dweight = torch.empty(row, dtype=kind, device=device)
+        if bias_grad:
+            dbias = torch.empty(row, dtype=kind, device=device)
+        _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle)
+    return dsrc, dweight, dbias
+
+
+# ------------------------------------------------------------------------------------------------ embedding lookup
+
+def _indices(indices: torch.Tensor) -> _Rows:
+    return _rows(indices.unsqueeze(-1), 1, "Indices")
+
+
+def _matrix(t: torch.Tensor, what: str) -> _Rows:
+    if t.dim() != 2:
+        raise _invalid(f"{what} must have two dimensions")
+    return _rows(t, 1, what)
+
+
+def _embedding(dst, indices, table, scale, handle):
+    i, t, d = _indices(indices), _matrix(table, "Table"), _rows(dst, 1, "Output")
+    _check(_lib().b200ppEmbedding(C.byref(i), C.byref(t), C.byref(d), scale, handle))
+
+
+def embedding_into(dst: torch.Tensor, indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *, stream=None) -> torch.Tensor:
+    """Embedding lookup into ``dst`` (the shape of ``indices`` followed by the number of columns): see :func:`embedding`."""
+    device = _device_of(table, indices, dst)
+    if table.dim() != 2 or dst.shape != (*indices.shape, table.shape[1]):
+        raise _invalid("The output must have the indices' shape followed by the table's number of columns")
+    with _Launch(device, stream) as handle:
+        _embedding(dst, indices, table, scale, handle)
+    return dst
+
+
+def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *, data_type: Optional[torch.dtype] = None,
+              stream=None) -> torch.Tensor:
+    """``scale * table[indices]``: ``indices`` (uint8, int32 or int64, any shape) select rows of ``table`` [rows, columns]
+    (float16, bfloat16 or float32) -- tokens, positions, class labels, the colours of a label map. An index outside the table
+    gives zeros. The result has ``data_type`` (default: that of ``table``)."""
+    device = _device_of(table, indices)
+    if table.dim() != 2:
+        raise _invalid("Table must have two dimensions")
+    with _Launch(device, stream) as handle:
+        dst = torch.empty((*indices.shape, table.shape[1]), dtype=data_type or table.dtype, device=device)
+        _embedding(dst, indices, table, scale, handle)
+    return dst
+
+
+def _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate, device, handle):
+    g, i, d = _rows(grad, 1, "Gradient"), _indices(indices), _matrix(dtable, "Table gradient")
+    op = _EmbeddingGradOp(scale, int(accumulate), -1 if padding_index is None else int(padding_index))
+    L = _lib()
+    keep, ws, size = _workspace(L.b200ppEmbeddingBackwardWorkspace, g, device)
+    _check(L.b200ppEmbeddingBackward(C.byref(g), C.byref(i), C.byref(d), C.byref(op), ws, size, handle))
+
+
+def embedding_backward_into(dtable: torch.Tensor, grad: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, *,
+                            padding_index: Optional[int] = None, accumulate: bool = False, stream=None) -> torch.Tensor:
+    """The gradient of :func:`embedding` with respect to the table into ``dtable``, or added to it with ``accumulate``
+    (rows no index names are then left alone): see :func:`embedding_backward`."""
+    device = _device_of(dtable, grad, indices)
+    if dtable.dim() != 2 or grad.shape != (*indices.shape, dtable.shape[1]):
+        raise _invalid("The gradient must have the indices' shape followed by the table's number of columns")
+    with _Launch(device, stream) as handle:
+        _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate, device, handle)
+    return dtable
+
+
+def embedding_backward(grad: torch.Tensor, indices: torch.Tensor, rows: int, scale: float = 1.0, *,
+                       padding_index: Optional[int] = None, data_type: torch.dtype = torch.float32, stream=None) -> torch.Tensor:
+    """The gradient of :func:`embedding` with respect to a table of ``rows`` rows: row v is ``scale`` times the sum of the rows
+    of ``grad`` whose index is v, zero if there is none. Indices outside the table and those equal to ``padding_index`` take
+    no part. The sums are float32 in an order that depends on the indices alone, rounded to ``data_type`` once."""
+    device = _device_of(grad, indices)
+    if grad.dim() < 1 or grad.shape[:-1] != indices.shape:
+        raise _invalid("The gradient must have the indices' shape followed by the table's number of columns")
+    with _Launch(device, stream) as handle:
+        dtable = torch.empty((int(rows), grad.shape[-1]), dtype=data_type, device=device)
+        _embedding_backward(dtable, grad, indices, scale, padding_index, False, device, handle)
+    return dtable
+
+
+__all__ = ["layernorm", "layernorm_into", "layernorm_backward", "layernorm_backward_into", "embedding", "embedding_into",
+           "embedding_backward", "embedding_backward_into"]
