@@ -1,0 +1,240 @@
+// Host side of the embedding lookup and its gradient: argument validation, kernel selection and launch.
+#include "embedding_kernels.cuh"
+#include "row_host.h"
+
+#include <algorithm>
+#include <atomic>
+
+using namespace b200pp;
+
+namespace {
+
+int check_indices(const B200ppRows *indices)
+{
+    if (indices->dtype != B200PP_U8 && indices->dtype != B200PP_S32 && indices->dtype != B200PP_S64)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Indices must be uint8, int32 or int64");
+    if (indices->cols != 1)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Indices must have one column");
+    return B200PP_SUCCESS;
+}
+
+} // namespace
+
+namespace {
+
+template<int TABLE, int W>
+int launch_embedding(EmbeddingKParams &p, cudaStream_t stream)
+{
+    // lanes per row: a warp, fewer for rows that would leave half of it idle; up to four vectors per lane
+    int lanes = 32;
+    while (lanes > 1 && (lanes / 2) * W >= p.cols) lanes /= 2;
+    const int u = p.cols <= lanes * W ? 1 : p.cols <= lanes * W * 2 ? 2 : 4;
+    p.blocks    = (p.cols + lanes * W * u - 1) / (lanes * W * u);
+    const dim3               block(lanes, 256 / lanes);
+    const unsigned long long jobs = static_cast<unsigned long long>(p.count) * p.blocks, ctas = (jobs + block.y - 1) / block.y;
+    if (ctas > 0x7fffffffull)
+        return fail(B200PP_ERROR_OVERFLOW, "Output is too large");
+    const unsigned grid = static_cast<unsigned>(ctas);
+    if (u == 1)
+        embedding_kernel<TABLE, W, 1><<<grid, block, 0, stream>>>(p);
+    else if (u == 2)
+        embedding_kernel<TABLE, W, 2><<<grid, block, 0, stream>>>(p);
+    else
+        embedding_kernel<TABLE, W, 4><<<grid, block, 0, stream>>>(p);
+    return check_launch("Embedding");
+}
+
+template<int TABLE>
+int launch_embedding(EmbeddingKParams &p, int width, cudaStream_t stream)
+{
+    if (width == 8)
+        return launch_embedding<TABLE, 8>(p, stream);
+    if (width == 4)
+        return launch_embedding<TABLE, 4>(p, stream);
+    if (width == 2)
+        return launch_embedding<TABLE, 2>(p, stream);
+    return launch_embedding<TABLE, 1>(p, stream);
+}
+
+} // namespace
+
+extern "C" int b200ppEmbedding(const B200ppRows *indices, const B200ppRows *table, const B200ppRows *dst, float scale,
+                               cudaStream_t stream)
+{
+    if (!indices || !table || !dst)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
+    if (!is_float(table->dtype) || !is_float(dst->dtype))
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Invalid DataType");
+    if (table->cols != dst->cols)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Table and output have different numbers of columns");
+    EmbeddingKParams p{};
+    long long        count = 0, dstRows = 0, rows = 0;
+    int              st;
+    if ((st = check_indices(indices)) || (st = take_rows(indices, "Indices", false, p.indices, count))
+        || (st = take_rows(table, "Table", false, p.table, rows)) || (st = take_rows(dst, "Output", true, p.dst, dstRows)))
+        return st;
+    if (count != dstRows)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Indices and output have different numbers of rows");
+    if (count == 0)
+        return B200PP_SUCCESS;
+    p.indexType = indices->dtype;
+    p.tableType = table->dtype;
+    p.dstType   = dst->dtype;
+    p.count     = static_cast<unsigned>(count);
+    p.rows      = static_cast<int>(rows);
+    p.cols      = static_cast<int>(dst->cols);
+    p.scale     = scale;
+    const int elem = row_elem_size(dst->dtype);
+    if (p.cols < 8 && p.dst.n2 == 0 && (count == 1 || p.dst.s2 == static_cast<long long>(p.cols) * elem)
+        && (reinterpret_cast<uintptr_t>(p.dst.base) & (8 * elem - 1)) == 0)
+    {
+        const unsigned long long ctas = (static_cast<unsigned long long>(count) * p.cols + 2047) / 2048; // at most 2^31 * 7 / 2^11
+        embedding_short_rows_kernel<<<static_cast<unsigned>(ctas), 256, 0, stream>>>(p);
+        return check_launch("Embedding");
+    }
+    VecWidth width(p.cols);
+    width.take(p.table, row_elem_size(table->dtype));
+    width.take(p.dst, elem);
+    if (table->dtype == B200PP_F16)
+        return launch_embedding<B200PP_F16>(p, width.width, stream);
+    if (table->dtype == B200PP_BF16)
+        return launch_embedding<B200PP_BF16>(p, width.width, stream);
+    return launch_embedding<B200PP_F32>(p, width.width, stream);
+}
+
+namespace {
+
+// Layout of the gradient's workspace.
+struct EmbeddingGradPlan
+{
+    unsigned unit, units;
+    size_t   keys[2], order[2], partials, bytes;
+};
+
+EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
+{
+    EmbeddingGradPlan w{};
+    w.unit       = 32;
+    w.units      = static_cast<unsigned>((count + w.unit - 1) / w.unit);
+    size_t at    = 0;
+    const size_t list = align_up(static_cast<size_t>(count) * sizeof(unsigned));
+    for (int k = 0; k < 2; ++k)
+    {
+        w.keys[k] = at;
+        at += list;
+        w.order[k] = at;
+        at += list;
+    }
+    w.partials = at;
+    w.bytes    = at + static_cast<size_t>(w.units) * 2 * cols * sizeof(float);
+    return w;
+}
+
+// Raises a kernel's dynamic shared-memory limit, once per device.
+template<typename K>
+int raise_smem(K kernel, int bytes, std::atomic<unsigned long long> &done)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit))
+        return B200PP_SUCCESS;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess)
+    {
+        cudaGetLastError();
+        return fail(B200PP_ERROR_INTERNAL, "Cannot raise a kernel's shared memory to %d bytes: %s", bytes, cudaGetErrorString(e));
+    }
+    done.fetch_or(bit);
+    return B200PP_SUCCESS;
+}
+
+} // namespace
+
+extern "C" int b200ppEmbeddingBackwardWorkspace(const B200ppRows *grad, size_t *bytes)
+{
+    if (!grad || !bytes)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
+    RowMap     m;
+    long long  count = 0;
+    B200ppRows t     = *grad;
+    t.base           = reinterpret_cast<void *>(uintptr_t(256));
+    if (int st = take_rows(&t, "Gradient", false, m, count))
+        return st;
+    *bytes = count > 0 ? plan_embedding_grad(count, t.cols).bytes : 0;
+    return B200PP_SUCCESS;
+}
+
+extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows *indices, const B200ppRows *dtable,
+                                       const B200ppEmbeddingGradOp *op, void *workspace, size_t workspaceBytes,
+                                       cudaStream_t stream)
+{
+    if (!grad || !indices || !dtable || !op)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
+    if (!is_float(grad->dtype) || !is_float(dtable->dtype))
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Invalid DataType");
+    if (grad->cols != dtable->cols)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Gradient and table have different numbers of columns");
+    EmbeddingGradKParams p{};
+    long long            count = 0, gradRows = 0, rows = 0;
+    int                  st;
+    if ((st = check_indices(indices)) || (st = take_rows(indices, "Indices", false, p.indices, count))
+        || (st = take_rows(grad, "Gradient", false, p.grad, gradRows)) || (st = take_rows(dtable, "Table gradient", true, p.dtable, rows)))
+        return st;
+    if (count != gradRows)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Indices and gradient have different numbers of rows");
+    if (rows == 0)
+        return B200PP_SUCCESS;
+    const EmbeddingGradPlan w = plan_embedding_grad(count, grad->cols);
+    if (count > 0 && (st = check_workspace(workspace, workspaceBytes, w.bytes)))
+        return st;
+    uint8_t *ws  = static_cast<uint8_t *>(workspace);
+    p.gradType   = grad->dtype;
+    p.indexType  = indices->dtype;
+    p.dtableType = dtable->dtype;
+    p.count      = static_cast<unsigned>(count);
+    p.rows       = static_cast<int>(rows);
+    p.cols       = static_cast<int>(grad->cols);
+    p.scale      = op->scale;
+    p.accumulate = op->accumulate != 0;
+    p.padding    = op->paddingIndex >= 0 && op->paddingIndex < rows ? static_cast<int>(op->paddingIndex) : -1;
+    p.unit       = w.unit;
+    if (!p.accumulate)
+    {
+        embedding_zero_kernel<<<std::min(static_cast<unsigned>(rows), 65535u), 256, 0, stream>>>(p);
+        if ((st = check_launch("EmbeddingBackward")))
+            return st;
+    }
+    if (count == 0)
+        return B200PP_SUCCESS;
+    for (int k = 0; k < 2; ++k)
+    {
+        p.keys[k]  = reinterpret_cast<unsigned *>(ws + w.keys[k]);
+        p.order[k] = reinterpret_cast<unsigned *>(ws + w.order[k]);
+    }
+    p.partials = reinterpret_cast<float *>(ws + w.partials);
+    int bits = 1; // of the largest key, `rows`
+    while (bits < 31 && (rows >> bits) != 0) ++bits;
+    p.passes    = (bits + kSortMaxBits - 1) / kSortMaxBits;
+    p.digitBits = (bits + p.passes - 1) / p.passes;
+    const int bins = 1 << p.digitBits;
+    static std::atomic<unsigned long long> raised{0};
+    if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(sort_smem_words(1 << kSortMaxBits) * sizeof(unsigned)), raised)))
+        return st;
+    embedding_sort_kernel<<<kSortCtas, kSortThreads, sort_smem_words(bins) * sizeof(unsigned), stream>>>(p);
+    if ((st = check_launch("EmbeddingBackward")))
+        return st;
+    const unsigned           blocks = (p.cols + 255u) / 256u;
+    const unsigned long long jobs   = static_cast<unsigned long long>(w.units) * blocks;
+    if ((jobs + 7) / 8 > 0x7fffffffull || blocks > 65535u)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Gradient is too large");
+    embedding_grad_runs_kernel<<<static_cast<unsigned>((jobs + 7) / 8), 256, 0, stream>>>(p);
+    if ((st = check_launch("EmbeddingBackward")))
+        return st;
+    if (w.units > 1)
+    {
+        embedding_grad_join_kernel<<<dim3(w.units - 1, blocks), 256, 0, stream>>>(p);
+        st = check_launch("EmbeddingBackward");
+    }
+    return st;
+}

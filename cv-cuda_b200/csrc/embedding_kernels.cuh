@@ -21,21 +21,78 @@ struct EmbeddingKParams
     unsigned count;
     int      rows, cols;
     float    scale;
+    unsigned blocks; // of a row
 };
 
-// One warp per row.
+// blockDim.x lanes of a warp per row, blockDim.y rows per CTA; a lane moves up to U vectors of W neighbouring elements, one
+// block of blockDim.x * U vectors of the row at a time. All loads of a block are issued before the first is used.
+template<int TABLE, int W, int U>
 __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingKParams p)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (unsigned long long i = blockIdx.x * 8ull + warp; i < p.count; i += gridDim.x * 8ull)
+    const unsigned long long job = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const unsigned           r   = static_cast<unsigned>(p.blocks == 1 ? job : job / p.blocks);
+    if (job >= static_cast<unsigned long long>(p.count) * p.blocks)
+        return;
+    const int      span = blockDim.x * W;
+    const int      c0   = static_cast<int>(job - static_cast<unsigned long long>(r) * p.blocks) * (span * U) + threadIdx.x * W;
+    const int      id   = load_index(p.indices, p.indexType, r, p.rows);
+    uint8_t       *y    = p.dst.at(r);
+    const uint8_t *t    = p.table.at(max(id, 0));
+    Vec<TABLE, W>  raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
     {
-        const unsigned r  = static_cast<unsigned>(i);
-        const int      id = load_index(p.indices, p.indexType, r, p.rows);
-        uint8_t       *y  = p.dst.at(r);
-        const uint8_t *t  = p.table.at(max(id, 0));
-        for (long long c = lane; c < p.cols; c += 32)
-            store_elem_as(y, c, p.dstType, id < 0 ? 0.0f : load_elem(t, c, p.tableType) * p.scale);
+        const int c = c0 + u * span;
+        raw[u]      = zero_raw<kElemBytes<TABLE> * W>();
+        if (id >= 0 && c < p.cols)
+            raw[u] = load_raw<kElemBytes<TABLE> * W>(t + static_cast<long long>(c) * kElemBytes<TABLE>);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+    {
+        const int c = c0 + u * span;
+        float     v[W];
+        unpack<TABLE, W>(raw[u], v);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = id < 0 ? 0.0f : v[i] * p.scale;
+        if (c < p.cols)
+            store_vec<W>(y, c, p.dstType, v);
+    }
+}
+
+// Rows of a few elements that follow one another without gaps (a palette's colours): a thread makes eight neighbouring elements of
+// the output, whichever rows they belong to, and stores them as one vector.
+__global__ void __launch_bounds__(256) embedding_short_rows_kernel(const EmbeddingKParams p)
+{
+    const unsigned long long total = static_cast<unsigned long long>(p.count) * p.cols;
+    const unsigned long long e0    = (static_cast<unsigned long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
+    if (e0 >= total)
+        return;
+    unsigned       r  = static_cast<unsigned>(e0 / p.cols);
+    int            c  = static_cast<int>(e0 - static_cast<unsigned long long>(r) * p.cols);
+    int            id = load_index(p.indices, p.indexType, r, p.rows);
+    const uint8_t *t  = p.table.at(max(id, 0));
+    float          v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        v[i] = 0.0f;
+        if (e0 + i < total)
+        {
+            if (id >= 0)
+                v[i] = load_elem(t, c, p.tableType) * p.scale;
+            if (++c == p.cols && e0 + i + 1 < total)
+            {
+                c  = 0;
+                id = load_index(p.indices, p.indexType, ++r, p.rows);
+                t  = p.table.at(max(id, 0));
+            }
+        }
+    }
+    if (e0 + 8 <= total)
+        store_vec<8>(p.dst.base, e0, p.dstType, v);
+    else
+        for (int i = 0; i < 8 && e0 + i < total; ++i) store_elem_as(p.dst.base, e0 + i, p.dstType, v[i]);
 }
 
 struct EmbeddingGradKParams
@@ -69,7 +126,7 @@ inline size_t sort_smem_words(int bins)
     return static_cast<size_t>(bins) * (kSortThreads / 32) + bins + 32;
 }
 
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) embedding_sort_kernel(const EmbeddingGradKParams p)
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const EmbeddingGradKParams p)
 {
     namespace cg = cooperative_groups;
     extern __shared__ unsigned smem[];

@@ -19,6 +19,8 @@ struct LayerNormKParams
     const uint8_t *weight, *bias;
     float          epsilon, fcols; // fcols: the number of columns
     float         *mean, *rstd;
+    unsigned       chunks;   // of a long row
+    float2        *partials; // [rows][chunks]
 };
 
 struct LayerNormGradKParams
@@ -35,39 +37,201 @@ struct LayerNormGradKParams
     int            parts;
 };
 
-// One CTA per row, any row length.
-template<int SRC>
-__global__ void __launch_bounds__(256) layernorm_row_kernel(const LayerNormKParams p)
+// A thread holds E values of its row: vectors of W neighbouring elements, T vectors apart (T: the threads of the row), so that
+// every load and store of a warp covers one contiguous span.
+template<int W>
+__device__ __forceinline__ int vec_at(int v, int t, int threads)
 {
-    __shared__ float scratch[32];
-    for (unsigned r = blockIdx.x; r < p.rows; r += gridDim.x)
+    return (v * threads + t) * W;
+}
+
+// Sum over the `lanes` neighbouring lanes (a power of two) a row has in a warp, or over the block.
+template<bool BLOCK>
+__device__ __forceinline__ float row_sum(float v, int lanes, float *scratch)
+{
+    if constexpr (!BLOCK)
     {
-        const uint8_t *x = p.src.at(r);
-        uint8_t       *y = p.dst.at(r);
-        float          s = 0.0f;
-        for (int c = threadIdx.x; c < p.cols; c += blockDim.x) s += load_elem<SRC>(x, c);
-        const float mean = block_sum(s, scratch) / p.fcols;
-        float       q    = 0.0f;
-        for (int c = threadIdx.x; c < p.cols; c += blockDim.x)
-        {
-            const float d = load_elem<SRC>(x, c) - mean;
-            q             = fmaf(d, d, q);
-        }
-        const float rstd = 1.0f / sqrtf(block_sum(q, scratch) / p.fcols + p.epsilon);
-        if (threadIdx.x == 0)
-        {
-            if (p.mean)
-                p.mean[r] = mean;
-            if (p.rstd)
-                p.rstd[r] = rstd;
-        }
-        for (int c = threadIdx.x; c < p.cols; c += blockDim.x)
-        {
-            const float w = p.weight ? load_elem(p.weight, c, p.weightType) : 1.0f;
-            const float b = p.bias ? load_elem(p.bias, c, p.biasType) : 0.0f;
-            store_elem_as(y, c, p.dstType, fmaf((load_elem<SRC>(x, c) - mean) * rstd, w, b));
-        }
+        for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
     }
+    else
+    {
+        // one barrier per sum: consecutive sums use different halves of the scratch memory
+        v = warp_sum(v);
+        if ((threadIdx.x & 31) == 0)
+            scratch[threadIdx.x >> 5] = v;
+        __syncthreads();
+        const float s = (threadIdx.x & 31) < ((blockDim.x + 31) >> 5) ? scratch[threadIdx.x & 31] : 0.0f;
+        return warp_sum(s);
+    }
+}
+
+// y of one thread's values.
+template<int E, int W>
+__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const float *x, float mean, float rstd, int c0,
+                                                int step, int end)
+{
+#pragma unroll
+    for (int v = 0; v < E / W; ++v)
+    {
+        const int c = c0 + v * step;
+        if (c >= end)
+            break;
+        float w[W], b[W], o[W];
+        if (p.weight)
+            load_vec<W>(p.weight, c, p.weightType, w);
+        if (p.bias)
+            load_vec<W>(p.bias, c, p.biasType, b);
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+        {
+            const float h = (x[v * W + i] - mean) * rstd;
+            o[i]          = p.weight ? (p.bias ? fmaf(h, w[i], b[i]) : h * w[i]) : (p.bias ? h + b[i] : h);
+        }
+        store_vec<W>(y, c, p.dstType, o);
+    }
+}
+
+// Forward, rows that fit into registers. BLOCK: one CTA per row; otherwise blockDim.x lanes of a warp per row and
+// blockDim.y rows per CTA. The statistics come from the registers (the variance about the mean), so the row is read once.
+template<int SRC, int E, int W, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? (E <= 16 ? 512 : 1024) : 256) layernorm_kernel(const LayerNormKParams p)
+{
+    __shared__ float scratch[2][32];
+    const int        t = threadIdx.x, threads = blockDim.x;
+    const unsigned   r = BLOCK ? blockIdx.x : blockIdx.x * blockDim.y + threadIdx.y;
+    if (!BLOCK && r - threadIdx.y % (32u / threads) >= p.rows) // all rows of the warp
+        return;
+    const bool     live = BLOCK || r < p.rows;
+    const uint8_t *x    = p.src.at(live ? r : p.rows - 1);
+    Vec<SRC, W>    raw[E / W];
+#pragma unroll
+    for (int v = 0; v < E / W; ++v)
+    {
+        const int c = vec_at<W>(v, t, threads);
+        raw[v]      = zero_raw<kElemBytes<SRC> * W>();
+        if (c < p.cols)
+            raw[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
+    }
+    float xv[E], s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < E / W; ++v)
+    {
+        unpack<SRC, W>(raw[v], xv + v * W);
+#pragma unroll
+        for (int i = 0; i < W; ++i) s += xv[v * W + i];
+    }
+    const float mean = row_sum<BLOCK>(s, threads, scratch[0]) / p.fcols;
+    float       q    = 0.0f;
+#pragma unroll
+    for (int v = 0; v < E / W; ++v)
+        if (vec_at<W>(v, t, threads) < p.cols)
+        {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+            {
+                const float d = xv[v * W + i] - mean;
+                q             = fmaf(d, d, q);
+            }
+        }
+    const float rstd = 1.0f / sqrtf(row_sum<BLOCK>(q, threads, scratch[1]) / p.fcols + p.epsilon);
+    if (!live)
+        return;
+    if (t == 0)
+    {
+        if (p.mean)
+            p.mean[r] = mean;
+        if (p.rstd)
+            p.rstd[r] = rstd;
+    }
+    layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, t * W, threads * W, p.cols);
+}
+
+// Forward, longer rows: two kernels over chunks of kChunk values. The first leaves each chunk's mean and sum of squared distances
+// to it; the second joins those of its row (as Chan, Golub and LeVeque do for two sets) and normalises its chunk. It takes the
+// chunks in reverse order, so that the ones read last by the first kernel are still in L2.
+constexpr int kChunk        = 8192;
+constexpr int kChunkThreads = 256;
+
+template<int SRC, int W>
+__device__ __forceinline__ void load_chunk(const uint8_t *x, int c0, int end, float (&xv)[kChunk / kChunkThreads])
+{
+    constexpr int V = kChunk / kChunkThreads / W;
+    Vec<SRC, W>   raw[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+    {
+        const int c = c0 + vec_at<W>(v, threadIdx.x, kChunkThreads);
+        raw[v]      = zero_raw<kElemBytes<SRC> * W>();
+        if (c < end)
+            raw[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) unpack<SRC, W>(raw[v], xv + v * W);
+}
+
+template<int SRC, int W>
+__global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_stats_kernel(const LayerNormKParams p)
+{
+    __shared__ float scratch[2][32];
+    constexpr int    E   = kChunk / kChunkThreads;
+    const unsigned   r   = blockIdx.x / p.chunks;
+    const long long  at  = static_cast<long long>(blockIdx.x - r * p.chunks) * kChunk;
+    const int        c0  = static_cast<int>(at);
+    const int        end = min(static_cast<long long>(p.cols), at + kChunk);
+    float            xv[E], s = 0.0f, q = 0.0f;
+    load_chunk<SRC, W>(p.src.at(r), c0, end, xv);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += xv[e];
+    const float mean = row_sum<true>(s, 0, scratch[0]) / static_cast<float>(end - c0);
+#pragma unroll
+    for (int v = 0; v < E / W; ++v)
+        if (c0 + vec_at<W>(v, threadIdx.x, kChunkThreads) < end)
+        {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+            {
+                const float d = xv[v * W + i] - mean;
+                q             = fmaf(d, d, q);
+            }
+        }
+    q = row_sum<true>(q, 0, scratch[1]);
+    if (threadIdx.x == 0)
+        p.partials[blockIdx.x] = make_float2(mean, q);
+}
+
+template<int SRC, int W>
+__global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(const LayerNormKParams p)
+{
+    __shared__ float scratch[2][32];
+    constexpr int    E   = kChunk / kChunkThreads;
+    const unsigned   job = gridDim.x - 1 - blockIdx.x;
+    const unsigned   r   = job / p.chunks;
+    const long long  at  = static_cast<long long>(job - r * p.chunks) * kChunk;
+    const int        c0  = static_cast<int>(at);
+    const int        end = min(static_cast<long long>(p.cols), at + kChunk);
+    float            xv[E];
+    load_chunk<SRC, W>(p.src.at(r), c0, end, xv);
+    const float2 *part = p.partials + static_cast<unsigned long long>(r) * p.chunks;
+    const float   tail = static_cast<float>(p.cols - static_cast<long long>(p.chunks - 1) * kChunk); // length of the last chunk
+    float         s    = 0.0f;
+    for (unsigned k = threadIdx.x; k < p.chunks; k += kChunkThreads) s += part[k].x * (k + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
+    const float mean = row_sum<true>(s, 0, scratch[0]) / p.fcols;
+    float       q    = 0.0f;
+    for (unsigned k = threadIdx.x; k < p.chunks; k += kChunkThreads)
+    {
+        const float d = part[k].x - mean;
+        q += part[k].y + d * d * (k + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<true>(q, 0, scratch[1]) / p.fcols + p.epsilon);
+    if (c0 == 0 && threadIdx.x == 0)
+    {
+        if (p.mean)
+            p.mean[r] = mean;
+        if (p.rstd)
+            p.rstd[r] = rstd;
+    }
+    layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, c0 + threadIdx.x * W, kChunkThreads * W, end);
 }
 
 // dx, one CTA per row, any row length.

@@ -123,6 +123,181 @@ __device__ __forceinline__ void store_elem_as(uint8_t *row, long long i, int dty
     }
 }
 
+// ---- vectors of W neighbouring elements (W * size bytes, on a boundary of as many bytes)
+
+template<int BYTES>
+struct RawVec
+{
+    unsigned w[BYTES / 4];
+};
+template<>
+struct RawVec<2>
+{
+    unsigned short w[1];
+};
+template<>
+struct RawVec<1>
+{
+    unsigned char w[1];
+};
+
+// Size of an element type in bytes.
+template<int DT>
+constexpr int kElemBytes = sizeof(typename Elem<DT>::type);
+
+template<int DT, int W>
+using Vec = RawVec<kElemBytes<DT> * W>;
+
+// Plain loads (not the read-only path): the operators may be asked to write over what they read.
+template<int BYTES>
+__device__ __forceinline__ RawVec<BYTES> load_raw(const uint8_t *p)
+{
+    RawVec<BYTES> r;
+    if constexpr (BYTES == 32)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+                     : "l"(p));
+    else if constexpr (BYTES == 16)
+    {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    }
+    else if constexpr (BYTES == 8)
+    {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        r.w[0] = v.x, r.w[1] = v.y;
+    }
+    else if constexpr (BYTES == 4)
+        r.w[0] = *reinterpret_cast<const unsigned *>(p);
+    else if constexpr (BYTES == 2)
+        r.w[0] = *reinterpret_cast<const unsigned short *>(p);
+    else
+        r.w[0] = *p;
+    return r;
+}
+
+template<int BYTES>
+__device__ __forceinline__ void store_raw(uint8_t *p, const RawVec<BYTES> &r)
+{
+    if constexpr (BYTES == 32)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]),
+                     "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7])
+                     : "memory");
+    else if constexpr (BYTES == 16)
+        *reinterpret_cast<uint4 *>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    else if constexpr (BYTES == 8)
+        *reinterpret_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
+    else if constexpr (BYTES == 4)
+        *reinterpret_cast<unsigned *>(p) = r.w[0];
+    else if constexpr (BYTES == 2)
+        *reinterpret_cast<unsigned short *>(p) = r.w[0];
+    else
+        *p = r.w[0];
+}
+
+template<int BYTES>
+__device__ __forceinline__ RawVec<BYTES> zero_raw()
+{
+    RawVec<BYTES> r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(r.w) / sizeof(r.w[0])); ++i) r.w[i] = 0;
+    return r;
+}
+
+template<int DT, int W>
+__device__ __forceinline__ void unpack(const Vec<DT, W> &r, float *v)
+{
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+    {
+        if constexpr (DT == B200PP_F32)
+            v[i] = __uint_as_float(r.w[i]);
+        else if constexpr (DT == B200PP_U8)
+        {
+            if constexpr (W >= 4) // the byte becomes the low mantissa bits of 2^23, which is subtracted: exact
+                v[i] = __uint_as_float(__byte_perm(r.w[i / 4], 0x4B000000u, 0x7540u + i % 4)) - 8388608.0f;
+            else if constexpr (W == 2)
+                v[i] = static_cast<float>((r.w[0] >> (8 * i)) & 0xffu);
+            else
+                v[i] = static_cast<float>(r.w[0]);
+        }
+        else
+        {
+            const unsigned bits = W == 1 ? r.w[0] : (i & 1) ? r.w[i / 2] >> 16 : r.w[i / 2] & 0xffffu;
+            if constexpr (DT == B200PP_BF16)
+                v[i] = __uint_as_float(bits << 16);
+            else
+                v[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+        }
+    }
+}
+
+template<int DT, int W>
+__device__ __forceinline__ Vec<DT, W> pack(const float *v)
+{
+    Vec<DT, W> r;
+    if constexpr (DT == B200PP_F32)
+    {
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = __float_as_uint(v[i]);
+    }
+    else if constexpr (W == 1)
+        r.w[0] = DT == B200PP_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[0])) : __half_as_ushort(__float2half_rn(v[0]));
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < W; i += 2)
+        {
+            if constexpr (DT == B200PP_BF16)
+            {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+                r.w[i / 2]             = *reinterpret_cast<const unsigned *>(&h);
+            }
+            else
+            {
+                const __half2 h = __floats2half2_rn(v[i], v[i + 1]);
+                r.w[i / 2]      = *reinterpret_cast<const unsigned *>(&h);
+            }
+        }
+    }
+    return r;
+}
+
+template<int DT, int W>
+__device__ __forceinline__ void load_vec(const uint8_t *row, long long i, float *v)
+{
+    unpack<DT, W>(load_raw<kElemBytes<DT> * W>(row + i * kElemBytes<DT>), v);
+}
+
+template<int DT, int W>
+__device__ __forceinline__ void store_vec(uint8_t *row, long long i, const float *v)
+{
+    store_raw<kElemBytes<DT> * W>(row + i * kElemBytes<DT>, pack<DT, W>(v));
+}
+
+// float16, bfloat16 or float32, chosen at run time.
+template<int W>
+__device__ __forceinline__ void load_vec(const uint8_t *row, long long i, int dtype, float *v)
+{
+    if (dtype == B200PP_F32)
+        load_vec<B200PP_F32, W>(row, i, v);
+    else if (dtype == B200PP_BF16)
+        load_vec<B200PP_BF16, W>(row, i, v);
+    else
+        load_vec<B200PP_F16, W>(row, i, v);
+}
+
+template<int W>
+__device__ __forceinline__ void store_vec(uint8_t *row, long long i, int dtype, const float *v)
+{
+    if (dtype == B200PP_F32)
+        store_vec<B200PP_F32, W>(row, i, v);
+    else if (dtype == B200PP_BF16)
+        store_vec<B200PP_BF16, W>(row, i, v);
+    else
+        store_vec<B200PP_F16, W>(row, i, v);
+}
+
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll

@@ -15,6 +15,9 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import math
+import struct
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -44,6 +47,15 @@ class _EmbeddingGradOp(C.Structure):
 _TYPES = {torch.uint8: 0, torch.float32: 6, torch.float16: 7, torch.bfloat16: 8, torch.int32: 5, torch.int64: 9}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
+# the handle of torch's current stream without building a Stream object, where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+@lru_cache(maxsize=None)
+def _cuda(device: int) -> torch.device:
+    return torch.device("cuda", device)
+
+
 _bound: Optional[C.CDLL] = None
 
 
@@ -51,14 +63,14 @@ def _lib() -> C.CDLL:
     global _bound
     L = ops.lib()
     if _bound is not L:
-        R, S = C.POINTER(_Rows), C.POINTER(C.c_size_t)
+        R = S = O = C.c_void_p
         for name, args in (("LayerNormWorkspace", [R, S]),
-                           ("LayerNorm", [R, R, C.POINTER(_LayerNormOp), C.c_void_p, C.c_size_t, C.c_void_p]),
+                           ("LayerNorm", [R, R, O, C.c_void_p, C.c_size_t, C.c_void_p]),
                            ("LayerNormBackwardWorkspace", [R, S]),
-                           ("LayerNormBackward", [R, R, R, C.POINTER(_LayerNormGradOp), C.c_void_p, C.c_size_t, C.c_void_p]),
+                           ("LayerNormBackward", [R, R, R, O, C.c_void_p, C.c_size_t, C.c_void_p]),
                            ("Embedding", [R, R, R, C.c_float, C.c_void_p]),
                            ("EmbeddingBackwardWorkspace", [R, S]),
-                           ("EmbeddingBackward", [R, R, R, C.POINTER(_EmbeddingGradOp), C.c_void_p, C.c_size_t, C.c_void_p])):
+                           ("EmbeddingBackward", [R, R, R, O, C.c_void_p, C.c_size_t, C.c_void_p])):
             f = getattr(L, "b200pp" + name)
             f.restype, f.argtypes = C.c_int, args
         _bound = L
@@ -71,34 +83,41 @@ def _invalid(message: str) -> Error:
     return Error(Status.ERROR_INVALID_ARGUMENT, message)
 
 
-def _device_of(*tensors) -> torch.device:
-    """The device the call runs on: that of the CUDA tensors, which must agree (page-locked host tensors follow)."""
-    dev = None
+def _device_of(*tensors) -> int:
+    """Index of the device the call runs on: that of the CUDA tensors, which must agree (page-locked host tensors follow)."""
+    dev = -1
     for t in tensors:
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors")
         if t.is_cuda:
-            if dev is None:
-                dev = t.device
-            elif t.device != dev:
-                raise _invalid(f"Tensors are on different devices ({dev} and {t.device})")
+            d = t.get_device()
+            if dev < 0:
+                dev = d
+            elif d != dev:
+                raise _invalid(f"Tensors are on different devices (cuda:{dev} and cuda:{d})")
         elif not t.is_pinned():
             raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors")
-    return dev if dev is not None else torch.device("cuda", torch.cuda.current_device())
+    return dev if dev >= 0 else torch.cuda.current_device()
 
 
-def _rows(t: torch.Tensor, axes: int, what: str) -> _Rows:
-    """The rows that the last `axes` dimensions of `t` make, in the order of the others."""
-    shape, stride, lead = t.shape, t.stride(), t.dim() - axes
-    cols, es = 1, t.element_size()
-    for k in range(t.dim() - 1, lead - 1, -1):
-        if stride[k] != cols and shape[k] != 1 and t.numel():
-            raise _invalid(f"{what}: the last {axes} dimension(s) must be contiguous")
+def _view(t: torch.Tensor, axes: int, what: str):
+    """(columns, [(count, stride in elements)]): the rows the last `axes` dimensions of `t` make, in the order of the others,
+    dimensions that continue one another merged."""
+    shape, lead = t.shape, t.dim() - axes
+    cols = 1
+    for k in range(lead, lead + axes):
         cols *= shape[k]
-    r = _Rows(t.data_ptr(), _TYPES.get(t.dtype, -1), cols)
-    dims = []  # (count, stride in elements), dimensions that continue one another merged
+    if t.is_contiguous():
+        return cols, ((t.numel() // cols if cols else math.prod(shape[:lead]), cols),)
+    stride = t.stride()
+    step = 1
+    for k in range(t.dim() - 1, lead - 1, -1):
+        if stride[k] != step and shape[k] != 1:
+            raise _invalid(f"{what}: the last {axes} dimension(s) must be contiguous")
+        step *= shape[k]
+    dims = []
     for k in range(lead):
         n, s = shape[k], stride[k]
         if n == 1:
@@ -107,19 +126,29 @@ def _rows(t: torch.Tensor, axes: int, what: str) -> _Rows:
             dims[-1] = (dims[-1][0] * n, s)
         else:
             dims.append((n, s))
-    if not t.numel():
-        dims = [(shape[k], 0) for k in range(lead)]
-        n = 1
-        for d in dims:
-            n *= d[0]
-        dims = [(n, cols)]
     if len(dims) > 3:
         raise _invalid(f"{what} has more than three independently strided dimensions of rows")
+    return cols, dims
+
+
+# A B200ppRows as bytes, which ctypes passes by address: a third of the time a ctypes.Structure takes to fill in.
+_pack_rows = struct.Struct("=Qi4xq3q3q").pack
+assert struct.calcsize("=Qi4xq3q3q") == C.sizeof(_Rows)
+
+
+def _rows(t: torch.Tensor, axes: int, what: str):
+    """(B200ppRows as bytes, columns, rows)."""
+    cols, dims = _view(t, axes, what)
+    es = t.element_size()
+    code = _TYPES.get(t.dtype, -1)
+    if len(dims) == 1:
+        n, s = dims[0]
+        return _pack_rows(t.data_ptr(), code, cols, n, 1, 1, s * es, 0, 0), cols, n
+    c, d, rows = [1, 1, 1], [0, 0, 0], 1
     for k, (n, s) in enumerate(dims):
-        r.count[k], r.stride[k] = n, s * es
-    for k in range(len(dims), 3):
-        r.count[k] = 1
-    return r
+        c[k], d[k] = n, s * es
+        rows *= n
+    return _pack_rows(t.data_ptr(), code, cols, *c, *d), cols, rows
 
 
 def _axes_of(t: torch.Tensor, axes: int) -> int:
@@ -140,29 +169,28 @@ def _param(t: Optional[torch.Tensor], numel: int, what: str, kinds=_FLOATS) -> T
     return t.data_ptr(), _TYPES[t.dtype]
 
 
-class _Launch(contextlib.AbstractContextManager):
-    """Makes `device` and the launch stream torch's current ones, so that what the call allocates belongs to that stream;
+class _Launch:
+    """Makes the device and the launch stream torch's current ones, so that what the call allocates belongs to that stream;
     gives the stream's handle. Does nothing where they are current already."""
 
-    def __init__(self, device: torch.device, stream):
+    __slots__ = ("handle", "_stack")
+
+    def __init__(self, device: int, stream):
         self._stack = None
-        other = device.index is not None and device.index != torch.cuda.current_device()
-        if stream is None:
-            if other:
-                self._stack = contextlib.ExitStack()
-                self._stack.enter_context(torch.cuda.device(device))
-            self.handle = torch.cuda.current_stream(device).cuda_stream
+        other = device != torch.cuda.current_device()
+        current = _raw_stream(device)
+        self.handle = current if stream is None else ops._stream_handle(stream)
+        if not other and self.handle == current:
             return
-        self.handle = ops._stream_handle(stream)
-        if other or self.handle != torch.cuda.current_stream(device).cuda_stream:
-            self._stack = contextlib.ExitStack()
-            if other:
-                self._stack.enter_context(torch.cuda.device(device))
-            if isinstance(stream, torch.cuda.Stream):
-                if stream.device != device:
-                    raise _invalid(f"The stream belongs to {stream.device}, the tensors to {device}")
-            else:
+        self._stack = contextlib.ExitStack()
+        if other:
+            self._stack.enter_context(torch.cuda.device(device))
+        if self.handle != current:
+            if not isinstance(stream, torch.cuda.Stream):
                 stream = torch.cuda.ExternalStream(self.handle, device=device) if self.handle else torch.cuda.default_stream(device)
+            elif stream.device.index != device:
+                self._stack.close()
+                raise _invalid(f"The stream belongs to {stream.device}, the tensors to cuda:{device}")
             self._stack.enter_context(torch.cuda.stream(stream))
 
     def __enter__(self):
@@ -172,30 +200,34 @@ class _Launch(contextlib.AbstractContextManager):
         return self._stack.__exit__(*exc) if self._stack is not None else None
 
 
-def _workspace(query, rows: _Rows, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+def _workspace(query, rows: bytes, device: int):
+    """(tensor that keeps it alive, address, size) of the scratch memory `query` asks for."""
     n = C.c_size_t(0)
-    _check(query(C.byref(rows), C.byref(n)))
+    _check(query(rows, C.byref(n)))
     if n.value == 0:
         return None, None, 0
-    t = torch.empty(n.value, dtype=torch.uint8, device=device)
+    t = torch.empty(n.value, dtype=torch.uint8, device=_cuda(device))
     return t, t.data_ptr(), n.value
 
 
 # ------------------------------------------------------------------------------------------------ LayerNorm
 
+_WHOLE_ROWS = 8192  # rows up to this length need no workspace (row_ops.h)
+
+
 def _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle):
-    s = _rows(src, axes, "Input")
-    d = _rows(dst, axes, "Output")
-    count = src.numel() // s.cols if s.cols else 0
-    op = _LayerNormOp()
-    op.weight, op.weightType = _param(weight, s.cols, "weight")
-    op.bias, op.biasType = _param(bias, s.cols, "bias")
-    op.epsilon = epsilon
-    op.mean, _ = _param(mean, count, "mean", (torch.float32,))
-    op.rstd, _ = _param(rstd, count, "rstd", (torch.float32,))
+    s, cols, count = _rows(src, axes, "Input")
+    d = _rows(dst, axes, "Output")[0]
+    w, wt = _param(weight, cols, "weight")
+    b, bt = _param(bias, cols, "bias")
+    op = _LayerNormOp(w, b, wt, bt, epsilon, _param(mean, count, "mean", (torch.float32,))[0],
+                      _param(rstd, count, "rstd", (torch.float32,))[0])
     L = _lib()
-    keep, ws, size = _workspace(L.b200ppLayerNormWorkspace, s, device)
-    _check(L.b200ppLayerNorm(C.byref(s), C.byref(d), C.byref(op), ws, size, handle))
+    keep = ws = None
+    size = 0
+    if cols > _WHOLE_ROWS:
+        keep, ws, size = _workspace(L.b200ppLayerNormWorkspace, s, device)
+    _check(L.b200ppLayerNorm(s, d, C.byref(op), ws, size, handle))
 
 
 def layernorm_into(dst: torch.Tensor, src: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -224,30 +256,29 @@ def layernorm(src: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Op
     axes = _axes_of(src, axes)
     kind = data_type or (src.dtype if src.dtype != torch.uint8 else torch.float32)
     with _Launch(device, stream) as handle:
-        dst = torch.empty(src.shape, dtype=kind, device=device)
+        dst = torch.empty(src.shape, dtype=kind, device=_cuda(device))
         mean = rstd = None
         if stats:
-            mean = torch.empty(src.shape[:src.dim() - axes], dtype=torch.float32, device=device)
+            mean = torch.empty(src.shape[:src.dim() - axes], dtype=torch.float32, device=_cuda(device))
             rstd = torch.empty_like(mean)
         _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle)
     return (dst, mean, rstd) if stats else dst
 
 
 def _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle):
-    g, s = _rows(grad, axes, "Gradient"), _rows(src, axes, "Input")
-    d = _rows(dsrc, axes, "Input gradient") if dsrc is not None else None
-    count = src.numel() // s.cols if s.cols else 0
-    op = _LayerNormGradOp()
-    op.mean, _ = _param(mean, count, "mean", (torch.float32,))
-    op.rstd, _ = _param(rstd, count, "rstd", (torch.float32,))
-    op.weight, op.weightType = _param(weight, s.cols, "weight")
-    op.dweight, op.dweightType = _param(dweight, s.cols, "weight gradient")
-    op.dbias, op.dbiasType = _param(dbias, s.cols, "bias gradient")
+    s, cols, count = _rows(src, axes, "Input")
+    g = _rows(grad, axes, "Gradient")[0]
+    d = None if dsrc is None else _rows(dsrc, axes, "Input gradient")[0]
+    w, wt = _param(weight, cols, "weight")
+    dw, dwt = _param(dweight, cols, "weight gradient")
+    db, dbt = _param(dbias, cols, "bias gradient")
+    op = _LayerNormGradOp(_param(mean, count, "mean", (torch.float32,))[0], _param(rstd, count, "rstd", (torch.float32,))[0], w, wt,
+                          dw, db, dwt, dbt)
     L = _lib()
     keep, ws, size = (None, None, 0)
     if dweight is not None or dbias is not None:
         keep, ws, size = _workspace(L.b200ppLayerNormBackwardWorkspace, s, device)
-    _check(L.b200ppLayerNormBackward(C.byref(g), C.byref(s), C.byref(d) if d is not None else None, C.byref(op), ws, size, handle))
+    _check(L.b200ppLayerNormBackward(g, s, d, C.byref(op), ws, size, handle))
 
 
 def layernorm_backward_into(dsrc: Optional[torch.Tensor], dweight: Optional[torch.Tensor], dbias: Optional[torch.Tensor],
@@ -278,31 +309,24 @@ def layernorm_backward(grad: torch.Tensor, src: torch.Tensor, mean: torch.Tensor
         dsrc = dweight = dbias = None
         row = src.shape[src.dim() - axes:]
         if src_grad:
-            dsrc = torch.empty(src.shape, dtype=data_type or (src.dtype if src.dtype != torch.uint8 else grad.dtype), device=device)
+            dsrc = torch.empty(src.shape, dtype=data_type or (src.dtype if src.dtype != torch.uint8 else grad.dtype), device=_cuda(device))
         kind = weight.dtype if weight is not None else torch.float32
         if weight_grad:
-            dweight = torch.empty(row, dtype=kind, device=device)
+            dweight = torch.empty(row, dtype=kind, device=_cuda(device))
         if bias_grad:
-            dbias = torch.empty(row, dtype=kind, device=device)
+            dbias = torch.empty(row, dtype=kind, device=_cuda(device))
         _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle)
     return dsrc, dweight, dbias
 
 
 # ------------------------------------------------------------------------------------------------ embedding lookup
 
-def _indices(indices: torch.Tensor) -> _Rows:
-    return _rows(indices.unsqueeze(-1), 1, "Indices")
-
-
-def _matrix(t: torch.Tensor, what: str) -> _Rows:
-    if t.dim() != 2:
-        raise _invalid(f"{what} must have two dimensions")
-    return _rows(t, 1, what)
+def _indices(indices: torch.Tensor) -> bytes:
+    return _rows(indices, 0, "Indices")[0]
 
 
 def _embedding(dst, indices, table, scale, handle):
-    i, t, d = _indices(indices), _matrix(table, "Table"), _rows(dst, 1, "Output")
-    _check(_lib().b200ppEmbedding(C.byref(i), C.byref(t), C.byref(d), scale, handle))
+    _check(_lib().b200ppEmbedding(_indices(indices), _rows(table, 1, "Table")[0], _rows(dst, 1, "Output")[0], scale, handle))
 
 
 def embedding_into(dst: torch.Tensor, indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *, stream=None) -> torch.Tensor:
@@ -324,17 +348,17 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *,
     if table.dim() != 2:
         raise _invalid("Table must have two dimensions")
     with _Launch(device, stream) as handle:
-        dst = torch.empty((*indices.shape, table.shape[1]), dtype=data_type or table.dtype, device=device)
+        dst = torch.empty((*indices.shape, table.shape[1]), dtype=data_type or table.dtype, device=_cuda(device))
         _embedding(dst, indices, table, scale, handle)
     return dst
 
 
 def _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate, device, handle):
-    g, i, d = _rows(grad, 1, "Gradient"), _indices(indices), _matrix(dtable, "Table gradient")
+    g = _rows(grad, 1, "Gradient")[0]
     op = _EmbeddingGradOp(scale, int(accumulate), -1 if padding_index is None else int(padding_index))
     L = _lib()
     keep, ws, size = _workspace(L.b200ppEmbeddingBackwardWorkspace, g, device)
-    _check(L.b200ppEmbeddingBackward(C.byref(g), C.byref(i), C.byref(d), C.byref(op), ws, size, handle))
+    _check(L.b200ppEmbeddingBackward(g, _indices(indices), _rows(dtable, 1, "Table gradient")[0], C.byref(op), ws, size, handle))
 
 
 def embedding_backward_into(dtable: torch.Tensor, grad: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, *,
@@ -358,7 +382,7 @@ def embedding_backward(grad: torch.Tensor, indices: torch.Tensor, rows: int, sca
     if grad.dim() < 1 or grad.shape[:-1] != indices.shape:
         raise _invalid("The gradient must have the indices' shape followed by the table's number of columns")
     with _Launch(device, stream) as handle:
-        dtable = torch.empty((int(rows), grad.shape[-1]), dtype=data_type, device=device)
+        dtable = torch.empty((int(rows), grad.shape[-1]), dtype=data_type, device=_cuda(device))
         _embedding_backward(dtable, grad, indices, scale, padding_index, False, device, handle)
     return dtable
 
