@@ -1,4 +1,4 @@
-// Host side of LayerNorm and its gradient: argument validation, kernel selection and launch.
+// Host side of LayerNorm: argument validation, kernel selection and launch.
 #include "layernorm_kernels.cuh"
 #include "row_host.h"
 
@@ -144,115 +144,3 @@ extern "C" int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, con
     }
     return check_launch("LayerNorm");
 }
-
-// Parts the rows are divided into for the sums over the rows.
-static int layernorm_grad_parts(long long rows, long long cols)
-{
-    const long long blocks = (cols + 31) / 32;
-    return static_cast<int>(std::max(1LL, std::min({(rows + 31) / 32, (kSms * 8 + blocks - 1) / blocks, 65535LL})));
-}
-
-extern "C" int b200ppLayerNormBackwardWorkspace(const B200ppRows *src, size_t *bytes)
-{
-    if (!src || !bytes)
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
-    RowMap    m;
-    long long rows = 0;
-    B200ppRows t   = *src;
-    t.base         = reinterpret_cast<void *>(uintptr_t(256));
-    if (int st = take_rows(&t, "Input", false, m, rows))
-        return st;
-    *bytes = static_cast<size_t>(layernorm_grad_parts(rows, t.cols)) * 2 * t.cols * sizeof(float);
-    return B200PP_SUCCESS;
-}
-
-namespace {
-
-template<int SRC>
-void launch_layernorm_grad(const LayerNormGradKParams &p, cudaStream_t stream, int &status)
-{
-    // the sums over the rows first: dsrc may be written over grad or src
-    if (p.dweight || p.dbias)
-    {
-        const dim3 grid((p.cols + 31u) / 32u, p.parts);
-        layernorm_grad_columns_kernel<SRC><<<grid, 256, 0, stream>>>(p);
-        if ((status = check_launch("LayerNormBackward")))
-            return;
-        layernorm_grad_join_kernel<<<(p.cols + 255u) / 256u, 256, 0, stream>>>(p);
-        if ((status = check_launch("LayerNormBackward")))
-            return;
-    }
-    if (p.dsrc.base)
-    {
-        layernorm_grad_row_kernel<SRC><<<std::min(p.rows, 65535u), 256, 0, stream>>>(p);
-        status = check_launch("LayerNormBackward");
-    }
-}
-
-} // namespace
-
-extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows *src, const B200ppRows *dsrc,
-                                       const B200ppLayerNormGradOp *op, void *workspace, size_t workspaceBytes,
-                                       cudaStream_t stream)
-{
-    if (!grad || !src || !op)
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
-    if (!dsrc && !op->dweight && !op->dbias)
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "No gradient is asked for");
-    if ((!is_float(src->dtype) && src->dtype != B200PP_U8) || !is_float(grad->dtype) || (dsrc && !is_float(dsrc->dtype)))
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Invalid DataType");
-    if (src->cols != grad->cols || (dsrc && src->cols != dsrc->cols))
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Input and gradient shapes are different");
-    LayerNormGradKParams p{};
-    long long            rows = 0, gradRows = 0, dsrcRows = 0;
-    int                  st;
-    if ((st = take_rows(src, "Input", false, p.src, rows)) || (st = take_rows(grad, "Gradient", false, p.grad, gradRows))
-        || (dsrc && (st = take_rows(dsrc, "Input gradient", true, p.dsrc, dsrcRows)))
-        || (st = check_param(op->weight, op->weightType, "weight"))
-        || (st = check_param(op->dweight, op->dweightType, "weight gradient"))
-        || (st = check_param(op->dbias, op->dbiasType, "bias gradient")) || (st = check_param(op->mean, B200PP_F32, "mean"))
-        || (st = check_param(op->rstd, B200PP_F32, "rstd")))
-        return st;
-    if (rows != gradRows || (dsrc && rows != dsrcRows))
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Input and gradient shapes are different");
-    if (rows > 0 && (!op->mean || !op->rstd))
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "The backward pass needs the forward pass's mean and rstd");
-    p.cols  = static_cast<int>(src->cols);
-    p.parts = layernorm_grad_parts(rows, p.cols);
-    if (op->dweight || op->dbias)
-        if ((st = check_workspace(workspace, workspaceBytes, static_cast<size_t>(p.parts) * 2 * p.cols * sizeof(float))))
-            return st;
-    p.rows        = static_cast<unsigned>(rows);
-    p.gradType    = grad->dtype;
-    p.dsrcType    = dsrc ? dsrc->dtype : 0;
-    p.weightType  = op->weightType;
-    p.dweightType = op->dweightType;
-    p.dbiasType   = op->dbiasType;
-    p.weight      = static_cast<const uint8_t *>(op->weight);
-    p.mean        = op->mean;
-    p.rstd        = op->rstd;
-    p.fcols       = static_cast<float>(p.cols);
-    p.dweight     = static_cast<uint8_t *>(op->dweight);
-    p.dbias       = static_cast<uint8_t *>(op->dbias);
-    p.partials    = static_cast<float *>(workspace);
-    if (rows == 0)
-        p.dsrc.base = nullptr;
-    int status = B200PP_SUCCESS;
-    switch (src->dtype)
-    {
-    case B200PP_U8:
-        launch_layernorm_grad<B200PP_U8>(p, stream, status);
-        break;
-    case B200PP_F16:
-        launch_layernorm_grad<B200PP_F16>(p, stream, status);
-        break;
-    case B200PP_BF16:
-        launch_layernorm_grad<B200PP_BF16>(p, stream, status);
-        break;
-    default:
-        launch_layernorm_grad<B200PP_F32>(p, stream, status);
-        break;
-    }
-    return status;
-}
-

@@ -1,0 +1,281 @@
+// Gradient of LayerNorm: h = (x - m) r, g = dy w, dx = r (g - mean(g) - h mean(g h)); dw = sum over the rows of dy h, db = sum over
+// the rows of dy. Bound: HBM (two tensors read, one written, about one operation per byte).
+//
+// The sums over the rows are split over a fixed number of parts, added up by a second kernel in a fixed order: no atomics, equal
+// inputs give equal bits.
+#ifndef CVCUDA_B200_LAYERNORM_GRAD_KERNELS_CUH
+#define CVCUDA_B200_LAYERNORM_GRAD_KERNELS_CUH
+
+#include "layernorm_kernels.cuh"
+
+namespace b200pp {
+
+struct LayerNormGradKParams
+{
+    RowMap         grad, src, dsrc;
+    unsigned       rows;
+    int            cols;
+    int            gradType, dsrcType, weightType, dweightType, dbiasType;
+    const uint8_t *weight;
+    const float   *mean, *rstd;
+    float          fcols;
+    uint8_t       *dweight, *dbias;
+    float         *partials; // [parts][2][cols]
+    int            parts;
+};
+
+// Rows that fit into registers, all gradients in one pass over the data. blockDim.x threads per row (BLOCK: whole warps, otherwise
+// part of one), blockDim.y rows per CTA at a time. A CTA walks down its share of the rows; each thread keeps its columns of the
+// weight and of the sums over the rows in registers, and loads its part of the next row before it works on the present one.
+constexpr int kGradResident8  = 768; // threads that fit on an SM, by the registers per thread the launch bound leaves (80)
+constexpr int kGradResident16 = 512; // (128)
+
+template<int SRC, int GRAD, int E, int W, bool BLOCK>
+__global__ void __launch_bounds__(E == 8 ? kGradResident8 : kGradResident16) layernorm_grad_kernel(const LayerNormGradKParams p)
+{
+    constexpr int           V     = E / W;
+    constexpr bool          AHEAD = E == 8; // with sixteen values there are no registers left for the next row
+    __shared__ float2       scratch[2][16]; // two halves, used in turn: one barrier per row
+    extern __shared__ float sums[];         // [2][cols]
+    const int               t = threadIdx.x, threads = blockDim.x, g = threadIdx.y, groups = blockDim.y;
+    const int               tid = g * threads + t, warp = tid >> 5;
+    float                   w[E], dw[E], db[E];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+    {
+        const int c = vec_at<W>(v, t, threads);
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[v * W + i] = 1.0f, dw[v * W + i] = 0.0f, db[v * W + i] = 0.0f;
+        if (p.weight && c < p.cols)
+            load_vec<W>(p.weight, c, p.weightType, w + v * W);
+    }
+    Vec<SRC, W>  xr[V];
+    Vec<GRAD, W> gr[V];
+    float        mean = 0.0f, rstd = 0.0f;
+    auto         fetch = [&](unsigned long long r) {
+        const bool     live = r < p.rows;
+        const uint8_t *x = nullptr, *dy = nullptr;
+        mean = rstd = 0.0f; // a row that is not there: h = 0 and dy = 0
+        if (live)
+        {
+            x    = p.src.at(static_cast<unsigned>(r));
+            dy   = p.grad.at(static_cast<unsigned>(r));
+            mean = p.mean[r];
+            rstd = p.rstd[r];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+        {
+            const int c = vec_at<W>(v, t, threads);
+            xr[v]       = zero_raw<kElemBytes<SRC> * W>();
+            gr[v]       = zero_raw<kElemBytes<GRAD> * W>();
+            if (live && c < p.cols)
+            {
+                xr[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
+                gr[v] = load_raw<kElemBytes<GRAD> * W>(dy + static_cast<long long>(c) * kElemBytes<GRAD>);
+            }
+        }
+    };
+    const unsigned long long step = static_cast<unsigned long long>(gridDim.x) * groups;
+    unsigned long long       r    = static_cast<unsigned long long>(blockIdx.x) * groups + g;
+    int                      half = 0;
+    if (AHEAD)
+        fetch(r);
+    // every thread of the CTA takes the same number of turns
+    for (unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * groups; first < p.rows; first += step)
+    {
+        if (!AHEAD)
+            fetch(r);
+        float       h[E], gv[E], s1 = 0.0f, s2 = 0.0f;
+        const float rs = rstd;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+        {
+            unpack<SRC, W>(xr[v], h + v * W);
+            unpack<GRAD, W>(gr[v], gv + v * W);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+        {
+            h[e]  = (h[e] - mean) * rs;
+            db[e] += gv[e];
+            dw[e] = fmaf(gv[e], h[e], dw[e]);
+            gv[e] *= w[e];
+            s1 += gv[e];
+            s2 = fmaf(gv[e], h[e], s2);
+        }
+        const unsigned long long now = r;
+        r += step;
+        if (AHEAD)
+            fetch(r);
+        if (!p.dsrc.base)
+            continue;
+        if constexpr (BLOCK)
+        {
+            s1 = warp_sum(s1);
+            s2 = warp_sum(s2);
+            if ((t & 31) == 0)
+                scratch[half][warp] = make_float2(s1, s2);
+            __syncthreads();
+            s1 = s2 = 0.0f;
+            for (int k = 0; k < threads >> 5; ++k)
+            {
+                const float2 o = scratch[half][g * (threads >> 5) + k];
+                s1 += o.x;
+                s2 += o.y;
+            }
+            half ^= 1;
+        }
+        else
+            for (int o = threads >> 1; o > 0; o >>= 1)
+            {
+                s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+                s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+            }
+        if (now >= p.rows)
+            continue;
+        const float c1 = s1 / p.fcols, c2 = s2 / p.fcols;
+        uint8_t    *dx = p.dsrc.at(static_cast<unsigned>(now));
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+        {
+            const int c = vec_at<W>(v, t, threads);
+            if (c >= p.cols)
+                break;
+            float o[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] = rs * (gv[v * W + i] - c1 - h[v * W + i] * c2);
+            store_vec<W>(dx, c, p.dsrcType, o);
+        }
+    }
+    if (!p.partials)
+        return;
+    // the CTA's sums: over the rows of a warp by shuffles, over the warps (BLOCK: over the rows) one after another
+    float    *part  = p.partials + static_cast<long long>(blockIdx.x) * 2 * p.cols;
+    int       slot  = g, slots = groups;
+    bool      holds = true;
+    if constexpr (!BLOCK)
+    {
+        for (int o = threads; o < 32; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+            {
+                dw[e] += __shfl_xor_sync(0xffffffffu, dw[e], o);
+                db[e] += __shfl_xor_sync(0xffffffffu, db[e], o);
+            }
+        slot  = warp;
+        slots = (threads * groups) >> 5;
+        holds = (tid & 31) < threads;
+    }
+    for (int s = 0; s < slots; ++s)
+    {
+        if (slot == s && holds)
+        {
+            float *to = s + 1 < slots ? sums : part;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+            {
+                const int c = vec_at<W>(e / W, t, threads) + e % W;
+                if (c < p.cols)
+                {
+                    to[c]          = s > 0 ? sums[c] + dw[e] : dw[e];
+                    to[p.cols + c] = s > 0 ? sums[p.cols + c] + db[e] : db[e];
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// dx, one CTA per row, any row length.
+template<int SRC>
+__global__ void __launch_bounds__(256) layernorm_grad_row_kernel(const LayerNormGradKParams p)
+{
+    __shared__ float scratch[32];
+    for (unsigned r = blockIdx.x; r < p.rows; r += gridDim.x)
+    {
+        const uint8_t *x = p.src.at(r), *dy = p.grad.at(r);
+        uint8_t       *dx   = p.dsrc.at(r);
+        const float    mean = p.mean[r], rstd = p.rstd[r];
+        float          s1 = 0.0f, s2 = 0.0f;
+        for (int c = threadIdx.x; c < p.cols; c += blockDim.x)
+        {
+            const float w = p.weight ? load_elem(p.weight, c, p.weightType) : 1.0f;
+            const float g = load_elem(dy, c, p.gradType) * w;
+            s1 += g;
+            s2 = fmaf(g, (load_elem<SRC>(x, c) - mean) * rstd, s2);
+        }
+        const float c1 = block_sum(s1, scratch) / p.fcols;
+        const float c2 = block_sum(s2, scratch) / p.fcols;
+        for (int c = threadIdx.x; c < p.cols; c += blockDim.x)
+        {
+            const float w = p.weight ? load_elem(p.weight, c, p.weightType) : 1.0f;
+            const float g = load_elem(dy, c, p.gradType) * w;
+            const float h = (load_elem<SRC>(x, c) - mean) * rstd;
+            store_elem_as(dx, c, p.dsrcType, rstd * (g - c1 - h * c2));
+        }
+    }
+}
+
+// dw and db: a CTA sums one part of the rows for 32 columns; layernorm_grad_join_kernel adds the parts up.
+template<int SRC>
+__global__ void __launch_bounds__(256) layernorm_grad_columns_kernel(const LayerNormGradKParams p)
+{
+    __shared__ float sw[8][32], sb[8][32];
+    const int        lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long  c    = static_cast<long long>(blockIdx.x) * 32 + lane;
+    const unsigned   per  = (p.rows + p.parts - 1) / p.parts;
+    const unsigned   r0   = min(p.rows, static_cast<unsigned>(blockIdx.y) * per), r1 = min(p.rows, r0 + per);
+    float            dw = 0.0f, db = 0.0f;
+    if (c < p.cols)
+        for (unsigned r = r0 + warp; r < r1; r += 8)
+        {
+            const float g = load_elem(p.grad.at(r), c, p.gradType);
+            db += g;
+            dw = fmaf(g, (load_elem<SRC>(p.src.at(r), c) - p.mean[r]) * p.rstd[r], dw);
+        }
+    sw[warp][lane] = dw;
+    sb[warp][lane] = db;
+    __syncthreads();
+    if (warp == 0 && c < p.cols)
+    {
+        for (int k = 1; k < 8; ++k)
+        {
+            dw += sw[k][lane];
+            db += sb[k][lane];
+        }
+        float *part       = p.partials + static_cast<long long>(blockIdx.y) * 2 * p.cols;
+        part[c]           = dw;
+        part[p.cols + c]  = db;
+    }
+}
+
+// Adds up the parts: a thread takes every 32nd part of a column, the 32 threads of the column are joined in order.
+__global__ void __launch_bounds__(1024) layernorm_grad_join_kernel(const LayerNormGradKParams p)
+{
+    __shared__ float   sum[32][33];
+    const long long    c = static_cast<long long>(blockIdx.x) * 32 + threadIdx.x; // of 2 * cols
+    const long long    n = 2LL * p.cols;
+    float              s = 0.0f;
+    if (c < n)
+        for (int k = threadIdx.y; k < p.parts; k += 32) s += p.partials[k * n + c];
+    sum[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    // one warp per column now
+    s                 = warp_sum(sum[threadIdx.x][threadIdx.y]);
+    const long long o = static_cast<long long>(blockIdx.x) * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && o < n)
+    {
+        if (o < p.cols)
+        {
+            if (p.dweight)
+                store_elem_as(p.dweight, o, p.dweightType, s);
+        }
+        else if (p.dbias)
+            store_elem_as(p.dbias, o - p.cols, p.dbiasType, s);
+    }
+}
+
+} // namespace b200pp
+
+#endif

@@ -1,5 +1,5 @@
 // Host side of the plain-C launch layer: argument validation, kernel selection and launch.
-// The translation unit that contains the device code of the image operators (layernorm.cu and embedding.cu: that of the row operators).
+// The translation unit that contains the device code of the image operators (layernorm*.cu and embedding.cu: that of the row operators).
 #include "border_kernels.cuh"
 #include "convert_kernels.cuh"
 #include "host_common.h"
