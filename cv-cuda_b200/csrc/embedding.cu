@@ -22,6 +22,18 @@ int check_indices(const B200ppRows *indices)
 
 namespace {
 
+template<int C>
+void launch_short_rows(const EmbeddingKParams &p, cudaStream_t stream)
+{
+    const unsigned long long tiles = (static_cast<unsigned long long>(p.count) * C + 2047) / 2048; // at most 2^31 * 7 / 2^11
+    // the copy to shared memory pays from the second index per table row on
+    if (static_cast<long long>(p.rows) * C <= kShortTable && p.count >= 2u * p.rows)
+        embedding_short_rows_kernel<C, true><<<static_cast<unsigned>(std::min<unsigned long long>(tiles, kSms * 8)), 256,
+                                               p.rows * C * static_cast<int>(sizeof(float)), stream>>>(p);
+    else
+        embedding_short_rows_kernel<C, false><<<static_cast<unsigned>(tiles), 256, 0, stream>>>(p);
+}
+
 template<int TABLE, int W>
 int launch_embedding(EmbeddingKParams &p, cudaStream_t stream)
 {
@@ -88,8 +100,30 @@ extern "C" int b200ppEmbedding(const B200ppRows *indices, const B200ppRows *tabl
     if (p.cols < 8 && p.dst.n2 == 0 && (count == 1 || p.dst.s2 == static_cast<long long>(p.cols) * elem)
         && (reinterpret_cast<uintptr_t>(p.dst.base) & (8 * elem - 1)) == 0)
     {
-        const unsigned long long ctas = (static_cast<unsigned long long>(count) * p.cols + 2047) / 2048; // at most 2^31 * 7 / 2^11
-        embedding_short_rows_kernel<<<static_cast<unsigned>(ctas), 256, 0, stream>>>(p);
+        switch (p.cols)
+        {
+        case 1:
+            launch_short_rows<1>(p, stream);
+            break;
+        case 2:
+            launch_short_rows<2>(p, stream);
+            break;
+        case 3:
+            launch_short_rows<3>(p, stream);
+            break;
+        case 4:
+            launch_short_rows<4>(p, stream);
+            break;
+        case 5:
+            launch_short_rows<5>(p, stream);
+            break;
+        case 6:
+            launch_short_rows<6>(p, stream);
+            break;
+        default:
+            launch_short_rows<7>(p, stream);
+            break;
+        }
         return check_launch("Embedding");
     }
     VecWidth width(p.cols);
@@ -107,14 +141,17 @@ namespace {
 // Layout of the gradient's workspace.
 struct EmbeddingGradPlan
 {
-    unsigned unit, units;
+    unsigned unit, units, blocks;
     size_t   keys[2], order[2], partials, bytes;
 };
 
 EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
 {
     EmbeddingGradPlan w{};
+    // 32 positions per warp; fewer where that would leave the GPU short of warps
+    w.blocks     = static_cast<unsigned>((cols + kGradCols - 1) / kGradCols);
     w.unit       = 32;
+    while (w.unit > 8 && count * w.blocks < static_cast<long long>(w.unit) * kSms * 16) w.unit /= 2;
     w.units      = static_cast<unsigned>((count + w.unit - 1) / w.unit);
     size_t at    = 0;
     const size_t list = align_up(static_cast<size_t>(count) * sizeof(unsigned));
@@ -128,6 +165,20 @@ EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
     w.partials = at;
     w.bytes    = at + static_cast<size_t>(w.units) * 2 * cols * sizeof(float);
     return w;
+}
+
+template<int GRAD>
+void launch_runs(const EmbeddingGradKParams &p, int width, cudaStream_t stream)
+{
+    const unsigned grid = static_cast<unsigned>((static_cast<unsigned long long>(p.units) * p.blocks + 7) / 8);
+    if (width == 8)
+        embedding_grad_runs_kernel<GRAD, 8><<<grid, 256, 0, stream>>>(p);
+    else if (width == 4)
+        embedding_grad_runs_kernel<GRAD, 4><<<grid, 256, 0, stream>>>(p);
+    else if (width == 2)
+        embedding_grad_runs_kernel<GRAD, 2><<<grid, 256, 0, stream>>>(p);
+    else
+        embedding_grad_runs_kernel<GRAD, 1><<<grid, 256, 0, stream>>>(p);
 }
 
 // Raises a kernel's dynamic shared-memory limit, once per device.
@@ -185,6 +236,8 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "Indices and gradient have different numbers of rows");
     if (rows == 0)
         return B200PP_SUCCESS;
+    if (count == 0 && op->accumulate)
+        return B200PP_SUCCESS;
     const EmbeddingGradPlan w = plan_embedding_grad(count, grad->cols);
     if (count > 0 && (st = check_workspace(workspace, workspaceBytes, w.bytes)))
         return st;
@@ -199,14 +252,8 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     p.accumulate = op->accumulate != 0;
     p.padding    = op->paddingIndex >= 0 && op->paddingIndex < rows ? static_cast<int>(op->paddingIndex) : -1;
     p.unit       = w.unit;
-    if (!p.accumulate)
-    {
-        embedding_zero_kernel<<<std::min(static_cast<unsigned>(rows), 65535u), 256, 0, stream>>>(p);
-        if ((st = check_launch("EmbeddingBackward")))
-            return st;
-    }
-    if (count == 0)
-        return B200PP_SUCCESS;
+    p.units      = w.units;
+    p.blocks     = w.blocks;
     for (int k = 0; k < 2; ++k)
     {
         p.keys[k]  = reinterpret_cast<unsigned *>(ws + w.keys[k]);
@@ -217,24 +264,46 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     while (bits < 31 && (rows >> bits) != 0) ++bits;
     p.passes    = (bits + kSortMaxBits - 1) / kSortMaxBits;
     p.digitBits = (bits + p.passes - 1) / p.passes;
-    const int bins = 1 << p.digitBits;
-    static std::atomic<unsigned long long> raised{0};
-    if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(sort_smem_words(1 << kSortMaxBits) * sizeof(unsigned)), raised)))
-        return st;
-    embedding_sort_kernel<<<kSortCtas, kSortThreads, sort_smem_words(bins) * sizeof(unsigned), stream>>>(p);
-    if ((st = check_launch("EmbeddingBackward")))
-        return st;
-    const unsigned           blocks = (p.cols + 255u) / 256u;
-    const unsigned long long jobs   = static_cast<unsigned long long>(w.units) * blocks;
-    if ((jobs + 7) / 8 > 0x7fffffffull || blocks > 65535u)
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Gradient is too large");
-    embedding_grad_runs_kernel<<<static_cast<unsigned>((jobs + 7) / 8), 256, 0, stream>>>(p);
-    if ((st = check_launch("EmbeddingBackward")))
-        return st;
-    if (w.units > 1)
+    // as few threads as hold the indices kSortKeys at a time: the tables of counts are per warp
+    int threads = 256;
+    while (threads < kSortMaxThreads && static_cast<long long>(threads) * kSortKeys * kSortCtas < count) threads *= 2;
+    p.sortWarps  = threads / 32;
+    int clusters = 1;
+    if (!p.accumulate)
     {
-        embedding_grad_join_kernel<<<dim3(w.units - 1, blocks), 256, 0, stream>>>(p);
-        st = check_launch("EmbeddingBackward");
+        VecWidth width(p.cols);
+        width.take(p.dtable, row_elem_size(p.dtableType));
+        p.zeroWidth             = width.width;
+        const long long rowSize = static_cast<long long>(p.cols) * row_elem_size(p.dtableType);
+        // a cluster per 256 KB to clear, at most as many as fit on the GPU beside the one that sorts
+        clusters += static_cast<int>(std::max(1LL, std::min(16LL, rows * rowSize / (256 << 10))));
+        p.zeroCtas  = (clusters - 1) * kSortCtas;
+        p.skipNamed = std::min(count, rows) * rowSize / p.zeroCtas > 2 * count * row_elem_size(p.indexType);
+        threads = kSortMaxThreads; // for those that clear
     }
-    return st;
+    const size_t smem = std::max(sort_smem_words(p.sortWarps * 32, 1 << p.digitBits), static_cast<size_t>(kZeroRows / 32)) * sizeof(unsigned);
+    static std::atomic<unsigned long long> raised{0};
+    if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(sort_smem_words(kSortMaxThreads, 1 << kSortMaxBits) * sizeof(unsigned)),
+                         raised)))
+        return st;
+    const unsigned long long jobs = static_cast<unsigned long long>(w.units) * w.blocks;
+    if (jobs > 0x7fffffffull || w.blocks > 65535u)
+        return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
+    embedding_sort_kernel<<<clusters * kSortCtas, threads, smem, stream>>>(p);
+    if ((st = check_launch("EmbeddingBackward")) || count == 0)
+        return st;
+    VecWidth width(p.cols);
+    width.take(p.grad, row_elem_size(p.gradType));
+    width.take(p.dtable, row_elem_size(p.dtableType));
+    width.take(p.partials, p.cols * static_cast<long long>(sizeof(float)), sizeof(float));
+    if (p.gradType == B200PP_F16)
+        launch_runs<B200PP_F16>(p, width.width, stream);
+    else if (p.gradType == B200PP_BF16)
+        launch_runs<B200PP_BF16>(p, width.width, stream);
+    else
+        launch_runs<B200PP_F32>(p, width.width, stream);
+    if ((st = check_launch("EmbeddingBackward")) || w.units == 1)
+        return st;
+    embedding_grad_join_kernel<<<dim3((w.units - 1 + 7) / 8, w.blocks), 256, 0, stream>>>(p);
+    return check_launch("EmbeddingBackward");
 }

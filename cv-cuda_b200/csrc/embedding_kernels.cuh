@@ -47,52 +47,64 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingKParams p
         if (id >= 0 && c < p.cols)
             raw[u] = load_raw<kElemBytes<TABLE> * W>(t + static_cast<long long>(c) * kElemBytes<TABLE>);
     }
+    float v[U * W];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-    {
-        const int c = c0 + u * span;
-        float     v[W];
-        unpack<TABLE, W>(raw[u], v);
+    for (int u = 0; u < U; ++u) unpack<TABLE, W>(raw[u], v + u * W);
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = id < 0 ? 0.0f : v[i] * p.scale;
-        if (c < p.cols)
-            store_vec<W>(y, c, p.dstType, v);
-    }
+    for (int i = 0; i < U * W; ++i) v[i] = id < 0 ? 0.0f : v[i] * p.scale;
+    store_vecs<W, U>(y, p.dstType, c0, span, p.cols, v);
 }
 
-// Rows of a few elements that follow one another without gaps (a palette's colours): a thread makes eight neighbouring elements of
-// the output, whichever rows they belong to, and stores them as one vector.
+// Rows of C elements (a palette's colours) that follow one another without gaps: a thread makes eight neighbouring elements of the
+// output, whichever rows they belong to, and stores them as one vector. SHARED: the table, times the scale, is copied to shared
+// memory first. Gathers bound this kernel: from L1 a warp's 32 addresses take a cycle per 128-byte line they touch (114 us for 16.6
+// million indices and a palette of 256 x 3 floats), from shared memory a cycle per clash of banks.
+constexpr int kShortTable = 8192; // floats of a table that is copied to shared memory
+
+template<int C, bool SHARED>
 __global__ void __launch_bounds__(256) embedding_short_rows_kernel(const EmbeddingKParams p)
 {
-    const unsigned long long total = static_cast<unsigned long long>(p.count) * p.cols;
-    const unsigned long long e0    = (static_cast<unsigned long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
-    if (e0 >= total)
-        return;
-    unsigned       r  = static_cast<unsigned>(e0 / p.cols);
-    int            c  = static_cast<int>(e0 - static_cast<unsigned long long>(r) * p.cols);
-    int            id = load_index(p.indices, p.indexType, r, p.rows);
-    const uint8_t *t  = p.table.at(max(id, 0));
-    float          v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
+    constexpr int                N = (C + 6) / C + 1; // rows that eight elements can lie in
+    extern __shared__ float      table[];
+    const unsigned long long     total = static_cast<unsigned long long>(p.count) * C;
+    if constexpr (SHARED)
     {
-        v[i] = 0.0f;
-        if (e0 + i < total)
-        {
-            if (id >= 0)
-                v[i] = load_elem(t, c, p.tableType) * p.scale;
-            if (++c == p.cols && e0 + i + 1 < total)
-            {
-                c  = 0;
-                id = load_index(p.indices, p.indexType, ++r, p.rows);
-                t  = p.table.at(max(id, 0));
-            }
-        }
+        for (int i = threadIdx.x; i < p.rows * C; i += 256)
+            table[i] = load_elem(p.table.at(i / C), i % C, p.tableType) * p.scale;
+        __syncthreads();
     }
-    if (e0 + 8 <= total)
-        store_vec<8>(p.dst.base, e0, p.dstType, v);
-    else
-        for (int i = 0; i < 8 && e0 + i < total; ++i) store_elem_as(p.dst.base, e0 + i, p.dstType, v[i]);
+    for (unsigned long long tile = blockIdx.x * 2048ull; tile < total; tile += gridDim.x * 2048ull)
+    {
+        const unsigned long long e0 = tile + threadIdx.x * 8;
+        if (e0 >= total)
+            break;
+        const unsigned r0 = static_cast<unsigned>(e0 / C);
+        const int      c0 = static_cast<int>(e0 - static_cast<unsigned long long>(r0) * C);
+        int            id[N];
+        const uint8_t *row[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) id[k] = r0 + k < p.count ? load_index(p.indices, p.indexType, r0 + k, p.rows) : -1;
+#pragma unroll
+        for (int k = 0; k < N; ++k) row[k] = SHARED ? nullptr : p.table.at(max(id[k], 0));
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            // element c0 + i of the rows from r0 on
+            const bool over = c0 + i % C >= C;
+            const int  lo = i / C, hi = lo < N - 1 ? lo + 1 : N - 1;
+            const int  c = over ? c0 + i % C - C : c0 + i % C;
+            const int  n = over ? id[hi] : id[lo];
+            v[i]         = 0.0f;
+            if (n >= 0)
+                v[i] = SHARED ? table[n * C + c] : load_elem(over ? row[hi] : row[lo], c, p.tableType) * p.scale;
+        }
+        uint8_t *y = p.dst.base + e0 * (p.dstType == B200PP_F32 ? 4 : 2);
+        if (e0 + 8 <= total)
+            store_vecs<8, 1>(y, p.dstType, 0, 8, 8, v);
+        else
+            store_vecs<1, 8>(y, p.dstType, 0, 1, static_cast<int>(total - e0), v);
+    }
 }
 
 struct EmbeddingGradKParams
@@ -103,224 +115,462 @@ struct EmbeddingGradKParams
     int       rows, cols;
     float     scale;
     int       accumulate;
-    int       padding; // -1: none
+    int       padding;            // -1: none
     unsigned *keys[2], *order[2]; // count entries each; the sorted ones are keys[0], order[0]
-    int       passes, digitBits;
-    float    *partials; // [units][2][cols]
-    unsigned  unit;     // sorted positions per unit
+    int       passes, digitBits, sortWarps;
+    int       zeroCtas, zeroWidth, skipNamed; // CTAs that clear the table, their vector width, whether they leave out named rows
+    float    *partials;                       // [units][2][cols]
+    unsigned  unit, units;                    // sorted positions per unit (at most 32)
+    unsigned  blocks;                         // column blocks of kGradCols
 };
 
-// ---- sort: positions 0..count-1 by index, stable; indices that take no part get the key `rows` and end up last.
+// ---- first kernel: sort the positions 0..count-1 by index, stable; indices that take no part get the key `rows` and end up
+// last. Meanwhile the other CTAs clear the table.
 //
-// One cluster of kSortCtas CTAs, a least-significant-digit radix sort. Each warp owns a contiguous range of the positions
-// and counts its digits in a table of its own (lanes with equal digits find one another with a match instruction, so no
-// atomics and a fixed order); a prefix over the warps, the CTAs (through distributed shared memory) and the digits turns the
-// counts into the places each warp writes to. The arrays between the passes are in global memory (they stay in L2); the
-// cluster barrier orders the passes.
-constexpr int kSortCtas    = 8;
-constexpr int kSortThreads = 1024;
-constexpr int kSortMaxBits = 10;
+// Cluster 0 sorts: a least-significant-digit radix sort over kSortCtas CTAs. Each warp owns a contiguous range of the positions and
+// counts its digits in a table of its own; a prefix over the warps, the CTAs (through distributed shared memory) and the digits
+// turns the counts into the places each warp writes to. Within a warp, lanes with equal digits find one another with a match
+// instruction, so the order is that of the positions. The arrays between the passes are in global memory (they stay in L2); the
+// cluster barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and most counts of
+// indices are small; clearing the table, which takes longer for the usual sizes, hides it.
+constexpr int kSortCtas       = 8;
+constexpr int kSortMaxThreads = 1024;
+constexpr int kSortMaxBits    = 10;
+constexpr int kSortKeys       = 8; // keys a lane holds at a time
 
-inline size_t sort_smem_words(int bins)
+inline size_t sort_smem_words(int threads, int bins)
 {
-    return static_cast<size_t>(bins) * (kSortThreads / 32) + bins + 32;
+    return static_cast<size_t>(bins) * (threads / 32) + bins + 32;
 }
 
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const EmbeddingGradKParams p)
+__device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, unsigned *smem)
 {
-    namespace cg = cooperative_groups;
-    extern __shared__ unsigned smem[];
-    cg::cluster_group          cluster = cg::this_cluster();
-    const unsigned             rank    = cluster.block_rank();
-    const int                  lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int              kWarps = kSortThreads / 32;
-    const int                  bins   = 1 << p.digitBits;
-    unsigned                  *hist   = smem;                 // [warps][bins]
-    unsigned                  *total  = smem + kWarps * bins; // [bins], read by the other CTAs
-    unsigned                  *wsum   = total + bins;         // [32]
+    namespace cg               = cooperative_groups;
+    cg::cluster_group cluster  = cg::this_cluster();
+    const unsigned    rank     = cluster.block_rank();
+    const int         lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = p.sortWarps;
+    const int         bins  = 1 << p.digitBits;
+    unsigned         *hist  = smem;                // [warps][bins]
+    unsigned         *total = smem + warps * bins; // [bins], read by the other CTAs
+    unsigned         *wsum  = total + bins;        // [32]
+    unsigned         *mine  = hist + warp * bins;
 
-    const unsigned long long perWarp = ((static_cast<unsigned long long>(p.count) + kSortCtas * kWarps - 1) / (kSortCtas * kWarps) + 31) / 32 * 32;
-    const unsigned long long first   = (static_cast<unsigned long long>(rank) * kWarps + warp) * perWarp;
-    const unsigned           i0      = static_cast<unsigned>(first < p.count ? first : p.count);
-    const unsigned           i1      = static_cast<unsigned>(first + perWarp < p.count ? first + perWarp : p.count);
-    unsigned                *mine    = hist + warp * bins;
+    constexpr unsigned       kTile   = 32 * kSortKeys;
+    const unsigned long long perWarp = (static_cast<unsigned long long>(p.count) + kSortCtas * warps - 1) / (kSortCtas * warps);
+    const unsigned long long span    = (perWarp + 31) / 32 * 32;
+    const unsigned long long first   = (static_cast<unsigned long long>(rank) * warps + warp) * span;
+    const unsigned           i0      = static_cast<unsigned>(warp < warps && first < p.count ? first : p.count);
+    const unsigned           i1      = static_cast<unsigned>(warp < warps && first + span < p.count ? first + span : p.count);
 
     for (int pass = 0; pass < p.passes; ++pass)
     {
-        // the last pass writes to array 0
-        const int       to    = (p.passes - 1 - pass) & 1;
+        const int       to    = (p.passes - 1 - pass) & 1; // the last pass writes to array 0
         const unsigned *keys  = p.keys[to ^ 1];
         const unsigned *order = p.order[to ^ 1];
         const int       shift = pass * p.digitBits;
-        auto            key_at = [&](unsigned i) {
-            if (pass > 0)
-                return keys[i];
-            const int id = load_index(p.indices, p.indexType, i, p.rows);
-            return id < 0 || id == p.padding ? static_cast<unsigned>(p.rows) : static_cast<unsigned>(id);
+        unsigned        key[kSortKeys], pos[kSortKeys];
+        auto            load = [&](unsigned tile) {
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k)
+            {
+                const unsigned i = tile + 32 * k + lane;
+                key[k] = pos[k] = 0;
+                if (i < i1)
+                {
+                    if (pass > 0)
+                    {
+                        key[k] = keys[i];
+                        pos[k] = order[i];
+                    }
+                    else
+                    {
+                        const int id = load_index(p.indices, p.indexType, i, p.rows);
+                        key[k]       = static_cast<unsigned>(id < 0 || id == p.padding ? p.rows : id);
+                        pos[k]       = i;
+                    }
+                }
+            }
         };
-        for (int b = threadIdx.x; b < kWarps * bins; b += kSortThreads) hist[b] = 0;
+        for (int b = threadIdx.x; b < warps * bins; b += threads) hist[b] = 0;
         __syncthreads();
-        for (unsigned i = i0 + lane; i - lane < i1; i += 32)
+        for (unsigned tile = i0; tile < i1; tile += kTile)
         {
-            const bool     in    = i < i1;
-            const unsigned digit = in ? (key_at(i) >> shift) & (bins - 1) : bins;
-            const unsigned same  = __match_any_sync(0xffffffffu, digit);
-            if (in && lane == __ffs(same) - 1)
-                mine[digit] += __popc(same);
-            __syncwarp();
+            load(tile);
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k)
+                if (tile + 32 * k + lane < i1)
+                    atomicAdd(mine + ((key[k] >> shift) & (bins - 1)), 1u); // counts: their order does not matter
         }
         __syncthreads();
-        // bins <= threads: thread b does digit b
-        unsigned sum = 0;
-        if (static_cast<int>(threadIdx.x) < bins)
+        // counts of the digit over the warps before each, and over all
+        for (int b = threadIdx.x; b < bins; b += threads)
         {
-            for (int w = 0; w < kWarps; ++w)
+            unsigned sum = 0;
+            for (int w = 0; w < warps; ++w)
             {
-                const unsigned n                = hist[w * bins + threadIdx.x];
-                hist[w * bins + threadIdx.x] = sum;
+                const unsigned n   = hist[w * bins + b];
+                hist[w * bins + b] = sum;
                 sum += n;
             }
-            total[threadIdx.x] = sum;
+            total[b] = sum;
         }
         cluster.sync();
-        unsigned before = 0, all = 0;
-        if (static_cast<int>(threadIdx.x) < bins)
-            for (unsigned c = 0; c < kSortCtas; ++c)
-            {
-                const unsigned n = cluster.map_shared_rank(total, c)[threadIdx.x];
-                before += c < rank ? n : 0;
-                all += n;
-            }
-        // exclusive prefix of `all` over the digits
-        unsigned incl = all;
-        for (int o = 1; o < 32; o <<= 1)
+        // where each digit of this CTA starts: the digits below it everywhere, and its own in the CTAs before
+        unsigned below = 0; // of the digits this thread does not see (those before its stretch of bins / threads)
         {
-            const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
-            incl += lane >= o ? up : 0;
-        }
-        if (lane == 31)
-            wsum[warp] = incl;
-        __syncthreads();
-        if (warp == 0)
-        {
-            unsigned v = wsum[lane];
+            const int per = (bins + threads - 1) / threads, b0 = min(bins, static_cast<int>(threadIdx.x) * per), b1 = min(bins, b0 + per);
+            unsigned  all = 0;
+            for (int b = b0; b < b1; ++b)
+                for (unsigned c = 0; c < kSortCtas; ++c) all += cluster.map_shared_rank(total, c)[b];
+            unsigned incl = all;
             for (int o = 1; o < 32; o <<= 1)
             {
-                const unsigned up = __shfl_up_sync(0xffffffffu, v, o);
-                v += lane >= o ? up : 0;
+                const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
+                incl += lane >= o ? up : 0;
             }
-            wsum[lane] = v;
-        }
-        __syncthreads();
-        const unsigned base = incl - all + (warp > 0 ? wsum[warp - 1] : 0) + before;
-        if (static_cast<int>(threadIdx.x) < bins)
-            for (int w = 0; w < kWarps; ++w) hist[w * bins + threadIdx.x] += base;
-        __syncthreads();
-        for (unsigned i = i0 + lane; i - lane < i1; i += 32)
-        {
-            const bool     in    = i < i1;
-            const unsigned key   = in ? key_at(i) : 0;
-            const unsigned pos   = in ? (pass > 0 ? order[i] : i) : 0;
-            const unsigned digit = in ? (key >> shift) & (bins - 1) : bins;
-            const unsigned same  = __match_any_sync(0xffffffffu, digit);
-            if (in)
+            if (lane == 31)
+                wsum[warp] = incl;
+            __syncthreads();
+            if (warp == 0)
             {
-                const unsigned at = mine[digit] + __popc(same & ((1u << lane) - 1));
-                p.keys[to][at]    = key;
-                p.order[to][at]   = pos;
+                unsigned v = lane < threads >> 5 ? wsum[lane] : 0;
+                for (int o = 1; o < 32; o <<= 1)
+                {
+                    const unsigned up = __shfl_up_sync(0xffffffffu, v, o);
+                    v += lane >= o ? up : 0;
+                }
+                wsum[lane] = v;
             }
-            __syncwarp();
-            if (in && lane == __ffs(same) - 1)
-                mine[digit] += __popc(same);
-            __syncwarp();
+            __syncthreads();
+            below = incl - all + (warp > 0 ? wsum[warp - 1] : 0);
+            for (int b = b0; b < b1; ++b)
+            {
+                unsigned before = 0, here = 0;
+                for (unsigned c = 0; c < kSortCtas; ++c)
+                {
+                    const unsigned n = cluster.map_shared_rank(total, c)[b];
+                    before += c < rank ? n : 0;
+                    here += n;
+                }
+                for (int w = 0; w < warps; ++w) hist[w * bins + b] += below + before;
+                below += here;
+            }
         }
-        cluster.sync(); // also keeps `total` until every CTA has read it
+        __syncthreads();
+        for (unsigned tile = i0; tile < i1; tile += kTile)
+        {
+            if (i1 - i0 > kTile)
+                load(tile); // otherwise the keys are still there
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k)
+            {
+                if (tile + 32 * k >= i1)
+                    break;
+                const bool     in    = tile + 32 * k + lane < i1;
+                const unsigned digit = in ? (key[k] >> shift) & (bins - 1) : bins;
+                const unsigned same  = __match_any_sync(0xffffffffu, digit);
+                if (in)
+                {
+                    const unsigned at = mine[digit] + __popc(same & ((1u << lane) - 1));
+                    p.keys[to][at]    = key[k];
+                    p.order[to][at]   = pos[k];
+                }
+                __syncwarp();
+                if (in && lane == __ffs(same) - 1)
+                    mine[digit] += __popc(same);
+                __syncwarp();
+            }
+        }
+        cluster.sync(); // the next pass reads what this one wrote; also keeps `total` until every CTA has read it
     }
 }
 
-__global__ void __launch_bounds__(256) embedding_zero_kernel(const EmbeddingGradKParams p)
+template<int W>
+__device__ __forceinline__ void embedding_clear_row(const EmbeddingGradKParams &p, unsigned r)
 {
-    for (unsigned r = blockIdx.x; r < static_cast<unsigned>(p.rows); r += gridDim.x)
+    uint8_t *d    = p.dtable.at(r);
+    float    z[W] = {};
+    for (long long c = static_cast<int>(threadIdx.x & 31) * W; c < p.cols; c += 32 * W)
+        store_vecs<W, 1>(d, p.dtableType, static_cast<int>(c), 0, p.cols, z);
+}
+
+// Clears this CTA's share of the table's rows: all of them, or (skipNamed) those no index names, found by going through the indices
+// once with a bit per row -- worth it where the rows that need not be written twice are more bytes than the indices.
+constexpr int kZeroRows  = 32768; // rows a CTA has bits for at a time
+constexpr int kScanAhead = 8;     // indices a thread loads at a time
+
+__device__ __forceinline__ void embedding_clear(const EmbeddingGradKParams &p, unsigned *named)
+{
+    const unsigned cta  = blockIdx.x - kSortCtas;
+    const unsigned per  = (static_cast<unsigned>(p.rows) + p.zeroCtas - 1) / p.zeroCtas;
+    const unsigned from = min(static_cast<unsigned>(p.rows), cta * per), to = min(static_cast<unsigned>(p.rows), from + per);
+    for (unsigned r0 = from; r0 < to; r0 += kZeroRows)
     {
-        uint8_t *d = p.dtable.at(r);
-        for (long long c = threadIdx.x; c < p.cols; c += blockDim.x) store_elem_as(d, c, p.dtableType, 0.0f);
+        const unsigned r1 = min(to, r0 + kZeroRows);
+        if (p.skipNamed)
+        {
+            for (unsigned k = threadIdx.x; k < kZeroRows / 32; k += blockDim.x) named[k] = 0;
+            __syncthreads();
+            for (unsigned long long i0 = threadIdx.x; i0 < p.count; i0 += kScanAhead * blockDim.x)
+            {
+                int id[kScanAhead]; // all loads before the first is used
+#pragma unroll
+                for (int k = 0; k < kScanAhead; ++k)
+                {
+                    const unsigned long long i = i0 + k * blockDim.x;
+                    id[k]                      = i < p.count ? load_index(p.indices, p.indexType, static_cast<unsigned>(i), p.rows) : -1;
+                }
+#pragma unroll
+                for (int k = 0; k < kScanAhead; ++k)
+                {
+                    const unsigned d = static_cast<unsigned>(id[k]) - r0; // -1: far above
+                    if (d < r1 - r0 && id[k] != p.padding)
+                        atomicOr(named + d / 32, 1u << (d % 32));
+                }
+            }
+            __syncthreads();
+        }
+        for (unsigned r = r0 + (threadIdx.x >> 5); r < r1; r += blockDim.x >> 5)
+        {
+            if (p.skipNamed && (named[(r - r0) / 32] >> ((r - r0) % 32) & 1))
+                continue;
+            if (p.zeroWidth == 8)
+                embedding_clear_row<8>(p, r);
+            else if (p.zeroWidth == 4)
+                embedding_clear_row<4>(p, r);
+            else if (p.zeroWidth == 2)
+                embedding_clear_row<2>(p, r);
+            else
+                embedding_clear_row<1>(p, r);
+        }
+        __syncthreads();
     }
 }
 
-__device__ __forceinline__ void embedding_grad_store(const EmbeddingGradKParams &p, unsigned key, long long c, float sum)
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortMaxThreads, 1)
+    embedding_sort_kernel(const EmbeddingGradKParams p)
 {
+    extern __shared__ unsigned smem[];
+    if (blockIdx.x < kSortCtas)
+        embedding_sort(p, smem);
+    else
+        embedding_clear(p, smem);
+}
+
+// ---- second kernel: a warp sums the runs of equal keys that start among `unit` neighbouring sorted positions, for kGradCols
+// columns. A run of up to kShortRun positions is summed by the warp it starts in, wherever it ends. Longer runs are summed unit
+// by unit into `partials` -- slot 0: the run comes from the unit before, slot 1: it starts here -- and joined by the third kernel.
+constexpr int kShortRun  = 32;
+constexpr int kGradCols  = 256; // eight per lane
+constexpr int kGradAhead = 8;   // rows loaded before the first is added
+
+// Puts a lane's eight sums where they belong: into `partial` or, if that is null, into the table. Not inlined: it would be there
+// once for each of the rows a warp has in flight, and code that runs once is as slow as it can be fetched (7 times slower for
+// few indices).
+template<int W>
+__device__ __noinline__ void embedding_grad_put(const EmbeddingGradKParams &p, float *partial, unsigned key, int c, float s0, float s1,
+                                                float s2, float s3, float s4, float s5, float s6, float s7)
+{
+    // vectors of four: 256-bit accesses in a function that is not inlined end this ptxas (12.9) with a segmentation fault
+    constexpr int P = W == 8 ? 4 : W, N = 8 / P, kStep = W == 8 ? 4 : 32 * W;
+    float         v[8] = {s0, s1, s2, s3, s4, s5, s6, s7};
+    if (partial)
+    {
+        store_vecs<B200PP_F32, P, N>(reinterpret_cast<uint8_t *>(partial), c, kStep, p.cols, v);
+        return;
+    }
     uint8_t *d = p.dtable.at(key);
-    float    v = sum * p.scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= p.scale;
     if (p.accumulate)
-        v += load_elem(d, c, p.dtableType);
-    store_elem_as(d, c, p.dtableType, v);
+    {
+        float old[8];
+        load_vecs<P, N>(d, p.dtableType, c, kStep, p.cols, old);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += old[i];
+    }
+    store_vecs<P, N>(d, p.dtableType, c, kStep, p.cols, v);
 }
 
-// A warp sums the runs of equal keys among `unit` neighbouring sorted positions, for 256 columns. A run that lies inside the
-// unit goes to the table; what belongs to a run that crosses the unit's ends goes to `partials`: slot 0 the run that comes
-// from the unit before, slot 1 the one that starts here and goes on.
-__global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const EmbeddingGradKParams p)
+template<int GRAD, int W>
+__global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
-    const int          lane   = threadIdx.x & 31;
-    const unsigned     blocks = (p.cols + 255u) / 256u;
-    const unsigned     units  = (p.count + p.unit - 1) / p.unit;
-    unsigned long long job    = blockIdx.x * 8ull + (threadIdx.x >> 5);
-    if (job >= static_cast<unsigned long long>(units) * blocks)
+    constexpr int            V    = 8 / W;
+    constexpr unsigned       kAll = 0xffffffffu;
+    const int                lane = threadIdx.x & 31;
+    const unsigned long long job  = blockIdx.x * 8ull + (threadIdx.x >> 5);
+    if (job >= static_cast<unsigned long long>(p.units) * p.blocks)
         return;
-    const unsigned  u  = static_cast<unsigned>(job / blocks);
-    const long long c0 = static_cast<long long>(job % blocks) * 256 + lane;
-    const unsigned  i0 = u * p.unit, i1 = min(p.count, i0 + p.unit);
-    float           acc[8] = {};
-    unsigned        cur    = p.keys[0][i0];
-    bool            head   = i0 > 0 && p.keys[0][i0 - 1] == cur;
-    for (unsigned i = i0; i < i1; ++i)
+    const unsigned u    = static_cast<unsigned>(job / p.blocks);
+    const int      c0   = static_cast<int>(job - static_cast<unsigned long long>(u) * p.blocks) * kGradCols + lane * W;
+    const unsigned i0   = u * p.unit;
+    const int      n    = static_cast<int>(min(p.count - i0, p.unit));
+    const unsigned none = static_cast<unsigned>(p.rows);
+    // keys of the 32 positions before the unit (lane l: i0 - 1 - l), of the 32 from its start on and of the 32 after those
+    const unsigned  i   = i0 + lane;
+    const unsigned  bk  = static_cast<unsigned>(lane) < i0 ? p.keys[0][i0 - 1 - lane] : none;
+    const unsigned  k0  = i < p.count ? p.keys[0][i] : none;
+    const unsigned  k1  = i + 32u < p.count ? p.keys[0][i + 32] : none;
+    const unsigned  o0  = i < p.count ? p.order[0][i] : 0;
+    const unsigned  o1  = i + 32u < p.count ? p.order[0][i + 32] : 0;
+    const unsigned  key = __shfl_sync(kAll, k0, 0);
+    if (key == none)
+        return;
+    // the run at the unit's start: `back` positions of it lie before (32: at least); how far it goes on
+    const unsigned other = __ballot_sync(kAll, bk != key);
+    const int      back  = other ? __ffs(other) - 1 : 32;
+    const unsigned d0 = __ballot_sync(kAll, k0 != key), d1 = __ballot_sync(kAll, k1 != key);
+    const int      on    = d0 ? __ffs(d0) - 1 : d1 ? 31 + __ffs(d1) : 64;
+    // what this warp sums: positions from..to, counted from the unit's start
+    int  from = 0, to = n;
+    bool head = back > 0; // the first run belongs to `partials`
+    if (back > 0 && back + on <= kShortRun)
     {
-        if (cur == static_cast<unsigned>(p.rows))
-            return;
-        const uint8_t *g = p.grad.at(p.order[0][i]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (c0 + 32 * k < p.cols)
-                acc[k] += load_elem(g, c0 + 32 * k, p.gradType);
-        const unsigned next = i + 1 < p.count ? p.keys[0][i + 1] : static_cast<unsigned>(p.rows);
-        if (next == cur && i + 1 < i1)
-            continue;
-        const bool tail = next == cur;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-        {
-            if (c0 + 32 * k < p.cols)
-            {
-                if (head || tail)
-                    p.partials[(static_cast<long long>(u) * 2 + (head ? 0 : 1)) * p.cols + c0 + 32 * k] = acc[k];
-                else
-                    embedding_grad_store(p, cur, c0 + 32 * k, acc[k]);
-            }
-            acc[k] = 0.0f;
-        }
+        from = on; // the warp before does it
         head = false;
-        cur  = next;
+    }
+    if (from >= n)
+        return;
+    // the run at the unit's end
+    const unsigned endKey = __shfl_sync(kAll, k0, n - 1), next = __shfl_sync(kAll, n < 32 ? k0 : k1, n & 31);
+    bool           tail   = false; // the last run belongs to `partials`
+    if (next == endKey && endKey != none)
+    {
+        const unsigned e0 = __ballot_sync(kAll, k0 == endKey), e1 = __ballot_sync(kAll, k1 == endKey);
+        const int      start = __ffs(e0) - 1, end = start + __popc(e0) + (start + __popc(e0) == 32 ? __popc(e1) : 0);
+        tail                 = (head && endKey == key) || end - start > kShortRun;
+        if (!tail)
+            to = end;
+    }
+    const unsigned s0 = __ballot_sync(kAll, k0 != none);
+    const int      valid = __popc(s0) + __popc(__ballot_sync(kAll, k1 != none));
+    to                   = min(to, valid);
+    const uint8_t *r0 = k0 != none ? p.grad.at(o0) : nullptr, *r1 = k1 != none ? p.grad.at(o1) : nullptr;
+    // bit j of ends: position j is the last of its run
+    const unsigned f0 = __shfl_down_sync(kAll, k0, 1), f1 = __shfl_down_sync(kAll, k1, 1), g1 = __shfl_sync(kAll, k1, 0);
+    unsigned long long ends = __ballot_sync(kAll, k0 != (lane < 31 ? f0 : g1));
+    ends |= static_cast<unsigned long long>(__ballot_sync(kAll, k1 != f1 || lane == 31)) << 32;
+    ends |= 1ull << (to - 1);
+    float acc[8] = {};
+    for (int j = from; j < to; j += kGradAhead)
+    {
+        Vec<GRAD, W> raw[kGradAhead][V];
+#pragma unroll
+        for (int a = 0; a < kGradAhead; ++a)
+        {
+            const unsigned long long at0 = __shfl_sync(kAll, reinterpret_cast<unsigned long long>(r0), (j + a) & 31);
+            const unsigned long long at1 = __shfl_sync(kAll, reinterpret_cast<unsigned long long>(r1), (j + a) & 31);
+            const uint8_t           *row = reinterpret_cast<const uint8_t *>(j + a < 32 ? at0 : at1);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+            {
+                const int c = c0 + v * 32 * W;
+                raw[a][v]   = zero_raw<kElemBytes<GRAD> * W>();
+                if (j + a < to && c < p.cols)
+                    raw[a][v] = load_raw<kElemBytes<GRAD> * W>(row + static_cast<long long>(c) * kElemBytes<GRAD>);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < kGradAhead; ++a)
+        {
+            const int q = j + a;
+            if (q >= to)
+                break;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+            {
+                float g[W];
+                unpack<GRAD, W>(raw[a][v], g);
+#pragma unroll
+                for (int k = 0; k < W; ++k) acc[v * W + k] += g[k];
+            }
+            if (!((ends >> q) & 1))
+                continue;
+            const unsigned kq   = __shfl_sync(kAll, q < 32 ? k0 : k1, q & 31);
+            float         *part = nullptr;
+            if (head || (tail && q + 1 == to))
+                part = p.partials + (static_cast<long long>(u) * 2 + (head ? 0 : 1)) * p.cols;
+            embedding_grad_put<W>(p, part, kq, c0, acc[0], acc[1], acc[2], acc[3], acc[4], acc[5], acc[6], acc[7]);
+#pragma unroll
+            for (int z = 0; z < 8; ++z) acc[z] = 0.0f;
+            head = false;
+        }
     }
 }
 
-// The runs that cross units: the unit a run starts in adds up its parts, in order.
-__global__ void __launch_bounds__(256) embedding_grad_join_kernel(const EmbeddingGradKParams p)
+// ---- third kernel: the runs longer than kShortRun that cross units. A CTA looks after eight units: a warp each finds out whether
+// such a run starts in its unit; the CTA then adds up the run's parts for kGradCols columns, each warp a contiguous share of the
+// units, the warps one after another.
+__global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
-    const unsigned  u    = blockIdx.x;
-    const unsigned  last = min(p.count, (u + 1) * p.unit) - 1; // its last position
-    const unsigned  key  = p.keys[0][last];
-    const long long c    = static_cast<long long>(blockIdx.y) * 256 + threadIdx.x;
-    if (last + 1 >= p.count || key == static_cast<unsigned>(p.rows) || p.keys[0][last + 1] != key)
-        return; // nothing goes on
-    const unsigned first = u * p.unit;
-    if (p.keys[0][first] == key && first > 0 && p.keys[0][first - 1] == key)
-        return; // it started before
-    if (c >= p.cols)
-        return;
-    float sum = p.partials[(static_cast<long long>(u) * 2 + 1) * p.cols + c];
-    for (unsigned long long i = last + 1ull; i < p.count && p.keys[0][i] == key; i += p.unit)
-        sum += p.partials[static_cast<long long>(i / p.unit) * 2 * p.cols + c];
-    embedding_grad_store(p, key, c, sum);
+    __shared__ float    sums[8][kGradCols];
+    __shared__ unsigned keys[8];
+    constexpr unsigned kAll = 0xffffffffu;
+    const unsigned     none = static_cast<unsigned>(p.rows);
+    const int          lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    {
+        const unsigned u = blockIdx.x * 8 + warp;
+        unsigned       k = none;
+        if (u + 1 < p.units) // not the last unit, so it is full
+        {
+            const unsigned first = u * p.unit;
+            const unsigned mine  = p.keys[0][min(first + lane, p.count - 1)]; // the unit after this one has a position at least
+            const unsigned prev  = first > 0 ? p.keys[0][first - 1] : none;
+            const unsigned last = __shfl_sync(kAll, mine, p.unit - 1), after = p.keys[0][first + p.unit];
+            const unsigned same  = __ballot_sync(kAll, mine == last);
+            const unsigned start = first + __ffs(same) - 1;
+            if (last != none && after == last && !(start == first && prev == last) && start + kShortRun < p.count
+                && p.keys[0][start + kShortRun] == last)
+                k = last;
+        }
+        if (lane == 0)
+            keys[warp] = k;
+    }
+    __syncthreads();
+    for (int l = 0; l < 8; ++l)
+    {
+        const unsigned u = blockIdx.x * 8 + l, k = keys[l];
+        if (k == none)
+            continue;
+        unsigned       more = 0; // units the run goes on in
+        for (;;)
+        {
+            const unsigned long long at = (static_cast<unsigned long long>(u) + 1 + more + lane) * p.unit;
+            const unsigned           on = __ballot_sync(kAll, at < p.count && p.keys[0][at] == k);
+            more += on == kAll ? 32 : __ffs(~on) - 1;
+            if (on != kAll)
+                break;
+        }
+        // share of this warp: parts from..to of 0 (slot 1 of unit u) and 1..more (slot 0 of unit u + part)
+        const unsigned per = (more + 8) / 8, from = min(more + 1, warp * per), to = min(more + 1, from + per);
+        const int      c0  = blockIdx.y * kGradCols + lane;
+        float          s[8] = {};
+#pragma unroll 2
+        for (unsigned m = from; m < to; ++m)
+        {
+            const float *part = p.partials + (static_cast<unsigned long long>(u + m) * 2 + (m == 0 ? 1 : 0)) * p.cols;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + 32 * j < p.cols)
+                    s[j] += part[c0 + 32 * j];
+        }
+        __syncthreads(); // the sums of the run before are taken
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[warp][lane + 32 * j] = s[j];
+        __syncthreads();
+        // the first warp hands the totals over: lane l has columns l, l + 32, ...
+        if (warp == 0)
+        {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+            {
+                s[j] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) s[j] += sums[w][lane + 32 * j];
+            }
+            embedding_grad_put<1>(p, nullptr, k, c0, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]);
+        }
+    }
 }
 
 } // namespace b200pp

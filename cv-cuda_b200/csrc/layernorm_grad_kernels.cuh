@@ -34,45 +34,40 @@ template<int SRC, int GRAD, int E, int W, bool BLOCK>
 __global__ void __launch_bounds__(E == 8 ? kGradResident8 : kGradResident16) layernorm_grad_kernel(const LayerNormGradKParams p)
 {
     constexpr int           V     = E / W;
-    constexpr bool          AHEAD = E == 8; // with sixteen values there are no registers left for the next row
+    constexpr bool          AHEAD = E == 8 && W >= 4; // otherwise there are no registers left for the next row
     __shared__ float2       scratch[2][16]; // two halves, used in turn: one barrier per row
     extern __shared__ float sums[];         // [2][cols]
     const int               t = threadIdx.x, threads = blockDim.x, g = threadIdx.y, groups = blockDim.y;
     const int               tid = g * threads + t, warp = tid >> 5;
+    const RowSpan<E, W, BLOCK> at(t);
     float                   w[E], dw[E], db[E];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-    {
-        const int c = vec_at<W>(v, t, threads);
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[v * W + i] = 1.0f, dw[v * W + i] = 0.0f, db[v * W + i] = 0.0f;
-        if (p.weight && c < p.cols)
-            load_vec<W>(p.weight, c, p.weightType, w + v * W);
-    }
+    for (int e = 0; e < E; ++e) w[e] = 1.0f, dw[e] = 0.0f, db[e] = 0.0f;
+    if (p.weight)
+        load_vecs<W, V>(p.weight, p.weightType, at.c, at.step, p.cols, w);
     Vec<SRC, W>  xr[V];
     Vec<GRAD, W> gr[V];
     float        mean = 0.0f, rstd = 0.0f;
     auto         fetch = [&](unsigned long long r) {
-        const bool     live = r < p.rows;
+        mean = rstd = 0.0f; // a row that is not there, and what lies behind a row's end: h = 0 and dy = 0
+        const int end = r < p.rows ? p.cols : 0;
         const uint8_t *x = nullptr, *dy = nullptr;
-        mean = rstd = 0.0f; // a row that is not there: h = 0 and dy = 0
-        if (live)
+        if (end)
         {
-            x    = p.src.at(static_cast<unsigned>(r));
-            dy   = p.grad.at(static_cast<unsigned>(r));
+            x    = p.src.at(static_cast<unsigned>(r)) + static_cast<long long>(at.c) * kElemBytes<SRC>;
+            dy   = p.grad.at(static_cast<unsigned>(r)) + static_cast<long long>(at.c) * kElemBytes<GRAD>;
             mean = p.mean[r];
             rstd = p.rstd[r];
         }
 #pragma unroll
         for (int v = 0; v < V; ++v)
         {
-            const int c = vec_at<W>(v, t, threads);
-            xr[v]       = zero_raw<kElemBytes<SRC> * W>();
-            gr[v]       = zero_raw<kElemBytes<GRAD> * W>();
-            if (live && c < p.cols)
+            xr[v] = zero_raw<kElemBytes<SRC> * W>();
+            gr[v] = zero_raw<kElemBytes<GRAD> * W>();
+            if (at.c + v * at.step < end)
             {
-                xr[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
-                gr[v] = load_raw<kElemBytes<GRAD> * W>(dy + static_cast<long long>(c) * kElemBytes<GRAD>);
+                xr[v] = load_raw<kElemBytes<SRC> * W>(x + v * at.step * kElemBytes<SRC>);
+                gr[v] = load_raw<kElemBytes<GRAD> * W>(dy + v * at.step * kElemBytes<GRAD>);
             }
         }
     };
@@ -137,16 +132,8 @@ __global__ void __launch_bounds__(E == 8 ? kGradResident8 : kGradResident16) lay
         const float c1 = s1 / p.fcols, c2 = s2 / p.fcols;
         uint8_t    *dx = p.dsrc.at(static_cast<unsigned>(now));
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-        {
-            const int c = vec_at<W>(v, t, threads);
-            if (c >= p.cols)
-                break;
-            float o[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) o[i] = rs * (gv[v * W + i] - c1 - h[v * W + i] * c2);
-            store_vec<W>(dx, c, p.dsrcType, o);
-        }
+        for (int e = 0; e < E; ++e) gv[e] = rs * (gv[e] - c1 - h[e] * c2);
+        store_vecs<W, V>(dx, p.dsrcType, at.c, at.step, p.cols, gv);
     }
     if (!p.partials)
         return;
@@ -175,7 +162,7 @@ __global__ void __launch_bounds__(E == 8 ? kGradResident8 : kGradResident16) lay
 #pragma unroll
             for (int e = 0; e < E; ++e)
             {
-                const int c = vec_at<W>(e / W, t, threads) + e % W;
+                const int c = at.c + e / W * at.step + e % W;
                 if (c < p.cols)
                 {
                     to[c]          = s > 0 ? sums[c] + dw[e] : dw[e];

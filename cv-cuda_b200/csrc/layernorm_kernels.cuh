@@ -22,13 +22,20 @@ struct LayerNormKParams
     float2        *partials; // [rows][chunks]
 };
 
-// A thread holds E values of its row: vectors of W neighbouring elements, T vectors apart (T: the threads of the row), so that
-// every load and store of a warp covers one contiguous span.
-template<int W>
-__device__ __forceinline__ int vec_at(int v, int t, int threads)
+// A thread holds E values of its row, as vectors of W neighbouring elements: lane l of warp k of the row has vectors l, l + 32, ...
+// of the warp's 32 E elements, so that every load and store of a warp covers one contiguous span, at offsets known at compile
+// time. (Rows of fewer than 32 lanes: l, l + lanes, ...)
+template<int E, int W, bool BLOCK>
+struct RowSpan
 {
-    return (v * threads + t) * W;
-}
+    int c, step; // first element of the thread, distance to its next vector
+
+    __device__ __forceinline__ explicit RowSpan(int t)
+        : c(BLOCK ? (t >> 5) * (32 * E) + (t & 31) * W : t * W)
+        , step(BLOCK || E > 8 ? 32 * W : static_cast<int>(blockDim.x) * W)
+    {
+    }
+};
 
 // Sum over the `lanes` neighbouring lanes (a power of two) a row has in a warp, or over the block.
 template<bool BLOCK>
@@ -51,29 +58,31 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *scratch)
     }
 }
 
-// y of one thread's values.
+// Weights and biases of eight values (1 and 0 where there are none).
+template<int W>
+__device__ __forceinline__ void layernorm_affine(const LayerNormKParams &p, int c, int step, int end, float *w, float *b)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.0f, b[i] = 0.0f;
+    if (p.weight)
+        load_vecs<W, 8 / W>(p.weight, p.weightType, c, step, end, w);
+    if (p.bias)
+        load_vecs<W, 8 / W>(p.bias, p.biasType, c, step, end, b);
+}
+
+// y of a thread's values, eight at a time.
 template<int E, int W>
-__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const float *x, float mean, float rstd, int c0,
+__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const float *x, float mean, float rstd, int c,
                                                 int step, int end)
 {
 #pragma unroll
-    for (int v = 0; v < E / W; ++v)
+    for (int k = 0; k < E / 8; ++k, c += 8 / W * step)
     {
-        const int c = c0 + v * step;
-        if (c >= end)
-            break;
-        float w[W], b[W], o[W];
-        if (p.weight)
-            load_vec<W>(p.weight, c, p.weightType, w);
-        if (p.bias)
-            load_vec<W>(p.bias, c, p.biasType, b);
+        float w[8], b[8];
+        layernorm_affine<W>(p, c, step, end, w, b);
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-        {
-            const float h = (x[v * W + i] - mean) * rstd;
-            o[i]          = p.weight ? (p.bias ? fmaf(h, w[i], b[i]) : h * w[i]) : (p.bias ? h + b[i] : h);
-        }
-        store_vec<W>(y, c, p.dstType, o);
+        for (int i = 0; i < 8; ++i) b[i] = fmaf((x[k * 8 + i] - mean) * rstd, w[i], b[i]);
+        store_vecs<W, 8 / W>(y, p.dstType, c, step, end, b);
     }
 }
 
@@ -87,30 +96,21 @@ __global__ void __launch_bounds__(BLOCK ? (E <= 16 ? 512 : 1024) : 256) layernor
     const unsigned   r = BLOCK ? blockIdx.x : blockIdx.x * blockDim.y + threadIdx.y;
     if (!BLOCK && r - threadIdx.y % (32u / threads) >= p.rows) // all rows of the warp
         return;
-    const bool     live = BLOCK || r < p.rows;
-    const uint8_t *x    = p.src.at(live ? r : p.rows - 1);
-    Vec<SRC, W>    raw[E / W];
+    const bool                 live = BLOCK || r < p.rows;
+    const RowSpan<E, W, BLOCK> at(t);
+    float                      xv[E], s = 0.0f;
+    load_vecs<SRC, W, E / W>(p.src.at(live ? r : p.rows - 1), at.c, at.step, p.cols, xv);
+    // with eight values there are registers left to fetch the weights at the same time as the row
+    float w[8], b[8];
+    if constexpr (E == 8)
+        layernorm_affine<W>(p, at.c, at.step, p.cols, w, b);
 #pragma unroll
-    for (int v = 0; v < E / W; ++v)
-    {
-        const int c = vec_at<W>(v, t, threads);
-        raw[v]      = zero_raw<kElemBytes<SRC> * W>();
-        if (c < p.cols)
-            raw[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
-    }
-    float xv[E], s = 0.0f;
-#pragma unroll
-    for (int v = 0; v < E / W; ++v)
-    {
-        unpack<SRC, W>(raw[v], xv + v * W);
-#pragma unroll
-        for (int i = 0; i < W; ++i) s += xv[v * W + i];
-    }
+    for (int e = 0; e < E; ++e) s += xv[e];
     const float mean = row_sum<BLOCK>(s, threads, scratch[0]) / p.fcols;
     float       q    = 0.0f;
 #pragma unroll
     for (int v = 0; v < E / W; ++v)
-        if (vec_at<W>(v, t, threads) < p.cols)
+        if (at.c + v * at.step < p.cols)
         {
 #pragma unroll
             for (int i = 0; i < W; ++i)
@@ -129,7 +129,14 @@ __global__ void __launch_bounds__(BLOCK ? (E <= 16 ? 512 : 1024) : 256) layernor
         if (p.rstd)
             p.rstd[r] = rstd;
     }
-    layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, t * W, threads * W, p.cols);
+    if constexpr (E == 8)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = fmaf((xv[i] - mean) * rstd, w[i], b[i]);
+        store_vecs<W, 8 / W>(p.dst.at(r), p.dstType, at.c, at.step, p.cols, b);
+    }
+    else
+        layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, at.c, at.step, p.cols);
 }
 
 // Forward, longer rows: two kernels over chunks of kChunk values. The first leaves each chunk's mean and sum of squared distances
@@ -137,23 +144,6 @@ __global__ void __launch_bounds__(BLOCK ? (E <= 16 ? 512 : 1024) : 256) layernor
 // chunks in reverse order, so that the ones read last by the first kernel are still in L2.
 constexpr int kChunk        = 8192;
 constexpr int kChunkThreads = 256;
-
-template<int SRC, int W>
-__device__ __forceinline__ void load_chunk(const uint8_t *x, int c0, int end, float (&xv)[kChunk / kChunkThreads])
-{
-    constexpr int V = kChunk / kChunkThreads / W;
-    Vec<SRC, W>   raw[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-    {
-        const int c = c0 + vec_at<W>(v, threadIdx.x, kChunkThreads);
-        raw[v]      = zero_raw<kElemBytes<SRC> * W>();
-        if (c < end)
-            raw[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) unpack<SRC, W>(raw[v], xv + v * W);
-}
 
 template<int SRC, int W>
 __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_stats_kernel(const LayerNormKParams p)
@@ -165,13 +155,14 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_stats_kernel(co
     const int        c0  = static_cast<int>(at);
     const int        end = min(static_cast<long long>(p.cols), at + kChunk);
     float            xv[E], s = 0.0f, q = 0.0f;
-    load_chunk<SRC, W>(p.src.at(r), c0, end, xv);
+    const RowSpan<E, W, true> span(threadIdx.x);
+    load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, xv);
 #pragma unroll
     for (int e = 0; e < E; ++e) s += xv[e];
     const float mean = row_sum<true>(s, 0, scratch[0]) / static_cast<float>(end - c0);
 #pragma unroll
     for (int v = 0; v < E / W; ++v)
-        if (c0 + vec_at<W>(v, threadIdx.x, kChunkThreads) < end)
+        if (c0 + span.c + v * span.step < end)
         {
 #pragma unroll
             for (int i = 0; i < W; ++i)
@@ -196,7 +187,8 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
     const int        c0  = static_cast<int>(at);
     const int        end = min(static_cast<long long>(p.cols), at + kChunk);
     float            xv[E];
-    load_chunk<SRC, W>(p.src.at(r), c0, end, xv);
+    const RowSpan<E, W, true> span(threadIdx.x);
+    load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, xv);
     const float2 *part = p.partials + static_cast<unsigned long long>(r) * p.chunks;
     const float   tail = static_cast<float>(p.cols - static_cast<long long>(p.chunks - 1) * kChunk); // length of the last chunk
     float         s    = 0.0f;
@@ -216,7 +208,7 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
         if (p.rstd)
             p.rstd[r] = rstd;
     }
-    layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, c0 + threadIdx.x * W, kChunkThreads * W, end);
+    layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, c0 + span.c, span.step, end);
 }
 
 } // namespace b200pp

@@ -275,27 +275,52 @@ __device__ __forceinline__ void store_vec(uint8_t *row, long long i, const float
     store_raw<kElemBytes<DT> * W>(row + i * kElemBytes<DT>, pack<DT, W>(v));
 }
 
-// float16, bfloat16 or float32, chosen at run time.
-template<int W>
-__device__ __forceinline__ void load_vec(const uint8_t *row, long long i, int dtype, float *v)
+// N neighbouring vectors, `step` elements apart, of float16, bfloat16 or float32 chosen at run time: the type is looked at once for
+// all of them. Vectors that start at or after `end` are left out (load: their values are not set).
+template<int DT, int W, int N>
+__device__ __forceinline__ void load_vecs(const uint8_t *row, int c, int step, int end, float *v)
 {
-    if (dtype == B200PP_F32)
-        load_vec<B200PP_F32, W>(row, i, v);
-    else if (dtype == B200PP_BF16)
-        load_vec<B200PP_BF16, W>(row, i, v);
-    else
-        load_vec<B200PP_F16, W>(row, i, v);
+    Vec<DT, W> raw[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+    {
+        raw[k] = zero_raw<kElemBytes<DT> * W>();
+        if (c + k * step < end)
+            raw[k] = load_raw<kElemBytes<DT> * W>(row + static_cast<long long>(c + k * step) * kElemBytes<DT>);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) unpack<DT, W>(raw[k], v + k * W);
 }
 
-template<int W>
-__device__ __forceinline__ void store_vec(uint8_t *row, long long i, int dtype, const float *v)
+template<int W, int N>
+__device__ __forceinline__ void load_vecs(const uint8_t *row, int dtype, int c, int step, int end, float *v)
 {
     if (dtype == B200PP_F32)
-        store_vec<B200PP_F32, W>(row, i, v);
+        load_vecs<B200PP_F32, W, N>(row, c, step, end, v);
     else if (dtype == B200PP_BF16)
-        store_vec<B200PP_BF16, W>(row, i, v);
+        load_vecs<B200PP_BF16, W, N>(row, c, step, end, v);
     else
-        store_vec<B200PP_F16, W>(row, i, v);
+        load_vecs<B200PP_F16, W, N>(row, c, step, end, v);
+}
+
+template<int DT, int W, int N>
+__device__ __forceinline__ void store_vecs(uint8_t *row, int c, int step, int end, const float *v)
+{
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (c + k * step < end)
+            store_vec<DT, W>(row, c + k * step, v + k * W);
+}
+
+template<int W, int N>
+__device__ __forceinline__ void store_vecs(uint8_t *row, int dtype, int c, int step, int end, const float *v)
+{
+    if (dtype == B200PP_F32)
+        store_vecs<B200PP_F32, W, N>(row, c, step, end, v);
+    else if (dtype == B200PP_BF16)
+        store_vecs<B200PP_BF16, W, N>(row, c, step, end, v);
+    else
+        store_vecs<B200PP_F16, W, N>(row, c, step, end, v);
 }
 
 __device__ __forceinline__ float warp_sum(float v)
