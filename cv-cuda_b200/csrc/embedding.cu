@@ -22,16 +22,26 @@ int check_indices(const B200ppRows *indices)
 
 namespace {
 
+template<int C, int R>
+void launch_short_rows(const EmbeddingKParams &p, cudaStream_t stream)
+{
+    const unsigned tiles = (p.count + 256u * R - 1) / (256u * R);
+    const int      lines = 8 * 32 * C * static_cast<int>(sizeof(uint4));
+    // the copy to shared memory pays from the second index per table row on
+    if (static_cast<long long>(p.rows) * C <= kShortTable && p.count >= 2u * p.rows)
+        embedding_short_rows_kernel<C, R, true><<<std::min(tiles, kSms * 8u), 256, lines + p.rows * C * static_cast<int>(sizeof(float)),
+                                                  stream>>>(p);
+    else
+        embedding_short_rows_kernel<C, R, false><<<tiles, 256, lines, stream>>>(p);
+}
+
 template<int C>
 void launch_short_rows(const EmbeddingKParams &p, cudaStream_t stream)
 {
-    const unsigned long long tiles = (static_cast<unsigned long long>(p.count) * C + 2047) / 2048; // at most 2^31 * 7 / 2^11
-    // the copy to shared memory pays from the second index per table row on
-    if (static_cast<long long>(p.rows) * C <= kShortTable && p.count >= 2u * p.rows)
-        embedding_short_rows_kernel<C, true><<<static_cast<unsigned>(std::min<unsigned long long>(tiles, kSms * 8)), 256,
-                                               p.rows * C * static_cast<int>(sizeof(float)), stream>>>(p);
+    if (p.dstType == B200PP_F32)
+        launch_short_rows<C, 4>(p, stream);
     else
-        embedding_short_rows_kernel<C, false><<<static_cast<unsigned>(tiles), 256, 0, stream>>>(p);
+        launch_short_rows<C, 8>(p, stream);
 }
 
 template<int TABLE, int W>
@@ -98,7 +108,7 @@ extern "C" int b200ppEmbedding(const B200ppRows *indices, const B200ppRows *tabl
     p.scale     = scale;
     const int elem = row_elem_size(dst->dtype);
     if (p.cols < 8 && p.dst.n2 == 0 && (count == 1 || p.dst.s2 == static_cast<long long>(p.cols) * elem)
-        && (reinterpret_cast<uintptr_t>(p.dst.base) & (8 * elem - 1)) == 0)
+        && (reinterpret_cast<uintptr_t>(p.dst.base) & 15) == 0)
     {
         switch (p.cols)
         {
@@ -142,7 +152,7 @@ namespace {
 struct EmbeddingGradPlan
 {
     unsigned unit, units, blocks;
-    size_t   keys[2], order[2], partials, bytes;
+    size_t   entries[2], partials, bytes;
 };
 
 EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
@@ -154,13 +164,10 @@ EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
     while (w.unit > 8 && count * w.blocks < static_cast<long long>(w.unit) * kSms * 16) w.unit /= 2;
     w.units      = static_cast<unsigned>((count + w.unit - 1) / w.unit);
     size_t at    = 0;
-    const size_t list = align_up(static_cast<size_t>(count) * sizeof(unsigned));
     for (int k = 0; k < 2; ++k)
     {
-        w.keys[k] = at;
-        at += list;
-        w.order[k] = at;
-        at += list;
+        w.entries[k] = at;
+        at += align_up(static_cast<size_t>(count) * sizeof(uint2));
     }
     w.partials = at;
     w.bytes    = at + static_cast<size_t>(w.units) * 2 * cols * sizeof(float);
@@ -254,20 +261,15 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     p.unit       = w.unit;
     p.units      = w.units;
     p.blocks     = w.blocks;
-    for (int k = 0; k < 2; ++k)
-    {
-        p.keys[k]  = reinterpret_cast<unsigned *>(ws + w.keys[k]);
-        p.order[k] = reinterpret_cast<unsigned *>(ws + w.order[k]);
-    }
+    for (int k = 0; k < 2; ++k) p.entries[k] = reinterpret_cast<uint2 *>(ws + w.entries[k]);
     p.partials = reinterpret_cast<float *>(ws + w.partials);
     int bits = 1; // of the largest key, `rows`
     while (bits < 31 && (rows >> bits) != 0) ++bits;
     p.passes    = (bits + kSortMaxBits - 1) / kSortMaxBits;
     p.digitBits = (bits + p.passes - 1) / p.passes;
-    // as few threads as hold the indices kSortKeys at a time: the tables of counts are per warp
-    int threads = 256;
-    while (threads < kSortMaxThreads && static_cast<long long>(threads) * kSortKeys * kSortCtas < count) threads *= 2;
-    p.sortWarps  = threads / 32;
+    // as few warps as hold the indices kSortKeys at a time: each has a table of counts
+    p.sortWarps = 8;
+    while (p.sortWarps < kSortThreads / 32 && static_cast<long long>(p.sortWarps) * 32 * kSortKeys * kSortCtas < count) p.sortWarps *= 2;
     int clusters = 1;
     if (!p.accumulate)
     {
@@ -276,20 +278,19 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
         p.zeroWidth             = width.width;
         const long long rowSize = static_cast<long long>(p.cols) * row_elem_size(p.dtableType);
         // a cluster per 256 KB to clear, at most as many as fit on the GPU beside the one that sorts
-        clusters += static_cast<int>(std::max(1LL, std::min(16LL, rows * rowSize / (256 << 10))));
+        clusters += static_cast<int>(std::max(1LL, std::min(14LL, rows * rowSize / (256 << 10))));
         p.zeroCtas  = (clusters - 1) * kSortCtas;
         p.skipNamed = std::min(count, rows) * rowSize / p.zeroCtas > 2 * count * row_elem_size(p.indexType);
-        threads = kSortMaxThreads; // for those that clear
     }
-    const size_t smem = std::max(sort_smem_words(p.sortWarps * 32, 1 << p.digitBits), static_cast<size_t>(kZeroRows / 32)) * sizeof(unsigned);
+    const size_t smem = std::max(sort_smem_words(p.sortWarps, 1 << p.digitBits), static_cast<size_t>(kZeroRows / 32)) * sizeof(unsigned);
     static std::atomic<unsigned long long> raised{0};
-    if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(sort_smem_words(kSortMaxThreads, 1 << kSortMaxBits) * sizeof(unsigned)),
+    if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(sort_smem_words(kSortThreads / 32, 1 << kSortMaxBits) * sizeof(unsigned)),
                          raised)))
         return st;
     const unsigned long long jobs = static_cast<unsigned long long>(w.units) * w.blocks;
     if (jobs > 0x7fffffffull || w.blocks > 65535u)
         return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
-    embedding_sort_kernel<<<clusters * kSortCtas, threads, smem, stream>>>(p);
+    embedding_sort_kernel<<<clusters * kSortCtas, kSortThreads, smem, stream>>>(p);
     if ((st = check_launch("EmbeddingBackward")) || count == 0)
         return st;
     VecWidth width(p.cols);

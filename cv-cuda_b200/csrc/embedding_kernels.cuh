@@ -55,55 +55,92 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingKParams p
     store_vecs<W, U>(y, p.dstType, c0, span, p.cols, v);
 }
 
-// Rows of C elements (a palette's colours) that follow one another without gaps: a thread makes eight neighbouring elements of the
-// output, whichever rows they belong to, and stores them as one vector. SHARED: the table, times the scale, is copied to shared
-// memory first. Gathers bound this kernel: from L1 a warp's 32 addresses take a cycle per 128-byte line they touch (114 us for 16.6
-// million indices and a palette of 256 x 3 floats), from shared memory a cycle per clash of banks.
-constexpr int kShortTable = 8192; // floats of a table that is copied to shared memory
+// Rows of C elements (a palette's colours) that follow one another without gaps. A thread makes R rows, R * C elements of 16 * C
+// bytes in all (R = 8 for 16-bit elements, 4 for 32-bit ones), and the warp stores its 512 * C bytes from shared memory as whole
+// lines. SHARED: the table, times the scale, is copied to shared memory first: gathers from L1 take a cycle for each 128-byte line a
+// warp's addresses touch (114 us for 16.6 million indices and a palette of 256 x 3 floats), from shared memory one for each clash of
+// banks.
+constexpr int kShortTable = 4096; // floats of a table that is copied to shared memory
 
-template<int C, bool SHARED>
+template<int IT, int R>
+__device__ __forceinline__ void load_short_indices(const EmbeddingKParams &p, unsigned r0, int *id)
+{
+    typedef typename Index<IT>::type T;
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+    {
+        id[k] = -1;
+        if (r0 + k < p.count)
+        {
+            const long long v = *reinterpret_cast<const T *>(p.indices.at(r0 + k));
+            id[k]             = v >= 0 && v < p.rows ? static_cast<int>(v) : -1;
+        }
+    }
+}
+
+template<int C, int R, bool SHARED>
 __global__ void __launch_bounds__(256) embedding_short_rows_kernel(const EmbeddingKParams p)
 {
-    constexpr int                N = (C + 6) / C + 1; // rows that eight elements can lie in
-    extern __shared__ float      table[];
-    const unsigned long long     total = static_cast<unsigned long long>(p.count) * C;
+    extern __shared__ uint4  short_smem[]; // [8 warps][32 * C], then the table
+    float                   *table = reinterpret_cast<float *>(short_smem + 8 * 32 * C);
+    const int                lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint4                   *mine = short_smem + warp * (32 * C);
     if constexpr (SHARED)
     {
         for (int i = threadIdx.x; i < p.rows * C; i += 256)
             table[i] = load_elem(p.table.at(i / C), i % C, p.tableType) * p.scale;
         __syncthreads();
     }
-    for (unsigned long long tile = blockIdx.x * 2048ull; tile < total; tile += gridDim.x * 2048ull)
+    constexpr unsigned kWarpRows = 32 * R;
+    for (unsigned long long w0 = (static_cast<unsigned long long>(blockIdx.x) * 8 + warp) * kWarpRows; w0 < p.count;
+         w0 += static_cast<unsigned long long>(gridDim.x) * 8 * kWarpRows)
     {
-        const unsigned long long e0 = tile + threadIdx.x * 8;
-        if (e0 >= total)
-            break;
-        const unsigned r0 = static_cast<unsigned>(e0 / C);
-        const int      c0 = static_cast<int>(e0 - static_cast<unsigned long long>(r0) * C);
-        int            id[N];
-        const uint8_t *row[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) id[k] = r0 + k < p.count ? load_index(p.indices, p.indexType, r0 + k, p.rows) : -1;
-#pragma unroll
-        for (int k = 0; k < N; ++k) row[k] = SHARED ? nullptr : p.table.at(max(id[k], 0));
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-        {
-            // element c0 + i of the rows from r0 on
-            const bool over = c0 + i % C >= C;
-            const int  lo = i / C, hi = lo < N - 1 ? lo + 1 : N - 1;
-            const int  c = over ? c0 + i % C - C : c0 + i % C;
-            const int  n = over ? id[hi] : id[lo];
-            v[i]         = 0.0f;
-            if (n >= 0)
-                v[i] = SHARED ? table[n * C + c] : load_elem(over ? row[hi] : row[lo], c, p.tableType) * p.scale;
-        }
-        uint8_t *y = p.dst.base + e0 * (p.dstType == B200PP_F32 ? 4 : 2);
-        if (e0 + 8 <= total)
-            store_vecs<8, 1>(y, p.dstType, 0, 8, 8, v);
+        const unsigned r0 = static_cast<unsigned>(w0) + lane * R;
+        int            id[R];
+        if (p.indexType == B200PP_U8)
+            load_short_indices<B200PP_U8, R>(p, r0, id);
+        else if (p.indexType == B200PP_S32)
+            load_short_indices<B200PP_S32, R>(p, r0, id);
         else
-            store_vecs<1, 8>(y, p.dstType, 0, 1, static_cast<int>(total - e0), v);
+            load_short_indices<B200PP_S64, R>(p, r0, id);
+        float v[R * C];
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+        {
+            const uint8_t *row = SHARED ? nullptr : p.table.at(max(id[k], 0));
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+            {
+                v[k * C + c] = 0.0f;
+                if (id[k] >= 0)
+                    v[k * C + c] = SHARED ? table[id[k] * C + c] : load_elem(row, c, p.tableType) * p.scale;
+            }
+        }
+        __syncwarp(); // the lines of the turn before are stored
+        uint8_t *to = reinterpret_cast<uint8_t *>(mine + lane * C);
+        if constexpr (R == 4)
+        {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                mine[lane * C + i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                                __float_as_uint(v[4 * i + 3]));
+        }
+        else
+            store_vecs<8, C>(to, p.dstType, 0, 8, 8 * C, v);
+        __syncwarp();
+        constexpr int kElem = 16 / R; // bytes: 2 or 4
+        uint8_t      *y     = p.dst.base + w0 * (C * kElem);
+        if (w0 + kWarpRows <= p.count)
+        {
+#pragma unroll
+            for (int i = 0; i < C; ++i) reinterpret_cast<uint4 *>(y)[i * 32 + lane] = mine[i * 32 + lane];
+        }
+        else
+        {
+            const int bytes = static_cast<int>(p.count - w0) * (C * kElem);
+            for (int i = lane * 2; i < bytes; i += 64)
+                *reinterpret_cast<unsigned short *>(y + i) = *reinterpret_cast<unsigned short *>(reinterpret_cast<uint8_t *>(mine) + i);
+        }
     }
 }
 
@@ -116,7 +153,7 @@ struct EmbeddingGradKParams
     float     scale;
     int       accumulate;
     int       padding;            // -1: none
-    unsigned *keys[2], *order[2]; // count entries each; the sorted ones are keys[0], order[0]
+    uint2    *entries[2];         // (index, position), count each; entries[0] holds the sorted ones
     int       passes, digitBits, sortWarps;
     int       zeroCtas, zeroWidth, skipNamed; // CTAs that clear the table, their vector width, whether they leave out named rows
     float    *partials;                       // [units][2][cols]
@@ -129,18 +166,17 @@ struct EmbeddingGradKParams
 //
 // Cluster 0 sorts: a least-significant-digit radix sort over kSortCtas CTAs. Each warp owns a contiguous range of the positions and
 // counts its digits in a table of its own; a prefix over the warps, the CTAs (through distributed shared memory) and the digits
-// turns the counts into the places each warp writes to. Within a warp, lanes with equal digits find one another with a match
-// instruction, so the order is that of the positions. The arrays between the passes are in global memory (they stay in L2); the
+// turns the counts into the places each warp writes to. The arrays between the passes are in global memory (they stay in L2); the
 // cluster barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and most counts of
 // indices are small; clearing the table, which takes longer for the usual sizes, hides it.
 constexpr int kSortCtas       = 8;
-constexpr int kSortMaxThreads = 1024;
+constexpr int kSortThreads    = 1024;
 constexpr int kSortMaxBits    = 10;
 constexpr int kSortKeys       = 8; // keys a lane holds at a time
 
-inline size_t sort_smem_words(int threads, int bins)
+inline size_t sort_smem_words(int warps, int bins)
 {
-    return static_cast<size_t>(bins) * (threads / 32) + bins + 32;
+    return static_cast<size_t>(bins) * warps + bins + 32;
 }
 
 __device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, unsigned *smem)
@@ -164,29 +200,24 @@ __device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, un
 
     for (int pass = 0; pass < p.passes; ++pass)
     {
-        const int       to    = (p.passes - 1 - pass) & 1; // the last pass writes to array 0
-        const unsigned *keys  = p.keys[to ^ 1];
-        const unsigned *order = p.order[to ^ 1];
-        const int       shift = pass * p.digitBits;
-        unsigned        key[kSortKeys], pos[kSortKeys];
-        auto            load = [&](unsigned tile) {
+        const int    to    = (p.passes - 1 - pass) & 1; // the last pass writes to array 0
+        const uint2 *from  = p.entries[to ^ 1];
+        const int    shift = pass * p.digitBits;
+        uint2        entry[kSortKeys];
+        auto         load = [&](unsigned tile) {
 #pragma unroll
             for (int k = 0; k < kSortKeys; ++k)
             {
                 const unsigned i = tile + 32 * k + lane;
-                key[k] = pos[k] = 0;
+                entry[k]         = make_uint2(0, 0);
                 if (i < i1)
                 {
                     if (pass > 0)
-                    {
-                        key[k] = keys[i];
-                        pos[k] = order[i];
-                    }
+                        entry[k] = from[i];
                     else
                     {
                         const int id = load_index(p.indices, p.indexType, i, p.rows);
-                        key[k]       = static_cast<unsigned>(id < 0 || id == p.padding ? p.rows : id);
-                        pos[k]       = i;
+                        entry[k]     = make_uint2(static_cast<unsigned>(id < 0 || id == p.padding ? p.rows : id), i);
                     }
                 }
             }
@@ -199,86 +230,92 @@ __device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, un
 #pragma unroll
             for (int k = 0; k < kSortKeys; ++k)
                 if (tile + 32 * k + lane < i1)
-                    atomicAdd(mine + ((key[k] >> shift) & (bins - 1)), 1u); // counts: their order does not matter
+                    atomicAdd(mine + ((entry[k].x >> shift) & (bins - 1)), 1u); // counts: their order does not matter
         }
         __syncthreads();
-        // counts of the digit over the warps before each, and over all
-        for (int b = threadIdx.x; b < bins; b += threads)
+        // thread b: digit b (there are at most as many as threads). Its counts over the warps before each, and over all
+        const bool has = static_cast<int>(threadIdx.x) < bins;
+        unsigned  *col = hist + threadIdx.x;
+        if (has)
         {
             unsigned sum = 0;
+#pragma unroll 8
             for (int w = 0; w < warps; ++w)
             {
-                const unsigned n   = hist[w * bins + b];
-                hist[w * bins + b] = sum;
+                const unsigned n = col[w * bins];
+                col[w * bins]    = sum;
                 sum += n;
             }
-            total[b] = sum;
+            total[threadIdx.x] = sum;
         }
         cluster.sync();
-        // where each digit of this CTA starts: the digits below it everywhere, and its own in the CTAs before
-        unsigned below = 0; // of the digits this thread does not see (those before its stretch of bins / threads)
+        // where the digit starts for this CTA: the digits below it everywhere, and its own in the CTAs before
+        unsigned before = 0, all = 0;
+        if (has)
         {
-            const int per = (bins + threads - 1) / threads, b0 = min(bins, static_cast<int>(threadIdx.x) * per), b1 = min(bins, b0 + per);
-            unsigned  all = 0;
-            for (int b = b0; b < b1; ++b)
-                for (unsigned c = 0; c < kSortCtas; ++c) all += cluster.map_shared_rank(total, c)[b];
-            unsigned incl = all;
+            unsigned n[kSortCtas];
+#pragma unroll
+            for (int c = 0; c < kSortCtas; ++c) n[c] = cluster.map_shared_rank(total, c)[threadIdx.x];
+#pragma unroll
+            for (int c = 0; c < kSortCtas; ++c)
+            {
+                before += c < static_cast<int>(rank) ? n[c] : 0;
+                all += n[c];
+            }
+        }
+        unsigned incl = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
+            incl += lane >= o ? up : 0;
+        }
+        if (lane == 31)
+            wsum[warp] = incl;
+        __syncthreads();
+        if (warp == 0)
+        {
+            unsigned v = lane < threads >> 5 ? wsum[lane] : 0;
+#pragma unroll
             for (int o = 1; o < 32; o <<= 1)
             {
-                const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
-                incl += lane >= o ? up : 0;
+                const unsigned up = __shfl_up_sync(0xffffffffu, v, o);
+                v += lane >= o ? up : 0;
             }
-            if (lane == 31)
-                wsum[warp] = incl;
-            __syncthreads();
-            if (warp == 0)
-            {
-                unsigned v = lane < threads >> 5 ? wsum[lane] : 0;
-                for (int o = 1; o < 32; o <<= 1)
-                {
-                    const unsigned up = __shfl_up_sync(0xffffffffu, v, o);
-                    v += lane >= o ? up : 0;
-                }
-                wsum[lane] = v;
-            }
-            __syncthreads();
-            below = incl - all + (warp > 0 ? wsum[warp - 1] : 0);
-            for (int b = b0; b < b1; ++b)
-            {
-                unsigned before = 0, here = 0;
-                for (unsigned c = 0; c < kSortCtas; ++c)
-                {
-                    const unsigned n = cluster.map_shared_rank(total, c)[b];
-                    before += c < rank ? n : 0;
-                    here += n;
-                }
-                for (int w = 0; w < warps; ++w) hist[w * bins + b] += below + before;
-                below += here;
-            }
+            wsum[lane] = v;
+        }
+        __syncthreads();
+        if (has)
+        {
+            const unsigned base = incl - all + (warp > 0 ? wsum[warp - 1] : 0) + before;
+#pragma unroll 8
+            for (int w = 0; w < warps; ++w) col[w * bins] += base;
         }
         __syncthreads();
         for (unsigned tile = i0; tile < i1; tile += kTile)
         {
             if (i1 - i0 > kTile)
-                load(tile); // otherwise the keys are still there
+                load(tile); // otherwise the entries are still there
+            // lanes with the same digit find one another; the first of them takes as many places as they are. The barriers of the
+            // warp keep the steps' atomics in order; their results are not waited for until all are under way.
+            unsigned same[kSortKeys], place[kSortKeys];
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k)
+                same[k] = __match_any_sync(0xffffffffu, tile + 32 * k + lane < i1 ? (entry[k].x >> shift) & (bins - 1) : bins);
 #pragma unroll
             for (int k = 0; k < kSortKeys; ++k)
             {
-                if (tile + 32 * k >= i1)
-                    break;
-                const bool     in    = tile + 32 * k + lane < i1;
-                const unsigned digit = in ? (key[k] >> shift) & (bins - 1) : bins;
-                const unsigned same  = __match_any_sync(0xffffffffu, digit);
-                if (in)
-                {
-                    const unsigned at = mine[digit] + __popc(same & ((1u << lane) - 1));
-                    p.keys[to][at]    = key[k];
-                    p.order[to][at]   = pos[k];
-                }
+                place[k] = 0;
+                if (tile + 32 * k + lane < i1 && lane == __ffs(same[k]) - 1)
+                    place[k] = atomicAdd(mine + ((entry[k].x >> shift) & (bins - 1)), static_cast<unsigned>(__popc(same[k])));
                 __syncwarp();
-                if (in && lane == __ffs(same) - 1)
-                    mine[digit] += __popc(same);
-                __syncwarp();
+            }
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k)
+            {
+                const unsigned at = __shfl_sync(0xffffffffu, place[k], __ffs(same[k]) - 1) + __popc(same[k] & ((1u << lane) - 1));
+                if (tile + 32 * k + lane < i1)
+                    p.entries[to][at] = entry[k];
             }
         }
         cluster.sync(); // the next pass reads what this one wrote; also keeps `total` until every CTA has read it
@@ -347,7 +384,7 @@ __device__ __forceinline__ void embedding_clear(const EmbeddingGradKParams &p, u
     }
 }
 
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortMaxThreads, 1)
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1)
     embedding_sort_kernel(const EmbeddingGradKParams p)
 {
     extern __shared__ unsigned smem[];
@@ -362,7 +399,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortMaxThre
 // by unit into `partials` -- slot 0: the run comes from the unit before, slot 1: it starts here -- and joined by the third kernel.
 constexpr int kShortRun  = 32;
 constexpr int kGradCols  = 256; // eight per lane
-constexpr int kGradAhead = 8;   // rows loaded before the first is added
+constexpr int kGradAhead = 4;   // rows loaded before the first is added
 
 // Puts a lane's eight sums where they belong: into `partial` or, if that is null, into the table. Not inlined: it would be there
 // once for each of the rows a warp has in flight, and code that runs once is as slow as it can be fetched (7 times slower for
@@ -393,7 +430,7 @@ __device__ __noinline__ void embedding_grad_put(const EmbeddingGradKParams &p, f
 }
 
 template<int GRAD, int W>
-__global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const __grid_constant__ EmbeddingGradKParams p)
+__global__ void __launch_bounds__(256, 3) embedding_grad_runs_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
     constexpr int            V    = 8 / W;
     constexpr unsigned       kAll = 0xffffffffu;
@@ -408,11 +445,11 @@ __global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const __grid_c
     const unsigned none = static_cast<unsigned>(p.rows);
     // keys of the 32 positions before the unit (lane l: i0 - 1 - l), of the 32 from its start on and of the 32 after those
     const unsigned  i   = i0 + lane;
-    const unsigned  bk  = static_cast<unsigned>(lane) < i0 ? p.keys[0][i0 - 1 - lane] : none;
-    const unsigned  k0  = i < p.count ? p.keys[0][i] : none;
-    const unsigned  k1  = i + 32u < p.count ? p.keys[0][i + 32] : none;
-    const unsigned  o0  = i < p.count ? p.order[0][i] : 0;
-    const unsigned  o1  = i + 32u < p.count ? p.order[0][i + 32] : 0;
+    const unsigned  bk  = static_cast<unsigned>(lane) < i0 ? p.entries[0][i0 - 1 - lane].x : none;
+    const unsigned  k0  = i < p.count ? p.entries[0][i].x : none;
+    const unsigned  k1  = i + 32u < p.count ? p.entries[0][i + 32].x : none;
+    const unsigned  o0  = i < p.count ? p.entries[0][i].y : 0;
+    const unsigned  o1  = i + 32u < p.count ? p.entries[0][i + 32].y : 0;
     const unsigned  key = __shfl_sync(kAll, k0, 0);
     if (key == none)
         return;
@@ -514,13 +551,13 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
         if (u + 1 < p.units) // not the last unit, so it is full
         {
             const unsigned first = u * p.unit;
-            const unsigned mine  = p.keys[0][min(first + lane, p.count - 1)]; // the unit after this one has a position at least
-            const unsigned prev  = first > 0 ? p.keys[0][first - 1] : none;
-            const unsigned last = __shfl_sync(kAll, mine, p.unit - 1), after = p.keys[0][first + p.unit];
+            const unsigned mine  = p.entries[0][min(first + lane, p.count - 1)].x; // the unit after this one has a position at least
+            const unsigned prev  = first > 0 ? p.entries[0][first - 1].x : none;
+            const unsigned last = __shfl_sync(kAll, mine, p.unit - 1), after = p.entries[0][first + p.unit].x;
             const unsigned same  = __ballot_sync(kAll, mine == last);
             const unsigned start = first + __ffs(same) - 1;
             if (last != none && after == last && !(start == first && prev == last) && start + kShortRun < p.count
-                && p.keys[0][start + kShortRun] == last)
+                && p.entries[0][start + kShortRun].x == last)
                 k = last;
         }
         if (lane == 0)
@@ -536,7 +573,7 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
         for (;;)
         {
             const unsigned long long at = (static_cast<unsigned long long>(u) + 1 + more + lane) * p.unit;
-            const unsigned           on = __ballot_sync(kAll, at < p.count && p.keys[0][at] == k);
+            const unsigned           on = __ballot_sync(kAll, at < p.count && p.entries[0][at].x == k);
             more += on == kAll ? 32 : __ffs(~on) - 1;
             if (on != kAll)
                 break;

@@ -118,6 +118,7 @@ extern "C" int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, con
     p.biasType   = op->biasType;
     p.epsilon    = op->epsilon;
     p.fcols      = static_cast<float>(p.cols);
+    p.invCols    = 1.0f / p.fcols;
     p.mean       = op->mean;
     p.rstd       = op->rstd;
     p.chunks     = static_cast<unsigned>(chunks);

@@ -20,14 +20,20 @@ GradPlan plan_layernorm_grad(long long rows, long long cols)
     GradPlan g{};
     if (cols <= 8192)
     {
-        g.values = cols <= 4096 ? 8 : 16;
-        if (cols <= 256)
-            for (g.threads = 4; g.threads * 8 < cols;) g.threads *= 2;
+        // a warp per row, or part of one, up to 768 columns; above, whole warps with sixteen values per thread
+        if (cols <= 768)
+        {
+            g.values = cols <= 256 ? 8 : cols <= 512 ? 16 : 24;
+            for (g.threads = 4; g.threads < 32 && g.threads * 8 < cols;) g.threads *= 2;
+        }
         else
-            g.threads = static_cast<int>((cols + 32 * g.values - 1) / (32 * g.values) * 32);
+        {
+            g.values  = 16;
+            g.threads = static_cast<int>((cols + 511) / 512 * 32);
+        }
         g.groups              = std::max(1, 256 / g.threads);
         const long long turns = (rows + g.groups - 1) / g.groups;
-        const int       ctas  = kSms * std::max(1, (g.values == 8 ? kGradResident8 : kGradResident16) / (g.threads * g.groups));
+        const int       ctas  = kSms * std::max(1, kGradResident / (g.threads * g.groups));
         g.parts               = static_cast<int>(std::max(1LL, std::min<long long>(turns, ctas)));
         return g;
     }
@@ -46,10 +52,12 @@ void launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStrea
 {
     const dim3 block(g.threads, g.groups);
     const int  smem = p.partials && g.groups > 1 ? 2 * p.cols * static_cast<int>(sizeof(float)) : 0;
-    if (g.threads <= 32)
+    if (g.values == 8)
         layernorm_grad_kernel<SRC, GRAD, 8, W, false><<<p.parts, block, smem, stream>>>(p);
-    else if (g.values == 8)
-        layernorm_grad_kernel<SRC, GRAD, 8, W, true><<<p.parts, block, smem, stream>>>(p);
+    else if (g.values == 24)
+        layernorm_grad_kernel<SRC, GRAD, 24, W, false><<<p.parts, block, smem, stream>>>(p);
+    else if (g.threads == 32)
+        layernorm_grad_kernel<SRC, GRAD, 16, W, false><<<p.parts, block, smem, stream>>>(p);
     else
         layernorm_grad_kernel<SRC, GRAD, 16, W, true><<<p.parts, block, smem, stream>>>(p);
 }
@@ -171,6 +179,7 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     p.mean        = op->mean;
     p.rstd        = op->rstd;
     p.fcols       = static_cast<float>(p.cols);
+    p.invCols     = 1.0f / p.fcols;
     p.dweight     = static_cast<uint8_t *>(op->dweight);
     p.dbias       = static_cast<uint8_t *>(op->dbias);
     if (rows == 0)

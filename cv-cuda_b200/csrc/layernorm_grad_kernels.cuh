@@ -18,122 +18,124 @@ struct LayerNormGradKParams
     int            gradType, dsrcType, weightType, dweightType, dbiasType;
     const uint8_t *weight;
     const float   *mean, *rstd;
-    float          fcols;
+    float          fcols, invCols;
     uint8_t       *dweight, *dbias;
     float         *partials; // [parts][2][cols]
     int            parts;
 };
 
 // Rows that fit into registers, all gradients in one pass over the data. blockDim.x threads per row (BLOCK: whole warps, otherwise
-// part of one), blockDim.y rows per CTA at a time. A CTA walks down its share of the rows; each thread keeps its columns of the
-// weight and of the sums over the rows in registers, and loads its part of the next row before it works on the present one.
-constexpr int kGradResident8  = 768; // threads that fit on an SM, by the registers per thread the launch bound leaves (80)
-constexpr int kGradResident16 = 512; // (128)
+// a warp, or part of one for eight values a lane), blockDim.y rows per CTA at a time. A CTA walks down its share of the rows; each
+// thread keeps its columns of the sums over the rows in registers. What a row costs besides its values -- addresses, shuffles, the
+// barrier -- is why a thread has up to 24 values: with eight (and the next row loaded ahead) 50176 rows of 768 bfloat16 took 62 us.
+constexpr int kGradResident = 512; // threads that fit on an SM, by the registers per thread the launch bound leaves (128)
 
 template<int SRC, int GRAD, int E, int W, bool BLOCK>
-__global__ void __launch_bounds__(E == 8 ? kGradResident8 : kGradResident16) layernorm_grad_kernel(const LayerNormGradKParams p)
+__global__ void __launch_bounds__(BLOCK ? kGradResident : 256, BLOCK ? 1 : 2) layernorm_grad_kernel(const LayerNormGradKParams p)
 {
-    constexpr int           V     = E / W;
-    constexpr bool          AHEAD = E == 8 && W >= 4; // otherwise there are no registers left for the next row
-    __shared__ float2       scratch[2][16]; // two halves, used in turn: one barrier per row
-    extern __shared__ float sums[];         // [2][cols]
-    const int               t = threadIdx.x, threads = blockDim.x, g = threadIdx.y, groups = blockDim.y;
-    const int               tid = g * threads + t, warp = tid >> 5;
+    constexpr int              V = E / W;
+    __shared__ float2          scratch[2][16]; // two halves, used in turn: one barrier per row
+    extern __shared__ float    sums[];         // [2][cols]
+    const int                  t = threadIdx.x, threads = !BLOCK && E > 8 ? 32 : blockDim.x, g = threadIdx.y, groups = blockDim.y;
+    const int                  tid = g * threads + t, warp = tid >> 5;
     const RowSpan<E, W, BLOCK> at(t);
-    float                   w[E], dw[E], db[E];
+    f32x2                      dw[E / 2], db[E / 2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = 1.0f, dw[e] = 0.0f, db[e] = 0.0f;
-    if (p.weight)
-        load_vecs<W, V>(p.weight, p.weightType, at.c, at.step, p.cols, w);
-    Vec<SRC, W>  xr[V];
-    Vec<GRAD, W> gr[V];
-    float        mean = 0.0f, rstd = 0.0f;
-    auto         fetch = [&](unsigned long long r) {
-        mean = rstd = 0.0f; // a row that is not there, and what lies behind a row's end: h = 0 and dy = 0
-        const int end = r < p.rows ? p.cols : 0;
-        const uint8_t *x = nullptr, *dy = nullptr;
-        if (end)
-        {
-            x    = p.src.at(static_cast<unsigned>(r)) + static_cast<long long>(at.c) * kElemBytes<SRC>;
-            dy   = p.grad.at(static_cast<unsigned>(r)) + static_cast<long long>(at.c) * kElemBytes<GRAD>;
-            mean = p.mean[r];
-            rstd = p.rstd[r];
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-        {
-            xr[v] = zero_raw<kElemBytes<SRC> * W>();
-            gr[v] = zero_raw<kElemBytes<GRAD> * W>();
-            if (at.c + v * at.step < end)
-            {
-                xr[v] = load_raw<kElemBytes<SRC> * W>(x + v * at.step * kElemBytes<SRC>);
-                gr[v] = load_raw<kElemBytes<GRAD> * W>(dy + v * at.step * kElemBytes<GRAD>);
-            }
-        }
-    };
+    for (int i = 0; i < E / 2; ++i) dw[i] = db[i] = both(0.0f);
     const unsigned long long step = static_cast<unsigned long long>(gridDim.x) * groups;
     unsigned long long       r    = static_cast<unsigned long long>(blockIdx.x) * groups + g;
     int                      half = 0;
-    if (AHEAD)
-        fetch(r);
     // every thread of the CTA takes the same number of turns
-    for (unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * groups; first < p.rows; first += step)
+    for (unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * groups; first < p.rows; first += step, r += step)
     {
-        if (!AHEAD)
-            fetch(r);
-        float       h[E], gv[E], s1 = 0.0f, s2 = 0.0f;
-        const float rs = rstd;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
+        const bool     live = r < p.rows;
+        const int      end  = live ? p.cols : 0; // a row that is not there, and what lies behind a row's end: x = dy = 0
+        const unsigned row  = live ? static_cast<unsigned>(r) : 0;
+        const float    mean = live ? p.mean[row] : 0.0f, rstd = live ? p.rstd[row] : 0.0f;
+        f32x2          h[E / 2], gv[E / 2], s1 = both(0.0f), s2 = both(0.0f);
         {
-            unpack<SRC, W>(xr[v], h + v * W);
-            unpack<GRAD, W>(gr[v], gv + v * W);
+            Vec<SRC, W>    xr[V];
+            Vec<GRAD, W>   gr[V];
+            const uint8_t *x = p.src.at(row), *dy = p.grad.at(row);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+            {
+                const int c = at.c + v * at.step;
+                xr[v]       = zero_raw<kElemBytes<SRC> * W>();
+                gr[v]       = zero_raw<kElemBytes<GRAD> * W>();
+                if (c < end)
+                {
+                    xr[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
+                    gr[v] = load_raw<kElemBytes<GRAD> * W>(dy + static_cast<long long>(c) * kElemBytes<GRAD>);
+                }
+            }
+            float f[E];
+#pragma unroll
+            for (int v = 0; v < V; ++v) unpack<SRC, W>(xr[v], f + v * W);
+            pairs<E>(f, h);
+#pragma unroll
+            for (int v = 0; v < V; ++v) unpack<GRAD, W>(gr[v], f + v * W);
+            pairs<E>(f, gv);
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int i = 0; i < E / 2; ++i)
         {
-            h[e]  = (h[e] - mean) * rs;
-            db[e] += gv[e];
-            dw[e] = fmaf(gv[e], h[e], dw[e]);
-            gv[e] *= w[e];
-            s1 += gv[e];
-            s2 = fmaf(gv[e], h[e], s2);
+            h[i]  = mul2(add2(h[i], both(-mean)), both(rstd));
+            db[i] = add2(db[i], gv[i]);
+            dw[i] = fma2(gv[i], h[i], dw[i]);
         }
-        const unsigned long long now = r;
-        r += step;
-        if (AHEAD)
-            fetch(r);
         if (!p.dsrc.base)
             continue;
+        if (p.weight) // from L1: there are no registers to keep it
+        {
+#pragma unroll
+            for (int k = 0; k < E / 8; ++k)
+            {
+                float f[8];
+                f32x2 w[4];
+                load_vecs<W, 8 / W>(p.weight, p.weightType, at.c + 8 / W * k * at.step, at.step, p.cols, f);
+                pairs<8>(f, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gv[4 * k + i] = mul2(gv[4 * k + i], w[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i)
+        {
+            s1 = add2(s1, gv[i]);
+            s2 = fma2(gv[i], h[i], s2);
+        }
+        float t1 = lo2(s1) + hi2(s1), t2 = lo2(s2) + hi2(s2);
         if constexpr (BLOCK)
         {
-            s1 = warp_sum(s1);
-            s2 = warp_sum(s2);
+            t1 = warp_sum(t1);
+            t2 = warp_sum(t2);
             if ((t & 31) == 0)
-                scratch[half][warp] = make_float2(s1, s2);
+                scratch[half][warp] = make_float2(t1, t2);
             __syncthreads();
-            s1 = s2 = 0.0f;
+            t1 = t2 = 0.0f;
             for (int k = 0; k < threads >> 5; ++k)
             {
                 const float2 o = scratch[half][g * (threads >> 5) + k];
-                s1 += o.x;
-                s2 += o.y;
+                t1 += o.x;
+                t2 += o.y;
             }
             half ^= 1;
         }
         else
             for (int o = threads >> 1; o > 0; o >>= 1)
             {
-                s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-                s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+                t1 += __shfl_xor_sync(0xffffffffu, t1, o);
+                t2 += __shfl_xor_sync(0xffffffffu, t2, o);
             }
-        if (now >= p.rows)
+        if (!live)
             continue;
-        const float c1 = s1 / p.fcols, c2 = s2 / p.fcols;
-        uint8_t    *dx = p.dsrc.at(static_cast<unsigned>(now));
+        const float c1 = t1 * p.invCols, c2 = t2 * p.invCols;
+        float       f[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) gv[e] = rs * (gv[e] - c1 - h[e] * c2);
-        store_vecs<W, V>(dx, p.dsrcType, at.c, at.step, p.cols, gv);
+        for (int i = 0; i < E / 2; ++i) gv[i] = mul2(add2(fma2(h[i], both(-c2), gv[i]), both(-c1)), both(rstd));
+        singles<E>(gv, f);
+        store_vecs<W, V>(p.dsrc.at(row), p.dsrcType, at.c, at.step, p.cols, f);
     }
     if (!p.partials)
         return;
@@ -141,14 +143,17 @@ __global__ void __launch_bounds__(E == 8 ? kGradResident8 : kGradResident16) lay
     float    *part  = p.partials + static_cast<long long>(blockIdx.x) * 2 * p.cols;
     int       slot  = g, slots = groups;
     bool      holds = true;
+    float     fw[E], fb[E];
+    singles<E>(dw, fw);
+    singles<E>(db, fb);
     if constexpr (!BLOCK)
     {
         for (int o = threads; o < 32; o <<= 1)
 #pragma unroll
             for (int e = 0; e < E; ++e)
             {
-                dw[e] += __shfl_xor_sync(0xffffffffu, dw[e], o);
-                db[e] += __shfl_xor_sync(0xffffffffu, db[e], o);
+                fw[e] += __shfl_xor_sync(0xffffffffu, fw[e], o);
+                fb[e] += __shfl_xor_sync(0xffffffffu, fb[e], o);
             }
         slot  = warp;
         slots = (threads * groups) >> 5;
@@ -165,8 +170,8 @@ __global__ void __launch_bounds__(E == 8 ? kGradResident8 : kGradResident16) lay
                 const int c = at.c + e / W * at.step + e % W;
                 if (c < p.cols)
                 {
-                    to[c]          = s > 0 ? sums[c] + dw[e] : dw[e];
-                    to[p.cols + c] = s > 0 ? sums[p.cols + c] + db[e] : db[e];
+                    to[c]          = s > 0 ? sums[c] + fw[e] : fw[e];
+                    to[p.cols + c] = s > 0 ? sums[p.cols + c] + fb[e] : fb[e];
                 }
             }
         }

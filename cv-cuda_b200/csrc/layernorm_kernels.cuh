@@ -16,7 +16,7 @@ struct LayerNormKParams
     int            cols;
     int            dstType, weightType, biasType;
     const uint8_t *weight, *bias;
-    float          epsilon, fcols; // fcols: the number of columns
+    float          epsilon, fcols, invCols; // the number of columns and its reciprocal
     float         *mean, *rstd;
     unsigned       chunks;   // of a long row
     float2        *partials; // [rows][chunks]
@@ -60,66 +60,117 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *scratch)
 
 // Weights and biases of eight values (1 and 0 where there are none).
 template<int W>
-__device__ __forceinline__ void layernorm_affine(const LayerNormKParams &p, int c, int step, int end, float *w, float *b)
+__device__ __forceinline__ void layernorm_affine(const LayerNormKParams &p, int c, int step, int end, f32x2 *w, f32x2 *b)
 {
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 1.0f, b[i] = 0.0f;
+    for (int i = 0; i < 4; ++i) w[i] = both(1.0f), b[i] = both(0.0f);
     if (p.weight)
-        load_vecs<W, 8 / W>(p.weight, p.weightType, c, step, end, w);
+    {
+        load_vecs<W, 8 / W>(p.weight, p.weightType, c, step, end, v);
+        pairs<8>(v, w);
+    }
     if (p.bias)
-        load_vecs<W, 8 / W>(p.bias, p.biasType, c, step, end, b);
+    {
+        load_vecs<W, 8 / W>(p.bias, p.biasType, c, step, end, v);
+        pairs<8>(v, b);
+    }
+}
+
+// y of eight values, given their distances d to the mean.
+template<int W>
+__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const f32x2 *d, float rstd, const f32x2 *w,
+                                                const f32x2 *b, int c, int step, int end)
+{
+    f32x2 o[4];
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = fma2(mul2(d[i], both(rstd)), w[i], b[i]);
+    singles<8>(o, v);
+    store_vecs<W, 8 / W>(y, p.dstType, c, step, end, v);
 }
 
 // y of a thread's values, eight at a time.
 template<int E, int W>
-__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const float *x, float mean, float rstd, int c,
-                                                int step, int end)
+__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const f32x2 *d, float rstd, int c, int step, int end)
 {
 #pragma unroll
     for (int k = 0; k < E / 8; ++k, c += 8 / W * step)
     {
-        float w[8], b[8];
+        f32x2 w[4], b[4];
         layernorm_affine<W>(p, c, step, end, w, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = fmaf((x[k * 8 + i] - mean) * rstd, w[i], b[i]);
-        store_vecs<W, 8 / W>(y, p.dstType, c, step, end, b);
+        layernorm_store<W>(p, y, d + 4 * k, rstd, w, b, c, step, end);
     }
 }
 
-// Forward, rows that fit into registers. BLOCK: one CTA per row; otherwise blockDim.x lanes of a warp per row and
-// blockDim.y rows per CTA. The statistics come from the registers (the variance about the mean), so the row is read once.
+// Sum of a thread's values; the values that lie behind the row's end are zero.
+template<int E>
+__device__ __forceinline__ float sum_pairs(const f32x2 *x)
+{
+    f32x2 a = x[0], b = x[1];
+#pragma unroll
+    for (int i = 2; i < E / 2; i += 2)
+    {
+        a = add2(a, x[i]);
+        b = add2(b, x[i + 1]);
+    }
+    a = add2(a, b);
+    return lo2(a) + hi2(a);
+}
+
+// Replaces a thread's values by their distances to the mean (0 behind the row's end) and gives the sum of the squares.
+template<int E, int W>
+__device__ __forceinline__ float centre(f32x2 *x, float mean, int c, int step, int end)
+{
+    if (c + (E / W - 1) * step >= end) // part of them lies behind the end
+    {
+        float v[E];
+        singles<E>(x, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (c + e / W * step >= end)
+                v[e] = mean;
+        pairs<E>(v, x);
+    }
+    f32x2 a = both(0.0f), b = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < E / 2; i += 2)
+    {
+        x[i]     = add2(x[i], both(-mean));
+        x[i + 1] = add2(x[i + 1], both(-mean));
+        a        = fma2(x[i], x[i], a);
+        b        = fma2(x[i + 1], x[i + 1], b);
+    }
+    a = add2(a, b);
+    return lo2(a) + hi2(a);
+}
+
+// Forward, rows that fit into registers. BLOCK: one CTA per row; otherwise blockDim.x lanes of a warp per row (32 for more than
+// eight values a lane) and blockDim.y rows per CTA. The statistics come from the registers (the variance about the mean), so the
+// row is read once.
 template<int SRC, int E, int W, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? (E <= 16 ? 512 : 1024) : 256) layernorm_kernel(const LayerNormKParams p)
 {
     __shared__ float scratch[2][32];
-    const int        t = threadIdx.x, threads = blockDim.x;
+    const int        t = threadIdx.x, threads = !BLOCK && E > 8 ? 32 : blockDim.x;
     const unsigned   r = BLOCK ? blockIdx.x : blockIdx.x * blockDim.y + threadIdx.y;
     if (!BLOCK && r - threadIdx.y % (32u / threads) >= p.rows) // all rows of the warp
         return;
     const bool                 live = BLOCK || r < p.rows;
     const RowSpan<E, W, BLOCK> at(t);
-    float                      xv[E], s = 0.0f;
-    load_vecs<SRC, W, E / W>(p.src.at(live ? r : p.rows - 1), at.c, at.step, p.cols, xv);
+    f32x2                      x[E / 2];
+    {
+        float v[E];
+        load_vecs<SRC, W, E / W>(p.src.at(live ? r : p.rows - 1), at.c, at.step, p.cols, v);
+        pairs<E>(v, x);
+    }
     // with eight values there are registers left to fetch the weights at the same time as the row
-    float w[8], b[8];
+    f32x2 w[4], b[4];
     if constexpr (E == 8)
         layernorm_affine<W>(p, at.c, at.step, p.cols, w, b);
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += xv[e];
-    const float mean = row_sum<BLOCK>(s, threads, scratch[0]) / p.fcols;
-    float       q    = 0.0f;
-#pragma unroll
-    for (int v = 0; v < E / W; ++v)
-        if (at.c + v * at.step < p.cols)
-        {
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-            {
-                const float d = xv[v * W + i] - mean;
-                q             = fmaf(d, d, q);
-            }
-        }
-    const float rstd = 1.0f / sqrtf(row_sum<BLOCK>(q, threads, scratch[1]) / p.fcols + p.epsilon);
+    const float mean = divide_count(row_sum<BLOCK>(sum_pairs<E>(x), threads, scratch[0]), p.fcols, p.invCols);
+    const float q    = centre<E, W>(x, mean, at.c, at.step, p.cols);
+    const float rstd = rsqrtf(row_sum<BLOCK>(q, threads, scratch[1]) * p.invCols + p.epsilon);
     if (!live)
         return;
     if (t == 0)
@@ -130,13 +181,9 @@ __global__ void __launch_bounds__(BLOCK ? (E <= 16 ? 512 : 1024) : 256) layernor
             p.rstd[r] = rstd;
     }
     if constexpr (E == 8)
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = fmaf((xv[i] - mean) * rstd, w[i], b[i]);
-        store_vecs<W, 8 / W>(p.dst.at(r), p.dstType, at.c, at.step, p.cols, b);
-    }
+        layernorm_store<W>(p, p.dst.at(r), x, rstd, w, b, at.c, at.step, p.cols);
     else
-        layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, at.c, at.step, p.cols);
+        layernorm_store<E, W>(p, p.dst.at(r), x, rstd, at.c, at.step, p.cols);
 }
 
 // Forward, longer rows: two kernels over chunks of kChunk values. The first leaves each chunk's mean and sum of squared distances
@@ -154,24 +201,15 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_stats_kernel(co
     const long long  at  = static_cast<long long>(blockIdx.x - r * p.chunks) * kChunk;
     const int        c0  = static_cast<int>(at);
     const int        end = min(static_cast<long long>(p.cols), at + kChunk);
-    float            xv[E], s = 0.0f, q = 0.0f;
     const RowSpan<E, W, true> span(threadIdx.x);
-    load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, xv);
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += xv[e];
-    const float mean = row_sum<true>(s, 0, scratch[0]) / static_cast<float>(end - c0);
-#pragma unroll
-    for (int v = 0; v < E / W; ++v)
-        if (c0 + span.c + v * span.step < end)
-        {
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-            {
-                const float d = xv[v * W + i] - mean;
-                q             = fmaf(d, d, q);
-            }
-        }
-    q = row_sum<true>(q, 0, scratch[1]);
+    f32x2                     x[E / 2];
+    {
+        float v[E];
+        load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, v);
+        pairs<E>(v, x);
+    }
+    const float mean = row_sum<true>(sum_pairs<E>(x), 0, scratch[0]) / static_cast<float>(end - c0);
+    const float q    = row_sum<true>(centre<E, W>(x, mean, c0 + span.c, span.step, end), 0, scratch[1]);
     if (threadIdx.x == 0)
         p.partials[blockIdx.x] = make_float2(mean, q);
 }
@@ -186,21 +224,25 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
     const long long  at  = static_cast<long long>(job - r * p.chunks) * kChunk;
     const int        c0  = static_cast<int>(at);
     const int        end = min(static_cast<long long>(p.cols), at + kChunk);
-    float            xv[E];
     const RowSpan<E, W, true> span(threadIdx.x);
-    load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, xv);
+    f32x2                     x[E / 2];
+    {
+        float v[E];
+        load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, v);
+        pairs<E>(v, x);
+    }
     const float2 *part = p.partials + static_cast<unsigned long long>(r) * p.chunks;
     const float   tail = static_cast<float>(p.cols - static_cast<long long>(p.chunks - 1) * kChunk); // length of the last chunk
     float         s    = 0.0f;
     for (unsigned k = threadIdx.x; k < p.chunks; k += kChunkThreads) s += part[k].x * (k + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
-    const float mean = row_sum<true>(s, 0, scratch[0]) / p.fcols;
+    const float mean = divide_count(row_sum<true>(s, 0, scratch[0]), p.fcols, p.invCols);
     float       q    = 0.0f;
     for (unsigned k = threadIdx.x; k < p.chunks; k += kChunkThreads)
     {
         const float d = part[k].x - mean;
         q += part[k].y + d * d * (k + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
     }
-    const float rstd = 1.0f / sqrtf(row_sum<true>(q, 0, scratch[1]) / p.fcols + p.epsilon);
+    const float rstd = rsqrtf(row_sum<true>(q, 0, scratch[1]) * p.invCols + p.epsilon);
     if (c0 == 0 && threadIdx.x == 0)
     {
         if (p.mean)
@@ -208,7 +250,9 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
         if (p.rstd)
             p.rstd[r] = rstd;
     }
-    layernorm_store<E, W>(p, p.dst.at(r), xv, mean, rstd, c0 + span.c, span.step, end);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) x[i] = add2(x[i], both(-mean));
+    layernorm_store<E, W>(p, p.dst.at(r), x, rstd, c0 + span.c, span.step, end);
 }
 
 } // namespace b200pp

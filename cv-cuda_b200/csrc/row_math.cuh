@@ -323,6 +323,68 @@ __device__ __forceinline__ void store_vecs(uint8_t *row, int dtype, int c, int s
         store_vecs<B200PP_F16, W, N>(row, c, step, end, v);
 }
 
+// ---- two float32 values in a 64-bit register: sm_100 adds, multiplies and fuses both with one instruction, each rounded as the
+// scalar instruction rounds it. The row operators' kernels issue about as many instructions as HBM gives them time for, so this
+// counts.
+typedef unsigned long long f32x2;
+
+__device__ __forceinline__ f32x2 make2(float lo, float hi)
+{
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ f32x2 both(float v)
+{
+    return make2(v, v);
+}
+
+__device__ __forceinline__ float lo2(f32x2 v)
+{
+    return __uint_as_float(static_cast<unsigned>(v));
+}
+
+__device__ __forceinline__ float hi2(f32x2 v)
+{
+    return __uint_as_float(static_cast<unsigned>(v >> 32));
+}
+
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+template<int N>
+__device__ __forceinline__ void pairs(const float *v, f32x2 *p)
+{
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) p[i] = make2(v[2 * i], v[2 * i + 1]);
+}
+
+template<int N>
+__device__ __forceinline__ void singles(const f32x2 *p, float *v)
+{
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) v[2 * i] = lo2(p[i]), v[2 * i + 1] = hi2(p[i]);
+}
+
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll
@@ -342,6 +404,31 @@ __device__ __forceinline__ float block_sum(float v, float *scratch)
     float s = (threadIdx.x & 31) < warps ? scratch[threadIdx.x & 31] : 0.0f;
     return warp_sum(s);
 }
+
+// s / n for a count n and inv = 1 / n rounded: one step of division by residual. A sum of n equal values gives the value itself.
+__device__ __forceinline__ float divide_count(float s, float n, float inv)
+{
+    const float q = s * inv;
+    return fmaf(fmaf(-q, n, s), inv, q);
+}
+
+template<int DT>
+struct Index;
+template<>
+struct Index<B200PP_U8>
+{
+    typedef uint8_t type;
+};
+template<>
+struct Index<B200PP_S32>
+{
+    typedef int type;
+};
+template<>
+struct Index<B200PP_S64>
+{
+    typedef long long type;
+};
 
 // Index i of a set of indices; -1 if it lies outside [0, rows).
 __device__ __forceinline__ int load_index(const RowMap &m, int dtype, unsigned i, int rows)
