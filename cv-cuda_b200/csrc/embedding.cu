@@ -3,7 +3,6 @@
 #include "row_host.h"
 
 #include <algorithm>
-#include <atomic>
 
 using namespace b200pp;
 
@@ -186,25 +185,6 @@ void launch_runs(const EmbeddingGradKParams &p, int width, cudaStream_t stream)
         embedding_grad_runs_kernel<GRAD, 2><<<grid, 256, 0, stream>>>(p);
     else
         embedding_grad_runs_kernel<GRAD, 1><<<grid, 256, 0, stream>>>(p);
-}
-
-// Raises a kernel's dynamic shared-memory limit, once per device.
-template<typename K>
-int raise_smem(K kernel, int bytes, std::atomic<unsigned long long> &done)
-{
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit))
-        return B200PP_SUCCESS;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess)
-    {
-        cudaGetLastError();
-        return fail(B200PP_ERROR_INTERNAL, "Cannot raise a kernel's shared memory to %d bytes: %s", bytes, cudaGetErrorString(e));
-    }
-    done.fetch_or(bit);
-    return B200PP_SUCCESS;
 }
 
 } // namespace

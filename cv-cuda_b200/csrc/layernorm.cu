@@ -16,15 +16,29 @@ long long layernorm_chunks(long long cols)
     return cols > kLongRow ? (cols + kChunk - 1) / kChunk : 0;
 }
 
+template<int SRC, int E, int W>
+int launch_warp(const LayerNormKParams &p, int lanes, cudaStream_t stream)
+{
+    constexpr int                          kRing = RowStage<SRC, W, E / W>::kThread * 256 * kWarpStages;
+    static std::atomic<unsigned long long> raised{0};
+    if (kRing > 32 * 1024) // a launch gets 48 KB unasked, static memory included
+        if (int st = raise_smem(layernorm_warp_kernel<SRC, E, W>, kRing, raised))
+            return st;
+    const dim3     block(lanes, 256 / lanes);
+    const unsigned turns = (p.rows + block.y - 1) / block.y;
+    layernorm_warp_kernel<SRC, E, W><<<std::min(turns, static_cast<unsigned>(kSms * kWarpCtas<E>)), block, kRing, stream>>>(p);
+    return B200PP_SUCCESS;
+}
+
 template<int SRC, int W>
-void launch_layernorm(const LayerNormKParams &p, cudaStream_t stream)
+int launch_layernorm(const LayerNormKParams &p, cudaStream_t stream)
 {
     const int cols = p.cols;
     if (p.chunks)
     {
         layernorm_chunk_stats_kernel<SRC, W><<<p.rows * p.chunks, kChunkThreads, 0, stream>>>(p);
         layernorm_chunk_apply_kernel<SRC, W><<<p.rows * p.chunks, kChunkThreads, 0, stream>>>(p);
-        return;
+        return B200PP_SUCCESS;
     }
     if (cols > 1024 || (cols > 256 && p.rows <= static_cast<unsigned>(kSms)))
     {
@@ -32,38 +46,34 @@ void launch_layernorm(const LayerNormKParams &p, cudaStream_t stream)
         // that the GPU is not full anyway.
         auto threads = [cols](int e) { return dim3((cols + 32 * e - 1) / (32 * e) * 32); };
         if (cols <= 4096 && p.rows <= static_cast<unsigned>(kSms))
-            layernorm_kernel<SRC, 8, W, true><<<p.rows, threads(8), 0, stream>>>(p);
+            layernorm_block_kernel<SRC, 8, W><<<p.rows, threads(8), 0, stream>>>(p);
         else if (cols <= 8192)
-            layernorm_kernel<SRC, 16, W, true><<<p.rows, threads(16), 0, stream>>>(p);
+            layernorm_block_kernel<SRC, 16, W><<<p.rows, threads(16), 0, stream>>>(p);
         else
-            layernorm_kernel<SRC, 32, W, true><<<p.rows, threads(32), 0, stream>>>(p);
-        return;
+            layernorm_block_kernel<SRC, 32, W><<<p.rows, threads(32), 0, stream>>>(p);
+        return B200PP_SUCCESS;
     }
     int lanes = 4;
     while (lanes < 32 && lanes * 8 < cols) lanes *= 2;
-    const dim3     block(lanes, 256 / lanes);
-    const unsigned grid = (p.rows + block.y - 1) / block.y;
     if (cols <= 256)
-        layernorm_kernel<SRC, 8, W, false><<<grid, block, 0, stream>>>(p);
-    else if (cols <= 512)
-        layernorm_kernel<SRC, 16, W, false><<<grid, block, 0, stream>>>(p);
-    else if (cols <= 768)
-        layernorm_kernel<SRC, 24, W, false><<<grid, block, 0, stream>>>(p);
-    else
-        layernorm_kernel<SRC, 32, W, false><<<grid, block, 0, stream>>>(p);
+        return launch_warp<SRC, 8, W>(p, lanes, stream);
+    if (cols <= 512)
+        return launch_warp<SRC, 16, W>(p, lanes, stream);
+    if (cols <= 768)
+        return launch_warp<SRC, 24, W>(p, lanes, stream);
+    return launch_warp<SRC, 32, W>(p, lanes, stream);
 }
 
 template<int SRC>
-void launch_layernorm(const LayerNormKParams &p, int width, cudaStream_t stream)
+int launch_layernorm(const LayerNormKParams &p, int width, cudaStream_t stream)
 {
     if (width == 8)
-        launch_layernorm<SRC, 8>(p, stream);
-    else if (width == 4)
-        launch_layernorm<SRC, 4>(p, stream);
-    else if (width == 2)
-        launch_layernorm<SRC, 2>(p, stream);
-    else
-        launch_layernorm<SRC, 1>(p, stream);
+        return launch_layernorm<SRC, 8>(p, stream);
+    if (width == 4)
+        return launch_layernorm<SRC, 4>(p, stream);
+    if (width == 2)
+        return launch_layernorm<SRC, 2>(p, stream);
+    return launch_layernorm<SRC, 1>(p, stream);
 }
 
 } // namespace
@@ -128,20 +138,15 @@ extern "C" int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, con
     width.take(p.dst, row_elem_size(dst->dtype));
     width.take(p.weight, 0, row_elem_size(p.weightType));
     width.take(p.bias, 0, row_elem_size(p.biasType));
-    switch (src->dtype)
-    {
-    case B200PP_U8:
-        launch_layernorm<B200PP_U8>(p, width.width, stream);
-        break;
-    case B200PP_F16:
-        launch_layernorm<B200PP_F16>(p, width.width, stream);
-        break;
-    case B200PP_BF16:
-        launch_layernorm<B200PP_BF16>(p, width.width, stream);
-        break;
-    default:
-        launch_layernorm<B200PP_F32>(p, width.width, stream);
-        break;
-    }
+    if (src->dtype == B200PP_U8)
+        st = launch_layernorm<B200PP_U8>(p, width.width, stream);
+    else if (src->dtype == B200PP_F16)
+        st = launch_layernorm<B200PP_F16>(p, width.width, stream);
+    else if (src->dtype == B200PP_BF16)
+        st = launch_layernorm<B200PP_BF16>(p, width.width, stream);
+    else
+        st = launch_layernorm<B200PP_F32>(p, width.width, stream);
+    if (st)
+        return st;
     return check_launch("LayerNorm");
 }

@@ -47,45 +47,57 @@ size_t grad_workspace(const GradPlan &g, long long cols)
     return static_cast<size_t>(g.parts) * 2 * cols * sizeof(float);
 }
 
-template<int SRC, int GRAD, int W>
-void launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
+template<int SRC, int GRAD, int E, int W, bool BLOCK>
+int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
 {
-    const dim3 block(g.threads, g.groups);
-    const int  smem = p.partials && g.groups > 1 ? 2 * p.cols * static_cast<int>(sizeof(float)) : 0;
+    typedef GradRing<SRC, GRAD, E, W>      Ring;
+    static std::atomic<unsigned long long> raised{0};
+    const int                              threads = g.threads * g.groups;
+    const int ring = Ring::kThread * Ring::kStages * threads, sums = p.partials ? 2 * p.cols * static_cast<int>(sizeof(float)) : 0;
+    const int smem = std::max(ring, sums);
+    if (smem > 32 * 1024) // a launch gets 48 KB unasked, static memory included
+        if (int st = raise_smem(layernorm_grad_kernel<SRC, GRAD, E, W, BLOCK>,
+                                std::max(Ring::kThread * Ring::kStages * kGradResident, 2 * 8192 * static_cast<int>(sizeof(float))), raised))
+            return st;
+    layernorm_grad_kernel<SRC, GRAD, E, W, BLOCK><<<p.parts, dim3(g.threads, g.groups), smem, stream>>>(p);
+    return check_launch("LayerNormBackward");
+}
+
+template<int SRC, int GRAD, int W>
+int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
+{
     if (g.values == 8)
-        layernorm_grad_kernel<SRC, GRAD, 8, W, false><<<p.parts, block, smem, stream>>>(p);
-    else if (g.values == 24)
-        layernorm_grad_kernel<SRC, GRAD, 24, W, false><<<p.parts, block, smem, stream>>>(p);
-    else if (g.threads == 32)
-        layernorm_grad_kernel<SRC, GRAD, 16, W, false><<<p.parts, block, smem, stream>>>(p);
-    else
-        layernorm_grad_kernel<SRC, GRAD, 16, W, true><<<p.parts, block, smem, stream>>>(p);
+        return launch_one_pass<SRC, GRAD, 8, W, false>(p, g, stream);
+    if (g.values == 24)
+        return launch_one_pass<SRC, GRAD, 24, W, false>(p, g, stream);
+    if (g.threads == 32)
+        return launch_one_pass<SRC, GRAD, 16, W, false>(p, g, stream);
+    return launch_one_pass<SRC, GRAD, 16, W, true>(p, g, stream);
 }
 
 template<int SRC, int GRAD>
-void launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, int width, cudaStream_t stream)
+int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, int width, cudaStream_t stream)
 {
     if (width == 8)
-        launch_one_pass<SRC, GRAD, 8>(p, g, stream);
-    else if (width == 4)
-        launch_one_pass<SRC, GRAD, 4>(p, g, stream);
-    else if (width == 2)
-        launch_one_pass<SRC, GRAD, 2>(p, g, stream);
-    else
-        launch_one_pass<SRC, GRAD, 1>(p, g, stream);
+        return launch_one_pass<SRC, GRAD, 8>(p, g, stream);
+    if (width == 4)
+        return launch_one_pass<SRC, GRAD, 4>(p, g, stream);
+    if (width == 2)
+        return launch_one_pass<SRC, GRAD, 2>(p, g, stream);
+    return launch_one_pass<SRC, GRAD, 1>(p, g, stream);
 }
 
 // The pairs of element types the one-pass kernel is built for: gradients of the source's type or float32, any for uint8.
-bool launch_one_pass(int srcType, const LayerNormGradKParams &p, const GradPlan &g, int width, cudaStream_t stream)
+// -1: not this pair, or rows too long.
+int launch_one_pass(int srcType, const LayerNormGradKParams &p, const GradPlan &g, int width, cudaStream_t stream)
 {
     if (g.values == 0)
-        return false;
+        return -1;
     switch (srcType * 16 + p.gradType)
     {
-#define B200PP_PAIR(S, G)                               \
-    case S * 16 + G:                                    \
-        launch_one_pass<S, G>(p, g, width, stream);     \
-        return true;
+#define B200PP_PAIR(S, G) \
+    case S * 16 + G:      \
+        return launch_one_pass<S, G>(p, g, width, stream);
         B200PP_PAIR(B200PP_U8, B200PP_F32)
         B200PP_PAIR(B200PP_U8, B200PP_F16)
         B200PP_PAIR(B200PP_U8, B200PP_BF16)
@@ -96,7 +108,7 @@ bool launch_one_pass(int srcType, const LayerNormGradKParams &p, const GradPlan 
         B200PP_PAIR(B200PP_F32, B200PP_F32)
 #undef B200PP_PAIR
     }
-    return false;
+    return -1;
 }
 
 template<int SRC>
@@ -189,8 +201,9 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     width.take(p.grad, row_elem_size(p.gradType));
     width.take(p.dsrc, row_elem_size(p.dsrcType));
     width.take(p.weight, 0, row_elem_size(p.weightType));
-    if (launch_one_pass(src->dtype, p, plan, width.width, stream))
-        st = check_launch("LayerNormBackward");
+    st = launch_one_pass(src->dtype, p, plan, width.width, stream);
+    if (st >= 0)
+        ; // done, or refused
     else if (src->dtype == B200PP_U8)
         st = launch_two_pass<B200PP_U8>(p, stream);
     else if (src->dtype == B200PP_F16)

@@ -26,56 +26,76 @@ struct LayerNormGradKParams
 
 // Rows that fit into registers, all gradients in one pass over the data. blockDim.x threads per row (BLOCK: whole warps, otherwise
 // a warp, or part of one for eight values a lane), blockDim.y rows per CTA at a time. A CTA walks down its share of the rows; each
-// thread keeps its columns of the sums over the rows in registers. What a row costs besides its values -- addresses, shuffles, the
-// barrier -- is why a thread has up to 24 values: with eight (and the next row loaded ahead) 50176 rows of 768 bfloat16 took 62 us.
+// thread keeps its columns of the sums over the rows in registers, and the rows ahead are on their way through shared memory. What
+// a row costs besides its values -- addresses, shuffles, the barrier -- is why a thread has up to 24 values.
 constexpr int kGradResident = 512; // threads that fit on an SM, by the registers per thread the launch bound leaves (128)
+
+template<int SRC, int GRAD, int E, int W>
+struct GradRing
+{
+    typedef RowStage<SRC, W, E / W>  X;
+    typedef RowStage<GRAD, W, E / W> G;
+    static constexpr int kThread = X::kThread + G::kThread;
+    static constexpr int kStages = kThread * 3 * kGradResident <= 200 * 1024 ? 3 : 2; // what fits beside L1
+};
 
 template<int SRC, int GRAD, int E, int W, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? kGradResident : 256, BLOCK ? 1 : 2) layernorm_grad_kernel(const LayerNormGradKParams p)
 {
-    constexpr int              V = E / W;
+    typedef GradRing<SRC, GRAD, E, W> Ring;
+    typedef typename Ring::X          X;
+    typedef typename Ring::G          G;
+    constexpr int              V = E / W, kStages = Ring::kStages;
+    constexpr bool             kStaged = Ring::kThread > 0;
     __shared__ float2          scratch[2][16]; // two halves, used in turn: one barrier per row
-    extern __shared__ float    sums[];         // [2][cols]
+    extern __shared__ uint4    ring[];         // the stages; in the end the sums, [2][cols]
+    float                     *sums = reinterpret_cast<float *>(ring);
     const int                  t = threadIdx.x, threads = !BLOCK && E > 8 ? 32 : blockDim.x, g = threadIdx.y, groups = blockDim.y;
-    const int                  tid = g * threads + t, warp = tid >> 5;
+    const int                  tid = g * threads + t, warp = tid >> 5, all = threads * groups, stageBytes = Ring::kThread * all;
     const RowSpan<E, W, BLOCK> at(t);
+    const unsigned             ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
     f32x2                      dw[E / 2], db[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) dw[i] = db[i] = both(0.0f);
     const unsigned long long step = static_cast<unsigned long long>(gridDim.x) * groups;
     unsigned long long       r    = static_cast<unsigned long long>(blockIdx.x) * groups + g;
-    int                      half = 0;
+    int                      half = 0, stage = 0;
+    auto                     fetch = [&](int s, unsigned long long k) {
+        const bool live = k < p.rows;
+        X::fetch(ring0 + s * stageBytes, tid, all, live ? p.src.at(static_cast<unsigned>(k)) : nullptr, p.src.base, at.c, at.step, p.cols);
+        G::fetch(ring0 + s * stageBytes + X::kThread * all, tid, all, live ? p.grad.at(static_cast<unsigned>(k)) : nullptr, p.grad.base,
+                 at.c, at.step, p.cols);
+        copies_commit();
+    };
+    if constexpr (kStaged)
+    {
+#pragma unroll
+        for (int s = 0; s < kStages - 1; ++s) fetch(s, r + s * step);
+    }
+    float nextMean = r < p.rows ? p.mean[r] : 0.0f, nextRstd = r < p.rows ? p.rstd[r] : 0.0f;
     // every thread of the CTA takes the same number of turns
     for (unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * groups; first < p.rows; first += step, r += step)
     {
-        const bool     live = r < p.rows;
-        const int      end  = live ? p.cols : 0; // a row that is not there, and what lies behind a row's end: x = dy = 0
+        const bool     live = r < p.rows; // a row that is not there, and what lies behind a row's end: x = dy = 0
         const unsigned row  = live ? static_cast<unsigned>(r) : 0;
-        const float    mean = live ? p.mean[row] : 0.0f, rstd = live ? p.rstd[row] : 0.0f;
+        const float    mean = nextMean, rstd = nextRstd;
         f32x2          h[E / 2], gv[E / 2], s1 = both(0.0f), s2 = both(0.0f);
         {
-            Vec<SRC, W>    xr[V];
-            Vec<GRAD, W>   gr[V];
-            const uint8_t *x = p.src.at(row), *dy = p.grad.at(row);
-#pragma unroll
-            for (int v = 0; v < V; ++v)
+            if constexpr (kStaged)
             {
-                const int c = at.c + v * at.step;
-                xr[v]       = zero_raw<kElemBytes<SRC> * W>();
-                gr[v]       = zero_raw<kElemBytes<GRAD> * W>();
-                if (c < end)
-                {
-                    xr[v] = load_raw<kElemBytes<SRC> * W>(x + static_cast<long long>(c) * kElemBytes<SRC>);
-                    gr[v] = load_raw<kElemBytes<GRAD> * W>(dy + static_cast<long long>(c) * kElemBytes<GRAD>);
-                }
+                fetch(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
+                copies_wait<kStages - 1>();
             }
-            float f[E];
-#pragma unroll
-            for (int v = 0; v < V; ++v) unpack<SRC, W>(xr[v], f + v * W);
+            const bool more = r + step < p.rows;
+            nextMean        = more ? p.mean[r + step] : 0.0f;
+            nextRstd        = more ? p.rstd[r + step] : 0.0f;
+            float          f[E];
+            const uint8_t *from = reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes;
+            X::take(from, tid, all, X::kStaged || !live ? nullptr : p.src.at(row), at.c, at.step, p.cols, f);
             pairs<E>(f, h);
-#pragma unroll
-            for (int v = 0; v < V; ++v) unpack<GRAD, W>(gr[v], f + v * W);
+            G::take(from + X::kThread * all, tid, all, G::kStaged || !live ? nullptr : p.grad.at(row), at.c, at.step, p.cols, f);
             pairs<E>(f, gv);
+            stage = stage == kStages - 1 ? 0 : stage + 1;
         }
 #pragma unroll
         for (int i = 0; i < E / 2; ++i)
@@ -139,6 +159,11 @@ __global__ void __launch_bounds__(BLOCK ? kGradResident : 256, BLOCK ? 1 : 2) la
     }
     if (!p.partials)
         return;
+    if constexpr (kStaged)
+    {
+        copies_wait<0>(); // the sums take the ring's place
+        __syncthreads();
+    }
     // the CTA's sums: over the rows of a warp by shuffles, over the warps (BLOCK: over the rows) one after another
     float    *part  = p.partials + static_cast<long long>(blockIdx.x) * 2 * p.cols;
     int       slot  = g, slots = groups;

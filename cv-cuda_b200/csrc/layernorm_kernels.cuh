@@ -145,35 +145,99 @@ __device__ __forceinline__ float centre(f32x2 *x, float mean, int c, int step, i
     return lo2(a) + hi2(a);
 }
 
-// Forward, rows that fit into registers. BLOCK: one CTA per row; otherwise blockDim.x lanes of a warp per row (32 for more than
-// eight values a lane) and blockDim.y rows per CTA. The statistics come from the registers (the variance about the mean), so the
-// row is read once.
-template<int SRC, int E, int W, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? (E <= 16 ? 512 : 1024) : 256) layernorm_kernel(const LayerNormKParams p)
+// Forward, a warp per row, or part of one for up to 256 columns (eight values a lane): blockDim.x lanes per row, blockDim.y rows
+// per CTA. A warp walks down its share of the rows with the weights in registers; the rows ahead are on their way through shared
+// memory. The statistics come from the registers (the variance about the mean), so the row is read once.
+constexpr int kWarpStages = 3;
+
+template<int E>
+constexpr int kWarpCtas = E <= 8 ? 4 : E <= 16 ? 3 : 2; // of 256 threads on an SM, by the registers the launch bound leaves
+
+template<int SRC, int E, int W>
+__global__ void __launch_bounds__(256, kWarpCtas<E>) layernorm_warp_kernel(const LayerNormKParams p)
 {
-    __shared__ float scratch[2][32];
-    const int        t = threadIdx.x, threads = !BLOCK && E > 8 ? 32 : blockDim.x;
-    const unsigned   r = BLOCK ? blockIdx.x : blockIdx.x * blockDim.y + threadIdx.y;
-    if (!BLOCK && r - threadIdx.y % (32u / threads) >= p.rows) // all rows of the warp
-        return;
-    const bool                 live = BLOCK || r < p.rows;
-    const RowSpan<E, W, BLOCK> at(t);
-    f32x2                      x[E / 2];
+    typedef RowStage<SRC, W, E / W> Stage;
+    extern __shared__ uint4         ring[];
+    constexpr int                   kStage = Stage::kThread * 256;
+    const int                       t = threadIdx.x, lanes = E > 8 ? 32 : blockDim.x, tid = threadIdx.y * lanes + t;
+    const RowSpan<E, W, false>      at(t);
+    const unsigned                  ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
+    f32x2                           w[E / 2], b[E / 2];
+#pragma unroll
+    for (int k = 0; k < E / 8; ++k)
+        layernorm_affine<W>(p, at.c + 8 / W * k * at.step, at.step, p.cols, w + 4 * k, b + 4 * k);
+    const unsigned long long step = static_cast<unsigned long long>(gridDim.x) * blockDim.y;
+    const unsigned long long r0   = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    auto                     row  = [&](unsigned long long r) { return r < p.rows ? p.src.at(static_cast<unsigned>(r)) : nullptr; };
+    if constexpr (Stage::kStaged)
+    {
+#pragma unroll
+        for (int s = 0; s < kWarpStages - 1; ++s)
+        {
+            Stage::fetch(ring0 + s * kStage, tid, 256, row(r0 + s * step), p.src.base, at.c, at.step, p.cols);
+            copies_commit();
+        }
+    }
+    int stage = 0;
+    // the lanes of a warp take the same number of turns: those of the warp's first row
+    for (unsigned long long r = r0, first = r0 - threadIdx.y % (32u / lanes); first < p.rows; r += step, first += step)
+    {
+        f32x2 x[E / 2];
+        {
+            float v[E];
+            if constexpr (Stage::kStaged)
+            {
+                const int ahead = stage == 0 ? kWarpStages - 1 : stage - 1;
+                Stage::fetch(ring0 + ahead * kStage, tid, 256, row(r + (kWarpStages - 1) * step), p.src.base, at.c, at.step, p.cols);
+                copies_commit();
+                copies_wait<kWarpStages - 1>();
+            }
+            Stage::take(reinterpret_cast<const uint8_t *>(ring) + stage * kStage, tid, 256, Stage::kStaged ? nullptr : row(r), at.c, at.step,
+                        p.cols, v);
+            stage = stage == kWarpStages - 1 ? 0 : stage + 1;
+            pairs<E>(v, x);
+        }
+        const float mean = divide_count(row_sum<false>(sum_pairs<E>(x), lanes, nullptr), p.fcols, p.invCols);
+        const float q    = centre<E, W>(x, mean, at.c, at.step, p.cols);
+        const float rstd = rsqrtf(row_sum<false>(q, lanes, nullptr) * p.invCols + p.epsilon);
+        if (r >= p.rows)
+            continue;
+        if (t == 0)
+        {
+            if (p.mean)
+                p.mean[r] = mean;
+            if (p.rstd)
+                p.rstd[r] = rstd;
+        }
+        float v[E];
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) x[i] = fma2(mul2(x[i], both(rstd)), w[i], b[i]);
+        singles<E>(x, v);
+        store_vecs<W, E / W>(p.dst.at(static_cast<unsigned>(r)), p.dstType, at.c, at.step, p.cols, v);
+    }
+}
+
+// Forward, a CTA per row.
+template<int SRC, int E, int W>
+__global__ void __launch_bounds__(E <= 16 ? 512 : 1024) layernorm_block_kernel(const LayerNormKParams p)
+{
+    __shared__ float          scratch[2][32];
+    const unsigned            r = blockIdx.x;
+    const RowSpan<E, W, true> at(threadIdx.x);
+    f32x2                     x[E / 2];
     {
         float v[E];
-        load_vecs<SRC, W, E / W>(p.src.at(live ? r : p.rows - 1), at.c, at.step, p.cols, v);
+        load_vecs<SRC, W, E / W>(p.src.at(r), at.c, at.step, p.cols, v);
         pairs<E>(v, x);
     }
     // with eight values there are registers left to fetch the weights at the same time as the row
     f32x2 w[4], b[4];
     if constexpr (E == 8)
         layernorm_affine<W>(p, at.c, at.step, p.cols, w, b);
-    const float mean = divide_count(row_sum<BLOCK>(sum_pairs<E>(x), threads, scratch[0]), p.fcols, p.invCols);
+    const float mean = divide_count(row_sum<true>(sum_pairs<E>(x), 0, scratch[0]), p.fcols, p.invCols);
     const float q    = centre<E, W>(x, mean, at.c, at.step, p.cols);
-    const float rstd = rsqrtf(row_sum<BLOCK>(q, threads, scratch[1]) * p.invCols + p.epsilon);
-    if (!live)
-        return;
-    if (t == 0)
+    const float rstd = rsqrtf(row_sum<true>(q, 0, scratch[1]) * p.invCols + p.epsilon);
+    if (threadIdx.x == 0)
     {
         if (p.mean)
             p.mean[r] = mean;

@@ -5,6 +5,7 @@
 #include "host_common.h"
 #include "row_math.cuh"
 
+#include <atomic>
 #include <cstdlib>
 
 namespace b200pp {
@@ -161,6 +162,25 @@ struct VecWidth
         take(m.base, m.s0 | m.s1 | m.s2, elem);
     }
 };
+
+// Raises a kernel's dynamic shared-memory limit, once per device.
+template<typename K>
+int raise_smem(K kernel, int bytes, std::atomic<unsigned long long> &done)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit))
+        return B200PP_SUCCESS;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess)
+    {
+        cudaGetLastError();
+        return fail(B200PP_ERROR_INTERNAL, "Cannot raise a kernel's shared memory to %d bytes: %s", bytes, cudaGetErrorString(e));
+    }
+    done.fetch_or(bit);
+    return B200PP_SUCCESS;
+}
 
 } // namespace b200pp
 

@@ -323,6 +323,89 @@ __device__ __forceinline__ void store_vecs(uint8_t *row, int dtype, int c, int s
         store_vecs<B200PP_F16, W, N>(row, c, step, end, v);
 }
 
+// ---- rows on their way through shared memory: each thread copies its own vectors of the rows ahead with asynchronous copies and
+// reads them back itself, so there is nothing to synchronise and no register is held while HBM answers. Vectors of fewer than four
+// bytes cannot be copied like that; they are loaded when they are needed.
+
+template<int BYTES>
+__device__ __forceinline__ void copy_async(unsigned dst, const uint8_t *src, bool there)
+{
+    const int n = there ? BYTES : 0; // what is not there becomes zeros
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+
+__device__ __forceinline__ void copies_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// All but the N latest groups are there.
+template<int N>
+__device__ __forceinline__ void copies_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The part of a ring that belongs to one tensor: V vectors of W elements for each of the CTA's threads.
+template<int DT, int W, int V>
+struct RowStage
+{
+    static constexpr int  kBytes  = kElemBytes<DT> * W;
+    static constexpr bool kStaged = kBytes >= 4;
+    static constexpr int  kPart = kBytes > 16 ? 16 : kBytes, kParts = kBytes / kPart;
+    static constexpr int  kThread = kStaged ? kBytes * V : 0; // bytes per thread and stage
+
+    // `stage`: shared-memory address of the stage; `row`: the row, null if there is none
+    static __device__ __forceinline__ void fetch(unsigned stage, int tid, int threads, const uint8_t *row, const uint8_t *valid, int c,
+                                                 int step, int end)
+    {
+        if constexpr (kStaged)
+        {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int k = 0; k < kParts; ++k)
+                {
+                    const bool there = row != nullptr && c + v * step < end;
+                    copy_async<kPart>(stage + ((v * kParts + k) * threads + tid) * kPart,
+                                      there ? row + static_cast<long long>(c + v * step) * kElemBytes<DT> + k * kPart : valid, there);
+                }
+        }
+    }
+
+    // the thread's values, from the ring or (vectors that are not staged) from the row itself
+    static __device__ __forceinline__ void take(const uint8_t *stage, int tid, int threads, const uint8_t *row, int c, int step, int end,
+                                                float *out)
+    {
+        Vec<DT, W> raw[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+        {
+            if constexpr (kStaged)
+            {
+#pragma unroll
+                for (int k = 0; k < kParts; ++k)
+                {
+                    const RawVec<kPart> part = load_raw<kPart>(stage + ((v * kParts + k) * threads + tid) * kPart);
+#pragma unroll
+                    for (int i = 0; i < kPart / 4; ++i) raw[v].w[k * (kPart / 4) + i] = part.w[i];
+                }
+            }
+            else
+            {
+                raw[v] = zero_raw<kBytes>();
+                if (row != nullptr && c + v * step < end)
+                    raw[v] = load_raw<kBytes>(row + static_cast<long long>(c + v * step) * kElemBytes<DT>);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) unpack<DT, W>(raw[v], out + v * W);
+    }
+};
+
 // ---- two float32 values in a 64-bit register: sm_100 adds, multiplies and fuses both with one instruction, each rounded as the
 // scalar instruction rounds it. The row operators' kernels issue about as many instructions as HBM gives them time for, so this
 // counts.
