@@ -8,33 +8,43 @@ using namespace b200pp;
 
 namespace {
 
-// How the rows are dealt out. One-pass kernel: `threads` per row with `values` values each, `groups` rows per CTA, one part per CTA;
-// for longer rows (values = 0) the sums over the rows are a kernel of their own.
+// How the rows are dealt out. One-pass kernel: `threads` per row and CTA with `values` values each, `groups` rows per CTA, a cluster of
+// `ctas` CTAs with `span` columns each per row, one part per CTA or cluster; for longer rows (values = 0) the sums over the rows
+// are a kernel of their own.
 struct GradPlan
 {
-    int threads, groups, values, parts;
+    int threads, groups, values, ctas, span, parts;
 };
 
 GradPlan plan_layernorm_grad(long long rows, long long cols)
 {
     GradPlan g{};
-    if (cols <= 8192)
+    if (cols <= 8 * 16 * kGradResident)
     {
-        // a warp per row, or part of one, up to 768 columns; above, whole warps with sixteen values per thread
+        g.ctas = 1;
         if (cols <= 768)
         {
-            g.values = cols <= 256 ? 8 : cols <= 512 ? 16 : 24;
-            for (g.threads = 4; g.threads < 32 && g.threads * 8 < cols;) g.threads *= 2;
+            // as few lanes per row as leave little idle
+            static const int table[][3] = {{8, 1, 8},     {16, 2, 8},    {32, 4, 8},    {64, 4, 16},   {96, 4, 24},  {128, 8, 16},
+                                           {192, 8, 24},  {256, 16, 16}, {384, 16, 24}, {512, 32, 16}, {768, 32, 24}};
+            int              i = 0;
+            while (cols > table[i][0]) ++i;
+            g.threads = table[i][1];
+            g.values  = table[i][2];
         }
         else
         {
-            g.values  = 16;
-            g.threads = static_cast<int>((cols + 511) / 512 * 32);
+            g.values = 16;
+            while (g.ctas * 16 * kGradResident < cols) g.ctas *= 2;
+            g.threads = static_cast<int>((cols + g.ctas * 512 - 1) / (g.ctas * 512) * 32);
         }
-        g.groups              = std::max(1, 256 / g.threads);
+        g.span = g.threads * g.values;
+        // several rows per CTA as long as there are enough for all SMs; whole warps
+        g.groups = std::max(1, 256 / g.threads);
+        while (g.groups > 1 && g.groups * g.threads > 32 && rows < static_cast<long long>(g.groups) * kSms) g.groups /= 2;
         const long long turns = (rows + g.groups - 1) / g.groups;
-        const int       ctas  = kSms * std::max(1, kGradResident / (g.threads * g.groups));
-        g.parts               = static_cast<int>(std::max(1LL, std::min<long long>(turns, ctas)));
+        const int       most  = std::max(1, kSms * std::max(1, kGradResident / (g.threads * g.groups)) / g.ctas);
+        g.parts               = static_cast<int>(std::max(1LL, std::min<long long>(turns, most)));
         return g;
     }
     const long long blocks = (cols + 31) / 32;
@@ -47,19 +57,23 @@ size_t grad_workspace(const GradPlan &g, long long cols)
     return static_cast<size_t>(g.parts) * 2 * cols * sizeof(float);
 }
 
-template<int SRC, int GRAD, int E, int W, bool BLOCK>
+template<int SRC, int GRAD, int E, int W, bool WARP>
 int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
 {
     typedef GradRing<SRC, GRAD, E, W>      Ring;
     static std::atomic<unsigned long long> raised{0};
-    const int                              threads = g.threads * g.groups;
-    const int ring = Ring::kThread * Ring::kStages * threads, sums = p.partials ? 2 * p.cols * static_cast<int>(sizeof(float)) : 0;
+    const int                              warps = g.threads * g.groups / 32, slots = WARP ? warps : g.groups;
+    const int                              columns = WARP ? p.cols : g.span;
+    const int ring = Ring::bytes(g.threads, g.groups) * Ring::kStages;
+    const int sums = p.partials && slots > 1 ? slots * 2 * columns * static_cast<int>(sizeof(float)) : 0;
     const int smem = std::max(ring, sums);
     if (smem > 32 * 1024) // a launch gets 48 KB unasked, static memory included
-        if (int st = raise_smem(layernorm_grad_kernel<SRC, GRAD, E, W, BLOCK>,
-                                std::max(Ring::kThread * Ring::kStages * kGradResident, 2 * 8192 * static_cast<int>(sizeof(float))), raised))
+        if (int st = raise_smem(layernorm_grad_kernel<SRC, GRAD, E, W, WARP>, 208 * 1024, raised))
             return st;
-    layernorm_grad_kernel<SRC, GRAD, E, W, BLOCK><<<p.parts, dim3(g.threads, g.groups), smem, stream>>>(p);
+    ClusterLaunch launch(g.ctas, g.threads, smem, stream);
+    launch.cfg.blockDim.y = g.groups;
+    launch.cfg.gridDim    = dim3(p.parts * g.ctas);
+    cudaLaunchKernelEx(&launch.cfg, layernorm_grad_kernel<SRC, GRAD, E, W, WARP>, p, g.span);
     return check_launch("LayerNormBackward");
 }
 
@@ -67,24 +81,24 @@ template<int SRC, int GRAD, int W>
 int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
 {
     if (g.values == 8)
-        return launch_one_pass<SRC, GRAD, 8, W, false>(p, g, stream);
+        return launch_one_pass<SRC, GRAD, 8, W, true>(p, g, stream);
     if (g.values == 24)
-        return launch_one_pass<SRC, GRAD, 24, W, false>(p, g, stream);
-    if (g.threads == 32)
-        return launch_one_pass<SRC, GRAD, 16, W, false>(p, g, stream);
-    return launch_one_pass<SRC, GRAD, 16, W, true>(p, g, stream);
+        return launch_one_pass<SRC, GRAD, 24, W, true>(p, g, stream);
+    if (g.threads <= 32)
+        return launch_one_pass<SRC, GRAD, 16, W, true>(p, g, stream);
+    return launch_one_pass<SRC, GRAD, 16, W, false>(p, g, stream);
 }
 
 template<int SRC, int GRAD>
 int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, int width, cudaStream_t stream)
 {
-    if (width == 8)
-        return launch_one_pass<SRC, GRAD, 8>(p, g, stream);
-    if (width == 4)
+    // vectors of 16 bytes at most on the way through shared memory; of four elements at least, otherwise the rows' lines as they are
+    if constexpr (SRC != B200PP_F32 && GRAD != B200PP_F32)
+        if (width == 8)
+            return launch_one_pass<SRC, GRAD, 8>(p, g, stream);
+    if (width >= 4)
         return launch_one_pass<SRC, GRAD, 4>(p, g, stream);
-    if (width == 2)
-        return launch_one_pass<SRC, GRAD, 2>(p, g, stream);
-    return launch_one_pass<SRC, GRAD, 1>(p, g, stream);
+    return launch_one_pass<SRC, GRAD, 0>(p, g, stream);
 }
 
 // The pairs of element types the one-pass kernel is built for: gradients of the source's type or float32, any for uint8.

@@ -24,79 +24,96 @@ struct LayerNormGradKParams
     int            parts;
 };
 
-// Rows that fit into registers, all gradients in one pass over the data. blockDim.x threads per row (BLOCK: whole warps, otherwise
-// a warp, or part of one for eight values a lane), blockDim.y rows per CTA at a time. A CTA walks down its share of the rows; each
-// thread keeps its columns of the sums over the rows in registers, and the rows ahead are on their way through shared memory. What
-// a row costs besides its values -- addresses, shuffles, the barrier -- is why a thread has up to 24 values.
+// All gradients in one pass over the data. WARP: blockDim.x lanes of a warp per row (a power of two) and blockDim.y rows per CTA at a
+// time; otherwise whole warps per row, blockDim.y rows per CTA at a time, or -- for longer rows -- a cluster of up to eight CTAs with
+// `span` columns each per row. CTAs (clusters) walk down their share of the rows; each thread keeps its columns of the sums over the
+// rows in registers, and the rows ahead are on their way through shared memory. What a row costs besides its values -- addresses,
+// shuffles, the barrier -- is why a thread has up to 24 values.
 constexpr int kGradResident = 512; // threads that fit on an SM, by the registers per thread the launch bound leaves (128)
 
 template<int SRC, int GRAD, int E, int W>
 struct GradRing
 {
-    typedef RowStage<SRC, W, E / W>  X;
-    typedef RowStage<GRAD, W, E / W> G;
-    static constexpr int kThread = X::kThread + G::kThread;
+    typedef RowStage<SRC, E, W>  X;
+    typedef RowStage<GRAD, E, W> G;
+
+    static constexpr int kThread = E * (kElemBytes<SRC> + kElemBytes<GRAD>);
     static constexpr int kStages = kThread * 3 * kGradResident <= 200 * 1024 ? 3 : 2; // what fits beside L1
+
+    static __host__ __device__ constexpr int bytes(int threads, int groups)
+    {
+        return X::bytes(threads, groups) + G::bytes(threads, groups);
+    }
 };
 
-template<int SRC, int GRAD, int E, int W, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? kGradResident : 256, BLOCK ? 1 : 2) layernorm_grad_kernel(const LayerNormGradKParams p)
+template<int SRC, int GRAD, int E, int W, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) layernorm_grad_kernel(const LayerNormGradKParams p, int span)
 {
+    namespace cg = cooperative_groups;
     typedef GradRing<SRC, GRAD, E, W> Ring;
     typedef typename Ring::X          X;
     typedef typename Ring::G          G;
-    constexpr int              V = E / W, kStages = Ring::kStages;
-    constexpr bool             kStaged = Ring::kThread > 0;
-    __shared__ float2          scratch[2][16]; // two halves, used in turn: one barrier per row
-    extern __shared__ uint4    ring[];         // the stages; in the end the sums, [2][cols]
-    float                     *sums = reinterpret_cast<float *>(ring);
-    const int                  t = threadIdx.x, threads = !BLOCK && E > 8 ? 32 : blockDim.x, g = threadIdx.y, groups = blockDim.y;
-    const int                  tid = g * threads + t, warp = tid >> 5, all = threads * groups, stageBytes = Ring::kThread * all;
-    const RowSpan<E, W, BLOCK> at(t);
-    const unsigned             ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
-    f32x2                      dw[E / 2], db[E / 2];
+    constexpr int           kStages = Ring::kStages;
+    __shared__ float2       scratch[2][16]; // two halves, used in turn: one barrier per row
+    __shared__ float2       parts[2][8];    // of the CTAs of a cluster
+    extern __shared__ uint4 ring[];         // the stages; in the end the sums, [groups][2][columns]
+    const int       threads = blockDim.x, groups = blockDim.y;
+    const RowThread k    = row_thread<E, W, !WARP>(threadIdx.x, threads, threadIdx.y, groups);
+    const int       tid  = k.g * threads + k.t, warp = tid >> 5;
+    const int       xBytes = X::bytes(threads, groups), stageBytes = Ring::bytes(threads, groups);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int       ctas = WARP ? 1 : cluster.num_blocks(), rank = WARP ? 0 : cluster.block_rank();
+    const int       from = rank * span, end = WARP ? p.cols : min(p.cols - from, span); // this CTA's columns
+    const unsigned  ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
+    f32x2           dw[E / 2], db[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) dw[i] = db[i] = both(0.0f);
-    const unsigned long long step = static_cast<unsigned long long>(gridDim.x) * groups;
-    unsigned long long       r    = static_cast<unsigned long long>(blockIdx.x) * groups + g;
+    const unsigned long long step = static_cast<unsigned long long>(gridDim.x / ctas) * groups;
+    const unsigned long long base = static_cast<unsigned long long>(blockIdx.x / ctas) * groups;
+    unsigned long long       r    = base + k.g;
     int                      half = 0, stage = 0;
-    auto                     fetch = [&](int s, unsigned long long k) {
-        const bool live = k < p.rows;
-        X::fetch(ring0 + s * stageBytes, tid, all, live ? p.src.at(static_cast<unsigned>(k)) : nullptr, p.src.base, at.c, at.step, p.cols);
-        G::fetch(ring0 + s * stageBytes + X::kThread * all, tid, all, live ? p.grad.at(static_cast<unsigned>(k)) : nullptr, p.grad.base,
-                 at.c, at.step, p.cols);
+    auto xRow = [&](unsigned long long n) {
+        return n < p.rows ? p.src.at(static_cast<unsigned>(n)) + static_cast<long long>(from) * kElemBytes<SRC> : static_cast<const uint8_t *>(nullptr);
+    };
+    auto gRow = [&](unsigned long long n) {
+        return n < p.rows ? p.grad.at(static_cast<unsigned>(n)) + static_cast<long long>(from) * kElemBytes<GRAD> : static_cast<const uint8_t *>(nullptr);
+    };
+    auto fetch = [&](int s, unsigned long long n) {
+        X::fetch(ring0 + s * stageBytes, k, xRow(n), end);
+        G::fetch(ring0 + s * stageBytes + xBytes, k, gRow(n), end);
         copies_commit();
     };
-    if constexpr (kStaged)
-    {
+    auto meet = [&]() { // the threads of a row, where they read each other's copies
+        if constexpr (W == 0)
+        {
+            if constexpr (WARP)
+                __syncwarp();
+            else
+                __syncthreads();
+        }
+    };
 #pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) fetch(s, r + s * step);
-    }
+    for (int s = 0; s < kStages - 1; ++s) fetch(s, r + s * step);
     float nextMean = r < p.rows ? p.mean[r] : 0.0f, nextRstd = r < p.rows ? p.rstd[r] : 0.0f;
     // every thread of the CTA takes the same number of turns
-    for (unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * groups; first < p.rows; first += step, r += step)
+    for (unsigned long long first = base; first < p.rows; first += step, r += step)
     {
         const bool     live = r < p.rows; // a row that is not there, and what lies behind a row's end: x = dy = 0
         const unsigned row  = live ? static_cast<unsigned>(r) : 0;
         const float    mean = nextMean, rstd = nextRstd;
-        f32x2          h[E / 2], gv[E / 2], s1 = both(0.0f), s2 = both(0.0f);
+        f32x2          h[E / 2], gv[E / 2];
+        fetch(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
+        const bool more = r + step < p.rows;
+        nextMean        = more ? p.mean[r + step] : 0.0f;
+        nextRstd        = more ? p.rstd[r + step] : 0.0f;
+        copies_wait<kStages - 1>();
+        meet();
         {
-            if constexpr (kStaged)
-            {
-                fetch(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
-                copies_wait<kStages - 1>();
-            }
-            const bool more = r + step < p.rows;
-            nextMean        = more ? p.mean[r + step] : 0.0f;
-            nextRstd        = more ? p.rstd[r + step] : 0.0f;
-            float          f[E];
-            const uint8_t *from = reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes;
-            X::take(from, tid, all, X::kStaged || !live ? nullptr : p.src.at(row), at.c, at.step, p.cols, f);
-            pairs<E>(f, h);
-            G::take(from + X::kThread * all, tid, all, G::kStaged || !live ? nullptr : p.grad.at(row), at.c, at.step, p.cols, f);
-            pairs<E>(f, gv);
-            stage = stage == kStages - 1 ? 0 : stage + 1;
+            const uint8_t *at = reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes;
+            X::take(at, k, xRow(r), end, h);
+            G::take(at + xBytes, k, gRow(r), end, gv);
         }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
 #pragma unroll
         for (int i = 0; i < E / 2; ++i)
         {
@@ -105,20 +122,22 @@ __global__ void __launch_bounds__(BLOCK ? kGradResident : 256, BLOCK ? 1 : 2) la
             dw[i] = fma2(gv[i], h[i], dw[i]);
         }
         if (!p.dsrc.base)
+        {
+            meet();
             continue;
+        }
         if (p.weight) // from L1: there are no registers to keep it
         {
 #pragma unroll
-            for (int k = 0; k < E / 8; ++k)
+            for (int j = 0; j < E / 8; ++j)
             {
-                float f[8];
                 f32x2 w[4];
-                load_vecs<W, 8 / W>(p.weight, p.weightType, at.c + 8 / W * k * at.step, at.step, p.cols, f);
-                pairs<8>(f, w);
+                load_param<W>(p.weight, p.weightType, from + k.c + j * (8 / kStep<W>) * k.step, k.step, from + end, w);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) gv[4 * k + i] = mul2(gv[4 * k + i], w[i]);
+                for (int i = 0; i < 4; ++i) gv[4 * j + i] = mul2(gv[4 * j + i], w[i]);
             }
         }
+        f32x2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
         for (int i = 0; i < E / 2; ++i)
         {
@@ -126,53 +145,60 @@ __global__ void __launch_bounds__(BLOCK ? kGradResident : 256, BLOCK ? 1 : 2) la
             s2 = fma2(gv[i], h[i], s2);
         }
         float t1 = lo2(s1) + hi2(s1), t2 = lo2(s2) + hi2(s2);
-        if constexpr (BLOCK)
+        if constexpr (WARP)
         {
-            t1 = warp_sum(t1);
-            t2 = warp_sum(t2);
-            if ((t & 31) == 0)
-                scratch[half][warp] = make_float2(t1, t2);
-            __syncthreads();
-            t1 = t2 = 0.0f;
-            for (int k = 0; k < threads >> 5; ++k)
-            {
-                const float2 o = scratch[half][g * (threads >> 5) + k];
-                t1 += o.x;
-                t2 += o.y;
-            }
-            half ^= 1;
-        }
-        else
             for (int o = threads >> 1; o > 0; o >>= 1)
             {
                 t1 += __shfl_xor_sync(0xffffffffu, t1, o);
                 t2 += __shfl_xor_sync(0xffffffffu, t2, o);
             }
+            meet();
+        }
+        else
+        {
+            t1 = warp_sum(t1);
+            t2 = warp_sum(t2);
+            if ((k.t & 31) == 0)
+                scratch[half][warp] = make_float2(t1, t2);
+            __syncthreads();
+            t1 = t2 = 0.0f;
+            for (int i = 0; i < threads >> 5; ++i)
+            {
+                const float2 o = scratch[half][k.g * (threads >> 5) + i];
+                t1 += o.x;
+                t2 += o.y;
+            }
+            if (ctas > 1) // then there is one row at a time
+            {
+                if (k.t < ctas)
+                    *cluster.map_shared_rank(&parts[half][rank], k.t) = make_float2(t1, t2);
+                cluster.sync();
+                t1 = t2 = 0.0f;
+                for (int i = 0; i < ctas; ++i)
+                {
+                    t1 += parts[half][i].x;
+                    t2 += parts[half][i].y;
+                }
+            }
+            half ^= 1;
+        }
         if (!live)
             continue;
         const float c1 = t1 * p.invCols, c2 = t2 * p.invCols;
-        float       f[E];
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) gv[i] = mul2(add2(fma2(h[i], both(-c2), gv[i]), both(-c1)), both(rstd));
-        singles<E>(gv, f);
-        store_vecs<W, V>(p.dsrc.at(row), p.dsrcType, at.c, at.step, p.cols, f);
+        store_row<E, W>(p.dsrc.at(row) + static_cast<long long>(from) * (p.dsrcType == B200PP_F32 ? 4 : 2), p.dsrcType, k, end, gv);
     }
+    if (ctas > 1)
+        cluster.sync(); // no CTA leaves while another may still write to it
     if (!p.partials)
         return;
-    if constexpr (kStaged)
-    {
-        copies_wait<0>(); // the sums take the ring's place
-        __syncthreads();
-    }
-    // the CTA's sums: over the rows of a warp by shuffles, over the warps (BLOCK: over the rows) one after another
-    float    *part  = p.partials + static_cast<long long>(blockIdx.x) * 2 * p.cols;
-    int       slot  = g, slots = groups;
-    bool      holds = true;
-    float     fw[E], fb[E];
+    // the CTA's sums: over the rows of a warp by shuffles, then over the row groups (WARP: the warps) through shared memory
+    copies_wait<0>();
+    float fw[E], fb[E];
     singles<E>(dw, fw);
     singles<E>(db, fb);
-    if constexpr (!BLOCK)
-    {
+    if constexpr (WARP)
         for (int o = threads; o < 32; o <<= 1)
 #pragma unroll
             for (int e = 0; e < E; ++e)
@@ -180,27 +206,37 @@ __global__ void __launch_bounds__(BLOCK ? kGradResident : 256, BLOCK ? 1 : 2) la
                 fw[e] += __shfl_xor_sync(0xffffffffu, fw[e], o);
                 fb[e] += __shfl_xor_sync(0xffffffffu, fb[e], o);
             }
-        slot  = warp;
-        slots = (threads * groups) >> 5;
-        holds = (tid & 31) < threads;
-    }
-    for (int s = 0; s < slots; ++s)
+    const int  slot = WARP ? warp : k.g, slots = WARP ? (threads * groups) >> 5 : groups;
+    const bool holds = !WARP || (tid & 31) < threads;
+    const int  columns = WARP ? p.cols : span;
+    float     *sums = reinterpret_cast<float *>(ring);
+    float     *part = p.partials + static_cast<long long>(blockIdx.x / ctas) * 2 * p.cols + from;
+    __syncthreads(); // the ring is not needed any more
+    if (holds)
     {
-        if (slot == s && holds)
-        {
-            float *to = s + 1 < slots ? sums : part;
+        float *to = slots > 1 ? sums + slot * 2 * columns : part;
+        const int next = slots > 1 ? columns : p.cols;
 #pragma unroll
-            for (int e = 0; e < E; ++e)
+        for (int e = 0; e < E; ++e)
+        {
+            const int c = k.c + e / kStep<W> * k.step + e % kStep<W>;
+            if (c < end)
             {
-                const int c = at.c + e / W * at.step + e % W;
-                if (c < p.cols)
-                {
-                    to[c]          = s > 0 ? sums[c] + fw[e] : fw[e];
-                    to[p.cols + c] = s > 0 ? sums[p.cols + c] + fb[e] : fb[e];
-                }
+                to[c]        = fw[e];
+                to[next + c] = fb[e];
             }
         }
-        __syncthreads();
+    }
+    if (slots == 1)
+        return;
+    __syncthreads();
+    for (int c = tid; c < 2 * columns; c += threads * groups)
+    {
+        float s = 0.0f;
+        for (int i = 0; i < slots; ++i) s += sums[i * 2 * columns + c];
+        const int col = c < columns ? c : c - columns;
+        if (col < end)
+            part[c < columns ? col : p.cols + col] = s;
     }
 }
 

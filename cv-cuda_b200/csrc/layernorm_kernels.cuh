@@ -7,6 +7,8 @@
 
 #include "row_math.cuh"
 
+#include <cooperative_groups.h>
+
 namespace b200pp {
 
 struct LayerNormKParams
@@ -22,20 +24,9 @@ struct LayerNormKParams
     float2        *partials; // [rows][chunks]
 };
 
-// A thread holds E values of its row, as vectors of W neighbouring elements: lane l of warp k of the row has vectors l, l + 32, ...
-// of the warp's 32 E elements, so that every load and store of a warp covers one contiguous span, at offsets known at compile
-// time. (Rows of fewer than 32 lanes: l, l + lanes, ...)
-template<int E, int W, bool BLOCK>
-struct RowSpan
-{
-    int c, step; // first element of the thread, distance to its next vector
-
-    __device__ __forceinline__ explicit RowSpan(int t)
-        : c(BLOCK ? (t >> 5) * (32 * E) + (t & 31) * W : t * W)
-        , step(BLOCK || E > 8 ? 32 * W : static_cast<int>(blockDim.x) * W)
-    {
-    }
-};
+// Elements a thread's vectors are made of: W, or pairs where rows start anywhere (W = 0).
+template<int W>
+constexpr int kStep = W ? W : 2;
 
 // Sum over the `lanes` neighbouring lanes (a power of two) a row has in a warp, or over the block.
 template<bool BLOCK>
@@ -62,45 +53,12 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *scratch)
 template<int W>
 __device__ __forceinline__ void layernorm_affine(const LayerNormKParams &p, int c, int step, int end, f32x2 *w, f32x2 *b)
 {
-    float v[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = both(1.0f), b[i] = both(0.0f);
     if (p.weight)
-    {
-        load_vecs<W, 8 / W>(p.weight, p.weightType, c, step, end, v);
-        pairs<8>(v, w);
-    }
+        load_param<W>(p.weight, p.weightType, c, step, end, w);
     if (p.bias)
-    {
-        load_vecs<W, 8 / W>(p.bias, p.biasType, c, step, end, v);
-        pairs<8>(v, b);
-    }
-}
-
-// y of eight values, given their distances d to the mean.
-template<int W>
-__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const f32x2 *d, float rstd, const f32x2 *w,
-                                                const f32x2 *b, int c, int step, int end)
-{
-    f32x2 o[4];
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = fma2(mul2(d[i], both(rstd)), w[i], b[i]);
-    singles<8>(o, v);
-    store_vecs<W, 8 / W>(y, p.dstType, c, step, end, v);
-}
-
-// y of a thread's values, eight at a time.
-template<int E, int W>
-__device__ __forceinline__ void layernorm_store(const LayerNormKParams &p, uint8_t *y, const f32x2 *d, float rstd, int c, int step, int end)
-{
-#pragma unroll
-    for (int k = 0; k < E / 8; ++k, c += 8 / W * step)
-    {
-        f32x2 w[4], b[4];
-        layernorm_affine<W>(p, c, step, end, w, b);
-        layernorm_store<W>(p, y, d + 4 * k, rstd, w, b, c, step, end);
-    }
+        load_param<W>(p.bias, p.biasType, c, step, end, b);
 }
 
 // Sum of a thread's values; the values that lie behind the row's end are zero.
@@ -122,13 +80,13 @@ __device__ __forceinline__ float sum_pairs(const f32x2 *x)
 template<int E, int W>
 __device__ __forceinline__ float centre(f32x2 *x, float mean, int c, int step, int end)
 {
-    if (c + (E / W - 1) * step >= end) // part of them lies behind the end
+    if (c + (E / W - 1) * step + W > end) // part of them lies behind the end
     {
         float v[E];
         singles<E>(x, v);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (c + e / W * step >= end)
+            if (c + e / W * step + e % W >= end)
                 v[e] = mean;
         pairs<E>(v, x);
     }
@@ -145,9 +103,9 @@ __device__ __forceinline__ float centre(f32x2 *x, float mean, int c, int step, i
     return lo2(a) + hi2(a);
 }
 
-// Forward, a warp per row, or part of one for up to 256 columns (eight values a lane): blockDim.x lanes per row, blockDim.y rows
-// per CTA. A warp walks down its share of the rows with the weights in registers; the rows ahead are on their way through shared
-// memory. The statistics come from the registers (the variance about the mean), so the row is read once.
+// Forward, `blockDim.x` lanes of a warp per row (a power of two), blockDim.y rows per CTA, E values per lane. A warp walks down its
+// share of the rows with the weights in registers; the rows ahead are on their way through shared memory. The statistics come from
+// the registers (the variance about the mean), so the row is read once.
 constexpr int kWarpStages = 3;
 
 template<int E>
@@ -156,86 +114,181 @@ constexpr int kWarpCtas = E <= 8 ? 4 : E <= 16 ? 3 : 2; // of 256 threads on an 
 template<int SRC, int E, int W>
 __global__ void __launch_bounds__(256, kWarpCtas<E>) layernorm_warp_kernel(const LayerNormKParams p)
 {
-    typedef RowStage<SRC, W, E / W> Stage;
-    extern __shared__ uint4         ring[];
-    constexpr int                   kStage = Stage::kThread * 256;
-    const int                       t = threadIdx.x, lanes = E > 8 ? 32 : blockDim.x, tid = threadIdx.y * lanes + t;
-    const RowSpan<E, W, false>      at(t);
-    const unsigned                  ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
-    f32x2                           w[E / 2], b[E / 2];
+    typedef RowStage<SRC, E, W> Stage;
+    extern __shared__ uint4     ring[];
+    const int                   lanes = E == 32 ? 32 : blockDim.x, stageBytes = Stage::bytes(lanes, blockDim.y);
+    const RowThread             k     = row_thread<E, W, E == 32>(threadIdx.x, lanes, threadIdx.y, blockDim.y);
+    const unsigned              ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
+    f32x2                       w[E / 2], b[E / 2];
 #pragma unroll
-    for (int k = 0; k < E / 8; ++k)
-        layernorm_affine<W>(p, at.c + 8 / W * k * at.step, at.step, p.cols, w + 4 * k, b + 4 * k);
+    for (int i = 0; i < E / 8; ++i)
+        layernorm_affine<W>(p, k.c + 8 / kStep<W> * i * k.step, k.step, p.cols, w + 4 * i, b + 4 * i);
     const unsigned long long step = static_cast<unsigned long long>(gridDim.x) * blockDim.y;
     const unsigned long long r0   = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    auto                     row  = [&](unsigned long long r) { return r < p.rows ? p.src.at(static_cast<unsigned>(r)) : nullptr; };
-    if constexpr (Stage::kStaged)
-    {
+    auto row = [&](unsigned long long r) { return r < p.rows ? p.src.at(static_cast<unsigned>(r)) : static_cast<const uint8_t *>(nullptr); };
 #pragma unroll
-        for (int s = 0; s < kWarpStages - 1; ++s)
-        {
-            Stage::fetch(ring0 + s * kStage, tid, 256, row(r0 + s * step), p.src.base, at.c, at.step, p.cols);
-            copies_commit();
-        }
+    for (int s = 0; s < kWarpStages - 1; ++s)
+    {
+        Stage::fetch(ring0 + s * stageBytes, k, row(r0 + s * step), p.cols);
+        copies_commit();
     }
     int stage = 0;
     // the lanes of a warp take the same number of turns: those of the warp's first row
     for (unsigned long long r = r0, first = r0 - threadIdx.y % (32u / lanes); first < p.rows; r += step, first += step)
     {
+        Stage::fetch(ring0 + (stage == 0 ? kWarpStages - 1 : stage - 1) * stageBytes, k, row(r + (kWarpStages - 1) * step), p.cols);
+        copies_commit();
+        copies_wait<kWarpStages - 1>();
+        if (W == 0)
+            __syncwarp();
         f32x2 x[E / 2];
-        {
-            float v[E];
-            if constexpr (Stage::kStaged)
-            {
-                const int ahead = stage == 0 ? kWarpStages - 1 : stage - 1;
-                Stage::fetch(ring0 + ahead * kStage, tid, 256, row(r + (kWarpStages - 1) * step), p.src.base, at.c, at.step, p.cols);
-                copies_commit();
-                copies_wait<kWarpStages - 1>();
-            }
-            Stage::take(reinterpret_cast<const uint8_t *>(ring) + stage * kStage, tid, 256, Stage::kStaged ? nullptr : row(r), at.c, at.step,
-                        p.cols, v);
-            stage = stage == kWarpStages - 1 ? 0 : stage + 1;
-            pairs<E>(v, x);
-        }
+        Stage::take(reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes, k, row(r), p.cols, x);
+        stage = stage == kWarpStages - 1 ? 0 : stage + 1;
+        if (W == 0)
+            __syncwarp();
         const float mean = divide_count(row_sum<false>(sum_pairs<E>(x), lanes, nullptr), p.fcols, p.invCols);
-        const float q    = centre<E, W>(x, mean, at.c, at.step, p.cols);
+        const float q    = centre<E, kStep<W>>(x, mean, k.c, k.step, p.cols);
         const float rstd = rsqrtf(row_sum<false>(q, lanes, nullptr) * p.invCols + p.epsilon);
         if (r >= p.rows)
             continue;
-        if (t == 0)
+        if (k.t == 0)
         {
             if (p.mean)
                 p.mean[r] = mean;
             if (p.rstd)
                 p.rstd[r] = rstd;
         }
-        float v[E];
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) x[i] = fma2(mul2(x[i], both(rstd)), w[i], b[i]);
-        singles<E>(x, v);
-        store_vecs<W, E / W>(p.dst.at(static_cast<unsigned>(r)), p.dstType, at.c, at.step, p.cols, v);
+        store_row<E, W>(p.dst.at(static_cast<unsigned>(r)), p.dstType, k, p.cols, x);
     }
 }
 
-// Forward, a CTA per row.
+// Forward, longer rows: a CTA per row, or a cluster of up to eight CTAs with `span` columns each, which walk down their share of the
+// rows together. Each CTA takes the mean and the squares of its part; the parts are joined as Chan, Golub and LeVeque do (the mean
+// weighted by length, the squares plus the distances of the means) after one exchange through distributed shared memory. With
+// sixteen values per thread the weights stay in registers; thirty-two are for rows that sixteen do not reach.
+template<int E>
+constexpr int kClusterThreads = E <= 16 ? 512 : 768; // most threads of a CTA, by the registers they need
+template<int E>
+constexpr int kClusterStages = E <= 16 ? 3 : 2;
+
 template<int SRC, int E, int W>
-__global__ void __launch_bounds__(E <= 16 ? 512 : 1024) layernorm_block_kernel(const LayerNormKParams p)
+__global__ void __launch_bounds__(kClusterThreads<E>, 1) layernorm_cluster_kernel(const LayerNormKParams p, int span)
 {
-    __shared__ float          scratch[2][32];
-    const unsigned            r = blockIdx.x;
-    const RowSpan<E, W, true> at(threadIdx.x);
-    f32x2                     x[E / 2];
+    namespace cg = cooperative_groups;
+    typedef RowStage<SRC, E, W> Stage;
+    constexpr int               kStages = kClusterStages<E>;
+    extern __shared__ uint4     ring[];
+    __shared__ float            scratch[2][32];
+    __shared__ float2           parts[2][8];
+    cg::cluster_group           cluster = cg::this_cluster();
+    const int                   ctas = cluster.num_blocks(), rank = cluster.block_rank(), stageBytes = Stage::bytes(blockDim.x, 1);
+    const int                   from = rank * span, end = min(p.cols - from, span); // this CTA's columns
+    const RowThread             k     = row_thread<E, W, true>(threadIdx.x, blockDim.x, 0, 1);
+    const unsigned              ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
+    f32x2                       w[E <= 16 ? E / 2 : 4], b[E <= 16 ? E / 2 : 4];
+    if constexpr (E <= 16)
     {
-        float v[E];
-        load_vecs<SRC, W, E / W>(p.src.at(r), at.c, at.step, p.cols, v);
-        pairs<E>(v, x);
+#pragma unroll
+        for (int i = 0; i < E / 8; ++i)
+            layernorm_affine<W>(p, from + k.c + 8 / kStep<W> * i * k.step, k.step, from + end, w + 4 * i, b + 4 * i);
     }
-    // with eight values there are registers left to fetch the weights at the same time as the row
-    f32x2 w[4], b[4];
-    if constexpr (E == 8)
-        layernorm_affine<W>(p, at.c, at.step, p.cols, w, b);
-    const float mean = divide_count(row_sum<true>(sum_pairs<E>(x), 0, scratch[0]), p.fcols, p.invCols);
-    const float q    = centre<E, W>(x, mean, at.c, at.step, p.cols);
+    const unsigned long long step = gridDim.x / ctas;
+    unsigned long long       r    = blockIdx.x / ctas;
+    auto                     row  = [&](unsigned long long n) {
+        return n < p.rows ? p.src.at(static_cast<unsigned>(n)) + static_cast<long long>(from) * kElemBytes<SRC> : static_cast<const uint8_t *>(nullptr);
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s)
+    {
+        Stage::fetch(ring0 + s * stageBytes, k, row(r + s * step), end);
+        copies_commit();
+    }
+    const float n     = static_cast<float>(end), inv = 1.0f / n;
+    int         stage = 0, half = 0;
+    for (; r < p.rows; r += step)
+    {
+        // the stage before was read by every thread before a barrier of the last turn
+        Stage::fetch(ring0 + (stage == 0 ? kStages - 1 : stage - 1) * stageBytes, k, row(r + (kStages - 1) * step), end);
+        copies_commit();
+        copies_wait<kStages - 1>();
+        if (W == 0)
+            __syncthreads();
+        f32x2 x[E / 2];
+        Stage::take(reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes, k, row(r), end, x);
+        stage        = stage == kStages - 1 ? 0 : stage + 1;
+        float mean   = divide_count(row_sum<true>(sum_pairs<E>(x), 0, scratch[0]), n, inv);
+        float q      = row_sum<true>(centre<E, kStep<W>>(x, mean, k.c, k.step, end), 0, scratch[1]);
+        float centre = 0.0f; // distance of this CTA's mean to the row's
+        if (ctas > 1)
+        {
+            if (static_cast<int>(threadIdx.x) < ctas)
+                *cluster.map_shared_rank(&parts[half][rank], threadIdx.x) = make_float2(mean, q);
+            cluster.sync();
+            float sum = 0.0f;
+            for (int c = 0; c < ctas; ++c) sum += parts[half][c].x * static_cast<float>(min(p.cols - c * span, span));
+            const float whole = divide_count(sum, p.fcols, p.invCols);
+            q                 = 0.0f;
+            for (int c = 0; c < ctas; ++c)
+            {
+                const float d = parts[half][c].x - whole;
+                q += parts[half][c].y + d * d * static_cast<float>(min(p.cols - c * span, span));
+            }
+            centre = mean - whole;
+            mean   = whole;
+            half ^= 1; // the next turn's parts come while slower CTAs read these
+        }
+        const float rstd = rsqrtf(q * p.invCols + p.epsilon);
+        if (rank == 0 && threadIdx.x == 0)
+        {
+            if (p.mean)
+                p.mean[r] = mean;
+            if (p.rstd)
+                p.rstd[r] = rstd;
+        }
+        uint8_t *y = p.dst.at(static_cast<unsigned>(r)) + static_cast<long long>(from) * (p.dstType == B200PP_F32 ? 4 : 2);
+        if constexpr (E <= 16)
+        {
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) x[i] = fma2(mul2(add2(x[i], both(centre)), both(rstd)), w[i], b[i]);
+        }
+        else
+        {
+#pragma unroll
+            for (int j = 0; j < E / 8; ++j)
+            {
+                if (p.weight || p.bias)
+                    layernorm_affine<W>(p, from + k.c + 8 / kStep<W> * j * k.step, k.step, from + end, w, b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const f32x2 h = mul2(add2(x[4 * j + i], both(centre)), both(rstd));
+                    x[4 * j + i]  = p.weight || p.bias ? fma2(h, w[i], b[i]) : h;
+                }
+            }
+        }
+        store_row<E, W>(y, p.dstType, k, end, x);
+    }
+    if (ctas > 1)
+        cluster.sync(); // no CTA leaves while another may still write to it
+}
+
+// Forward, a CTA per row and eight values per thread, for so few rows that only latency counts: the weights are fetched at the same
+// time as the row.
+template<int SRC, int W>
+__global__ void __launch_bounds__(512) layernorm_few_kernel(const LayerNormKParams p)
+{
+    __shared__ float scratch[2][32];
+    const unsigned   r = blockIdx.x;
+    const RowThread  k = row_thread<8, W, true>(threadIdx.x, blockDim.x, 0, 1);
+    f32x2            x[4], w[4], b[4];
+    float            v[8];
+    load_vecs<SRC, W, 8 / W>(p.src.at(r), k.c, k.step, p.cols, v);
+    layernorm_affine<W>(p, k.c, k.step, p.cols, w, b);
+    pairs<8>(v, x);
+    const float mean = divide_count(row_sum<true>(sum_pairs<8>(x), 0, scratch[0]), p.fcols, p.invCols);
+    const float q    = centre<8, W>(x, mean, k.c, k.step, p.cols);
     const float rstd = rsqrtf(row_sum<true>(q, 0, scratch[1]) * p.invCols + p.epsilon);
     if (threadIdx.x == 0)
     {
@@ -244,14 +297,14 @@ __global__ void __launch_bounds__(E <= 16 ? 512 : 1024) layernorm_block_kernel(c
         if (p.rstd)
             p.rstd[r] = rstd;
     }
-    if constexpr (E == 8)
-        layernorm_store<W>(p, p.dst.at(r), x, rstd, w, b, at.c, at.step, p.cols);
-    else
-        layernorm_store<E, W>(p, p.dst.at(r), x, rstd, at.c, at.step, p.cols);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fma2(mul2(x[i], both(rstd)), w[i], b[i]);
+    singles<8>(x, v);
+    store_vecs<W, 8 / W>(p.dst.at(r), p.dstType, k.c, k.step, p.cols, v);
 }
 
-// Forward, longer rows: two kernels over chunks of kChunk values. The first leaves each chunk's mean and sum of squared distances
-// to it; the second joins those of its row (as Chan, Golub and LeVeque do for two sets) and normalises its chunk. It takes the
+// Forward, rows too long for that, or long and few: two kernels over chunks of kChunk values. The first leaves each chunk's mean and
+// sum of squared distances to it; the second joins those of its row, likewise, and normalises its chunk. It takes the
 // chunks in reverse order, so that the ones read last by the first kernel are still in L2.
 constexpr int kChunk        = 8192;
 constexpr int kChunkThreads = 256;
@@ -265,7 +318,7 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_stats_kernel(co
     const long long  at  = static_cast<long long>(blockIdx.x - r * p.chunks) * kChunk;
     const int        c0  = static_cast<int>(at);
     const int        end = min(static_cast<long long>(p.cols), at + kChunk);
-    const RowSpan<E, W, true> span(threadIdx.x);
+    const RowThread           span = row_thread<E, W, true>(threadIdx.x, kChunkThreads, 0, 1);
     f32x2                     x[E / 2];
     {
         float v[E];
@@ -288,7 +341,7 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
     const long long  at  = static_cast<long long>(job - r * p.chunks) * kChunk;
     const int        c0  = static_cast<int>(at);
     const int        end = min(static_cast<long long>(p.cols), at + kChunk);
-    const RowSpan<E, W, true> span(threadIdx.x);
+    const RowThread           span = row_thread<E, W, true>(threadIdx.x, kChunkThreads, 0, 1);
     f32x2                     x[E / 2];
     {
         float v[E];
@@ -316,7 +369,19 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
     }
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) x[i] = add2(x[i], both(-mean));
-    layernorm_store<E, W>(p, p.dst.at(r), x, rstd, c0 + span.c, span.step, end);
+    uint8_t *y = p.dst.at(r);
+#pragma unroll
+    for (int j = 0; j < E / 8; ++j)
+    {
+        const int c = c0 + span.c + 8 / W * j * span.step;
+        f32x2     w[4], b[4];
+        float     v[8];
+        layernorm_affine<W>(p, c, span.step, end, w, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = fma2(mul2(x[4 * j + i], both(rstd)), w[i], b[i]);
+        singles<8>(w, v);
+        store_vecs<W, 8 / W>(y, p.dstType, c, span.step, end, v);
+    }
 }
 
 } // namespace b200pp

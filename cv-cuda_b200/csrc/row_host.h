@@ -5,8 +5,12 @@
 #include "host_common.h"
 #include "row_math.cuh"
 
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 namespace b200pp {
 
@@ -181,6 +185,57 @@ int raise_smem(K kernel, int bytes, std::atomic<unsigned long long> &done)
     done.fetch_or(bit);
     return B200PP_SUCCESS;
 }
+
+// A launch in clusters of `ctas` CTAs.
+struct ClusterLaunch
+{
+    cudaLaunchConfig_t    cfg{};
+    cudaLaunchAttribute   attr{};
+
+    ClusterLaunch(int ctas, int threads, int smem, cudaStream_t stream)
+    {
+        cfg.blockDim         = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream           = stream;
+        attr.id              = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim  = {static_cast<unsigned>(ctas), 1, 1};
+        cfg.attrs            = &attr;
+        cfg.numAttrs         = 1;
+        cfg.gridDim          = dim3(ctas);
+    }
+
+    ClusterLaunch(const ClusterLaunch &) = delete;
+
+    // As many clusters as are resident at a time, at most one per row. How many that is depends on how the SMs are grouped, so
+    // the runtime is asked, once per shape.
+    template<typename K>
+    void fill(K kernel, unsigned rows)
+    {
+        static std::mutex                            mu;
+        static std::map<std::tuple<const void *, int, unsigned, unsigned, size_t>, int> known;
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const unsigned ctas = attr.val.clusterDim.x;
+        const auto     key  = std::make_tuple(reinterpret_cast<const void *>(kernel), dev, ctas, cfg.blockDim.x, cfg.dynamicSmemBytes);
+        int            most = 0;
+        {
+            std::lock_guard<std::mutex> lock(mu);
+            auto                        it = known.find(key);
+            if (it == known.end())
+            {
+                if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1)
+                {
+                    cudaGetLastError();
+                    most = kSms / static_cast<int>(ctas);
+                }
+                known[key] = most;
+            }
+            else
+                most = it->second;
+        }
+        cfg.gridDim.x = ctas * std::min(rows, static_cast<unsigned>(most));
+    }
+};
 
 } // namespace b200pp
 

@@ -323,89 +323,6 @@ __device__ __forceinline__ void store_vecs(uint8_t *row, int dtype, int c, int s
         store_vecs<B200PP_F16, W, N>(row, c, step, end, v);
 }
 
-// ---- rows on their way through shared memory: each thread copies its own vectors of the rows ahead with asynchronous copies and
-// reads them back itself, so there is nothing to synchronise and no register is held while HBM answers. Vectors of fewer than four
-// bytes cannot be copied like that; they are loaded when they are needed.
-
-template<int BYTES>
-__device__ __forceinline__ void copy_async(unsigned dst, const uint8_t *src, bool there)
-{
-    const int n = there ? BYTES : 0; // what is not there becomes zeros
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
-}
-
-__device__ __forceinline__ void copies_commit()
-{
-    asm volatile("cp.async.commit_group;" ::: "memory");
-}
-
-// All but the N latest groups are there.
-template<int N>
-__device__ __forceinline__ void copies_wait()
-{
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// The part of a ring that belongs to one tensor: V vectors of W elements for each of the CTA's threads.
-template<int DT, int W, int V>
-struct RowStage
-{
-    static constexpr int  kBytes  = kElemBytes<DT> * W;
-    static constexpr bool kStaged = kBytes >= 4;
-    static constexpr int  kPart = kBytes > 16 ? 16 : kBytes, kParts = kBytes / kPart;
-    static constexpr int  kThread = kStaged ? kBytes * V : 0; // bytes per thread and stage
-
-    // `stage`: shared-memory address of the stage; `row`: the row, null if there is none
-    static __device__ __forceinline__ void fetch(unsigned stage, int tid, int threads, const uint8_t *row, const uint8_t *valid, int c,
-                                                 int step, int end)
-    {
-        if constexpr (kStaged)
-        {
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-#pragma unroll
-                for (int k = 0; k < kParts; ++k)
-                {
-                    const bool there = row != nullptr && c + v * step < end;
-                    copy_async<kPart>(stage + ((v * kParts + k) * threads + tid) * kPart,
-                                      there ? row + static_cast<long long>(c + v * step) * kElemBytes<DT> + k * kPart : valid, there);
-                }
-        }
-    }
-
-    // the thread's values, from the ring or (vectors that are not staged) from the row itself
-    static __device__ __forceinline__ void take(const uint8_t *stage, int tid, int threads, const uint8_t *row, int c, int step, int end,
-                                                float *out)
-    {
-        Vec<DT, W> raw[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-        {
-            if constexpr (kStaged)
-            {
-#pragma unroll
-                for (int k = 0; k < kParts; ++k)
-                {
-                    const RawVec<kPart> part = load_raw<kPart>(stage + ((v * kParts + k) * threads + tid) * kPart);
-#pragma unroll
-                    for (int i = 0; i < kPart / 4; ++i) raw[v].w[k * (kPart / 4) + i] = part.w[i];
-                }
-            }
-            else
-            {
-                raw[v] = zero_raw<kBytes>();
-                if (row != nullptr && c + v * step < end)
-                    raw[v] = load_raw<kBytes>(row + static_cast<long long>(c + v * step) * kElemBytes<DT>);
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) unpack<DT, W>(raw[v], out + v * W);
-    }
-};
-
 // ---- two float32 values in a 64-bit register: sm_100 adds, multiplies and fuses both with one instruction, each rounded as the
 // scalar instruction rounds it. The row operators' kernels issue about as many instructions as HBM gives them time for, so this
 // counts.
@@ -486,6 +403,216 @@ __device__ __forceinline__ float block_sum(float v, float *scratch)
     __syncthreads();
     float s = (threadIdx.x & 31) < warps ? scratch[threadIdx.x & 31] : 0.0f;
     return warp_sum(s);
+}
+
+// ---- rows on their way through shared memory
+
+template<int BYTES>
+__device__ __forceinline__ void copy_async(unsigned dst, const uint8_t *src, int n)
+{
+    // n bytes of BYTES, zeros after them
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+
+__device__ __forceinline__ void copies_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// All but the N latest groups are there.
+template<int N>
+__device__ __forceinline__ void copies_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Who a thread is: thread t of the `threads` of a row (a power of two below 32, or whole warps), row group g of the CTA; a row's values are dealt out as vectors, the
+// thread's first at element c, `step` elements apart.
+struct RowThread
+{
+    int t, threads, g, groups, c, step;
+};
+
+// One stage of one tensor for all row groups of a CTA. E values per thread as vectors of W, W dividing the row and everything
+// aligned to it: each thread copies its own vectors and reads them back itself, so there is nothing to synchronise and no register
+// is held while HBM answers.
+template<int DT, int E, int W>
+struct RowStage
+{
+    static constexpr int kVec = kElemBytes<DT> * W, V = E / W; // 4 to 16 bytes
+
+    static __host__ __device__ constexpr int bytes(int threads, int groups)
+    {
+        return kVec * V * threads * groups;
+    }
+
+    // `row`: null if there is none; `end`: elements of the row
+    static __device__ __forceinline__ void fetch(unsigned stage, const RowThread &k, const uint8_t *row, int end)
+    {
+        const int tid = k.g * k.threads + k.t, all = k.threads * k.groups;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (row && k.c + v * k.step < end)
+                copy_async<kVec>(stage + (v * all + tid) * kVec, row + static_cast<long long>(k.c + v * k.step) * kElemBytes<DT>, kVec);
+    }
+
+    // The thread's values, zeros behind the row's end.
+    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *row, int end, f32x2 *out)
+    {
+        const int   tid = k.g * k.threads + k.t, all = k.threads * k.groups;
+        Vec<DT, W>  raw[V];
+        float       f[E];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+        {
+            raw[v] = zero_raw<kVec>();
+            if (row && k.c + v * k.step < end)
+                raw[v] = load_raw<kVec>(stage + (v * all + tid) * kVec);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) unpack<DT, W>(raw[v], f + v * W);
+        pairs<E>(f, out);
+    }
+};
+
+// The same for rows that start anywhere (W = 0): the 16-byte lines a row touches are copied as they are, by whichever thread of the
+// row, and each thread picks its pairs of elements out of them. (The first line may begin with bytes before the row: those of the
+// row before it, or, before the first row, of the same 16 bytes of memory as its first element.) The threads of a row have to meet
+// between the copies' end and `take`, and between `take` and the next copies to the stage.
+template<int DT, int E>
+struct RowStage<DT, E, 0>
+{
+    static constexpr int kSize = kElemBytes<DT>;
+
+    static __host__ __device__ constexpr int group_bytes(int threads)
+    {
+        return (threads * E * kSize + 15) / 16 * 16 + 32; // the lines, and a word more for the last pair
+    }
+
+    static __host__ __device__ constexpr int bytes(int threads, int groups)
+    {
+        return group_bytes(threads) * groups;
+    }
+
+    static __device__ __forceinline__ void fetch(unsigned stage, const RowThread &k, const uint8_t *row, int end)
+    {
+        if (!row)
+            return;
+        const int            off   = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
+        const int            bytes = off + min(end, k.threads * E) * kSize;
+        const unsigned       to    = stage + k.g * group_bytes(k.threads);
+        const uint8_t *const line  = row - off;
+        for (int q = k.t * 16; q < bytes; q += k.threads * 16) copy_async<16>(to + q, line + q, min(16, bytes - q));
+    }
+
+    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *row, int end, f32x2 *out)
+    {
+        const int       off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
+        const unsigned *w   = reinterpret_cast<const unsigned *>(stage + k.g * group_bytes(k.threads));
+#pragma unroll
+        for (int v = 0; v < E / 2; ++v)
+        {
+            const int c = k.c + v * k.step;
+            float     f[2] = {0.0f, 0.0f};
+            if (row && c < end)
+            {
+                const int      at = off + c * kSize;
+                const unsigned w0 = w[at >> 2], w1 = w[(at >> 2) + 1];
+                if constexpr (kSize == 4)
+                {
+                    f[0] = __uint_as_float(w0);
+                    f[1] = __uint_as_float(w1);
+                }
+                else
+                {
+                    const unsigned bits = __funnelshift_r(w0, w1, (at & 3) * 8);
+                    if constexpr (kSize == 2)
+                    {
+                        Vec<DT, 2> r;
+                        r.w[0] = bits;
+                        unpack<DT, 2>(r, f);
+                    }
+                    else
+                    {
+                        f[0] = static_cast<float>(bits & 0xffu);
+                        f[1] = static_cast<float>((bits >> 8) & 0xffu);
+                    }
+                }
+                if (c + 1 >= end)
+                    f[1] = 0.0f;
+            }
+            out[v] = make2(f[0], f[1]);
+        }
+    }
+};
+
+// How the threads of a row are laid out over its elements: with `lanes` = 32 or more, warp by warp, 32 E elements each; below, lane
+// by lane. W = 0 goes by pairs.
+// (WHOLE: whole warps, which lets the compiler know the distance between a thread's vectors.)
+template<int E, int W, bool WHOLE>
+__device__ __forceinline__ RowThread row_thread(int t, int threads, int g, int groups)
+{
+    constexpr int kW    = W ? W : 2;
+    const int     lanes = WHOLE ? 32 : threads;
+    return {t, threads, g, groups, (WHOLE ? (t >> 5) * (32 * E) + (t & 31) * kW : t * kW), lanes * kW};
+}
+
+// Eight neighbouring-by-vector values of a parameter (weight, bias), from the thread's vector at element c on.
+template<int W>
+__device__ __forceinline__ void load_param(const uint8_t *p, int dtype, int c, int step, int end, f32x2 *out)
+{
+    float f[8];
+    if constexpr (W > 0)
+        load_vecs<W, 8 / W>(p, dtype, c, step, end, f);
+    else
+    {
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+        {
+            f[2 * v]     = c + v * step < end ? load_elem(p, c + v * step, dtype) : 0.0f;
+            f[2 * v + 1] = c + v * step + 1 < end ? load_elem(p, c + v * step + 1, dtype) : 0.0f;
+        }
+    }
+    pairs<8>(f, out);
+}
+
+// A thread's values to its row.
+template<int DT, int E>
+__device__ __forceinline__ void store_pairs(uint8_t *row, int c, int step, int end, const float *f)
+{
+    const bool whole = (reinterpret_cast<uintptr_t>(row) & (2 * kElemBytes<DT> - 1)) == 0; // pairs start on even elements
+#pragma unroll
+    for (int v = 0; v < E / 2; ++v)
+    {
+        const int at = c + v * step;
+        if (whole && at + 1 < end)
+            store_vec<DT, 2>(row, at, f + 2 * v);
+        else
+        {
+            if (at < end)
+                store_elem_as<DT>(row, at, f[2 * v]);
+            if (at + 1 < end)
+                store_elem_as<DT>(row, at + 1, f[2 * v + 1]);
+        }
+    }
+}
+
+template<int E, int W>
+__device__ __forceinline__ void store_row(uint8_t *row, int dtype, const RowThread &k, int end, const f32x2 *x)
+{
+    float f[E];
+    singles<E>(x, f);
+    if constexpr (W > 0)
+        store_vecs<W, E / W>(row, dtype, k.c, k.step, end, f);
+    else if (dtype == B200PP_F32)
+        store_pairs<B200PP_F32, E>(row, k.c, k.step, end, f);
+    else if (dtype == B200PP_BF16)
+        store_pairs<B200PP_BF16, E>(row, k.c, k.step, end, f);
+    else
+        store_pairs<B200PP_F16, E>(row, k.c, k.step, end, f);
 }
 
 // s / n for a count n and inv = 1 / n rounded: one step of division by residual. A sum of n equal values gives the value itself.
