@@ -8,89 +8,65 @@ using namespace b200pp;
 
 namespace {
 
-// How a row is dealt out.
-//  - up to 1024 columns: `lanes` lanes of a warp with `values` values each, as few lanes as leave little idle: what a row costs besides
-//    its values -- shuffles, addresses -- is per lane;
-//  - up to kClusterCols: a CTA of up to 512 threads with sixteen values each, or a cluster of as many as that takes, up to eight;
-//    beyond 65536 columns thirty-two values and up to 768 threads;
-//  - longer rows, and long rows that are too few to fill the GPU like that: chunks, two kernels.
-struct RowPlan
+// How rows of up to 1024 columns are dealt out: `lanes` lanes of a warp with `values` values each, as few lanes as leave little idle.
+// What a row costs besides its values -- shuffles, addresses -- is per lane (468750 rows of 64 bfloat16: 24 us with four lanes of
+// sixteen values, 31 us with eight of eight).
+struct WarpPlan
 {
-    int       lanes, values, threads, ctas, span;
-    long long chunks;
+    int lanes, values;
 };
 
-constexpr long long kNoWorkspaceCols = 8192; // rows up to this length are never split into chunks (row_ops.h)
-
-RowPlan plan_layernorm(long long rows, long long cols)
+WarpPlan plan_warp(int cols)
 {
-    RowPlan r{};
-    if (cols <= 1024)
-    {
-        static const int table[][3] = {{8, 1, 8},    {16, 2, 8},   {32, 4, 8},   {64, 4, 16},  {96, 4, 24},  {128, 8, 16},
-                                       {192, 8, 24}, {256, 16, 16}, {384, 16, 24}, {512, 32, 16}, {768, 32, 24}, {1024, 32, 32}};
-        int              i = 0;
-        while (cols > table[i][0]) ++i;
-        r.lanes  = table[i][1];
-        r.values = table[i][2];
-        return r;
-    }
-    r.values             = cols <= 8 * 16 * kClusterThreads<16> ? 16 : 32;
-    const long long most = r.values == 16 ? 16 * kClusterThreads<16> : 32 * kClusterThreads<32>; // columns a CTA can take
-    r.ctas               = 1;
-    while (r.ctas * most < cols && r.ctas < 16) r.ctas *= 2;
-    if (r.ctas <= 8 && (cols <= kNoWorkspaceCols || rows * r.ctas >= kSms / 2))
-    {
-        // the same number of columns for each CTA of a row, in whole warps, so that every part starts on a vector
-        r.threads = static_cast<int>((cols + r.ctas * 32 * r.values - 1) / (r.ctas * 32 * r.values) * 32);
-        r.span    = r.threads * r.values;
-        return r;
-    }
-    r.ctas   = 0;
-    r.chunks = (cols + kChunk - 1) / kChunk;
-    return r;
+    static const int table[][3] = {{8, 1, 8},    {16, 2, 8},    {32, 4, 8},    {64, 4, 16},   {96, 4, 24},   {128, 8, 16},
+                                   {192, 8, 24}, {256, 16, 16}, {384, 16, 24}, {512, 32, 16}, {768, 32, 24}, {1024, 32, 32}};
+    int              i = 0;
+    while (cols > table[i][0]) ++i;
+    return {table[i][1], table[i][2]};
 }
 
-template<int SRC, int E, int W>
-int launch_warp(const LayerNormKParams &p, const RowPlan &plan, cudaStream_t stream)
+// Chunks of a row; 0 for those the other kernels take (no workspace up to 8192 columns, row_ops.h).
+long long layernorm_chunks(long long cols)
+{
+    return cols > kBlockCols ? (cols + kChunk - 1) / kChunk : 0;
+}
+
+template<int SRC, int E, int W, bool FULL>
+int launch_warp(const LayerNormKParams &p, const WarpPlan &plan, cudaStream_t stream)
 {
     static std::atomic<unsigned long long> raised{0};
     const dim3                             block(plan.lanes, 256 / plan.lanes);
     const int                              ring = RowStage<SRC, E, W>::bytes(block.x, block.y) * kWarpStages;
     if (ring > 32 * 1024) // a launch gets 48 KB unasked, static memory included
-        if (int st = raise_smem(layernorm_warp_kernel<SRC, E, W>, 112 * 1024, raised))
+        if (int st = raise_smem(layernorm_warp_kernel<SRC, E, W, FULL>, 112 * 1024, raised))
             return st;
     const unsigned turns = (p.rows + block.y - 1) / block.y;
-    layernorm_warp_kernel<SRC, E, W><<<std::min(turns, static_cast<unsigned>(kSms * kWarpCtas<E>)), block, ring, stream>>>(p);
-    return B200PP_SUCCESS;
-}
-
-template<int SRC, int E, int W>
-int launch_cluster(const LayerNormKParams &p, const RowPlan &plan, cudaStream_t stream)
-{
-    static std::atomic<unsigned long long> raised{0};
-    const int                              ring = RowStage<SRC, E, W>::bytes(plan.threads, 1) * kClusterStages<E>;
-    if (ring > 32 * 1024)
-        if (int st = raise_smem(layernorm_cluster_kernel<SRC, E, W>, 208 * 1024, raised))
-            return st;
-    ClusterLaunch launch(plan.ctas, plan.threads, ring, stream);
-    launch.fill(layernorm_cluster_kernel<SRC, E, W>, p.rows);
-    cudaLaunchKernelEx(&launch.cfg, layernorm_cluster_kernel<SRC, E, W>, p, plan.span); // check_launch reports a failure
+    layernorm_warp_kernel<SRC, E, W, FULL><<<std::min(turns, static_cast<unsigned>(kSms * kWarpCtas<E>)), block, ring, stream>>>(p);
     return B200PP_SUCCESS;
 }
 
 template<int SRC, int W>
-int launch_staged(const LayerNormKParams &p, const RowPlan &plan, cudaStream_t stream)
+int launch_staged(const LayerNormKParams &p, cudaStream_t stream)
 {
-    if (plan.ctas)
-        return plan.values == 16 ? launch_cluster<SRC, 16, W>(p, plan, stream) : launch_cluster<SRC, 32, W>(p, plan, stream);
+    if (p.cols > 1024)
+    {
+        static std::atomic<unsigned long long> raised{0};
+        const int                              threads = (p.cols + 511) / 512 * 32;
+        const int                              ring    = RowStage<SRC, 16, W>::bytes(threads, 1) * 3;
+        if (ring > 32 * 1024)
+            if (int st = raise_smem(layernorm_block_kernel<SRC, W>, 112 * 1024, raised))
+                return st;
+        layernorm_block_kernel<SRC, W><<<std::min(p.rows, static_cast<unsigned>(kSms * (512 / threads))), threads, ring, stream>>>(p);
+        return B200PP_SUCCESS;
+    }
+    const WarpPlan plan = plan_warp(p.cols);
     if (plan.values == 8)
-        return launch_warp<SRC, 8, W>(p, plan, stream);
-    if (plan.values == 16)
-        return launch_warp<SRC, 16, W>(p, plan, stream);
-    if (plan.values == 24)
-        return launch_warp<SRC, 24, W>(p, plan, stream);
-    return launch_warp<SRC, 32, W>(p, plan, stream);
+        return launch_warp<SRC, 8, W, false>(p, plan, stream);
+    if (plan.values == 32)
+        return launch_warp<SRC, 32, W, true>(p, plan, stream);
+    if (plan.lanes == 32)
+        return plan.values == 16 ? launch_warp<SRC, 16, W, true>(p, plan, stream) : launch_warp<SRC, 24, W, true>(p, plan, stream);
+    return plan.values == 16 ? launch_warp<SRC, 16, W, false>(p, plan, stream) : launch_warp<SRC, 24, W, false>(p, plan, stream);
 }
 
 template<int SRC, int W>
@@ -111,7 +87,7 @@ bool launch_direct(const LayerNormKParams &p, cudaStream_t stream)
 }
 
 template<int SRC>
-int launch_layernorm(const LayerNormKParams &p, const RowPlan &plan, int width, cudaStream_t stream)
+int launch_layernorm(const LayerNormKParams &p, int width, cudaStream_t stream)
 {
     if (width == 8 ? launch_direct<SRC, 8>(p, stream)
                    : width == 4 ? launch_direct<SRC, 4>(p, stream) : width == 2 ? launch_direct<SRC, 2>(p, stream) : launch_direct<SRC, 1>(p, stream))
@@ -119,10 +95,10 @@ int launch_layernorm(const LayerNormKParams &p, const RowPlan &plan, int width, 
     // vectors of 16 bytes at most on the way through shared memory; of four elements at least, otherwise the rows' lines as they are
     if constexpr (SRC != B200PP_F32)
         if (width == 8)
-            return launch_staged<SRC, 8>(p, plan, stream);
+            return launch_staged<SRC, 8>(p, stream);
     if (width >= 4)
-        return launch_staged<SRC, 4>(p, plan, stream);
-    return launch_staged<SRC, 0>(p, plan, stream);
+        return launch_staged<SRC, 4>(p, stream);
+    return launch_staged<SRC, 0>(p, stream);
 }
 
 } // namespace
@@ -137,7 +113,7 @@ extern "C" int b200ppLayerNormWorkspace(const B200ppRows *src, size_t *bytes)
     t.base          = reinterpret_cast<void *>(uintptr_t(256));
     if (int st = take_rows(&t, "Input", false, m, rows))
         return st;
-    *bytes = static_cast<size_t>(rows) * plan_layernorm(rows, t.cols).chunks * sizeof(float2);
+    *bytes = static_cast<size_t>(rows) * layernorm_chunks(t.cols) * sizeof(float2);
     return B200PP_SUCCESS;
 }
 
@@ -161,8 +137,7 @@ extern "C" int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, con
         return st;
     if (rows != dstRows)
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "Input and output shapes are different");
-    const RowPlan   plan   = plan_layernorm(rows, src->cols);
-    const long long chunks = plan.chunks;
+    const long long chunks = layernorm_chunks(src->cols);
     if ((st = check_workspace(workspace, workspaceBytes, static_cast<size_t>(rows) * chunks * sizeof(float2))))
         return st;
     if (rows * chunks > 0x7fffffffLL)
@@ -189,13 +164,13 @@ extern "C" int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, con
     width.take(p.weight, 0, row_elem_size(p.weightType));
     width.take(p.bias, 0, row_elem_size(p.biasType));
     if (src->dtype == B200PP_U8)
-        st = launch_layernorm<B200PP_U8>(p, plan, width.width, stream);
+        st = launch_layernorm<B200PP_U8>(p, width.width, stream);
     else if (src->dtype == B200PP_F16)
-        st = launch_layernorm<B200PP_F16>(p, plan, width.width, stream);
+        st = launch_layernorm<B200PP_F16>(p, width.width, stream);
     else if (src->dtype == B200PP_BF16)
-        st = launch_layernorm<B200PP_BF16>(p, plan, width.width, stream);
+        st = launch_layernorm<B200PP_BF16>(p, width.width, stream);
     else
-        st = launch_layernorm<B200PP_F32>(p, plan, width.width, stream);
+        st = launch_layernorm<B200PP_F32>(p, width.width, stream);
     if (st)
         return st;
     return check_launch("LayerNorm");

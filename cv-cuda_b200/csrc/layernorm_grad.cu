@@ -57,36 +57,36 @@ size_t grad_workspace(const GradPlan &g, long long cols)
     return static_cast<size_t>(g.parts) * 2 * cols * sizeof(float);
 }
 
-template<int SRC, int GRAD, int E, int W, bool WARP>
+template<int SRC, int GRAD, int E, int W, bool WARP, bool FULL>
 int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
 {
     typedef GradRing<SRC, GRAD, E, W>      Ring;
     static std::atomic<unsigned long long> raised{0};
     const int                              warps = g.threads * g.groups / 32, slots = WARP ? warps : g.groups;
     const int                              columns = WARP ? p.cols : g.span;
-    const int ring = Ring::bytes(g.threads, g.groups) * Ring::kStages;
+    const int ring = Ring::bytes(g.threads, g.groups) * Ring::kStages + g.threads * E * static_cast<int>(sizeof(float));
     const int sums = p.partials && slots > 1 ? slots * 2 * columns * static_cast<int>(sizeof(float)) : 0;
     const int smem = std::max(ring, sums);
     if (smem > 32 * 1024) // a launch gets 48 KB unasked, static memory included
-        if (int st = raise_smem(layernorm_grad_kernel<SRC, GRAD, E, W, WARP>, 208 * 1024, raised))
+        if (int st = raise_smem(layernorm_grad_kernel<SRC, GRAD, E, W, WARP, FULL>, 208 * 1024, raised))
             return st;
     ClusterLaunch launch(g.ctas, g.threads, smem, stream);
     launch.cfg.blockDim.y = g.groups;
     launch.cfg.gridDim    = dim3(p.parts * g.ctas);
-    cudaLaunchKernelEx(&launch.cfg, layernorm_grad_kernel<SRC, GRAD, E, W, WARP>, p, g.span);
+    cudaLaunchKernelEx(&launch.cfg, layernorm_grad_kernel<SRC, GRAD, E, W, WARP, FULL>, p, g.span);
     return check_launch("LayerNormBackward");
 }
 
 template<int SRC, int GRAD, int W>
 int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
 {
+    if (g.threads > 32)
+        return launch_one_pass<SRC, GRAD, 16, W, false, true>(p, g, stream);
     if (g.values == 8)
-        return launch_one_pass<SRC, GRAD, 8, W, true>(p, g, stream);
-    if (g.values == 24)
-        return launch_one_pass<SRC, GRAD, 24, W, true>(p, g, stream);
-    if (g.threads <= 32)
-        return launch_one_pass<SRC, GRAD, 16, W, true>(p, g, stream);
-    return launch_one_pass<SRC, GRAD, 16, W, false>(p, g, stream);
+        return launch_one_pass<SRC, GRAD, 8, W, true, false>(p, g, stream);
+    if (g.threads == 32)
+        return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, true, true>(p, g, stream) : launch_one_pass<SRC, GRAD, 24, W, true, true>(p, g, stream);
+    return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, true, false>(p, g, stream) : launch_one_pass<SRC, GRAD, 24, W, true, false>(p, g, stream);
 }
 
 template<int SRC, int GRAD>

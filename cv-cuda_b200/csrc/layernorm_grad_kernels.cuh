@@ -8,6 +8,8 @@
 
 #include "layernorm_kernels.cuh"
 
+#include <cooperative_groups.h>
+
 namespace b200pp {
 
 struct LayerNormGradKParams
@@ -38,7 +40,7 @@ struct GradRing
     typedef RowStage<GRAD, E, W> G;
 
     static constexpr int kThread = E * (kElemBytes<SRC> + kElemBytes<GRAD>);
-    static constexpr int kStages = kThread * 3 * kGradResident <= 200 * 1024 ? 3 : 2; // what fits beside L1
+    static constexpr int kStages = kThread * 3 * kGradResident <= 180 * 1024 ? 3 : 2; // what fits beside the weights and L1
 
     static __host__ __device__ constexpr int bytes(int threads, int groups)
     {
@@ -46,7 +48,8 @@ struct GradRing
     }
 };
 
-template<int SRC, int GRAD, int E, int W, bool WARP>
+// FULL: rows have whole warps.
+template<int SRC, int GRAD, int E, int W, bool WARP, bool FULL>
 __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) layernorm_grad_kernel(const LayerNormGradKParams p, int span)
 {
     namespace cg = cooperative_groups;
@@ -56,9 +59,9 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
     constexpr int           kStages = Ring::kStages;
     __shared__ float2       scratch[2][16]; // two halves, used in turn: one barrier per row
     __shared__ float2       parts[2][8];    // of the CTAs of a cluster
-    extern __shared__ uint4 ring[];         // the stages; in the end the sums, [groups][2][columns]
-    const int       threads = blockDim.x, groups = blockDim.y;
-    const RowThread k    = row_thread<E, W, !WARP>(threadIdx.x, threads, threadIdx.y, groups);
+    extern __shared__ uint4 ring[];         // the stages, then the weights; in the end the sums, [groups][2][columns]
+    const int       threads = WARP && FULL ? 32 : blockDim.x, groups = blockDim.y;
+    const RowThread k    = row_thread<E, W, FULL>(threadIdx.x, threads, threadIdx.y, groups);
     const int       tid  = k.g * threads + k.t, warp = tid >> 5;
     const int       xBytes = X::bytes(threads, groups), stageBytes = Ring::bytes(threads, groups);
     cg::cluster_group cluster = cg::this_cluster();
@@ -68,19 +71,18 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
     f32x2           dw[E / 2], db[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) dw[i] = db[i] = both(0.0f);
-    const unsigned long long step = static_cast<unsigned long long>(gridDim.x / ctas) * groups;
-    const unsigned long long base = static_cast<unsigned long long>(blockIdx.x / ctas) * groups;
-    unsigned long long       r    = base + k.g;
-    int                      half = 0, stage = 0;
-    auto xRow = [&](unsigned long long n) {
-        return n < p.rows ? p.src.at(static_cast<unsigned>(n)) + static_cast<long long>(from) * kElemBytes<SRC> : static_cast<const uint8_t *>(nullptr);
-    };
-    auto gRow = [&](unsigned long long n) {
-        return n < p.rows ? p.grad.at(static_cast<unsigned>(n)) + static_cast<long long>(from) * kElemBytes<GRAD> : static_cast<const uint8_t *>(nullptr);
-    };
-    auto fetch = [&](int s, unsigned long long n) {
-        X::fetch(ring0 + s * stageBytes, k, xRow(n), end);
-        G::fetch(ring0 + s * stageBytes + xBytes, k, gRow(n), end);
+    const unsigned step = gridDim.x / ctas * groups, base = blockIdx.x / ctas * groups;
+    unsigned       r    = base + k.g;
+    int            half = 0, stage = 0;
+    uint8_t       *ring8 = reinterpret_cast<uint8_t *>(ring);
+    auto xRow = [&](unsigned n) { return p.src.at(n) + static_cast<long long>(from) * kElemBytes<SRC>; };
+    auto gRow = [&](unsigned n) { return p.grad.at(n) + static_cast<long long>(from) * kElemBytes<GRAD>; };
+    auto fetch = [&](int s, unsigned n) {
+        if (n < p.rows)
+        {
+            X::fetch(ring0 + s * stageBytes, k, xRow(n), end);
+            G::fetch(ring0 + s * stageBytes + xBytes, k, gRow(n), end);
+        }
         copies_commit();
     };
     auto meet = [&]() { // the threads of a row, where they read each other's copies
@@ -93,40 +95,19 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
         }
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) fetch(s, r + s * step);
-    float nextMean = r < p.rows ? p.mean[r] : 0.0f, nextRstd = r < p.rows ? p.rstd[r] : 0.0f;
-    // every thread of the CTA takes the same number of turns
-    for (unsigned long long first = base; first < p.rows; first += step, r += step)
+    for (int s = 0; s < kStages; ++s)
     {
-        const bool     live = r < p.rows; // a row that is not there, and what lies behind a row's end: x = dy = 0
-        const unsigned row  = live ? static_cast<unsigned>(r) : 0;
-        const float    mean = nextMean, rstd = nextRstd;
-        f32x2          h[E / 2], gv[E / 2];
-        fetch(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
-        const bool more = r + step < p.rows;
-        nextMean        = more ? p.mean[r + step] : 0.0f;
-        nextRstd        = more ? p.rstd[r + step] : 0.0f;
-        copies_wait<kStages - 1>();
-        meet();
-        {
-            const uint8_t *at = reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes;
-            X::take(at, k, xRow(r), end, h);
-            G::take(at + xBytes, k, gRow(r), end, gv);
-        }
-        stage = stage == kStages - 1 ? 0 : stage + 1;
+        X::clear(ring8 + s * stageBytes, k, end);
+        G::clear(ring8 + s * stageBytes + xBytes, k, end);
+    }
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i)
-        {
-            h[i]  = mul2(add2(h[i], both(-mean)), both(rstd));
-            db[i] = add2(db[i], gv[i]);
-            dw[i] = fma2(gv[i], h[i], dw[i]);
-        }
-        if (!p.dsrc.base)
-        {
-            meet();
-            continue;
-        }
-        if (p.weight) // from L1: there are no registers to keep it
+    for (int s = 0; s < kStages - 1; ++s) fetch(s, r + s * step);
+    // the weights as float32, one copy for the row groups: thread t's vectors of four are `threads` apart, which no two lanes clash on.
+    // Registers would have to be shared with the sums (E = 24 has 48 of those), and from L1 they cost the conversion for each row.
+    f32x2 *weights = reinterpret_cast<f32x2 *>(ring8 + kStages * stageBytes);
+    if (p.weight && p.dsrc.base)
+    {
+        if (k.g == 0)
         {
 #pragma unroll
             for (int j = 0; j < E / 8; ++j)
@@ -134,7 +115,56 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
                 f32x2 w[4];
                 load_param<W>(p.weight, p.weightType, from + k.c + j * (8 / kStep<W>) * k.step, k.step, from + end, w);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) gv[4 * j + i] = mul2(gv[4 * j + i], w[i]);
+                for (int i = 0; i < 2; ++i)
+                    *reinterpret_cast<ulonglong2 *>(weights + ((2 * j + i) * threads + k.t) * 2) = make_ulonglong2(w[2 * i], w[2 * i + 1]);
+            }
+        }
+        __syncthreads();
+    }
+    float nextMean = r < p.rows ? p.mean[r] : 0.0f, nextRstd = r < p.rows ? p.rstd[r] : 0.0f;
+    // every thread of the CTA takes the same number of turns
+    for (unsigned first = base; first < p.rows; first += step, r += step)
+    {
+        const bool  live = r < p.rows;
+        const float mean = nextMean, rstd = nextRstd;
+        f32x2       h[E / 2], gv[E / 2];
+        fetch(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
+        const bool more = r + step < p.rows;
+        nextMean        = more ? p.mean[r + step] : 0.0f;
+        nextRstd        = more ? p.rstd[r + step] : 0.0f;
+        copies_wait<kStages - 1>();
+        meet();
+        {
+            const uint8_t *at = ring8 + stage * stageBytes;
+            const unsigned n  = live ? r : 0;
+            X::take(at, k, W == 0 ? xRow(n) : nullptr, h);
+            G::take(at + xBytes, k, W == 0 ? gRow(n) : nullptr, gv);
+        }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) h[i] = mul2(add2(h[i], both(-mean)), both(rstd));
+        if (live) // otherwise there are values of an earlier row in the stage
+        {
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i)
+            {
+                db[i] = add2(db[i], gv[i]);
+                dw[i] = fma2(gv[i], h[i], dw[i]);
+            }
+        }
+        if (!p.dsrc.base)
+        {
+            meet();
+            continue;
+        }
+        if (p.weight)
+        {
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i)
+            {
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(weights + (i * threads + k.t) * 2);
+                gv[2 * i]     = mul2(gv[2 * i], w.x);
+                gv[2 * i + 1] = mul2(gv[2 * i + 1], w.y);
             }
         }
         f32x2 s1 = both(0.0f), s2 = both(0.0f);
@@ -147,11 +177,8 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
         float t1 = lo2(s1) + hi2(s1), t2 = lo2(s2) + hi2(s2);
         if constexpr (WARP)
         {
-            for (int o = threads >> 1; o > 0; o >>= 1)
-            {
-                t1 += __shfl_xor_sync(0xffffffffu, t1, o);
-                t2 += __shfl_xor_sync(0xffffffffu, t2, o);
-            }
+            t1 = row_sum<false>(t1, threads, nullptr);
+            t2 = row_sum<false>(t2, threads, nullptr);
             meet();
         }
         else
@@ -187,7 +214,7 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
         const float c1 = t1 * p.invCols, c2 = t2 * p.invCols;
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) gv[i] = mul2(add2(fma2(h[i], both(-c2), gv[i]), both(-c1)), both(rstd));
-        store_row<E, W>(p.dsrc.at(row) + static_cast<long long>(from) * (p.dsrcType == B200PP_F32 ? 4 : 2), p.dsrcType, k, end, gv);
+        store_row<E, W>(p.dsrc.at(r) + static_cast<long long>(from) * (p.dsrcType == B200PP_F32 ? 4 : 2), p.dsrcType, k, end, gv);
     }
     if (ctas > 1)
         cluster.sync(); // no CTA leaves while another may still write to it

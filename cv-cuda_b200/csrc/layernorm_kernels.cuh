@@ -7,8 +7,6 @@
 
 #include "row_math.cuh"
 
-#include <cooperative_groups.h>
-
 namespace b200pp {
 
 struct LayerNormKParams
@@ -34,6 +32,8 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *scratch)
 {
     if constexpr (!BLOCK)
     {
+        if (lanes == 32)
+            return warp_sum(v);
         for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     }
@@ -111,38 +111,43 @@ constexpr int kWarpStages = 3;
 template<int E>
 constexpr int kWarpCtas = E <= 8 ? 4 : E <= 16 ? 3 : 2; // of 256 threads on an SM, by the registers the launch bound leaves
 
-template<int SRC, int E, int W>
+// FULL: 32 lanes per row.
+template<int SRC, int E, int W, bool FULL>
 __global__ void __launch_bounds__(256, kWarpCtas<E>) layernorm_warp_kernel(const LayerNormKParams p)
 {
     typedef RowStage<SRC, E, W> Stage;
     extern __shared__ uint4     ring[];
-    const int                   lanes = E == 32 ? 32 : blockDim.x, stageBytes = Stage::bytes(lanes, blockDim.y);
-    const RowThread             k     = row_thread<E, W, E == 32>(threadIdx.x, lanes, threadIdx.y, blockDim.y);
+    const int                   lanes = FULL ? 32 : blockDim.x, groups = FULL ? 8 : blockDim.y, stageBytes = Stage::bytes(lanes, groups);
+    const RowThread             k     = row_thread<E, W, FULL>(threadIdx.x, lanes, threadIdx.y, groups);
+    uint8_t                    *ring8 = reinterpret_cast<uint8_t *>(ring);
     const unsigned              ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
     f32x2                       w[E / 2], b[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 8; ++i)
         layernorm_affine<W>(p, k.c + 8 / kStep<W> * i * k.step, k.step, p.cols, w + 4 * i, b + 4 * i);
-    const unsigned long long step = static_cast<unsigned long long>(gridDim.x) * blockDim.y;
-    const unsigned long long r0   = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    auto row = [&](unsigned long long r) { return r < p.rows ? p.src.at(static_cast<unsigned>(r)) : static_cast<const uint8_t *>(nullptr); };
+    const unsigned step = gridDim.x * groups, r0 = blockIdx.x * groups + threadIdx.y;
+#pragma unroll
+    for (int s = 0; s < kWarpStages; ++s) Stage::clear(ring8 + s * stageBytes, k, p.cols);
 #pragma unroll
     for (int s = 0; s < kWarpStages - 1; ++s)
     {
-        Stage::fetch(ring0 + s * stageBytes, k, row(r0 + s * step), p.cols);
+        if (r0 + s * step < p.rows)
+            Stage::fetch(ring0 + s * stageBytes, k, p.src.at(r0 + s * step), p.cols);
         copies_commit();
     }
     int stage = 0;
     // the lanes of a warp take the same number of turns: those of the warp's first row
-    for (unsigned long long r = r0, first = r0 - threadIdx.y % (32u / lanes); first < p.rows; r += step, first += step)
+    for (unsigned r = r0, first = r0 - threadIdx.y % (32u / lanes); first < p.rows; r += step, first += step)
     {
-        Stage::fetch(ring0 + (stage == 0 ? kWarpStages - 1 : stage - 1) * stageBytes, k, row(r + (kWarpStages - 1) * step), p.cols);
+        const unsigned ahead = r + (kWarpStages - 1) * step;
+        if (ahead < p.rows)
+            Stage::fetch(ring0 + (stage == 0 ? kWarpStages - 1 : stage - 1) * stageBytes, k, p.src.at(ahead), p.cols);
         copies_commit();
         copies_wait<kWarpStages - 1>();
         if (W == 0)
             __syncwarp();
         f32x2 x[E / 2];
-        Stage::take(reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes, k, row(r), p.cols, x);
+        Stage::take(ring8 + stage * stageBytes, k, W == 0 ? p.src.at(min(r, p.rows - 1)) : nullptr, x);
         stage = stage == kWarpStages - 1 ? 0 : stage + 1;
         if (W == 0)
             __syncwarp();
@@ -160,118 +165,68 @@ __global__ void __launch_bounds__(256, kWarpCtas<E>) layernorm_warp_kernel(const
         }
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) x[i] = fma2(mul2(x[i], both(rstd)), w[i], b[i]);
-        store_row<E, W>(p.dst.at(static_cast<unsigned>(r)), p.dstType, k, p.cols, x);
+        store_row<E, W>(p.dst.at(r), p.dstType, k, p.cols, x);
     }
 }
 
-// Forward, longer rows: a CTA per row, or a cluster of up to eight CTAs with `span` columns each, which walk down their share of the
-// rows together. Each CTA takes the mean and the squares of its part; the parts are joined as Chan, Golub and LeVeque do (the mean
-// weighted by length, the squares plus the distances of the means) after one exchange through distributed shared memory. With
-// sixteen values per thread the weights stay in registers; thirty-two are for rows that sixteen do not reach.
-template<int E>
-constexpr int kClusterThreads = E <= 16 ? 512 : 768; // most threads of a CTA, by the registers they need
-template<int E>
-constexpr int kClusterStages = E <= 16 ? 3 : 2;
+// Forward, longer rows: a CTA per row, sixteen values per thread. (Clusters of CTAs for rows that do not fit into one were slower than
+// the two kernels over chunks below: 72 against 55 us for 256 uint8 images of 224 x 224 x 3. A CTA of so many threads is alone on
+// its SM, and nothing goes on there while it waits for its barriers.)
+constexpr int kBlockCols = 16 * 512;
 
-template<int SRC, int E, int W>
-__global__ void __launch_bounds__(kClusterThreads<E>, 1) layernorm_cluster_kernel(const LayerNormKParams p, int span)
+template<int SRC, int W>
+__global__ void __launch_bounds__(512) layernorm_block_kernel(const LayerNormKParams p)
 {
-    namespace cg = cooperative_groups;
+    constexpr int               E = 16, kStages = 3;
     typedef RowStage<SRC, E, W> Stage;
-    constexpr int               kStages = kClusterStages<E>;
     extern __shared__ uint4     ring[];
     __shared__ float            scratch[2][32];
-    __shared__ float2           parts[2][8];
-    cg::cluster_group           cluster = cg::this_cluster();
-    const int                   ctas = cluster.num_blocks(), rank = cluster.block_rank(), stageBytes = Stage::bytes(blockDim.x, 1);
-    const int                   from = rank * span, end = min(p.cols - from, span); // this CTA's columns
+    const int                   stageBytes = Stage::bytes(blockDim.x, 1);
     const RowThread             k     = row_thread<E, W, true>(threadIdx.x, blockDim.x, 0, 1);
+    uint8_t                    *ring8 = reinterpret_cast<uint8_t *>(ring);
     const unsigned              ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
-    f32x2                       w[E <= 16 ? E / 2 : 4], b[E <= 16 ? E / 2 : 4];
-    if constexpr (E <= 16)
-    {
+    f32x2                       w[E / 2], b[E / 2];
 #pragma unroll
-        for (int i = 0; i < E / 8; ++i)
-            layernorm_affine<W>(p, from + k.c + 8 / kStep<W> * i * k.step, k.step, from + end, w + 4 * i, b + 4 * i);
-    }
-    const unsigned long long step = gridDim.x / ctas;
-    unsigned long long       r    = blockIdx.x / ctas;
-    auto                     row  = [&](unsigned long long n) {
-        return n < p.rows ? p.src.at(static_cast<unsigned>(n)) + static_cast<long long>(from) * kElemBytes<SRC> : static_cast<const uint8_t *>(nullptr);
-    };
+    for (int i = 0; i < E / 8; ++i)
+        layernorm_affine<W>(p, k.c + 8 / kStep<W> * i * k.step, k.step, p.cols, w + 4 * i, b + 4 * i);
+    const unsigned step = gridDim.x;
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) Stage::clear(ring8 + s * stageBytes, k, p.cols);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s)
     {
-        Stage::fetch(ring0 + s * stageBytes, k, row(r + s * step), end);
+        if (blockIdx.x + s * step < p.rows)
+            Stage::fetch(ring0 + s * stageBytes, k, p.src.at(blockIdx.x + s * step), p.cols);
         copies_commit();
     }
-    const float n     = static_cast<float>(end), inv = 1.0f / n;
-    int         stage = 0, half = 0;
-    for (; r < p.rows; r += step)
+    int stage = 0;
+    for (unsigned r = blockIdx.x; r < p.rows; r += step)
     {
-        // the stage before was read by every thread before a barrier of the last turn
-        Stage::fetch(ring0 + (stage == 0 ? kStages - 1 : stage - 1) * stageBytes, k, row(r + (kStages - 1) * step), end);
+        // the stage this goes to was read by every thread before a barrier of the last turn
+        const unsigned ahead = r + (kStages - 1) * step;
+        if (ahead < p.rows)
+            Stage::fetch(ring0 + (stage == 0 ? kStages - 1 : stage - 1) * stageBytes, k, p.src.at(ahead), p.cols);
         copies_commit();
         copies_wait<kStages - 1>();
         if (W == 0)
             __syncthreads();
         f32x2 x[E / 2];
-        Stage::take(reinterpret_cast<const uint8_t *>(ring) + stage * stageBytes, k, row(r), end, x);
-        stage        = stage == kStages - 1 ? 0 : stage + 1;
-        float mean   = divide_count(row_sum<true>(sum_pairs<E>(x), 0, scratch[0]), n, inv);
-        float q      = row_sum<true>(centre<E, kStep<W>>(x, mean, k.c, k.step, end), 0, scratch[1]);
-        float centre = 0.0f; // distance of this CTA's mean to the row's
-        if (ctas > 1)
-        {
-            if (static_cast<int>(threadIdx.x) < ctas)
-                *cluster.map_shared_rank(&parts[half][rank], threadIdx.x) = make_float2(mean, q);
-            cluster.sync();
-            float sum = 0.0f;
-            for (int c = 0; c < ctas; ++c) sum += parts[half][c].x * static_cast<float>(min(p.cols - c * span, span));
-            const float whole = divide_count(sum, p.fcols, p.invCols);
-            q                 = 0.0f;
-            for (int c = 0; c < ctas; ++c)
-            {
-                const float d = parts[half][c].x - whole;
-                q += parts[half][c].y + d * d * static_cast<float>(min(p.cols - c * span, span));
-            }
-            centre = mean - whole;
-            mean   = whole;
-            half ^= 1; // the next turn's parts come while slower CTAs read these
-        }
-        const float rstd = rsqrtf(q * p.invCols + p.epsilon);
-        if (rank == 0 && threadIdx.x == 0)
+        Stage::take(ring8 + stage * stageBytes, k, W == 0 ? p.src.at(r) : nullptr, x);
+        stage            = stage == kStages - 1 ? 0 : stage + 1;
+        const float mean = divide_count(row_sum<true>(sum_pairs<E>(x), 0, scratch[0]), p.fcols, p.invCols);
+        const float q    = centre<E, kStep<W>>(x, mean, k.c, k.step, p.cols);
+        const float rstd = rsqrtf(row_sum<true>(q, 0, scratch[1]) * p.invCols + p.epsilon);
+        if (threadIdx.x == 0)
         {
             if (p.mean)
                 p.mean[r] = mean;
             if (p.rstd)
                 p.rstd[r] = rstd;
         }
-        uint8_t *y = p.dst.at(static_cast<unsigned>(r)) + static_cast<long long>(from) * (p.dstType == B200PP_F32 ? 4 : 2);
-        if constexpr (E <= 16)
-        {
 #pragma unroll
-            for (int i = 0; i < E / 2; ++i) x[i] = fma2(mul2(add2(x[i], both(centre)), both(rstd)), w[i], b[i]);
-        }
-        else
-        {
-#pragma unroll
-            for (int j = 0; j < E / 8; ++j)
-            {
-                if (p.weight || p.bias)
-                    layernorm_affine<W>(p, from + k.c + 8 / kStep<W> * j * k.step, k.step, from + end, w, b);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                {
-                    const f32x2 h = mul2(add2(x[4 * j + i], both(centre)), both(rstd));
-                    x[4 * j + i]  = p.weight || p.bias ? fma2(h, w[i], b[i]) : h;
-                }
-            }
-        }
-        store_row<E, W>(y, p.dstType, k, end, x);
+        for (int i = 0; i < E / 2; ++i) x[i] = fma2(mul2(x[i], both(rstd)), w[i], b[i]);
+        store_row<E, W>(p.dst.at(r), p.dstType, k, p.cols, x);
     }
-    if (ctas > 1)
-        cluster.sync(); // no CTA leaves while another may still write to it
 }
 
 // Forward, a CTA per row and eight values per thread, for so few rows that only latency counts: the weights are fetched at the same
@@ -303,7 +258,7 @@ __global__ void __launch_bounds__(512) layernorm_few_kernel(const LayerNormKPara
     store_vecs<W, 8 / W>(p.dst.at(r), p.dstType, k.c, k.step, p.cols, v);
 }
 
-// Forward, rows too long for that, or long and few: two kernels over chunks of kChunk values. The first leaves each chunk's mean and
+// Forward, rows too long for that: two kernels over chunks of kChunk values. The first leaves each chunk's mean and
 // sum of squared distances to it; the second joins those of its row, likewise, and normalises its chunk. It takes the
 // chunks in reverse order, so that the ones read last by the first kernel are still in L2.
 constexpr int kChunk        = 8192;
@@ -312,55 +267,93 @@ constexpr int kChunkThreads = 256;
 template<int SRC, int W>
 __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_stats_kernel(const LayerNormKParams p)
 {
-    __shared__ float scratch[2][32];
-    constexpr int    E   = kChunk / kChunkThreads;
-    const unsigned   r   = blockIdx.x / p.chunks;
-    const long long  at  = static_cast<long long>(blockIdx.x - r * p.chunks) * kChunk;
-    const int        c0  = static_cast<int>(at);
-    const int        end = min(static_cast<long long>(p.cols), at + kChunk);
-    const RowThread           span = row_thread<E, W, true>(threadIdx.x, kChunkThreads, 0, 1);
-    f32x2                     x[E / 2];
+    constexpr int   E   = kChunk / kChunkThreads;
+    const unsigned  r   = blockIdx.x / p.chunks;
+    const long long at  = static_cast<long long>(blockIdx.x - r * p.chunks) * kChunk;
+    const int       end = static_cast<int>(min(static_cast<long long>(p.cols) - at, static_cast<long long>(kChunk)));
+    const uint8_t  *x8  = p.src.at(r) + at * kElemBytes<SRC>;
+    const RowThread k   = row_thread<E, W, true>(threadIdx.x, kChunkThreads, 0, 1);
+    if constexpr (SRC == B200PP_U8 && W >= 4)
     {
-        float v[E];
-        load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, v);
-        pairs<E>(v, x);
+        // whole numbers: sum and sum of squares (at most 8192 * 255^2 < 2^32) by the four-way dot product, exact
+        __shared__ unsigned total[2][8];
+        unsigned            s = 0, q = 0;
+#pragma unroll
+        for (int v = 0; v < E / W; ++v)
+            if (k.c + v * k.step < end)
+            {
+                const RawVec<W> raw = load_raw<W>(x8 + k.c + v * k.step);
+#pragma unroll
+                for (int i = 0; i < W / 4; ++i)
+                {
+                    s = __dp4a(raw.w[i], 0x01010101u, s);
+                    q = __dp4a(raw.w[i], raw.w[i], q);
+                }
+            }
+        s = __reduce_add_sync(0xffffffffu, s);
+        q = __reduce_add_sync(0xffffffffu, q);
+        if ((threadIdx.x & 31) == 0)
+            total[0][threadIdx.x >> 5] = s, total[1][threadIdx.x >> 5] = q;
+        __syncthreads();
+        if (threadIdx.x == 0)
+        {
+            s = q = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += total[0][i], q += total[1][i];
+            // n sum(x^2) - sum(x)^2, both below 2^46
+            const unsigned long long d = static_cast<unsigned long long>(end) * q - static_cast<unsigned long long>(s) * s;
+            p.partials[blockIdx.x]     = make_float2(static_cast<float>(s) / static_cast<float>(end), static_cast<float>(d) / static_cast<float>(end));
+        }
     }
-    const float mean = row_sum<true>(sum_pairs<E>(x), 0, scratch[0]) / static_cast<float>(end - c0);
-    const float q    = row_sum<true>(centre<E, W>(x, mean, c0 + span.c, span.step, end), 0, scratch[1]);
-    if (threadIdx.x == 0)
-        p.partials[blockIdx.x] = make_float2(mean, q);
+    else
+    {
+        __shared__ float scratch[2][32];
+        f32x2            x[E / 2];
+        {
+            float v[E];
+            load_vecs<SRC, W, E / W>(x8, k.c, k.step, end, v);
+            pairs<E>(v, x);
+        }
+        const float mean = row_sum<true>(sum_pairs<E>(x), 0, scratch[0]) / static_cast<float>(end);
+        const float q    = row_sum<true>(centre<E, W>(x, mean, k.c, k.step, end), 0, scratch[1]);
+        if (threadIdx.x == 0)
+            p.partials[blockIdx.x] = make_float2(mean, q);
+    }
 }
 
 template<int SRC, int W>
 __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(const LayerNormKParams p)
 {
-    __shared__ float scratch[2][32];
-    constexpr int    E   = kChunk / kChunkThreads;
-    const unsigned   job = gridDim.x - 1 - blockIdx.x;
-    const unsigned   r   = job / p.chunks;
-    const long long  at  = static_cast<long long>(job - r * p.chunks) * kChunk;
-    const int        c0  = static_cast<int>(at);
-    const int        end = min(static_cast<long long>(p.cols), at + kChunk);
-    const RowThread           span = row_thread<E, W, true>(threadIdx.x, kChunkThreads, 0, 1);
-    f32x2                     x[E / 2];
+    constexpr int   E   = kChunk / kChunkThreads;
+    const unsigned  job = gridDim.x - 1 - blockIdx.x, r = job / p.chunks;
+    const long long at  = static_cast<long long>(job - r * p.chunks) * kChunk;
+    const int       end = static_cast<int>(min(static_cast<long long>(p.cols) - at, static_cast<long long>(kChunk)));
+    const uint8_t  *x8  = p.src.at(r) + at * kElemBytes<SRC>;
+    uint8_t        *y   = p.dst.at(r) + at * (p.dstType == B200PP_F32 ? 4 : 2);
+    const RowThread k   = row_thread<E, W, true>(threadIdx.x, kChunkThreads, 0, 1);
+    Vec<SRC, W>     raw[E / W];
+#pragma unroll
+    for (int v = 0; v < E / W; ++v)
     {
-        float v[E];
-        load_vecs<SRC, W, E / W>(p.src.at(r), c0 + span.c, span.step, end, v);
-        pairs<E>(v, x);
+        raw[v] = zero_raw<kElemBytes<SRC> * W>();
+        if (k.c + v * k.step < end)
+            raw[v] = load_raw<kElemBytes<SRC> * W>(x8 + (k.c + v * k.step) * kElemBytes<SRC>);
     }
+    // every warp joins the parts for itself: nothing to wait for
+    const int     lane = threadIdx.x & 31;
     const float2 *part = p.partials + static_cast<unsigned long long>(r) * p.chunks;
     const float   tail = static_cast<float>(p.cols - static_cast<long long>(p.chunks - 1) * kChunk); // length of the last chunk
     float         s    = 0.0f;
-    for (unsigned k = threadIdx.x; k < p.chunks; k += kChunkThreads) s += part[k].x * (k + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
-    const float mean = divide_count(row_sum<true>(s, 0, scratch[0]), p.fcols, p.invCols);
+    for (unsigned i = lane; i < p.chunks; i += 32) s += part[i].x * (i + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
+    const float mean = divide_count(warp_sum(s), p.fcols, p.invCols);
     float       q    = 0.0f;
-    for (unsigned k = threadIdx.x; k < p.chunks; k += kChunkThreads)
+    for (unsigned i = lane; i < p.chunks; i += 32)
     {
-        const float d = part[k].x - mean;
-        q += part[k].y + d * d * (k + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
+        const float d = part[i].x - mean;
+        q += part[i].y + d * d * (i + 1 < p.chunks ? static_cast<float>(kChunk) : tail);
     }
-    const float rstd = rsqrtf(row_sum<true>(q, 0, scratch[1]) * p.invCols + p.epsilon);
-    if (c0 == 0 && threadIdx.x == 0)
+    const float rstd = rsqrtf(warp_sum(q) * p.invCols + p.epsilon);
+    if (at == 0 && threadIdx.x == 0)
     {
         if (p.mean)
             p.mean[r] = mean;
@@ -368,19 +361,24 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
             p.rstd[r] = rstd;
     }
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) x[i] = add2(x[i], both(-mean));
-    uint8_t *y = p.dst.at(r);
-#pragma unroll
     for (int j = 0; j < E / 8; ++j)
     {
-        const int c = c0 + span.c + 8 / W * j * span.step;
-        f32x2     w[4], b[4];
+        const int c = k.c + 8 / W * j * k.step;
+        f32x2     x[4], w[4], b[4];
         float     v[8];
-        layernorm_affine<W>(p, c, span.step, end, w, b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = fma2(mul2(x[4 * j + i], both(rstd)), w[i], b[i]);
-        singles<8>(w, v);
-        store_vecs<W, 8 / W>(y, p.dstType, c, span.step, end, v);
+        for (int i = 0; i < 8 / W; ++i) unpack<SRC, W>(raw[j * (8 / W) + i], v + i * W);
+        pairs<8>(v, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = mul2(add2(x[i], both(-mean)), both(rstd));
+        if (p.weight || p.bias)
+        {
+            layernorm_affine<W>(p, static_cast<int>(at) + c, k.step, static_cast<int>(at) + end, w, b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = fma2(x[i], w[i], b[i]);
+        }
+        singles<8>(x, v);
+        store_vecs<W, 8 / W>(y, p.dstType, c, k.step, end, v);
     }
 }
 

@@ -438,7 +438,7 @@ struct RowThread
 
 // One stage of one tensor for all row groups of a CTA. E values per thread as vectors of W, W dividing the row and everything
 // aligned to it: each thread copies its own vectors and reads them back itself, so there is nothing to synchronise and no register
-// is held while HBM answers.
+// is held while HBM answers. What lies behind a row's end is set to zero once (`clear`) and never copied over.
 template<int DT, int E, int W>
 struct RowStage
 {
@@ -449,29 +449,34 @@ struct RowStage
         return kVec * V * threads * groups;
     }
 
-    // `row`: null if there is none; `end`: elements of the row
-    static __device__ __forceinline__ void fetch(unsigned stage, const RowThread &k, const uint8_t *row, int end)
+    // `end`: elements of the row
+    static __device__ __forceinline__ void clear(uint8_t *stage, const RowThread &k, int end)
     {
         const int tid = k.g * k.threads + k.t, all = k.threads * k.groups;
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            if (row && k.c + v * k.step < end)
-                copy_async<kVec>(stage + (v * all + tid) * kVec, row + static_cast<long long>(k.c + v * k.step) * kElemBytes<DT>, kVec);
+            if (k.c + v * k.step >= end)
+                store_raw<kVec>(stage + (v * all + tid) * kVec, zero_raw<kVec>());
+    }
+
+    static __device__ __forceinline__ void fetch(unsigned stage, const RowThread &k, const uint8_t *row, int end)
+    {
+        const int      tid = k.g * k.threads + k.t, all = k.threads * k.groups;
+        const uint8_t *at  = row + k.c * kElemBytes<DT>;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (k.c + v * k.step < end)
+                copy_async<kVec>(stage + (v * all + tid) * kVec, at + v * k.step * kElemBytes<DT>, kVec);
     }
 
     // The thread's values, zeros behind the row's end.
-    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *row, int end, f32x2 *out)
+    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *, f32x2 *out)
     {
-        const int   tid = k.g * k.threads + k.t, all = k.threads * k.groups;
-        Vec<DT, W>  raw[V];
-        float       f[E];
+        const int  tid = k.g * k.threads + k.t, all = k.threads * k.groups;
+        Vec<DT, W> raw[V];
+        float      f[E];
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-        {
-            raw[v] = zero_raw<kVec>();
-            if (row && k.c + v * k.step < end)
-                raw[v] = load_raw<kVec>(stage + (v * all + tid) * kVec);
-        }
+        for (int v = 0; v < V; ++v) raw[v] = load_raw<kVec>(stage + (v * all + tid) * kVec);
 #pragma unroll
         for (int v = 0; v < V; ++v) unpack<DT, W>(raw[v], f + v * W);
         pairs<E>(f, out);
@@ -479,48 +484,62 @@ struct RowStage
 };
 
 // The same for rows that start anywhere (W = 0): the 16-byte lines a row touches are copied as they are, by whichever thread of the
-// row, and each thread picks its pairs of elements out of them. (The first line may begin with bytes before the row: those of the
-// row before it, or, before the first row, of the same 16 bytes of memory as its first element.) The threads of a row have to meet
-// between the copies' end and `take`, and between `take` and the next copies to the stage.
+// row, zeros after its end, and each thread picks its pairs of elements out of them. (The first line may begin with bytes before the
+// row: those of the row before it, or, before the first row, of the same 16 bytes of memory as its first element.) The threads of a
+// row have to meet between the copies' end and `take`, and between `take` and the next copies to the stage.
 template<int DT, int E>
 struct RowStage<DT, E, 0>
 {
     static constexpr int kSize = kElemBytes<DT>;
 
-    static __host__ __device__ constexpr int group_bytes(int threads)
+    static __host__ __device__ constexpr int lines(int threads)
     {
-        return (threads * E * kSize + 15) / 16 * 16 + 32; // the lines, and a word more for the last pair
+        return (threads * E * kSize + 15 + 15) / 16;
     }
 
     static __host__ __device__ constexpr int bytes(int threads, int groups)
     {
-        return group_bytes(threads) * groups;
+        return (lines(threads) * 16 + 16) * groups; // a word more for the last pair
     }
+
+    static __device__ __forceinline__ void clear(uint8_t *, const RowThread &, int) {}
 
     static __device__ __forceinline__ void fetch(unsigned stage, const RowThread &k, const uint8_t *row, int end)
     {
-        if (!row)
-            return;
         const int            off   = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
         const int            bytes = off + min(end, k.threads * E) * kSize;
-        const unsigned       to    = stage + k.g * group_bytes(k.threads);
+        const unsigned       to    = stage + k.g * bytes_of_group(k.threads);
         const uint8_t *const line  = row - off;
-        for (int q = k.t * 16; q < bytes; q += k.threads * 16) copy_async<16>(to + q, line + q, min(16, bytes - q));
+#pragma unroll 4
+        for (int q = k.t; q < lines(k.threads); q += k.threads)
+        {
+            const int n = min(16, max(0, bytes - q * 16));
+            copy_async<16>(to + q * 16, n > 0 ? line + q * 16 : line, n);
+        }
     }
 
-    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *row, int end, f32x2 *out)
+    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *row, f32x2 *out)
     {
-        const int       off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
-        const unsigned *w   = reinterpret_cast<const unsigned *>(stage + k.g * group_bytes(k.threads));
+        // the thread's first pair starts `at` bytes into the lines
+        const int       at    = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) + k.c * kSize;
+        const int       shift = (at & 3) * 8;
+        const unsigned *w     = reinterpret_cast<const unsigned *>(stage + k.g * bytes_of_group(k.threads)) + (at >> 2);
 #pragma unroll
         for (int v = 0; v < E / 2; ++v)
         {
-            const int c = k.c + v * k.step;
-            float     f[2] = {0.0f, 0.0f};
-            if (row && c < end)
+            float f[2];
+            if constexpr (kSize == 1)
             {
-                const int      at = off + c * kSize;
-                const unsigned w0 = w[at >> 2], w1 = w[(at >> 2) + 1];
+                // vectors are an even number of bytes apart, which need not be whole words
+                const int      b = at + v * k.step;
+                const unsigned *x = reinterpret_cast<const unsigned *>(stage + k.g * bytes_of_group(k.threads)) + (b >> 2);
+                const unsigned  bits = __funnelshift_r(x[0], x[1], (b & 3) * 8);
+                f[0]                 = static_cast<float>(bits & 0xffu);
+                f[1]                 = static_cast<float>((bits >> 8) & 0xffu);
+            }
+            else
+            {
+                const unsigned w0 = w[v * k.step * kSize / 4], w1 = w[v * k.step * kSize / 4 + 1];
                 if constexpr (kSize == 4)
                 {
                     f[0] = __uint_as_float(w0);
@@ -528,24 +547,19 @@ struct RowStage<DT, E, 0>
                 }
                 else
                 {
-                    const unsigned bits = __funnelshift_r(w0, w1, (at & 3) * 8);
-                    if constexpr (kSize == 2)
-                    {
-                        Vec<DT, 2> r;
-                        r.w[0] = bits;
-                        unpack<DT, 2>(r, f);
-                    }
-                    else
-                    {
-                        f[0] = static_cast<float>(bits & 0xffu);
-                        f[1] = static_cast<float>((bits >> 8) & 0xffu);
-                    }
+                    Vec<DT, 2> r;
+                    r.w[0] = __funnelshift_r(w0, w1, shift);
+                    unpack<DT, 2>(r, f);
                 }
-                if (c + 1 >= end)
-                    f[1] = 0.0f;
             }
             out[v] = make2(f[0], f[1]);
         }
+    }
+
+private:
+    static __host__ __device__ constexpr int bytes_of_group(int threads)
+    {
+        return lines(threads) * 16 + 16;
     }
 };
 
@@ -579,24 +593,37 @@ __device__ __forceinline__ void load_param(const uint8_t *p, int dtype, int c, i
     pairs<8>(f, out);
 }
 
-// A thread's values to its row.
+// A thread's values to its row, which may start anywhere.
 template<int DT, int E>
 __device__ __forceinline__ void store_pairs(uint8_t *row, int c, int step, int end, const float *f)
 {
     const bool whole = (reinterpret_cast<uintptr_t>(row) & (2 * kElemBytes<DT> - 1)) == 0; // pairs start on even elements
+    if (c + (E / 2 - 1) * step + 1 < end)
+    {
+        uint8_t *at = row + c * kElemBytes<DT>;
+        if (whole)
+        {
+#pragma unroll
+            for (int v = 0; v < E / 2; ++v) store_vec<DT, 2>(at, v * step, f + 2 * v);
+        }
+        else
+        {
+#pragma unroll
+            for (int v = 0; v < E / 2; ++v)
+            {
+                store_elem_as<DT>(at, v * step, f[2 * v]);
+                store_elem_as<DT>(at, v * step + 1, f[2 * v + 1]);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int v = 0; v < E / 2; ++v)
     {
-        const int at = c + v * step;
-        if (whole && at + 1 < end)
-            store_vec<DT, 2>(row, at, f + 2 * v);
-        else
-        {
-            if (at < end)
-                store_elem_as<DT>(row, at, f[2 * v]);
-            if (at + 1 < end)
-                store_elem_as<DT>(row, at + 1, f[2 * v + 1]);
-        }
+        if (c + v * step < end)
+            store_elem_as<DT>(row, c + v * step, f[2 * v]);
+        if (c + v * step + 1 < end)
+            store_elem_as<DT>(row, c + v * step + 1, f[2 * v + 1]);
     }
 }
 
