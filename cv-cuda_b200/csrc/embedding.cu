@@ -150,18 +150,16 @@ namespace {
 // Layout of the gradient's workspace.
 struct EmbeddingGradPlan
 {
-    unsigned unit, units, blocks;
+    unsigned units, groups, blocks;
     size_t   entries[2], partials, bytes;
 };
 
 EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
 {
     EmbeddingGradPlan w{};
-    // 32 positions per warp; fewer where that would leave the GPU short of warps
     w.blocks     = static_cast<unsigned>((cols + kGradCols - 1) / kGradCols);
-    w.unit       = 32;
-    while (w.unit > 8 && count * w.blocks < static_cast<long long>(w.unit) * kSms * 16) w.unit /= 2;
-    w.units      = static_cast<unsigned>((count + w.unit - 1) / w.unit);
+    w.units      = static_cast<unsigned>((count + kGradUnit - 1) / kGradUnit);
+    w.groups     = static_cast<unsigned>((count + kShortRun - 1) / kShortRun);
     size_t at    = 0;
     for (int k = 0; k < 2; ++k)
     {
@@ -169,14 +167,14 @@ EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
         at += align_up(static_cast<size_t>(count) * sizeof(uint2));
     }
     w.partials = at;
-    w.bytes    = at + static_cast<size_t>(w.units) * 2 * cols * sizeof(float);
+    w.bytes    = at + static_cast<size_t>(w.groups) * 2 * cols * sizeof(float);
     return w;
 }
 
 template<int GRAD>
 void launch_runs(const EmbeddingGradKParams &p, int width, cudaStream_t stream)
 {
-    const unsigned grid = static_cast<unsigned>((static_cast<unsigned long long>(p.units) * p.blocks + 7) / 8);
+    const unsigned grid = static_cast<unsigned>(((static_cast<unsigned long long>(p.units) + 2 * p.groups) * p.blocks + 7) / 8);
     if (width == 8)
         embedding_grad_runs_kernel<GRAD, 8><<<grid, 256, 0, stream>>>(p);
     else if (width == 4)
@@ -238,8 +236,8 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     p.scale      = op->scale;
     p.accumulate = op->accumulate != 0;
     p.padding    = op->paddingIndex >= 0 && op->paddingIndex < rows ? static_cast<int>(op->paddingIndex) : -1;
-    p.unit       = w.unit;
     p.units      = w.units;
+    p.groups     = w.groups;
     p.blocks     = w.blocks;
     for (int k = 0; k < 2; ++k) p.entries[k] = reinterpret_cast<uint2 *>(ws + w.entries[k]);
     p.partials = reinterpret_cast<float *>(ws + w.partials);
@@ -267,7 +265,7 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(sort_smem_words(kSortThreads / 32, 1 << kSortMaxBits) * sizeof(unsigned)),
                          raised)))
         return st;
-    const unsigned long long jobs = static_cast<unsigned long long>(w.units) * w.blocks;
+    const unsigned long long jobs = (static_cast<unsigned long long>(w.units) + 2 * w.groups) * w.blocks;
     if (jobs > 0x7fffffffull || w.blocks > 65535u)
         return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
     embedding_sort_kernel<<<clusters * kSortCtas, kSortThreads, smem, stream>>>(p);
@@ -283,8 +281,8 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
         launch_runs<B200PP_BF16>(p, width.width, stream);
     else
         launch_runs<B200PP_F32>(p, width.width, stream);
-    if ((st = check_launch("EmbeddingBackward")) || w.units == 1)
+    if ((st = check_launch("EmbeddingBackward")) || w.groups == 1)
         return st;
-    embedding_grad_join_kernel<<<dim3((w.units - 1 + 7) / 8, w.blocks), 256, 0, stream>>>(p);
+    embedding_grad_join_kernel<<<dim3((w.groups - 1 + 7) / 8, w.blocks), 256, 0, stream>>>(p);
     return check_launch("EmbeddingBackward");
 }

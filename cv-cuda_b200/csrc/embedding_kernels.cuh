@@ -156,8 +156,8 @@ struct EmbeddingGradKParams
     uint2    *entries[2];         // (index, position), count each; entries[0] holds the sorted ones
     int       passes, digitBits, sortWarps;
     int       zeroCtas, zeroWidth, skipNamed; // CTAs that clear the table, their vector width, whether they leave out named rows
-    float    *partials;                       // [units][2][cols]
-    unsigned  unit, units;                    // sorted positions per unit (at most 32)
+    float    *partials;                       // [groups][2][cols]
+    unsigned  units, groups;                  // of kGradUnit and kShortRun sorted positions
     unsigned  blocks;                         // column blocks of kGradCols
 };
 
@@ -394,12 +394,16 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
         embedding_clear(p, smem);
 }
 
-// ---- second kernel: a warp sums the runs of equal keys that start among `unit` neighbouring sorted positions, for kGradCols
-// columns. A run of up to kShortRun positions is summed by the warp it starts in, wherever it ends. Longer runs are summed unit
-// by unit into `partials` -- slot 0: the run comes from the unit before, slot 1: it starts here -- and joined by the third kernel.
+// ---- second kernel: sums the runs of equal keys among the sorted positions, a warp for kGradCols columns of each job.
+//  - Runs of up to kShortRun positions belong to the warp in whose unit of kGradUnit positions they start, wherever they end. It has
+//    the rows of a unit in flight at once; larger units left the GPU with little more than one wave of long-lived warps.
+//  - Longer runs are summed by groups of kShortRun positions into `partials` -- slot 0 for the run that comes from the group before,
+//    slot 1 for the one that starts in the group, a job each -- and joined by the third kernel.
+constexpr int kGradUnit  = 8;
 constexpr int kShortRun  = 32;
 constexpr int kGradCols  = 256; // eight per lane
-constexpr int kGradAhead = 4;   // rows loaded before the first is added
+template<int GRAD, int W>
+constexpr int kGradAhead = GRAD == B200PP_F32 || W == 1 ? 4 : 8; // rows loaded before the first is added: 32 registers
 
 // Puts a lane's eight sums where they belong: into `partial` or, if that is null, into the table. Not inlined: it would be there
 // once for each of the rows a warp has in flight, and code that runs once is as slow as it can be fetched (7 times slower for
@@ -432,72 +436,77 @@ __device__ __noinline__ void embedding_grad_put(const EmbeddingGradKParams &p, f
 template<int GRAD, int W>
 __global__ void __launch_bounds__(256, 3) embedding_grad_runs_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
-    constexpr int            V    = 8 / W;
+    constexpr int            V = 8 / W, kAhead = kGradAhead<GRAD, W>;
     constexpr unsigned       kAll = 0xffffffffu;
     const int                lane = threadIdx.x & 31;
     const unsigned long long job  = blockIdx.x * 8ull + (threadIdx.x >> 5);
-    if (job >= static_cast<unsigned long long>(p.units) * p.blocks)
+    const unsigned           item = static_cast<unsigned>(job / p.blocks); // the groups' slots, then the units
+    if (item >= 2 * p.groups + p.units)
         return;
-    const unsigned u    = static_cast<unsigned>(job / p.blocks);
-    const int      c0   = static_cast<int>(job - static_cast<unsigned long long>(u) * p.blocks) * kGradCols + lane * W;
-    const unsigned i0   = u * p.unit;
-    const int      n    = static_cast<int>(min(p.count - i0, p.unit));
-    const unsigned none = static_cast<unsigned>(p.rows);
-    // keys of the 32 positions before the unit (lane l: i0 - 1 - l), of the 32 from its start on and of the 32 after those
-    const unsigned  i   = i0 + lane;
-    const unsigned  bk  = static_cast<unsigned>(lane) < i0 ? p.entries[0][i0 - 1 - lane].x : none;
-    const unsigned  k0  = i < p.count ? p.entries[0][i].x : none;
-    const unsigned  k1  = i + 32u < p.count ? p.entries[0][i + 32].x : none;
-    const unsigned  o0  = i < p.count ? p.entries[0][i].y : 0;
-    const unsigned  o1  = i + 32u < p.count ? p.entries[0][i + 32].y : 0;
-    const unsigned  key = __shfl_sync(kAll, k0, 0);
-    if (key == none)
+    const int      c0    = static_cast<int>(job - static_cast<unsigned long long>(item) * p.blocks) * kGradCols + lane * W;
+    const bool     whole = item < 2 * p.groups;
+    const unsigned i0    = whole ? item / 2 * kShortRun : (item - 2 * p.groups) * kGradUnit;
+    const int      n     = static_cast<int>(min(p.count - i0, static_cast<unsigned>(whole ? kShortRun : kGradUnit)));
+    const unsigned none  = static_cast<unsigned>(p.rows);
+    // keys of the 32 positions before (lane l: i0 - 1 - l), of the 32 from i0 on and of the 32 after those
+    const unsigned i     = i0 + lane;
+    const unsigned bk    = static_cast<unsigned>(lane) < i0 ? p.entries[0][i0 - 1 - lane].x : none;
+    const uint2    e0    = i < p.count ? p.entries[0][i] : make_uint2(none, 0);
+    const uint2    e1    = i + 32u < p.count ? p.entries[0][i + 32] : make_uint2(none, 0);
+    const unsigned first = __shfl_sync(kAll, e0.x, 0);
+    if (first == none)
         return;
-    // the run at the unit's start: `back` positions of it lie before (32: at least); how far it goes on
-    const unsigned other = __ballot_sync(kAll, bk != key);
+    const int valid = __popc(__ballot_sync(kAll, e0.x != none)) + __popc(__ballot_sync(kAll, e1.x != none));
+    // the run at the start: `back` positions of it lie before (32: at least), it goes on for `on` (64: at least)
+    const unsigned other = __ballot_sync(kAll, bk != first);
     const int      back  = other ? __ffs(other) - 1 : 32;
-    const unsigned d0 = __ballot_sync(kAll, k0 != key), d1 = __ballot_sync(kAll, k1 != key);
+    const unsigned d0 = __ballot_sync(kAll, e0.x != first), d1 = __ballot_sync(kAll, e1.x != first);
     const int      on    = d0 ? __ffs(d0) - 1 : d1 ? 31 + __ffs(d1) : 64;
-    // what this warp sums: positions from..to, counted from the unit's start
-    int  from = 0, to = n;
-    bool head = back > 0; // the first run belongs to `partials`
-    if (back > 0 && back + on <= kShortRun)
+    // the run at the end: from position `start`, as far as it starts here, up to `stop` (beyond n if it goes on)
+    const unsigned endKey = __shfl_sync(kAll, e0.x, n - 1);
+    const unsigned m0 = __ballot_sync(kAll, e0.x == endKey), m1 = __ballot_sync(kAll, e1.x == endKey);
+    const int      start = __ffs(m0) - 1, stop = start + __popc(m0) + (start + __popc(m0) == 32 ? __popc(m1) : 0);
+    const bool     goes = endKey != none && stop > n, ours = start > 0 || back == 0; // it goes on; it starts here
+    const bool     tail = goes && ours && stop - start > kShortRun;
+    // what this job sums: positions from..to, counted from i0
+    int from, to;
+    if (whole)
     {
-        from = on; // the warp before does it
-        head = false;
-    }
-    if (from >= n)
-        return;
-    // the run at the unit's end
-    const unsigned endKey = __shfl_sync(kAll, k0, n - 1), next = __shfl_sync(kAll, n < 32 ? k0 : k1, n & 31);
-    bool           tail   = false; // the last run belongs to `partials`
-    if (next == endKey && endKey != none)
-    {
-        const unsigned e0 = __ballot_sync(kAll, k0 == endKey), e1 = __ballot_sync(kAll, k1 == endKey);
-        const int      start = __ffs(e0) - 1, end = start + __popc(e0) + (start + __popc(e0) == 32 ? __popc(e1) : 0);
-        tail                 = (head && endKey == key) || end - start > kShortRun;
-        if (!tail)
-            to = end;
-    }
-    const unsigned s0 = __ballot_sync(kAll, k0 != none);
-    const int      valid = __popc(s0) + __popc(__ballot_sync(kAll, k1 != none));
-    to                   = min(to, valid);
-    const uint8_t *r0 = k0 != none ? p.grad.at(o0) : nullptr, *r1 = k1 != none ? p.grad.at(o1) : nullptr;
-    // bit j of ends: position j is the last of its run
-    const unsigned f0 = __shfl_down_sync(kAll, k0, 1), f1 = __shfl_down_sync(kAll, k1, 1), g1 = __shfl_sync(kAll, k1, 0);
-    unsigned long long ends = __ballot_sync(kAll, k0 != (lane < 31 ? f0 : g1));
-    ends |= static_cast<unsigned long long>(__ballot_sync(kAll, k1 != f1 || lane == 31)) << 32;
-    ends |= 1ull << (to - 1);
-    float acc[8] = {};
-    for (int j = from; j < to; j += kGradAhead)
-    {
-        Vec<GRAD, W> raw[kGradAhead][V];
-#pragma unroll
-        for (int a = 0; a < kGradAhead; ++a)
+        if (item & 1)
         {
-            const unsigned long long at0 = __shfl_sync(kAll, reinterpret_cast<unsigned long long>(r0), (j + a) & 31);
-            const unsigned long long at1 = __shfl_sync(kAll, reinterpret_cast<unsigned long long>(r1), (j + a) & 31);
-            const uint8_t           *row = reinterpret_cast<const uint8_t *>(j + a < 32 ? at0 : at1);
+            if (!tail)
+                return;
+            from = start, to = n;
+        }
+        else
+        {
+            if (back == 0 || back + on <= kShortRun)
+                return;
+            from = 0, to = min(on, n);
+        }
+    }
+    else
+    {
+        from = back > 0 ? on : 0; // a run from before is done by the warp it starts with, or by groups
+        to   = min(tail ? start : goes && ours ? stop : n, valid);
+        if (from >= min(to, n))
+            return;
+    }
+    // bit j of ends: position j is the last of its run, as far as this job goes
+    const unsigned     f0 = __shfl_down_sync(kAll, e0.x, 1), f1 = __shfl_down_sync(kAll, e1.x, 1), g1 = __shfl_sync(kAll, e1.x, 0);
+    unsigned long long ends = __ballot_sync(kAll, e0.x != (lane < 31 ? f0 : g1));
+    ends |= static_cast<unsigned long long>(__ballot_sync(kAll, e1.x != f1 || lane == 31)) << 32;
+    ends |= 1ull << (to - 1);
+    float *const part   = whole ? p.partials + static_cast<long long>(item) * p.cols : nullptr;
+    float        acc[8] = {};
+    for (int j = from; j < to; j += kAhead)
+    {
+        Vec<GRAD, W> raw[kAhead][V];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+        {
+            const unsigned o0 = __shfl_sync(kAll, e0.y, (j + a) & 31), o1 = __shfl_sync(kAll, e1.y, (j + a) & 31);
+            const uint8_t *row = p.grad.at(j + a < 32 ? o0 : o1);
 #pragma unroll
             for (int v = 0; v < V; ++v)
             {
@@ -508,7 +517,7 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_runs_kernel(const __gri
             }
         }
 #pragma unroll
-        for (int a = 0; a < kGradAhead; ++a)
+        for (int a = 0; a < kAhead; ++a)
         {
             const int q = j + a;
             if (q >= to)
@@ -523,39 +532,33 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_runs_kernel(const __gri
             }
             if (!((ends >> q) & 1))
                 continue;
-            const unsigned kq   = __shfl_sync(kAll, q < 32 ? k0 : k1, q & 31);
-            float         *part = nullptr;
-            if (head || (tail && q + 1 == to))
-                part = p.partials + (static_cast<long long>(u) * 2 + (head ? 0 : 1)) * p.cols;
-            embedding_grad_put<W>(p, part, kq, c0, acc[0], acc[1], acc[2], acc[3], acc[4], acc[5], acc[6], acc[7]);
+            embedding_grad_put<W>(p, part, __shfl_sync(kAll, q < 32 ? e0.x : e1.x, q & 31), c0, acc[0], acc[1], acc[2], acc[3], acc[4],
+                                  acc[5], acc[6], acc[7]);
 #pragma unroll
             for (int z = 0; z < 8; ++z) acc[z] = 0.0f;
-            head = false;
         }
     }
 }
 
-// ---- third kernel: the runs longer than kShortRun that cross units. A CTA looks after eight units: a warp each finds out whether
-// such a run starts in its unit; the CTA then adds up the run's parts for kGradCols columns, each warp a contiguous share of the
-// units, the warps one after another.
+// ---- third kernel: the runs longer than kShortRun. A CTA looks after eight groups: a warp each finds out whether such a run starts in
+// its group; the CTA then adds up the run's parts for kGradCols columns, each warp a contiguous share of the groups, the warps one
+// after another.
 __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
     __shared__ float    sums[8][kGradCols];
     __shared__ unsigned keys[8];
-    constexpr unsigned kAll = 0xffffffffu;
-    const unsigned     none = static_cast<unsigned>(p.rows);
-    const int          lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr unsigned  kAll = 0xffffffffu;
+    const unsigned      none = static_cast<unsigned>(p.rows);
+    const int           lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     {
         const unsigned u = blockIdx.x * 8 + warp;
         unsigned       k = none;
-        if (u + 1 < p.units) // not the last unit, so it is full
+        if (u + 1 < p.groups) // not the last group, so it is full
         {
-            const unsigned first = u * p.unit;
-            const unsigned mine  = p.entries[0][min(first + lane, p.count - 1)].x; // the unit after this one has a position at least
-            const unsigned prev  = first > 0 ? p.entries[0][first - 1].x : none;
-            const unsigned last = __shfl_sync(kAll, mine, p.unit - 1), after = p.entries[0][first + p.unit].x;
-            const unsigned same  = __ballot_sync(kAll, mine == last);
-            const unsigned start = first + __ffs(same) - 1;
+            const unsigned first = u * kShortRun;
+            const unsigned mine = p.entries[0][first + lane].x, prev = first > 0 ? p.entries[0][first - 1].x : none;
+            const unsigned last = __shfl_sync(kAll, mine, 31), after = p.entries[0][first + kShortRun].x;
+            const unsigned start = first + __ffs(__ballot_sync(kAll, mine == last)) - 1;
             if (last != none && after == last && !(start == first && prev == last) && start + kShortRun < p.count
                 && p.entries[0][start + kShortRun].x == last)
                 k = last;
@@ -569,16 +572,16 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
         const unsigned u = blockIdx.x * 8 + l, k = keys[l];
         if (k == none)
             continue;
-        unsigned       more = 0; // units the run goes on in
+        unsigned more = 0; // groups the run goes on in
         for (;;)
         {
-            const unsigned long long at = (static_cast<unsigned long long>(u) + 1 + more + lane) * p.unit;
+            const unsigned long long at = (static_cast<unsigned long long>(u) + 1 + more + lane) * kShortRun;
             const unsigned           on = __ballot_sync(kAll, at < p.count && p.entries[0][at].x == k);
             more += on == kAll ? 32 : __ffs(~on) - 1;
             if (on != kAll)
                 break;
         }
-        // share of this warp: parts from..to of 0 (slot 1 of unit u) and 1..more (slot 0 of unit u + part)
+        // share of this warp: parts from..to of 0 (slot 1 of group u) and 1..more (slot 0 of group u + part)
         const unsigned per = (more + 8) / 8, from = min(more + 1, warp * per), to = min(more + 1, from + per);
         const int      c0  = blockIdx.y * kGradCols + lane;
         float          s[8] = {};

@@ -56,7 +56,7 @@ int launch_staged(const LayerNormKParams &p, cudaStream_t stream)
         if (ring > 32 * 1024)
             if (int st = raise_smem(layernorm_block_kernel<SRC, W>, 112 * 1024, raised))
                 return st;
-        layernorm_block_kernel<SRC, W><<<std::min(p.rows, static_cast<unsigned>(kSms * (512 / threads))), threads, ring, stream>>>(p);
+        layernorm_block_kernel<SRC, W><<<std::min(p.rows, static_cast<unsigned>(kSms * (kBlockResident / threads))), threads, ring, stream>>>(p);
         return B200PP_SUCCESS;
     }
     const WarpPlan plan = plan_warp(p.cols);

@@ -16,7 +16,7 @@ struct GradPlan
     int threads, groups, values, ctas, span, parts;
 };
 
-GradPlan plan_layernorm_grad(long long rows, long long cols)
+GradPlan plan_layernorm_grad(long long rows, long long cols, int elem)
 {
     GradPlan g{};
     if (cols <= 8 * 16 * kGradResident)
@@ -34,9 +34,11 @@ GradPlan plan_layernorm_grad(long long rows, long long cols)
         }
         else
         {
-            g.values = 16;
             while (g.ctas * 16 * kGradResident < cols) g.ctas *= 2;
-            g.threads = static_cast<int>((cols + g.ctas * 512 - 1) / (g.ctas * 512) * 32);
+            // sixteen values, or 24 where that lets two CTAs share an SM (shared memory is too small for two with float32 rows)
+            const long long part = (cols + g.ctas - 1) / g.ctas;
+            g.values             = elem < 4 && part > 16 * kGradResident / 2 && part <= 24 * kGradResident / 2 ? 24 : 16;
+            g.threads            = static_cast<int>((part + 32 * g.values - 1) / (32 * g.values) * 32);
         }
         g.span = g.threads * g.values;
         // several rows per CTA as long as there are enough for all SMs; whole warps
@@ -81,7 +83,8 @@ template<int SRC, int GRAD, int W>
 int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
 {
     if (g.threads > 32)
-        return launch_one_pass<SRC, GRAD, 16, W, false, true>(p, g, stream);
+        return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, false, true>(p, g, stream)
+                              : launch_one_pass<SRC, GRAD, 24, W, false, true>(p, g, stream);
     if (g.values == 8)
         return launch_one_pass<SRC, GRAD, 8, W, true, false>(p, g, stream);
     if (g.threads == 32)
@@ -156,7 +159,7 @@ extern "C" int b200ppLayerNormBackwardWorkspace(const B200ppRows *src, size_t *b
     t.base         = reinterpret_cast<void *>(uintptr_t(256));
     if (int st = take_rows(&t, "Input", false, m, rows))
         return st;
-    *bytes = grad_workspace(plan_layernorm_grad(rows, t.cols), t.cols);
+    *bytes = grad_workspace(plan_layernorm_grad(rows, t.cols, row_elem_size(t.dtype)), t.cols);
     return B200PP_SUCCESS;
 }
 
@@ -187,7 +190,7 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     if (rows > 0 && (!op->mean || !op->rstd))
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "The backward pass needs the forward pass's mean and rstd");
     p.cols  = static_cast<int>(src->cols);
-    const GradPlan plan = plan_layernorm_grad(rows, p.cols);
+    const GradPlan plan = plan_layernorm_grad(rows, p.cols, row_elem_size(src->dtype));
     p.parts             = plan.parts;
     if (op->dweight || op->dbias)
     {
@@ -228,6 +231,9 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
         st = launch_two_pass<B200PP_F32>(p, stream);
     if (st || !p.partials)
         return st;
-    layernorm_grad_join_kernel<<<(2u * p.cols + 31u) / 32u, dim3(32, 32), 0, stream>>>(p);
+    // as many threads share a column as there are parts for
+    const int  share = p.parts >= 64 ? 32 : p.parts >= 8 ? 8 : 1;
+    const dim3 block(share == 1 ? 128 : 32, share);
+    layernorm_grad_join_kernel<<<(2u * p.cols + block.x - 1) / block.x, block, 0, stream>>>(p);
     return check_launch("LayerNormBackward");
 }

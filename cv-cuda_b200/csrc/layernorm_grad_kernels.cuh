@@ -330,30 +330,38 @@ __global__ void __launch_bounds__(256) layernorm_grad_columns_kernel(const Layer
     }
 }
 
-// Adds up the parts: a thread takes every 32nd part of a column, the 32 threads of the column are joined in order.
+// Adds up the parts: blockDim.y threads share a column, each takes every blockDim.y-th part, and the first joins them in order.
 __global__ void __launch_bounds__(1024) layernorm_grad_join_kernel(const LayerNormGradKParams p)
 {
-    __shared__ float   sum[32][33];
-    const long long    c = static_cast<long long>(blockIdx.x) * 32 + threadIdx.x; // of 2 * cols
-    const long long    n = 2LL * p.cols;
-    float              s = 0.0f;
+    __shared__ float sum[32][33];
+    const long long  c = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, n = 2LL * p.cols; // column of dw, db
+    float            s = 0.0f;
     if (c < n)
-        for (int k = threadIdx.y; k < p.parts; k += 32) s += p.partials[k * n + c];
-    sum[threadIdx.y][threadIdx.x] = s;
-    __syncthreads();
-    // one warp per column now
-    s                 = warp_sum(sum[threadIdx.x][threadIdx.y]);
-    const long long o = static_cast<long long>(blockIdx.x) * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && o < n)
     {
-        if (o < p.cols)
-        {
-            if (p.dweight)
-                store_elem_as(p.dweight, o, p.dweightType, s);
-        }
-        else if (p.dbias)
-            store_elem_as(p.dbias, o - p.cols, p.dbiasType, s);
+#pragma unroll 4
+        for (int k = threadIdx.y; k < p.parts; k += blockDim.y) s += p.partials[k * n + c];
     }
+    if (blockDim.y > 1)
+    {
+        sum[threadIdx.y][threadIdx.x] = s;
+        __syncthreads();
+        if (threadIdx.y > 0)
+            return;
+        float t[4] = {};
+        for (int k = 0; k < static_cast<int>(blockDim.y); k += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] += sum[k + i][threadIdx.x];
+        s = (t[0] + t[1]) + (t[2] + t[3]);
+    }
+    if (c >= n)
+        return;
+    if (c < p.cols)
+    {
+        if (p.dweight)
+            store_elem_as(p.dweight, c, p.dweightType, s);
+    }
+    else if (p.dbias)
+        store_elem_as(p.dbias, c - p.cols, p.dbiasType, s);
 }
 
 } // namespace b200pp

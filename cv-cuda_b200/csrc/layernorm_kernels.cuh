@@ -172,10 +172,11 @@ __global__ void __launch_bounds__(256, kWarpCtas<E>) layernorm_warp_kernel(const
 // Forward, longer rows: a CTA per row, sixteen values per thread. (Clusters of CTAs for rows that do not fit into one were slower than
 // the two kernels over chunks below: 72 against 55 us for 256 uint8 images of 224 x 224 x 3. A CTA of so many threads is alone on
 // its SM, and nothing goes on there while it waits for its barriers.)
-constexpr int kBlockCols = 16 * 512;
+constexpr int kBlockCols     = 16 * 512;
+constexpr int kBlockResident = 768; // threads that fit on an SM, by the registers per thread the launch bound leaves (80)
 
 template<int SRC, int W>
-__global__ void __launch_bounds__(512) layernorm_block_kernel(const LayerNormKParams p)
+__global__ void __launch_bounds__(kBlockResident) layernorm_block_kernel(const LayerNormKParams p)
 {
     constexpr int               E = 16, kStages = 3;
     typedef RowStage<SRC, E, W> Stage;

@@ -47,7 +47,8 @@ class _EmbeddingGradOp(C.Structure):
 _TYPES = {torch.uint8: 0, torch.float32: 6, torch.float16: 7, torch.bfloat16: 8, torch.int32: 5, torch.int64: 9}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
-# the handle of torch's current stream without building a Stream object, where this torch has it
+# the current device, and the handle of its current stream without building a Stream object, where this torch has them
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
@@ -83,23 +84,27 @@ def _invalid(message: str) -> Error:
     return Error(Status.ERROR_INVALID_ARGUMENT, message)
 
 
-def _device_of(*tensors) -> int:
+def _device_of(first, *others) -> int:
     """Index of the device the call runs on: that of the CUDA tensors, which must agree (page-locked host tensors follow)."""
-    dev = -1
-    for t in tensors:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors")
-        if t.is_cuda:
-            d = t.get_device()
-            if dev < 0:
-                dev = d
-            elif d != dev:
-                raise _invalid(f"Tensors are on different devices (cuda:{dev} and cuda:{d})")
-        elif not t.is_pinned():
-            raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors")
+    try:
+        dev = first.get_device() if first.is_cuda else _host(first)
+        for t in others:
+            if t is not None:
+                d = t.get_device() if t.is_cuda else _host(t)
+                if d != dev:
+                    if dev < 0:
+                        dev = d
+                    elif d >= 0:
+                        raise _invalid(f"Tensors are on different devices (cuda:{dev} and cuda:{d})")
+    except AttributeError:
+        raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors") from None
     return dev if dev >= 0 else torch.cuda.current_device()
+
+
+def _host(t) -> int:
+    if not t.is_pinned():
+        raise _invalid("Arguments must be cuda-accessible, pitch-linear tensors")
+    return -1
 
 
 def _view(t: torch.Tensor, axes: int, what: str):
@@ -131,9 +136,13 @@ def _view(t: torch.Tensor, axes: int, what: str):
     return cols, dims
 
 
-# A B200ppRows as bytes, which ctypes passes by address: a third of the time a ctypes.Structure takes to fill in.
+# The C structures as bytes, which ctypes passes by address: a third of the time a ctypes.Structure takes to fill in.
 _pack_rows = struct.Struct("=Qi4xq3q3q").pack
-assert struct.calcsize("=Qi4xq3q3q") == C.sizeof(_Rows)
+_pack_ln = struct.Struct("=QQiif4xQQ").pack
+_pack_ln_grad = struct.Struct("=QQQi4xQQii").pack
+_pack_emb_grad = struct.Struct("=fiq").pack
+assert struct.calcsize("=Qi4xq3q3q") == C.sizeof(_Rows) and struct.calcsize("=QQiif4xQQ") == C.sizeof(_LayerNormOp)
+assert struct.calcsize("=QQQi4xQQii") == C.sizeof(_LayerNormGradOp) and struct.calcsize("=fiq") == C.sizeof(_EmbeddingGradOp)
 
 
 def _rows(t: torch.Tensor, axes: int, what: str):
@@ -158,10 +167,8 @@ def _axes_of(t: torch.Tensor, axes: int) -> int:
     return axes
 
 
-def _param(t: Optional[torch.Tensor], numel: int, what: str, kinds=_FLOATS) -> Tuple[Optional[int], int]:
-    """(address, type code) of a packed tensor of `numel` values, or (None, 0)."""
-    if t is None:
-        return None, 0
+def _param(t: torch.Tensor, numel: int, what: str, kinds=_FLOATS) -> Tuple[int, int]:
+    """(address, type code) of a packed tensor of `numel` values."""
     if t.dtype not in kinds:
         raise _invalid(f"Invalid DataType of the {what}")
     if t.numel() != numel or not t.is_contiguous():
@@ -169,45 +176,33 @@ def _param(t: Optional[torch.Tensor], numel: int, what: str, kinds=_FLOATS) -> T
     return t.data_ptr(), _TYPES[t.dtype]
 
 
-class _Launch:
-    """Makes the device and the launch stream torch's current ones, so that what the call allocates belongs to that stream;
-    gives the stream's handle. Does nothing where they are current already."""
-
-    __slots__ = ("handle", "_stack")
-
-    def __init__(self, device: int, stream):
-        self._stack = None
-        other = device != torch.cuda.current_device()
-        current = _raw_stream(device)
-        self.handle = current if stream is None else ops._stream_handle(stream)
-        if not other and self.handle == current:
-            return
-        self._stack = contextlib.ExitStack()
-        if other:
-            self._stack.enter_context(torch.cuda.device(device))
-        if self.handle != current:
-            if not isinstance(stream, torch.cuda.Stream):
-                stream = torch.cuda.ExternalStream(self.handle, device=device) if self.handle else torch.cuda.default_stream(device)
-            elif stream.device.index != device:
-                self._stack.close()
-                raise _invalid(f"The stream belongs to {stream.device}, the tensors to cuda:{device}")
-            self._stack.enter_context(torch.cuda.stream(stream))
-
-    def __enter__(self):
-        return self.handle
-
-    def __exit__(self, *exc):
-        return self._stack.__exit__(*exc) if self._stack is not None else None
+def _enter(device: int, stream):
+    """(handle of the launch stream, what to leave afterwards or None). Makes the device and the stream torch's current ones where
+    they are not, so that what the call allocates belongs to that stream."""
+    current = _raw_stream(device)
+    handle = current if stream is None else ops._stream_handle(stream)
+    other = device != _current_device()
+    if not other and handle == current:
+        return handle, None
+    stack = contextlib.ExitStack()
+    if other:
+        stack.enter_context(torch.cuda.device(device))
+    if handle != current:
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+        elif stream.device.index != device:
+            stack.close()
+            raise _invalid(f"The stream belongs to {stream.device}, the tensors to cuda:{device}")
+        stack.enter_context(torch.cuda.stream(stream))
+    return handle, stack
 
 
-def _workspace(query, rows: bytes, device: int):
-    """(tensor that keeps it alive, address, size) of the scratch memory `query` asks for."""
+@lru_cache(maxsize=1024)
+def _workspace_size(name: str, code: int, cols: int, rows: int) -> int:
+    """What the library asks for; it depends on the shape alone."""
     n = C.c_size_t(0)
-    _check(query(rows, C.byref(n)))
-    if n.value == 0:
-        return None, None, 0
-    t = torch.empty(n.value, dtype=torch.uint8, device=_cuda(device))
-    return t, t.data_ptr(), n.value
+    _check(getattr(_lib(), name)(_pack_rows(256, code, cols, rows, 1, 1, cols * 8, 0, 0), C.byref(n)))
+    return n.value
 
 
 # ------------------------------------------------------------------------------------------------ LayerNorm
@@ -215,19 +210,21 @@ def _workspace(query, rows: bytes, device: int):
 _WHOLE_ROWS = 8192  # rows up to this length need no workspace (row_ops.h)
 
 
-def _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle):
+def _layernorm(d, src, weight, bias, epsilon, axes, mean, rstd, device, handle):
+    """`d`: the output, as _rows packs it, or the tensor `src` is laid out like, freshly allocated."""
     s, cols, count = _rows(src, axes, "Input")
-    d = _rows(dst, axes, "Output")[0]
-    w, wt = _param(weight, cols, "weight")
-    b, bt = _param(bias, cols, "bias")
-    op = _LayerNormOp(w, b, wt, bt, epsilon, _param(mean, count, "mean", (torch.float32,))[0],
-                      _param(rstd, count, "rstd", (torch.float32,))[0])
-    L = _lib()
-    keep = ws = None
-    size = 0
+    if not isinstance(d, bytes):
+        d = _pack_rows(d.data_ptr(), _TYPES.get(d.dtype, -1), cols, count, 1, 1, cols * d.element_size(), 0, 0)
+    w, wt = _param(weight, cols, "weight") if weight is not None else (0, 0)
+    b, bt = _param(bias, cols, "bias") if bias is not None else (0, 0)
+    op = _pack_ln(w, b, wt, bt, epsilon, _param(mean, count, "mean", (torch.float32,))[0] if mean is not None else 0,
+                  _param(rstd, count, "rstd", (torch.float32,))[0] if rstd is not None else 0)
+    keep, ws, size = None, None, 0
     if cols > _WHOLE_ROWS:
-        keep, ws, size = _workspace(L.b200ppLayerNormWorkspace, s, device)
-    _check(L.b200ppLayerNorm(s, d, C.byref(op), ws, size, handle))
+        size = _workspace_size("b200ppLayerNormWorkspace", _TYPES.get(src.dtype, -1), cols, count)
+        keep = torch.empty(size, dtype=torch.uint8, device=_cuda(device))
+        ws = keep.data_ptr()
+    _check(_lib().b200ppLayerNorm(s, d, op, ws, size, handle))
 
 
 def layernorm_into(dst: torch.Tensor, src: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -239,8 +236,12 @@ def layernorm_into(dst: torch.Tensor, src: torch.Tensor, weight: Optional[torch.
     axes = _axes_of(src, axes)
     if dst.shape != src.shape:
         raise _invalid("Input and output shapes are different")
-    with _Launch(device, stream) as handle:
-        _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle)
+    handle, leave = _enter(device, stream)
+    try:
+        _layernorm(_rows(dst, axes, "Output")[0], src, weight, bias, epsilon, axes, mean, rstd, device, handle)
+    finally:
+        if leave is not None:
+            leave.close()
     return dst
 
 
@@ -255,30 +256,37 @@ def layernorm(src: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Op
     device = _device_of(src, weight, bias)
     axes = _axes_of(src, axes)
     kind = data_type or (src.dtype if src.dtype != torch.uint8 else torch.float32)
-    with _Launch(device, stream) as handle:
-        dst = torch.empty(src.shape, dtype=kind, device=_cuda(device))
+    handle, leave = _enter(device, stream)
+    try:
+        on = _cuda(device)
+        dst = torch.empty(src.shape, dtype=kind, device=on)
         mean = rstd = None
         if stats:
-            mean = torch.empty(src.shape[:src.dim() - axes], dtype=torch.float32, device=_cuda(device))
+            mean = torch.empty(src.shape[:src.dim() - axes], dtype=torch.float32, device=on)
             rstd = torch.empty_like(mean)
         _layernorm(dst, src, weight, bias, epsilon, axes, mean, rstd, device, handle)
+    finally:
+        if leave is not None:
+            leave.close()
     return (dst, mean, rstd) if stats else dst
 
 
-def _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle):
+def _layernorm_backward(d, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle):
     s, cols, count = _rows(src, axes, "Input")
     g = _rows(grad, axes, "Gradient")[0]
-    d = None if dsrc is None else _rows(dsrc, axes, "Input gradient")[0]
-    w, wt = _param(weight, cols, "weight")
-    dw, dwt = _param(dweight, cols, "weight gradient")
-    db, dbt = _param(dbias, cols, "bias gradient")
-    op = _LayerNormGradOp(_param(mean, count, "mean", (torch.float32,))[0], _param(rstd, count, "rstd", (torch.float32,))[0], w, wt,
-                          dw, db, dwt, dbt)
-    L = _lib()
-    keep, ws, size = (None, None, 0)
-    if dweight is not None or dbias is not None:
-        keep, ws, size = _workspace(L.b200ppLayerNormBackwardWorkspace, s, device)
-    _check(L.b200ppLayerNormBackward(g, s, d, C.byref(op), ws, size, handle))
+    if d is not None and not isinstance(d, bytes):
+        d = _pack_rows(d.data_ptr(), _TYPES.get(d.dtype, -1), cols, count, 1, 1, cols * d.element_size(), 0, 0)
+    w, wt = _param(weight, cols, "weight") if weight is not None else (0, 0)
+    dw, dwt = _param(dweight, cols, "weight gradient") if dweight is not None else (0, 0)
+    db, dbt = _param(dbias, cols, "bias gradient") if dbias is not None else (0, 0)
+    op = _pack_ln_grad(_param(mean, count, "mean", (torch.float32,))[0], _param(rstd, count, "rstd", (torch.float32,))[0], w, wt,
+                       dw, db, dwt, dbt)
+    keep, ws, size = None, None, 0
+    if dw or db:
+        size = _workspace_size("b200ppLayerNormBackwardWorkspace", _TYPES.get(src.dtype, -1), cols, count)
+        keep = torch.empty(size, dtype=torch.uint8, device=_cuda(device))
+        ws = keep.data_ptr()
+    _check(_lib().b200ppLayerNormBackward(g, s, d, op, ws, size, handle))
 
 
 def layernorm_backward_into(dsrc: Optional[torch.Tensor], dweight: Optional[torch.Tensor], dbias: Optional[torch.Tensor],
@@ -290,8 +298,13 @@ def layernorm_backward_into(dsrc: Optional[torch.Tensor], dweight: Optional[torc
     axes = _axes_of(src, axes)
     if grad.shape != src.shape or (dsrc is not None and dsrc.shape != src.shape):
         raise _invalid("Input and gradient shapes are different")
-    with _Launch(device, stream) as handle:
-        _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle)
+    handle, leave = _enter(device, stream)
+    try:
+        _layernorm_backward(None if dsrc is None else _rows(dsrc, axes, "Input gradient")[0], dweight, dbias, grad, src, mean, rstd,
+                            weight, axes, device, handle)
+    finally:
+        if leave is not None:
+            leave.close()
     return dsrc, dweight, dbias
 
 
@@ -305,17 +318,22 @@ def layernorm_backward(grad: torch.Tensor, src: torch.Tensor, mean: torch.Tensor
     axes = _axes_of(src, axes)
     if grad.shape != src.shape:
         raise _invalid("Input and gradient shapes are different")
-    with _Launch(device, stream) as handle:
+    handle, leave = _enter(device, stream)
+    try:
+        on = _cuda(device)
         dsrc = dweight = dbias = None
         row = src.shape[src.dim() - axes:]
         if src_grad:
-            dsrc = torch.empty(src.shape, dtype=data_type or (src.dtype if src.dtype != torch.uint8 else grad.dtype), device=_cuda(device))
+            dsrc = torch.empty(src.shape, dtype=data_type or (src.dtype if src.dtype != torch.uint8 else grad.dtype), device=on)
         kind = weight.dtype if weight is not None else torch.float32
         if weight_grad:
-            dweight = torch.empty(row, dtype=kind, device=_cuda(device))
+            dweight = torch.empty(row, dtype=kind, device=on)
         if bias_grad:
-            dbias = torch.empty(row, dtype=kind, device=_cuda(device))
+            dbias = torch.empty(row, dtype=kind, device=on)
         _layernorm_backward(dsrc, dweight, dbias, grad, src, mean, rstd, weight, axes, device, handle)
+    finally:
+        if leave is not None:
+            leave.close()
     return dsrc, dweight, dbias
 
 
@@ -325,17 +343,17 @@ def _indices(indices: torch.Tensor) -> bytes:
     return _rows(indices, 0, "Indices")[0]
 
 
-def _embedding(dst, indices, table, scale, handle):
-    _check(_lib().b200ppEmbedding(_indices(indices), _rows(table, 1, "Table")[0], _rows(dst, 1, "Output")[0], scale, handle))
-
-
 def embedding_into(dst: torch.Tensor, indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *, stream=None) -> torch.Tensor:
     """Embedding lookup into ``dst`` (the shape of ``indices`` followed by the number of columns): see :func:`embedding`."""
     device = _device_of(table, indices, dst)
     if table.dim() != 2 or dst.shape != (*indices.shape, table.shape[1]):
         raise _invalid("The output must have the indices' shape followed by the table's number of columns")
-    with _Launch(device, stream) as handle:
-        _embedding(dst, indices, table, scale, handle)
+    handle, leave = _enter(device, stream)
+    try:
+        _check(_lib().b200ppEmbedding(_indices(indices), _rows(table, 1, "Table")[0], _rows(dst, 1, "Output")[0], scale, handle))
+    finally:
+        if leave is not None:
+            leave.close()
     return dst
 
 
@@ -347,18 +365,25 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *,
     device = _device_of(table, indices)
     if table.dim() != 2:
         raise _invalid("Table must have two dimensions")
-    with _Launch(device, stream) as handle:
-        dst = torch.empty((*indices.shape, table.shape[1]), dtype=data_type or table.dtype, device=_cuda(device))
-        _embedding(dst, indices, table, scale, handle)
+    handle, leave = _enter(device, stream)
+    try:
+        i, _, count = _rows(indices, 0, "Indices")
+        t, cols, _ = _rows(table, 1, "Table")
+        dst = torch.empty((*indices.shape, cols), dtype=data_type or table.dtype, device=_cuda(device))
+        d = _pack_rows(dst.data_ptr(), _TYPES.get(dst.dtype, -1), cols, count, 1, 1, cols * dst.element_size(), 0, 0)
+        _check(_lib().b200ppEmbedding(i, t, d, scale, handle))
+    finally:
+        if leave is not None:
+            leave.close()
     return dst
 
 
 def _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate, device, handle):
-    g = _rows(grad, 1, "Gradient")[0]
-    op = _EmbeddingGradOp(scale, int(accumulate), -1 if padding_index is None else int(padding_index))
-    L = _lib()
-    keep, ws, size = _workspace(L.b200ppEmbeddingBackwardWorkspace, g, device)
-    _check(L.b200ppEmbeddingBackward(g, _indices(indices), _rows(dtable, 1, "Table gradient")[0], C.byref(op), ws, size, handle))
+    g, cols, count = _rows(grad, 1, "Gradient")
+    op = _pack_emb_grad(scale, int(accumulate), -1 if padding_index is None else int(padding_index))
+    size = _workspace_size("b200ppEmbeddingBackwardWorkspace", _TYPES.get(grad.dtype, -1), cols, count)
+    ws = torch.empty(size, dtype=torch.uint8, device=_cuda(device))
+    _check(_lib().b200ppEmbeddingBackward(g, _indices(indices), _rows(dtable, 1, "Table gradient")[0], op, ws.data_ptr(), size, handle))
 
 
 def embedding_backward_into(dtable: torch.Tensor, grad: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, *,
@@ -368,8 +393,12 @@ def embedding_backward_into(dtable: torch.Tensor, grad: torch.Tensor, indices: t
     device = _device_of(dtable, grad, indices)
     if dtable.dim() != 2 or grad.shape != (*indices.shape, dtable.shape[1]):
         raise _invalid("The gradient must have the indices' shape followed by the table's number of columns")
-    with _Launch(device, stream) as handle:
+    handle, leave = _enter(device, stream)
+    try:
         _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate, device, handle)
+    finally:
+        if leave is not None:
+            leave.close()
     return dtable
 
 
@@ -381,9 +410,13 @@ def embedding_backward(grad: torch.Tensor, indices: torch.Tensor, rows: int, sca
     device = _device_of(grad, indices)
     if grad.dim() < 1 or grad.shape[:-1] != indices.shape:
         raise _invalid("The gradient must have the indices' shape followed by the table's number of columns")
-    with _Launch(device, stream) as handle:
+    handle, leave = _enter(device, stream)
+    try:
         dtable = torch.empty((int(rows), grad.shape[-1]), dtype=data_type, device=_cuda(device))
         _embedding_backward(dtable, grad, indices, scale, padding_index, False, device, handle)
+    finally:
+        if leave is not None:
+            leave.close()
     return dtable
 
 
