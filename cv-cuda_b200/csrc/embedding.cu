@@ -150,14 +150,13 @@ namespace {
 // Layout of the gradient's workspace.
 struct EmbeddingGradPlan
 {
-    unsigned units, groups, blocks;
+    unsigned units, groups;
     size_t   entries[2], partials, bytes;
 };
 
 EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
 {
     EmbeddingGradPlan w{};
-    w.blocks     = static_cast<unsigned>((cols + kGradCols - 1) / kGradCols);
     w.units      = static_cast<unsigned>((count + kGradUnit - 1) / kGradUnit);
     w.groups     = static_cast<unsigned>((count + kShortRun - 1) / kShortRun);
     size_t at    = 0;
@@ -171,18 +170,54 @@ EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
     return w;
 }
 
-template<int GRAD>
-void launch_runs(const EmbeddingGradKParams &p, int width, cudaStream_t stream)
+template<int GRAD, int W>
+int launch_runs(EmbeddingGradKParams &p, cudaStream_t stream)
 {
-    const unsigned grid = static_cast<unsigned>(((static_cast<unsigned long long>(p.units) + 2 * p.groups) * p.blocks + 7) / 8);
+    p.blocks                      = static_cast<unsigned>((static_cast<long long>(p.cols) + kGradCols<W> - 1) / kGradCols<W>);
+    const unsigned long long jobs = (static_cast<unsigned long long>(p.units) + 2 * p.groups) * p.blocks;
+    if (jobs > 0x7fffffffull)
+        return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
+    Launch(dim3(static_cast<unsigned>((jobs + 7) / 8)), dim3(256), 0, stream, 1, true).run(embedding_grad_runs_kernel<GRAD, W>, p);
+    return check_launch("EmbeddingBackward");
+}
+
+template<int GRAD>
+int launch_runs(EmbeddingGradKParams &p, int width, cudaStream_t stream)
+{
     if (width == 8)
-        embedding_grad_runs_kernel<GRAD, 8><<<grid, 256, 0, stream>>>(p);
-    else if (width == 4)
-        embedding_grad_runs_kernel<GRAD, 4><<<grid, 256, 0, stream>>>(p);
-    else if (width == 2)
-        embedding_grad_runs_kernel<GRAD, 2><<<grid, 256, 0, stream>>>(p);
-    else
-        embedding_grad_runs_kernel<GRAD, 1><<<grid, 256, 0, stream>>>(p);
+        return launch_runs<GRAD, 8>(p, stream);
+    if (width == 4)
+        return launch_runs<GRAD, 4>(p, stream);
+    if (width == 2)
+        return launch_runs<GRAD, 2>(p, stream);
+    return launch_runs<GRAD, 1>(p, stream);
+}
+
+// CTAs of the cluster that sorts: one for few indices, then eight; sixteen, where the GPU has room for such a cluster, once the
+// indices take longer than the exchange between the CTAs (16384 indices: 18 us with eight, 14 us with sixteen; 5003: 10.3 us both).
+int sort_ctas(long long count, size_t smem)
+{
+    if (count <= 2048)
+        return 1;
+    if (count <= 8192)
+        return 8;
+    static std::atomic<unsigned long long> wide{0}, asked{0};
+    int                                    dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(asked.load() & bit))
+    {
+        int clusters = 0;
+        if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess)
+        {
+            Launch launch(dim3(16), dim3(kSortThreads), static_cast<int>(smem), nullptr, 16, false);
+            if (cudaOccupancyMaxActiveClusters(&clusters, embedding_sort_kernel, &launch.cfg) == cudaSuccess && clusters > 0)
+                wide.fetch_or(bit);
+        }
+        cudaGetLastError();
+        asked.fetch_or(bit);
+    }
+    return wide.load() & bit ? 16 : 8;
 }
 
 } // namespace
@@ -238,51 +273,58 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     p.padding    = op->paddingIndex >= 0 && op->paddingIndex < rows ? static_cast<int>(op->paddingIndex) : -1;
     p.units      = w.units;
     p.groups     = w.groups;
-    p.blocks     = w.blocks;
     for (int k = 0; k < 2; ++k) p.entries[k] = reinterpret_cast<uint2 *>(ws + w.entries[k]);
     p.partials = reinterpret_cast<float *>(ws + w.partials);
     int bits = 1; // of the largest key, `rows`
     while (bits < 31 && (rows >> bits) != 0) ++bits;
     p.passes    = (bits + kSortMaxBits - 1) / kSortMaxBits;
     p.digitBits = (bits + p.passes - 1) / p.passes;
-    // as few warps as hold the indices kSortKeys at a time: each has a table of counts
-    p.sortWarps = 8;
-    while (p.sortWarps < kSortThreads / 32 && static_cast<long long>(p.sortWarps) * 32 * kSortKeys * kSortCtas < count) p.sortWarps *= 2;
-    int clusters = 1;
+    static std::atomic<unsigned long long> raised{0};
+    const size_t                           most = sort_smem_words(kSortThreads / 32, 1 << kSortMaxBits) * sizeof(unsigned);
+    if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(most), raised)))
+        return st;
+    if (count > 0)
+    {
+        // as few warps as hold the indices kSortKeys at a time: each has a table of counts
+        const int ctas = sort_ctas(count, most);
+        p.sortWarps    = 4;
+        while (p.sortWarps < kSortThreads / 32 && static_cast<long long>(p.sortWarps) * 32 * kSortKeys * ctas < count) p.sortWarps *= 2;
+        const long long warps = static_cast<long long>(ctas) * p.sortWarps;
+        p.span                = static_cast<unsigned>(((count + warps - 1) / warps + 31) / 32 * 32);
+        const size_t smem     = sort_smem_words(p.sortWarps, 1 << p.digitBits) * sizeof(unsigned);
+        Launch(dim3(ctas), dim3(kSortThreads), static_cast<int>(smem), stream, ctas, false).run(embedding_sort_kernel, p);
+        if ((st = check_launch("EmbeddingBackward")))
+            return st;
+    }
     if (!p.accumulate)
     {
         VecWidth width(p.cols);
         width.take(p.dtable, row_elem_size(p.dtableType));
         p.zeroWidth             = width.width;
         const long long rowSize = static_cast<long long>(p.cols) * row_elem_size(p.dtableType);
-        // a cluster per 256 KB to clear, at most as many as fit on the GPU beside the one that sorts
-        clusters += static_cast<int>(std::max(1LL, std::min(14LL, rows * rowSize / (256 << 10))));
-        p.zeroCtas  = (clusters - 1) * kSortCtas;
-        p.skipNamed = std::min(count, rows) * rowSize / p.zeroCtas > 2 * count * row_elem_size(p.indexType);
+        const int       ctas    = static_cast<int>(std::max(1LL, std::min({2LL * kSms, rows * rowSize / (32 << 10), rows})));
+        p.skipNamed             = std::min(count, rows) * rowSize / ctas > 2 * count * row_elem_size(p.indexType);
+        Launch(dim3(ctas), dim3(kZeroThreads), 0, stream, 1, count > 0).run(embedding_clear_kernel, p);
+        if ((st = check_launch("EmbeddingBackward")))
+            return st;
     }
-    const size_t smem = std::max(sort_smem_words(p.sortWarps, 1 << p.digitBits), static_cast<size_t>(kZeroRows / 32)) * sizeof(unsigned);
-    static std::atomic<unsigned long long> raised{0};
-    if ((st = raise_smem(embedding_sort_kernel, static_cast<int>(sort_smem_words(kSortThreads / 32, 1 << kSortMaxBits) * sizeof(unsigned)),
-                         raised)))
-        return st;
-    const unsigned long long jobs = (static_cast<unsigned long long>(w.units) + 2 * w.groups) * w.blocks;
-    if (jobs > 0x7fffffffull || w.blocks > 65535u)
-        return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
-    embedding_sort_kernel<<<clusters * kSortCtas, kSortThreads, smem, stream>>>(p);
-    if ((st = check_launch("EmbeddingBackward")) || count == 0)
+    if (count == 0)
         return st;
     VecWidth width(p.cols);
     width.take(p.grad, row_elem_size(p.gradType));
     width.take(p.dtable, row_elem_size(p.dtableType));
     width.take(p.partials, p.cols * static_cast<long long>(sizeof(float)), sizeof(float));
     if (p.gradType == B200PP_F16)
-        launch_runs<B200PP_F16>(p, width.width, stream);
+        st = launch_runs<B200PP_F16>(p, width.width, stream);
     else if (p.gradType == B200PP_BF16)
-        launch_runs<B200PP_BF16>(p, width.width, stream);
+        st = launch_runs<B200PP_BF16>(p, width.width, stream);
     else
-        launch_runs<B200PP_F32>(p, width.width, stream);
-    if ((st = check_launch("EmbeddingBackward")) || w.groups == 1)
+        st = launch_runs<B200PP_F32>(p, width.width, stream);
+    if (st || w.groups == 1)
         return st;
-    embedding_grad_join_kernel<<<dim3((w.groups - 1 + 7) / 8, w.blocks), 256, 0, stream>>>(p);
+    const unsigned blocks = static_cast<unsigned>((static_cast<long long>(p.cols) + kJoinCols - 1) / kJoinCols);
+    if (blocks > 65535u)
+        return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
+    Launch(dim3((w.groups - 1 + 7) / 8, blocks), dim3(256), 0, stream, 1, true).run(embedding_grad_join_kernel, p);
     return check_launch("EmbeddingBackward");
 }

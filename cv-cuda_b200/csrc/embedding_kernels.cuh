@@ -155,48 +155,49 @@ struct EmbeddingGradKParams
     int       padding;            // -1: none
     uint2    *entries[2];         // (index, position), count each; entries[0] holds the sorted ones
     int       passes, digitBits, sortWarps;
-    int       zeroCtas, zeroWidth, skipNamed; // CTAs that clear the table, their vector width, whether they leave out named rows
+    unsigned  span;                 // positions of a warp that sorts
+    int       zeroWidth, skipNamed; // vectors that clear the table, whether rows that are named are left out
     float    *partials;                       // [groups][2][cols]
     unsigned  units, groups;                  // of kGradUnit and kShortRun sorted positions
-    unsigned  blocks;                         // column blocks of kGradCols
+    unsigned  blocks;                         // column blocks of kGradCols<W>
 };
 
-// ---- first kernel: sort the positions 0..count-1 by index, stable; indices that take no part get the key `rows` and end up
-// last. Meanwhile the other CTAs clear the table.
+// ---- first kernel: sort the positions 0..count-1 by index, stable; indices that take no part get the key `rows` and end up last.
 //
-// Cluster 0 sorts: a least-significant-digit radix sort over kSortCtas CTAs. Each warp owns a contiguous range of the positions and
-// counts its digits in a table of its own; a prefix over the warps, the CTAs (through distributed shared memory) and the digits
-// turns the counts into the places each warp writes to. The arrays between the passes are in global memory (they stay in L2); the
-// cluster barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and most counts of
-// indices are small; clearing the table, which takes longer for the usual sizes, hides it.
-constexpr int kSortCtas       = 8;
-constexpr int kSortThreads    = 1024;
-constexpr int kSortMaxBits    = 10;
-constexpr int kSortKeys       = 8; // keys a lane holds at a time
+// A least-significant-digit radix sort by one CTA or one cluster. Each warp owns a contiguous range of the positions and counts its
+// digits in a table of its own; a prefix over the warps, the CTAs (through distributed shared memory) and the digits turns the
+// counts into the places each warp writes to. The arrays between the passes are in global memory (they stay in L2); the cluster
+// barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and most counts of indices are
+// small; clearing the table goes on at the same time. Few indices cost latency -- the trips to memory, the barriers, code that is
+// fetched to run once (8 us for 1000) -- many the scattered stores and the ballots (25 us for 65536 of 50000, 59 us for 262144 of
+// 128000, sixteen CTAs). A match instruction instead of the ballots takes a turn for each different digit of a warp (43 us for the
+// 65536 with eight CTAs, where ballots take 34).
+constexpr int kSortThreads = 1024;
+constexpr int kSortMaxBits = 10;
+constexpr int kSortMaxCtas = 16;
+constexpr int kSortKeys    = 2; // keys a lane holds at a time: the code is short, most of it runs once and is waited for
 
 inline size_t sort_smem_words(int warps, int bins)
 {
     return static_cast<size_t>(bins) * warps + bins + 32;
 }
 
-__device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, unsigned *smem)
+__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const EmbeddingGradKParams p)
 {
-    namespace cg               = cooperative_groups;
-    cg::cluster_group cluster  = cg::this_cluster();
-    const unsigned    rank     = cluster.block_rank();
-    const int         lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = p.sortWarps;
+    namespace cg = cooperative_groups;
+    extern __shared__ unsigned smem[];
+    cudaTriggerProgrammaticLaunchCompletion(); // the table may be cleared meanwhile
+    cg::cluster_group cluster = cg::this_cluster();
+    const unsigned    rank = cluster.block_rank(), ctas = cluster.num_blocks();
+    const int         lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = kSortThreads, warps = p.sortWarps;
     const int         bins  = 1 << p.digitBits;
     unsigned         *hist  = smem;                // [warps][bins]
     unsigned         *total = smem + warps * bins; // [bins], read by the other CTAs
     unsigned         *wsum  = total + bins;        // [32]
     unsigned         *mine  = hist + warp * bins;
 
-    constexpr unsigned       kTile   = 32 * kSortKeys;
-    const unsigned long long perWarp = (static_cast<unsigned long long>(p.count) + kSortCtas * warps - 1) / (kSortCtas * warps);
-    const unsigned long long span    = (perWarp + 31) / 32 * 32;
-    const unsigned long long first   = (static_cast<unsigned long long>(rank) * warps + warp) * span;
-    const unsigned           i0      = static_cast<unsigned>(warp < warps && first < p.count ? first : p.count);
-    const unsigned           i1      = static_cast<unsigned>(warp < warps && first + span < p.count ? first + span : p.count);
+    constexpr unsigned kTile = 32 * kSortKeys;
+    const unsigned     i0    = warp < warps ? min(p.count, (rank * warps + warp) * p.span) : p.count, i1 = min(p.count, i0 + p.span);
 
     for (int pass = 0; pass < p.passes; ++pass)
     {
@@ -239,7 +240,7 @@ __device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, un
         if (has)
         {
             unsigned sum = 0;
-#pragma unroll 8
+#pragma unroll 4
             for (int w = 0; w < warps; ++w)
             {
                 const unsigned n = col[w * bins];
@@ -253,13 +254,13 @@ __device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, un
         unsigned before = 0, all = 0;
         if (has)
         {
-            unsigned n[kSortCtas];
+            unsigned n[kSortMaxCtas];
 #pragma unroll
-            for (int c = 0; c < kSortCtas; ++c) n[c] = cluster.map_shared_rank(total, c)[threadIdx.x];
+            for (unsigned c = 0; c < kSortMaxCtas; ++c) n[c] = c < ctas ? cluster.map_shared_rank(total, c)[threadIdx.x] : 0;
 #pragma unroll
-            for (int c = 0; c < kSortCtas; ++c)
+            for (unsigned c = 0; c < kSortMaxCtas; ++c)
             {
-                before += c < static_cast<int>(rank) ? n[c] : 0;
+                before += c < rank ? n[c] : 0;
                 all += n[c];
             }
         }
@@ -288,7 +289,7 @@ __device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, un
         if (has)
         {
             const unsigned base = incl - all + (warp > 0 ? wsum[warp - 1] : 0) + before;
-#pragma unroll 8
+#pragma unroll 4
             for (int w = 0; w < warps; ++w) col[w * bins] += base;
         }
         __syncthreads();
@@ -296,12 +297,24 @@ __device__ __forceinline__ void embedding_sort(const EmbeddingGradKParams &p, un
         {
             if (i1 - i0 > kTile)
                 load(tile); // otherwise the entries are still there
-            // lanes with the same digit find one another; the first of them takes as many places as they are. The barriers of the
-            // warp keep the steps' atomics in order; their results are not waited for until all are under way.
+            // lanes with the same digit find one another bit by bit; the first of them takes as many places as they are. The
+            // barriers of the warp keep the steps' atomics in order; their results are not waited for until all are under way.
             unsigned same[kSortKeys], place[kSortKeys];
 #pragma unroll
+            for (int k = 0; k < kSortKeys; ++k) same[k] = __ballot_sync(0xffffffffu, tile + 32 * k + lane < i1);
+#pragma unroll 1
+            for (int b = shift; b < shift + p.digitBits; ++b)
+#pragma unroll
+                for (int k = 0; k < kSortKeys; ++k)
+                {
+                    const bool     one  = entry[k].x >> b & 1;
+                    const unsigned ones = __ballot_sync(0xffffffffu, one);
+                    same[k] &= one ? ones : ~ones;
+                }
+#pragma unroll
             for (int k = 0; k < kSortKeys; ++k)
-                same[k] = __match_any_sync(0xffffffffu, tile + 32 * k + lane < i1 ? (entry[k].x >> shift) & (bins - 1) : bins);
+                if (tile + 32 * k + lane >= i1)
+                    same[k] = 0xffffffffu; // nobody
 #pragma unroll
             for (int k = 0; k < kSortKeys; ++k)
             {
@@ -331,30 +344,34 @@ __device__ __forceinline__ void embedding_clear_row(const EmbeddingGradKParams &
         store_vecs<W, 1>(d, p.dtableType, static_cast<int>(c), 0, p.cols, z);
 }
 
-// Clears this CTA's share of the table's rows: all of them, or (skipNamed) those no index names, found by going through the indices
-// once with a bit per row -- worth it where the rows that need not be written twice are more bytes than the indices.
+// ---- beside it: clears the table's rows, all of them, or (skipNamed) those no index names, found by going through the indices
+// once with a bit per row -- worth it where the rows that need not be written twice are more bytes than the indices. Launched while
+// the sort runs, on the SMs that leaves.
 constexpr int kZeroRows  = 32768; // rows a CTA has bits for at a time
 constexpr int kScanAhead = 8;     // indices a thread loads at a time
 
-__device__ __forceinline__ void embedding_clear(const EmbeddingGradKParams &p, unsigned *named)
+constexpr int kZeroThreads = 512;
+
+__global__ void __launch_bounds__(kZeroThreads) embedding_clear_kernel(const EmbeddingGradKParams p)
 {
-    const unsigned cta  = blockIdx.x - kSortCtas;
-    const unsigned per  = (static_cast<unsigned>(p.rows) + p.zeroCtas - 1) / p.zeroCtas;
-    const unsigned from = min(static_cast<unsigned>(p.rows), cta * per), to = min(static_cast<unsigned>(p.rows), from + per);
+    __shared__ unsigned named[kZeroRows / 32];
+    cudaTriggerProgrammaticLaunchCompletion();
+    const unsigned per  = (static_cast<unsigned>(p.rows) + gridDim.x - 1) / gridDim.x;
+    const unsigned from = min(static_cast<unsigned>(p.rows), blockIdx.x * per), to = min(static_cast<unsigned>(p.rows), from + per);
     for (unsigned r0 = from; r0 < to; r0 += kZeroRows)
     {
         const unsigned r1 = min(to, r0 + kZeroRows);
         if (p.skipNamed)
         {
-            for (unsigned k = threadIdx.x; k < kZeroRows / 32; k += blockDim.x) named[k] = 0;
+            for (unsigned k = threadIdx.x; k < (r1 - r0 + 31) / 32; k += kZeroThreads) named[k] = 0;
             __syncthreads();
-            for (unsigned long long i0 = threadIdx.x; i0 < p.count; i0 += kScanAhead * blockDim.x)
+            for (unsigned long long i0 = threadIdx.x; i0 < p.count; i0 += kScanAhead * kZeroThreads)
             {
                 int id[kScanAhead]; // all loads before the first is used
 #pragma unroll
                 for (int k = 0; k < kScanAhead; ++k)
                 {
-                    const unsigned long long i = i0 + k * blockDim.x;
+                    const unsigned long long i = i0 + k * kZeroThreads;
                     id[k]                      = i < p.count ? load_index(p.indices, p.indexType, static_cast<unsigned>(i), p.rows) : -1;
                 }
 #pragma unroll
@@ -367,7 +384,7 @@ __device__ __forceinline__ void embedding_clear(const EmbeddingGradKParams &p, u
             }
             __syncthreads();
         }
-        for (unsigned r = r0 + (threadIdx.x >> 5); r < r1; r += blockDim.x >> 5)
+        for (unsigned r = r0 + (threadIdx.x >> 5); r < r1; r += kZeroThreads / 32)
         {
             if (p.skipNamed && (named[(r - r0) / 32] >> ((r - r0) % 32) & 1))
                 continue;
@@ -382,72 +399,67 @@ __device__ __forceinline__ void embedding_clear(const EmbeddingGradKParams &p, u
         }
         __syncthreads();
     }
+    cudaGridDependencySynchronize(); // whoever waits for this kernel waits for the sort
 }
 
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1)
-    embedding_sort_kernel(const EmbeddingGradKParams p)
-{
-    extern __shared__ unsigned smem[];
-    if (blockIdx.x < kSortCtas)
-        embedding_sort(p, smem);
-    else
-        embedding_clear(p, smem);
-}
-
-// ---- second kernel: sums the runs of equal keys among the sorted positions, a warp for kGradCols columns of each job.
+// ---- second kernel: sums the runs of equal keys among the sorted positions, a warp for kGradCols<W> columns of each job.
 //  - Runs of up to kShortRun positions belong to the warp in whose unit of kGradUnit positions they start, wherever they end. It has
 //    the rows of a unit in flight at once; larger units left the GPU with little more than one wave of long-lived warps.
 //  - Longer runs are summed by groups of kShortRun positions into `partials` -- slot 0 for the run that comes from the group before,
 //    slot 1 for the one that starts in the group, a job each -- and joined by the third kernel.
 constexpr int kGradUnit  = 8;
 constexpr int kShortRun  = 32;
-constexpr int kGradCols  = 256; // eight per lane
-template<int GRAD, int W>
-constexpr int kGradAhead = GRAD == B200PP_F32 || W == 1 ? 4 : 8; // rows loaded before the first is added: 32 registers
-
-// Puts a lane's eight sums where they belong: into `partial` or, if that is null, into the table. Not inlined: it would be there
-// once for each of the rows a warp has in flight, and code that runs once is as slow as it can be fetched (7 times slower for
-// few indices).
 template<int W>
-__device__ __noinline__ void embedding_grad_put(const EmbeddingGradKParams &p, float *partial, unsigned key, int c, float s0, float s1,
-                                                float s2, float s3, float s4, float s5, float s6, float s7)
+constexpr int kGradCols = W >= 4 ? 256 : 128; // eight per lane, four where they are narrow vectors
+constexpr int kJoinCols = 256;
+constexpr int kGradAhead = 8; // rows loaded before the first is added
+
+// Puts a lane's sums where they belong: into `partial` or, if that is null, into the table. Not inlined: it would be there once for
+// each of the rows a warp has in flight, and code that runs once is as slow as it can be fetched (32 us instead of 19 for 5003 rows of
+// 333 floats). `N` values as vectors of W, `step` elements apart.
+template<int W, int N>
+__device__ __noinline__ void embedding_grad_put(const EmbeddingGradKParams &p, float *partial, unsigned key, int c, int step, float s0,
+                                                float s1, float s2, float s3, float s4, float s5, float s6, float s7)
 {
-    // vectors of four: 256-bit accesses in a function that is not inlined end this ptxas (12.9) with a segmentation fault
-    constexpr int P = W == 8 ? 4 : W, N = 8 / P, kStep = W == 8 ? 4 : 32 * W;
+    // vectors of four at most: 256-bit accesses in a function that is not inlined end this ptxas (12.9) with a segmentation fault
+    constexpr int P    = W == 8 ? 4 : W, M = N / P;
+    const int     by   = W == 8 ? 4 : step;
     float         v[8] = {s0, s1, s2, s3, s4, s5, s6, s7};
     if (partial)
     {
-        store_vecs<B200PP_F32, P, N>(reinterpret_cast<uint8_t *>(partial), c, kStep, p.cols, v);
+        store_vecs<B200PP_F32, P, M>(reinterpret_cast<uint8_t *>(partial), c, by, p.cols, v);
         return;
     }
     uint8_t *d = p.dtable.at(key);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= p.scale;
+    for (int i = 0; i < N; ++i) v[i] *= p.scale;
     if (p.accumulate)
     {
         float old[8];
-        load_vecs<P, N>(d, p.dtableType, c, kStep, p.cols, old);
+        load_vecs<P, M>(d, p.dtableType, c, by, p.cols, old);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += old[i];
+        for (int i = 0; i < N; ++i) v[i] += old[i];
     }
-    store_vecs<P, N>(d, p.dtableType, c, kStep, p.cols, v);
+    store_vecs<P, M>(d, p.dtableType, c, by, p.cols, v);
 }
 
 template<int GRAD, int W>
-__global__ void __launch_bounds__(256, 3) embedding_grad_runs_kernel(const __grid_constant__ EmbeddingGradKParams p)
+__global__ void __launch_bounds__(256, GRAD == B200PP_F32 && W >= 4 ? 2 : 3) embedding_grad_runs_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
-    constexpr int            V = 8 / W, kAhead = kGradAhead<GRAD, W>;
+    constexpr int            N = kGradCols<W> / 32, V = N / W, kAhead = kGradAhead;
     constexpr unsigned       kAll = 0xffffffffu;
     const int                lane = threadIdx.x & 31;
     const unsigned long long job  = blockIdx.x * 8ull + (threadIdx.x >> 5);
     const unsigned           item = static_cast<unsigned>(job / p.blocks); // the groups' slots, then the units
     if (item >= 2 * p.groups + p.units)
         return;
-    const int      c0    = static_cast<int>(job - static_cast<unsigned long long>(item) * p.blocks) * kGradCols + lane * W;
+    const int      c0    = static_cast<int>(job - static_cast<unsigned long long>(item) * p.blocks) * kGradCols<W> + lane * W;
     const bool     whole = item < 2 * p.groups;
     const unsigned i0    = whole ? item / 2 * kShortRun : (item - 2 * p.groups) * kGradUnit;
     const int      n     = static_cast<int>(min(p.count - i0, static_cast<unsigned>(whole ? kShortRun : kGradUnit)));
     const unsigned none  = static_cast<unsigned>(p.rows);
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     // keys of the 32 positions before (lane l: i0 - 1 - l), of the 32 from i0 on and of the 32 after those
     const unsigned i     = i0 + lane;
     const unsigned bk    = static_cast<unsigned>(lane) < i0 ? p.entries[0][i0 - 1 - lane].x : none;
@@ -532,24 +544,25 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_runs_kernel(const __gri
             }
             if (!((ends >> q) & 1))
                 continue;
-            embedding_grad_put<W>(p, part, __shfl_sync(kAll, q < 32 ? e0.x : e1.x, q & 31), c0, acc[0], acc[1], acc[2], acc[3], acc[4],
-                                  acc[5], acc[6], acc[7]);
+            embedding_grad_put<W, N>(p, part, __shfl_sync(kAll, q < 32 ? e0.x : e1.x, q & 31), c0, 32 * W, acc[0], acc[1], acc[2], acc[3],
+                                     acc[4], acc[5], acc[6], acc[7]);
 #pragma unroll
-            for (int z = 0; z < 8; ++z) acc[z] = 0.0f;
+            for (int z = 0; z < N; ++z) acc[z] = 0.0f;
         }
     }
 }
 
 // ---- third kernel: the runs longer than kShortRun. A CTA looks after eight groups: a warp each finds out whether such a run starts in
-// its group; the CTA then adds up the run's parts for kGradCols columns, each warp a contiguous share of the groups, the warps one
+// its group; the CTA then adds up the run's parts for kJoinCols columns, each warp a contiguous share of the groups, the warps one
 // after another.
 __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
-    __shared__ float    sums[8][kGradCols];
+    __shared__ float    sums[8][kJoinCols];
     __shared__ unsigned keys[8];
     constexpr unsigned  kAll = 0xffffffffu;
     const unsigned      none = static_cast<unsigned>(p.rows);
     const int           lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    cudaGridDependencySynchronize();
     {
         const unsigned u = blockIdx.x * 8 + warp;
         unsigned       k = none;
@@ -583,7 +596,7 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
         }
         // share of this warp: parts from..to of 0 (slot 1 of group u) and 1..more (slot 0 of group u + part)
         const unsigned per = (more + 8) / 8, from = min(more + 1, warp * per), to = min(more + 1, from + per);
-        const int      c0  = blockIdx.y * kGradCols + lane;
+        const int      c0  = blockIdx.y * kJoinCols + lane;
         float          s[8] = {};
 #pragma unroll 2
         for (unsigned m = from; m < to; ++m)
@@ -608,7 +621,7 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
 #pragma unroll
                 for (int w = 0; w < 8; ++w) s[j] += sums[w][lane + 32 * j];
             }
-            embedding_grad_put<1>(p, nullptr, k, c0, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]);
+            embedding_grad_put<1, 8>(p, nullptr, k, c0, 32, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]);
         }
     }
 }

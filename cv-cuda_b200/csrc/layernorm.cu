@@ -75,7 +75,7 @@ bool launch_direct(const LayerNormKParams &p, cudaStream_t stream)
     if (p.chunks)
     {
         layernorm_chunk_stats_kernel<SRC, W><<<p.rows * p.chunks, kChunkThreads, 0, stream>>>(p);
-        layernorm_chunk_apply_kernel<SRC, W><<<p.rows * p.chunks, kChunkThreads, 0, stream>>>(p);
+        Launch(dim3(p.rows * p.chunks), dim3(kChunkThreads), 0, stream, 1, true).run(layernorm_chunk_apply_kernel<SRC, W>, p);
         return true;
     }
     if (p.cols > 256 && p.cols <= 4096 && p.rows <= static_cast<unsigned>(kSms))

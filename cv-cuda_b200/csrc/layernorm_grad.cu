@@ -72,10 +72,8 @@ int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream
     if (smem > 32 * 1024) // a launch gets 48 KB unasked, static memory included
         if (int st = raise_smem(layernorm_grad_kernel<SRC, GRAD, E, W, WARP, FULL>, 208 * 1024, raised))
             return st;
-    ClusterLaunch launch(g.ctas, g.threads, smem, stream);
-    launch.cfg.blockDim.y = g.groups;
-    launch.cfg.gridDim    = dim3(p.parts * g.ctas);
-    cudaLaunchKernelEx(&launch.cfg, layernorm_grad_kernel<SRC, GRAD, E, W, WARP, FULL>, p, g.span);
+    Launch(dim3(p.parts * g.ctas), dim3(g.threads, g.groups), smem, stream, g.ctas, false)
+        .run(layernorm_grad_kernel<SRC, GRAD, E, W, WARP, FULL>, p, g.span);
     return check_launch("LayerNormBackward");
 }
 
@@ -234,6 +232,6 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     // as many threads share a column as there are parts for
     const int  share = p.parts >= 64 ? 32 : p.parts >= 8 ? 8 : 1;
     const dim3 block(share == 1 ? 128 : 32, share);
-    layernorm_grad_join_kernel<<<(2u * p.cols + block.x - 1) / block.x, block, 0, stream>>>(p);
+    Launch(dim3((2u * p.cols + block.x - 1) / block.x), block, 0, stream, 1, true).run(layernorm_grad_join_kernel, p);
     return check_launch("LayerNormBackward");
 }

@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
     __shared__ float2       scratch[2][16]; // two halves, used in turn: one barrier per row
     __shared__ float2       parts[2][8];    // of the CTAs of a cluster
     extern __shared__ uint4 ring[];         // the stages, then the weights; in the end the sums, [groups][2][columns]
+    cudaTriggerProgrammaticLaunchCompletion();
     const int       threads = WARP && FULL ? 32 : blockDim.x, groups = blockDim.y;
     const RowThread k    = row_thread<E, W, FULL>(threadIdx.x, threads, threadIdx.y, groups);
     const int       tid  = k.g * threads + k.t, warp = tid >> 5;
@@ -336,6 +337,7 @@ __global__ void __launch_bounds__(1024) layernorm_grad_join_kernel(const LayerNo
     __shared__ float sum[32][33];
     const long long  c = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, n = 2LL * p.cols; // column of dw, db
     float            s = 0.0f;
+    cudaGridDependencySynchronize(); // launched early
     if (c < n)
     {
 #pragma unroll 4

@@ -268,6 +268,7 @@ constexpr int kChunkThreads = 256;
 template<int SRC, int W>
 __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_stats_kernel(const LayerNormKParams p)
 {
+    cudaTriggerProgrammaticLaunchCompletion();
     constexpr int   E   = kChunk / kChunkThreads;
     const unsigned  r   = blockIdx.x / p.chunks;
     const long long at  = static_cast<long long>(blockIdx.x - r * p.chunks) * kChunk;
@@ -340,7 +341,8 @@ __global__ void __launch_bounds__(kChunkThreads) layernorm_chunk_apply_kernel(co
         if (k.c + v * k.step < end)
             raw[v] = load_raw<kElemBytes<SRC> * W>(x8 + (k.c + v * k.step) * kElemBytes<SRC>);
     }
-    // every warp joins the parts for itself: nothing to wait for
+    cudaGridDependencySynchronize(); // launched early: the values are on their way, the statistics may not be there yet
+    // every warp joins the parts for itself: no barrier
     const int     lane = threadIdx.x & 31;
     const float2 *part = p.partials + static_cast<unsigned long long>(r) * p.chunks;
     const float   tail = static_cast<float>(p.cols - static_cast<long long>(p.chunks - 1) * kChunk); // length of the last chunk

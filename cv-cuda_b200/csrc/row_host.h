@@ -8,9 +8,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>
-#include <map>
-#include <mutex>
-#include <tuple>
 
 namespace b200pp {
 
@@ -186,54 +183,41 @@ int raise_smem(K kernel, int bytes, std::atomic<unsigned long long> &done)
     return B200PP_SUCCESS;
 }
 
-// A launch in clusters of `ctas` CTAs.
-struct ClusterLaunch
+// A launch in clusters of `ctas` CTAs (1: none), and/or -- `early` -- one that may begin while the kernel before it on the stream
+// is still running, as soon as all CTAs of that one have allowed it: the kernel waits for it itself, before it touches what that one
+// writes.
+struct Launch
 {
-    cudaLaunchConfig_t    cfg{};
-    cudaLaunchAttribute   attr{};
+    cudaLaunchConfig_t  cfg{};
+    cudaLaunchAttribute attrs[2]{};
 
-    ClusterLaunch(int ctas, int threads, int smem, cudaStream_t stream)
+    Launch(dim3 grid, dim3 block, int smem, cudaStream_t stream, int ctas, bool early)
     {
-        cfg.blockDim         = dim3(threads);
+        cfg.gridDim          = grid;
+        cfg.blockDim         = block;
         cfg.dynamicSmemBytes = smem;
         cfg.stream           = stream;
-        attr.id              = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim  = {static_cast<unsigned>(ctas), 1, 1};
-        cfg.attrs            = &attr;
-        cfg.numAttrs         = 1;
-        cfg.gridDim          = dim3(ctas);
+        cfg.attrs            = attrs;
+        if (ctas > 1)
+        {
+            cudaLaunchAttribute &a = attrs[cfg.numAttrs++];
+            a.id                   = cudaLaunchAttributeClusterDimension;
+            a.val.clusterDim       = {static_cast<unsigned>(ctas), 1, 1};
+        }
+        if (early)
+        {
+            cudaLaunchAttribute &a                       = attrs[cfg.numAttrs++];
+            a.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+            a.val.programmaticStreamSerializationAllowed = 1;
+        }
     }
 
-    ClusterLaunch(const ClusterLaunch &) = delete;
+    Launch(const Launch &) = delete;
 
-    // As many clusters as are resident at a time, at most one per row. How many that is depends on how the SMs are grouped, so
-    // the runtime is asked, once per shape.
-    template<typename K>
-    void fill(K kernel, unsigned rows)
+    template<typename... P, typename... A>
+    void run(void (*kernel)(P...), A... args) // check_launch reports a failure
     {
-        static std::mutex                            mu;
-        static std::map<std::tuple<const void *, int, unsigned, unsigned, size_t>, int> known;
-        int dev = 0;
-        cudaGetDevice(&dev);
-        const unsigned ctas = attr.val.clusterDim.x;
-        const auto     key  = std::make_tuple(reinterpret_cast<const void *>(kernel), dev, ctas, cfg.blockDim.x, cfg.dynamicSmemBytes);
-        int            most = 0;
-        {
-            std::lock_guard<std::mutex> lock(mu);
-            auto                        it = known.find(key);
-            if (it == known.end())
-            {
-                if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1)
-                {
-                    cudaGetLastError();
-                    most = kSms / static_cast<int>(ctas);
-                }
-                known[key] = most;
-            }
-            else
-                most = it->second;
-        }
-        cfg.gridDim.x = ctas * std::min(rows, static_cast<unsigned>(most));
+        cudaLaunchKernelEx(&cfg, kernel, args...);
     }
 };
 
