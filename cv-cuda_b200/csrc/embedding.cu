@@ -300,10 +300,8 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     {
         VecWidth width(p.cols);
         width.take(p.dtable, row_elem_size(p.dtableType));
-        p.zeroWidth             = width.width;
-        const long long rowSize = static_cast<long long>(p.cols) * row_elem_size(p.dtableType);
-        const int       ctas    = static_cast<int>(std::max(1LL, std::min({2LL * kSms, rows * rowSize / (32 << 10), rows})));
-        p.skipNamed             = std::min(count, rows) * rowSize / ctas > 2 * count * row_elem_size(p.indexType);
+        p.zeroWidth         = width.width;
+        const unsigned ctas = static_cast<unsigned>(std::min<long long>((rows + kZeroThreads / 32 - 1) / (kZeroThreads / 32), kSms * 8));
         Launch(dim3(ctas), dim3(kZeroThreads), 0, stream, 1, count > 0).run(embedding_clear_kernel, p);
         if ((st = check_launch("EmbeddingBackward")))
             return st;

@@ -155,8 +155,8 @@ struct EmbeddingGradKParams
     int       padding;            // -1: none
     uint2    *entries[2];         // (index, position), count each; entries[0] holds the sorted ones
     int       passes, digitBits, sortWarps;
-    unsigned  span;                 // positions of a warp that sorts
-    int       zeroWidth, skipNamed; // vectors that clear the table, whether rows that are named are left out
+    unsigned  span;      // positions of a warp that sorts
+    int       zeroWidth; // of the vectors that clear the table
     float    *partials;                       // [groups][2][cols]
     unsigned  units, groups;                  // of kGradUnit and kShortRun sorted positions
     unsigned  blocks;                         // column blocks of kGradCols<W>
@@ -344,60 +344,23 @@ __device__ __forceinline__ void embedding_clear_row(const EmbeddingGradKParams &
         store_vecs<W, 1>(d, p.dtableType, static_cast<int>(c), 0, p.cols, z);
 }
 
-// ---- beside it: clears the table's rows, all of them, or (skipNamed) those no index names, found by going through the indices
-// once with a bit per row -- worth it where the rows that need not be written twice are more bytes than the indices. Launched while
-// the sort runs, on the SMs that leaves.
-constexpr int kZeroRows  = 32768; // rows a CTA has bits for at a time
-constexpr int kScanAhead = 8;     // indices a thread loads at a time
-
-constexpr int kZeroThreads = 512;
+// ---- beside it: clears the table, launched while the sort runs, on the SMs that leaves. All rows: rows that are written again
+// soon are still in L2 then, and finding out which those are took longer (a bit per row, 65536 indices of 50000: 86 us).
+constexpr int kZeroThreads = 256;
 
 __global__ void __launch_bounds__(kZeroThreads) embedding_clear_kernel(const EmbeddingGradKParams p)
 {
-    __shared__ unsigned named[kZeroRows / 32];
     cudaTriggerProgrammaticLaunchCompletion();
-    const unsigned per  = (static_cast<unsigned>(p.rows) + gridDim.x - 1) / gridDim.x;
-    const unsigned from = min(static_cast<unsigned>(p.rows), blockIdx.x * per), to = min(static_cast<unsigned>(p.rows), from + per);
-    for (unsigned r0 = from; r0 < to; r0 += kZeroRows)
+    for (unsigned r = blockIdx.x * (kZeroThreads / 32) + (threadIdx.x >> 5); r < static_cast<unsigned>(p.rows); r += gridDim.x * (kZeroThreads / 32))
     {
-        const unsigned r1 = min(to, r0 + kZeroRows);
-        if (p.skipNamed)
-        {
-            for (unsigned k = threadIdx.x; k < (r1 - r0 + 31) / 32; k += kZeroThreads) named[k] = 0;
-            __syncthreads();
-            for (unsigned long long i0 = threadIdx.x; i0 < p.count; i0 += kScanAhead * kZeroThreads)
-            {
-                int id[kScanAhead]; // all loads before the first is used
-#pragma unroll
-                for (int k = 0; k < kScanAhead; ++k)
-                {
-                    const unsigned long long i = i0 + k * kZeroThreads;
-                    id[k]                      = i < p.count ? load_index(p.indices, p.indexType, static_cast<unsigned>(i), p.rows) : -1;
-                }
-#pragma unroll
-                for (int k = 0; k < kScanAhead; ++k)
-                {
-                    const unsigned d = static_cast<unsigned>(id[k]) - r0; // -1: far above
-                    if (d < r1 - r0 && id[k] != p.padding)
-                        atomicOr(named + d / 32, 1u << (d % 32));
-                }
-            }
-            __syncthreads();
-        }
-        for (unsigned r = r0 + (threadIdx.x >> 5); r < r1; r += kZeroThreads / 32)
-        {
-            if (p.skipNamed && (named[(r - r0) / 32] >> ((r - r0) % 32) & 1))
-                continue;
-            if (p.zeroWidth == 8)
-                embedding_clear_row<8>(p, r);
-            else if (p.zeroWidth == 4)
-                embedding_clear_row<4>(p, r);
-            else if (p.zeroWidth == 2)
-                embedding_clear_row<2>(p, r);
-            else
-                embedding_clear_row<1>(p, r);
-        }
-        __syncthreads();
+        if (p.zeroWidth == 8)
+            embedding_clear_row<8>(p, r);
+        else if (p.zeroWidth == 4)
+            embedding_clear_row<4>(p, r);
+        else if (p.zeroWidth == 2)
+            embedding_clear_row<2>(p, r);
+        else
+            embedding_clear_row<1>(p, r);
     }
     cudaGridDependencySynchronize(); // whoever waits for this kernel waits for the sort
 }
@@ -411,7 +374,6 @@ constexpr int kGradUnit  = 8;
 constexpr int kShortRun  = 32;
 template<int W>
 constexpr int kGradCols = W >= 4 ? 256 : 128; // eight per lane, four where they are narrow vectors
-constexpr int kJoinCols = 256;
 constexpr int kGradAhead = 8; // rows loaded before the first is added
 
 // Puts a lane's sums where they belong: into `partial` or, if that is null, into the table. Not inlined: it would be there once for
@@ -513,20 +475,18 @@ __global__ void __launch_bounds__(256, GRAD == B200PP_F32 && W >= 4 ? 2 : 3) emb
     float        acc[8] = {};
     for (int j = from; j < to; j += kAhead)
     {
+        // nothing conditional about the loads, so that they all go out together: past the last row it is loaded again, past the
+        // last column the last vector is
         Vec<GRAD, W> raw[kAhead][V];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
         {
-            const unsigned o0 = __shfl_sync(kAll, e0.y, (j + a) & 31), o1 = __shfl_sync(kAll, e1.y, (j + a) & 31);
-            const uint8_t *row = p.grad.at(j + a < 32 ? o0 : o1);
+            const int      at = min(j + a, to - 1);
+            const unsigned o0 = __shfl_sync(kAll, e0.y, at & 31), o1 = __shfl_sync(kAll, e1.y, at & 31);
+            const uint8_t *row = p.grad.at(at < 32 ? o0 : o1);
 #pragma unroll
             for (int v = 0; v < V; ++v)
-            {
-                const int c = c0 + v * 32 * W;
-                raw[a][v]   = zero_raw<kElemBytes<GRAD> * W>();
-                if (j + a < to && c < p.cols)
-                    raw[a][v] = load_raw<kElemBytes<GRAD> * W>(row + static_cast<long long>(c) * kElemBytes<GRAD>);
-            }
+                raw[a][v] = load_raw<kElemBytes<GRAD> * W>(row + static_cast<long long>(min(c0 + v * 32 * W, p.cols - W)) * kElemBytes<GRAD>);
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
@@ -552,20 +512,35 @@ __global__ void __launch_bounds__(256, GRAD == B200PP_F32 && W >= 4 ? 2 : 3) emb
     }
 }
 
-// ---- third kernel: the runs longer than kShortRun. A CTA looks after eight groups: a warp each finds out whether such a run starts in
-// its group; the CTA then adds up the run's parts for kJoinCols columns, each warp a contiguous share of the groups, the warps one
-// after another.
+// ---- third kernel: the runs longer than kShortRun. A CTA looks after eight groups, a warp each: it finds out whether such a run
+// starts in its group and adds up the run's parts for kJoinCols columns. Runs of more than kJoinAlone groups are left to the whole CTA,
+// each warp a contiguous share of the groups, the warps one after another.
+constexpr int      kJoinCols  = 256;
+constexpr unsigned kJoinAlone = 16;
+
+// Adds the parts from..to of the run that starts in group u: 0 is slot 1 of that group, k slot 0 of group u + k.
+__device__ __forceinline__ void embedding_add_parts(const EmbeddingGradKParams &p, unsigned u, unsigned from, unsigned to, int c0, float (&s)[8])
+{
+#pragma unroll 2
+    for (unsigned m = from; m < to; ++m)
+    {
+        const float *part = p.partials + (static_cast<unsigned long long>(u + m) * 2 + (m == 0 ? 1 : 0)) * p.cols;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += part[min(c0 + 32 * j, p.cols - 1)];
+    }
+}
+
 __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_constant__ EmbeddingGradKParams p)
 {
     __shared__ float    sums[8][kJoinCols];
-    __shared__ unsigned keys[8];
+    __shared__ unsigned keys[8], parts[8]; // of the runs left to the whole CTA
     constexpr unsigned  kAll = 0xffffffffu;
     const unsigned      none = static_cast<unsigned>(p.rows);
-    const int           lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int           lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.y * kJoinCols + lane;
     cudaGridDependencySynchronize();
     {
         const unsigned u = blockIdx.x * 8 + warp;
-        unsigned       k = none;
+        unsigned       k = none, more = 0; // the run's key, the groups it goes on in
         if (u + 1 < p.groups) // not the last group, so it is full
         {
             const unsigned first = u * kShortRun;
@@ -576,17 +551,7 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
                 && p.entries[0][start + kShortRun].x == last)
                 k = last;
         }
-        if (lane == 0)
-            keys[warp] = k;
-    }
-    __syncthreads();
-    for (int l = 0; l < 8; ++l)
-    {
-        const unsigned u = blockIdx.x * 8 + l, k = keys[l];
-        if (k == none)
-            continue;
-        unsigned more = 0; // groups the run goes on in
-        for (;;)
+        while (k != none)
         {
             const unsigned long long at = (static_cast<unsigned long long>(u) + 1 + more + lane) * kShortRun;
             const unsigned           on = __ballot_sync(kAll, at < p.count && p.entries[0][at].x == k);
@@ -594,19 +559,25 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
             if (on != kAll)
                 break;
         }
-        // share of this warp: parts from..to of 0 (slot 1 of group u) and 1..more (slot 0 of group u + part)
-        const unsigned per = (more + 8) / 8, from = min(more + 1, warp * per), to = min(more + 1, from + per);
-        const int      c0  = blockIdx.y * kJoinCols + lane;
-        float          s[8] = {};
-#pragma unroll 2
-        for (unsigned m = from; m < to; ++m)
+        if (k != none && more <= kJoinAlone)
         {
-            const float *part = p.partials + (static_cast<unsigned long long>(u + m) * 2 + (m == 0 ? 1 : 0)) * p.cols;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + 32 * j < p.cols)
-                    s[j] += part[c0 + 32 * j];
+            float s[8] = {};
+            embedding_add_parts(p, u, 0, more + 1, c0, s);
+            embedding_grad_put<1, 8>(p, nullptr, k, c0, 32, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]);
+            k = none;
         }
+        if (lane == 0)
+            keys[warp] = k, parts[warp] = more + 1;
+    }
+    __syncthreads();
+    for (int l = 0; l < 8; ++l)
+    {
+        const unsigned k = keys[l];
+        if (k == none)
+            continue;
+        const unsigned per = (parts[l] + 7) / 8, from = min(parts[l], warp * per), to = min(parts[l], from + per);
+        float          s[8] = {};
+        embedding_add_parts(p, blockIdx.x * 8 + l, from, to, c0, s);
         __syncthreads(); // the sums of the run before are taken
 #pragma unroll
         for (int j = 0; j < 8; ++j) sums[warp][lane + 32 * j] = s[j];
