@@ -27,8 +27,8 @@ void launch_short_rows(const EmbeddingKParams &p, cudaStream_t stream)
     const unsigned tiles = (p.count + 256u * R - 1) / (256u * R);
     const int      lines = 8 * 32 * C * static_cast<int>(sizeof(uint4));
     // the copy to shared memory pays from the second index per table row on
-    if (static_cast<long long>(p.rows) * C <= kShortTable && p.count >= 2u * p.rows)
-        embedding_short_rows_kernel<C, R, true><<<std::min(tiles, kSms * 8u), 256, lines + p.rows * C * static_cast<int>(sizeof(float)),
+    if (static_cast<long long>(p.rows) * short_stride(C) <= kShortTable && p.count >= 2u * p.rows)
+        embedding_short_rows_kernel<C, R, true><<<std::min(tiles, kSms * 8u), 256, lines + p.rows * short_stride(C) * static_cast<int>(sizeof(float)),
                                                   stream>>>(p);
     else
         embedding_short_rows_kernel<C, R, false><<<tiles, 256, lines, stream>>>(p);
@@ -43,26 +43,39 @@ void launch_short_rows(const EmbeddingKParams &p, cudaStream_t stream)
         launch_short_rows<C, 8>(p, stream);
 }
 
+template<int TABLE, int W, int U>
+int launch_embedding(EmbeddingKParams &p, int lanes, cudaStream_t stream)
+{
+    constexpr int R = kLookupVectors<W> / U;
+    p.blocks        = static_cast<unsigned>((static_cast<long long>(p.cols) + lanes * W * U - 1) / (lanes * W * U));
+    const dim3               block(lanes, 256 / lanes);
+    const unsigned long long ctas = (static_cast<unsigned long long>(p.count) + R * block.y - 1) / (R * block.y) * p.blocks;
+    if (ctas > 0x7fffffffull)
+        return fail(B200PP_ERROR_OVERFLOW, "Output is too large");
+    if (p.dstType == TABLE)
+        embedding_kernel<TABLE, TABLE, W, U><<<static_cast<unsigned>(ctas), block, 0, stream>>>(p);
+    else
+        embedding_kernel<TABLE, -1, W, U><<<static_cast<unsigned>(ctas), block, 0, stream>>>(p);
+    return check_launch("Embedding");
+}
+
 template<int TABLE, int W>
 int launch_embedding(EmbeddingKParams &p, cudaStream_t stream)
 {
-    // lanes per row: a warp, fewer for rows that would leave half of it idle; up to four vectors per lane
+    // lanes per row: a warp, fewer for rows that would leave half of it idle; as many vectors per lane as the row has
     int lanes = 32;
     while (lanes > 1 && (lanes / 2) * W >= p.cols) lanes /= 2;
-    const int u = p.cols <= lanes * W ? 1 : p.cols <= lanes * W * 2 ? 2 : 4;
-    p.blocks    = (p.cols + lanes * W * u - 1) / (lanes * W * u);
-    const dim3               block(lanes, 256 / lanes);
-    const unsigned long long jobs = static_cast<unsigned long long>(p.count) * p.blocks, ctas = (jobs + block.y - 1) / block.y;
-    if (ctas > 0x7fffffffull)
-        return fail(B200PP_ERROR_OVERFLOW, "Output is too large");
-    const unsigned grid = static_cast<unsigned>(ctas);
-    if (u == 1)
-        embedding_kernel<TABLE, W, 1><<<grid, block, 0, stream>>>(p);
-    else if (u == 2)
-        embedding_kernel<TABLE, W, 2><<<grid, block, 0, stream>>>(p);
-    else
-        embedding_kernel<TABLE, W, 4><<<grid, block, 0, stream>>>(p);
-    return check_launch("Embedding");
+    const int vectors = (p.cols + lanes * W - 1) / (lanes * W);
+    // so few rows that the GPU is not full: one vector per lane, and as many lanes as there are
+    if (vectors == 1 || static_cast<long long>(p.count) * vectors <= kSms * 8)
+        return launch_embedding<TABLE, W, 1>(p, lanes, stream);
+    if (vectors == 2)
+        return launch_embedding<TABLE, W, 2>(p, lanes, stream);
+    if (kLookupVectors<W> == 4 || vectors <= 4)
+        return launch_embedding<TABLE, W, 4>(p, lanes, stream);
+    if constexpr (kLookupVectors<W> == 8)
+        return launch_embedding<TABLE, W, 8>(p, lanes, stream);
+    return B200PP_SUCCESS; // not reached
 }
 
 template<int TABLE>

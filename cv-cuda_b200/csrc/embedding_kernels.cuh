@@ -24,35 +24,60 @@ struct EmbeddingKParams
     unsigned blocks; // of a row
 };
 
-// blockDim.x lanes of a warp per row, blockDim.y rows per CTA; a lane moves up to U vectors of W neighbouring elements, one
-// block of blockDim.x * U vectors of the row at a time. All loads of a block are issued before the first is used.
-template<int TABLE, int W, int U>
+// `blockDim.x` lanes of a warp per row, R rows for each; a lane moves U vectors of W neighbouring elements of each, one block of
+// blockDim.x * U vectors of the row. All loads go out before the first is used, and none is conditional: past the row's end its last
+// vector is loaded again, for an index outside the table the first row. What bounds the kernel is how many bytes it has under way
+// and, for short rows, how many instructions a row takes (3.3 million rows of nine: 155 us with each lane of a row reading the
+// index), so a warp reads 32 indices at a time and hands them out. DST: the output's type, -1 for any.
+template<int W>
+constexpr int kLookupVectors = W == 8 ? 4 : 8; // U * R
+
+template<int TABLE, int DST, int W, int U>
 __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingKParams p)
 {
-    const unsigned long long job = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    const unsigned           r   = static_cast<unsigned>(p.blocks == 1 ? job : job / p.blocks);
-    if (job >= static_cast<unsigned long long>(p.count) * p.blocks)
-        return;
-    const int      span = blockDim.x * W;
-    const int      c0   = static_cast<int>(job - static_cast<unsigned long long>(r) * p.blocks) * (span * U) + threadIdx.x * W;
-    const int      id   = load_index(p.indices, p.indexType, r, p.rows);
-    uint8_t       *y    = p.dst.at(r);
-    const uint8_t *t    = p.table.at(max(id, 0));
-    Vec<TABLE, W>  raw[U];
+    constexpr int  R    = kLookupVectors<W> / U;
+    const unsigned tile = blockIdx.x / p.blocks;
+    const int      span = blockDim.x * W, tid = threadIdx.y * blockDim.x + threadIdx.x;
+    const int      c0   = static_cast<int>(blockIdx.x - tile * p.blocks) * (span * U) + threadIdx.x * W;
+    const int      rowsAtATime = 32 / blockDim.x, g = (tid & 31) / blockDim.x; // of the warp
+    // below 2^31 + 256 * 8
+    const unsigned base = (tile * 8 + (tid >> 5)) * (R * rowsAtATime);
+    int            id[R], mine = -1;
+    Vec<TABLE, W>  raw[R][U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int k = 0; k < R; ++k)
     {
-        const int c = c0 + u * span;
-        raw[u]      = zero_raw<kElemBytes<TABLE> * W>();
-        if (id >= 0 && c < p.cols)
-            raw[u] = load_raw<kElemBytes<TABLE> * W>(t + static_cast<long long>(c) * kElemBytes<TABLE>);
+        if ((k * rowsAtATime & 31) == 0)
+            mine = load_index(p.indices, p.indexType, min(base + k * rowsAtATime + (tid & 31), p.count - 1), p.rows);
+        id[k] = __shfl_sync(0xffffffffu, mine, (k * rowsAtATime & 31) + g);
     }
-    float v[U * W];
+    if (p.rows > 0)
+    {
 #pragma unroll
-    for (int u = 0; u < U; ++u) unpack<TABLE, W>(raw[u], v + u * W);
+        for (int k = 0; k < R; ++k)
+        {
+            const uint8_t *t = p.table.at(max(id[k], 0));
 #pragma unroll
-    for (int i = 0; i < U * W; ++i) v[i] = id < 0 ? 0.0f : v[i] * p.scale;
-    store_vecs<W, U>(y, p.dstType, c0, span, p.cols, v);
+            for (int u = 0; u < U; ++u)
+                raw[k][u] = load_raw<kElemBytes<TABLE> * W>(t + static_cast<long long>(min(c0 + u * span, p.cols - W)) * kElemBytes<TABLE>);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+    {
+        const unsigned r = base + k * rowsAtATime + g;
+        if (r >= p.count)
+            return;
+        float v[U * W];
+#pragma unroll
+        for (int u = 0; u < U; ++u) unpack<TABLE, W>(raw[k][u], v + u * W);
+#pragma unroll
+        for (int i = 0; i < U * W; ++i) v[i] = id[k] < 0 ? 0.0f : v[i] * p.scale;
+        if constexpr (DST < 0)
+            store_vecs<W, U>(p.dst.at(r), p.dstType, c0, span, p.cols, v);
+        else
+            store_vecs<DST, W, U>(p.dst.at(r), c0, span, p.cols, v);
+    }
 }
 
 // Rows of C elements (a palette's colours) that follow one another without gaps. A thread makes R rows, R * C elements of 16 * C
@@ -61,6 +86,12 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingKParams p
 // warp's addresses touch (114 us for 16.6 million indices and a palette of 256 x 3 floats), from shared memory one for each clash of
 // banks.
 constexpr int kShortTable = 4096; // floats of a table that is copied to shared memory
+
+// Distance of its rows: odd, so that they start in all banks.
+inline __host__ __device__ constexpr int short_stride(int c)
+{
+    return c | 1;
+}
 
 template<int IT, int R>
 __device__ __forceinline__ void load_short_indices(const EmbeddingKParams &p, unsigned r0, int *id)
@@ -82,13 +113,14 @@ template<int C, int R, bool SHARED>
 __global__ void __launch_bounds__(256) embedding_short_rows_kernel(const EmbeddingKParams p)
 {
     extern __shared__ uint4  short_smem[]; // [8 warps][32 * C], then the table
+    constexpr int            S     = short_stride(C);
     float                   *table = reinterpret_cast<float *>(short_smem + 8 * 32 * C);
     const int                lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint4                   *mine = short_smem + warp * (32 * C);
     if constexpr (SHARED)
     {
         for (int i = threadIdx.x; i < p.rows * C; i += 256)
-            table[i] = load_elem(p.table.at(i / C), i % C, p.tableType) * p.scale;
+            table[i / C * S + i % C] = load_elem(p.table.at(i / C), i % C, p.tableType) * p.scale;
         __syncthreads();
     }
     constexpr unsigned kWarpRows = 32 * R;
@@ -113,7 +145,7 @@ __global__ void __launch_bounds__(256) embedding_short_rows_kernel(const Embeddi
             {
                 v[k * C + c] = 0.0f;
                 if (id[k] >= 0)
-                    v[k * C + c] = SHARED ? table[id[k] * C + c] : load_elem(row, c, p.tableType) * p.scale;
+                    v[k * C + c] = SHARED ? table[id[k] * S + c] : load_elem(row, c, p.tableType) * p.scale;
             }
         }
         __syncwarp(); // the lines of the turn before are stored
