@@ -24,12 +24,12 @@ namespace {
 template<int C, int R>
 void launch_short_rows(const EmbeddingKParams &p, cudaStream_t stream)
 {
-    const unsigned tiles = (p.count + 256u * R - 1) / (256u * R);
-    const int      lines = 8 * 32 * C * static_cast<int>(sizeof(uint4));
+    const unsigned  tiles = (p.count + 256u * R - 1) / (256u * R);
+    const int       lines = 8 * 32 * C * static_cast<int>(sizeof(uint4));
+    const long long table = (static_cast<long long>(p.rows) + 1) * kShortStride<C, R> * (16 / R);
     // the copy to shared memory pays from the second index per table row on
-    if (static_cast<long long>(p.rows) * short_stride(C) <= kShortTable && p.count >= 2u * p.rows)
-        embedding_short_rows_kernel<C, R, true><<<std::min(tiles, kSms * 8u), 256, lines + p.rows * short_stride(C) * static_cast<int>(sizeof(float)),
-                                                  stream>>>(p);
+    if (table <= kShortTable && p.count >= 2u * p.rows)
+        embedding_short_rows_kernel<C, R, true><<<std::min(tiles, kSms * 8u), 256, lines + static_cast<int>(table), stream>>>(p);
     else
         embedding_short_rows_kernel<C, R, false><<<tiles, 256, lines, stream>>>(p);
 }
@@ -71,11 +71,14 @@ int launch_embedding(EmbeddingKParams &p, cudaStream_t stream)
         return launch_embedding<TABLE, W, 1>(p, lanes, stream);
     if (vectors == 2)
         return launch_embedding<TABLE, W, 2>(p, lanes, stream);
-    if (kLookupVectors<W> == 4 || vectors <= 4)
-        return launch_embedding<TABLE, W, 4>(p, lanes, stream);
     if constexpr (kLookupVectors<W> == 8)
-        return launch_embedding<TABLE, W, 8>(p, lanes, stream);
-    return B200PP_SUCCESS; // not reached
+    {
+        // the vectors of a lane's share of the row, rounded up to 4, 6 or 8
+        const int each = (vectors + (vectors + 7) / 8 - 1) / ((vectors + 7) / 8);
+        if (each > 4)
+            return each > 6 ? launch_embedding<TABLE, W, 8>(p, lanes, stream) : launch_embedding<TABLE, W, 6>(p, lanes, stream);
+    }
+    return launch_embedding<TABLE, W, 4>(p, lanes, stream);
 }
 
 template<int TABLE>

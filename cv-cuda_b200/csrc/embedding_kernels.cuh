@@ -82,29 +82,40 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingKParams p
 
 // Rows of C elements (a palette's colours) that follow one another without gaps. A thread makes R rows, R * C elements of 16 * C
 // bytes in all (R = 8 for 16-bit elements, 4 for 32-bit ones), and the warp stores its 512 * C bytes from shared memory as whole
-// lines. SHARED: the table, times the scale, is copied to shared memory first: gathers from L1 take a cycle for each 128-byte line a
-// warp's addresses touch (114 us for 16.6 million indices and a palette of 256 x 3 floats), from shared memory one for each clash of
-// banks.
-constexpr int kShortTable = 4096; // floats of a table that is copied to shared memory
+// lines. SHARED: the table's rows, times the scale and rounded to the output's type, are copied to shared memory first, with a row of
+// zeros for indices outside the table. Gathers bound this kernel: from L1 a warp's 32 addresses take a cycle for each 128-byte line
+// they touch (114 us for 16.6 million indices and a palette of 256 x 3 floats), from shared memory one for each clash of banks, which
+// 16-bit rows read whole (8 bytes for three) have half as many of as three floats read one by one (37 us).
+constexpr int kShortTable = 16384; // bytes of a table that is copied to shared memory
 
-// Distance of its rows: odd, so that they start in all banks.
-inline __host__ __device__ constexpr int short_stride(int c)
-{
-    return c | 1;
-}
+// Elements a row takes there: 16-bit rows a power of two, float32 rows an odd number, so that they start in all banks.
+template<int C, int R>
+constexpr int kShortStride = R == 4 ? C | 1 : C <= 2 ? C : C <= 4 ? 4 : 8;
 
 template<int IT, int R>
-__device__ __forceinline__ void load_short_indices(const EmbeddingKParams &p, unsigned r0, int *id)
+__device__ __forceinline__ void load_short_indices(const EmbeddingKParams &p, unsigned r0, int none, int *id)
 {
     typedef typename Index<IT>::type T;
+    if (IT == B200PP_U8 && R == 8 && p.indices.n2 == 0 && p.indices.s2 == 1 && (reinterpret_cast<uintptr_t>(p.indices.base) & 7) == 0
+        && r0 + 8 <= p.count) // r0 is a multiple of eight
+    {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p.indices.base + r0);
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+        {
+            id[k] = static_cast<int>((k < 4 ? v.x : v.y) >> (k % 4 * 8) & 0xffu);
+            id[k] = id[k] < p.rows ? id[k] : none;
+        }
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < R; ++k)
     {
-        id[k] = -1;
+        id[k] = none;
         if (r0 + k < p.count)
         {
             const long long v = *reinterpret_cast<const T *>(p.indices.at(r0 + k));
-            id[k]             = v >= 0 && v < p.rows ? static_cast<int>(v) : -1;
+            id[k]             = v >= 0 && v < p.rows ? static_cast<int>(v) : none;
         }
     }
 }
@@ -112,15 +123,16 @@ __device__ __forceinline__ void load_short_indices(const EmbeddingKParams &p, un
 template<int C, int R, bool SHARED>
 __global__ void __launch_bounds__(256) embedding_short_rows_kernel(const EmbeddingKParams p)
 {
+    constexpr int            S = kShortStride<C, R>;
     extern __shared__ uint4  short_smem[]; // [8 warps][32 * C], then the table
-    constexpr int            S     = short_stride(C);
-    float                   *table = reinterpret_cast<float *>(short_smem + 8 * 32 * C);
+    uint8_t                 *table = reinterpret_cast<uint8_t *>(short_smem + 8 * 32 * C);
     const int                lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint4                   *mine = short_smem + warp * (32 * C);
     if constexpr (SHARED)
     {
-        for (int i = threadIdx.x; i < p.rows * C; i += 256)
-            table[i / C * S + i % C] = load_elem(p.table.at(i / C), i % C, p.tableType) * p.scale;
+        for (int i = threadIdx.x; i < (p.rows + 1) * C; i += 256)
+            store_elem_as(table, i / C * S + i % C, p.dstType,
+                          i / C < p.rows ? load_elem(p.table.at(i / C), i % C, p.tableType) * p.scale : 0.0f);
         __syncthreads();
     }
     constexpr unsigned kWarpRows = 32 * R;
@@ -128,37 +140,70 @@ __global__ void __launch_bounds__(256) embedding_short_rows_kernel(const Embeddi
          w0 += static_cast<unsigned long long>(gridDim.x) * 8 * kWarpRows)
     {
         const unsigned r0 = static_cast<unsigned>(w0) + lane * R;
+        const int      none = SHARED ? p.rows : -1;
         int            id[R];
         if (p.indexType == B200PP_U8)
-            load_short_indices<B200PP_U8, R>(p, r0, id);
+            load_short_indices<B200PP_U8, R>(p, r0, none, id);
         else if (p.indexType == B200PP_S32)
-            load_short_indices<B200PP_S32, R>(p, r0, id);
+            load_short_indices<B200PP_S32, R>(p, r0, none, id);
         else
-            load_short_indices<B200PP_S64, R>(p, r0, id);
-        float v[R * C];
-#pragma unroll
-        for (int k = 0; k < R; ++k)
+            load_short_indices<B200PP_S64, R>(p, r0, none, id);
+        uint4 line[C]; // the thread's 16 * C bytes
+        if constexpr (SHARED && R == 8)
         {
-            const uint8_t *row = SHARED ? nullptr : p.table.at(max(id[k], 0));
+            unsigned short h[8 * C];
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int k = 0; k < 8; ++k)
             {
-                v[k * C + c] = 0.0f;
-                if (id[k] >= 0)
-                    v[k * C + c] = SHARED ? table[id[k] * S + c] : load_elem(row, c, p.tableType) * p.scale;
+                const RawVec<2 * S> e = load_raw<2 * S>(table + id[k] * (2 * S));
+#pragma unroll
+                for (int c = 0; c < C; ++c) h[k * C + c] = static_cast<unsigned short>(S == 1 ? e.w[0] : e.w[c / 2] >> (c % 2 * 16));
+            }
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                line[i] = make_uint4(h[8 * i] | h[8 * i + 1] << 16, h[8 * i + 2] | h[8 * i + 3] << 16, h[8 * i + 4] | h[8 * i + 5] << 16,
+                                     h[8 * i + 6] | h[8 * i + 7] << 16);
+        }
+        else
+        {
+            float v[R * C];
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+            {
+                const uint8_t *row = SHARED ? nullptr : p.table.at(max(id[k], 0));
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                {
+                    if constexpr (SHARED)
+                        v[k * C + c] = reinterpret_cast<const float *>(table)[id[k] * S + c];
+                    else
+                    {
+                        v[k * C + c] = 0.0f;
+                        if (id[k] >= 0)
+                            v[k * C + c] = load_elem(row, c, p.tableType) * p.scale;
+                    }
+                }
+            }
+            if constexpr (R == 4)
+            {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                    line[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                         __float_as_uint(v[4 * i + 3]));
+            }
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                {
+                    const RawVec<16> r = p.dstType == B200PP_BF16 ? pack<B200PP_BF16, 8>(v + 8 * i) : pack<B200PP_F16, 8>(v + 8 * i);
+                    line[i]            = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+                }
             }
         }
         __syncwarp(); // the lines of the turn before are stored
-        uint8_t *to = reinterpret_cast<uint8_t *>(mine + lane * C);
-        if constexpr (R == 4)
-        {
 #pragma unroll
-            for (int i = 0; i < C; ++i)
-                mine[lane * C + i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
-                                                __float_as_uint(v[4 * i + 3]));
-        }
-        else
-            store_vecs<8, C>(to, p.dstType, 0, 8, 8 * C, v);
+        for (int i = 0; i < C; ++i) mine[lane * C + i] = line[i];
         __syncwarp();
         constexpr int kElem = 16 / R; // bytes: 2 or 4
         uint8_t      *y     = p.dst.base + w0 * (C * kElem);

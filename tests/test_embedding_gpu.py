@@ -57,7 +57,8 @@ COLS = [1, 2, 3, 4, 5, 7, 8, 9, 16, 31, 32, 33, 64, 100, 255, 256, 257, 333, 512
 
 
 @pytest.mark.parametrize("cols", COLS)
-@pytest.mark.parametrize("table,dst,ids", [("f32", "f32", "i32"), ("bf16", "bf16", "i64"), ("f16", "f32", "u8"), ("f32", "f16", "i64")])
+@pytest.mark.parametrize("table,dst,ids", [("f32", "f32", "i32"), ("bf16", "bf16", "i64"), ("f16", "f32", "u8"), ("f32", "f16", "i64"),
+                                           ("bf16", "bf16", "u8")])
 def test_lookup(pkg, cols, table, dst, ids):
     t = values((211, cols), KINDS[table], cols)
     for shape in ((1,), (7,), (3, 130), (2049,)):
@@ -111,6 +112,18 @@ def test_lookup_strides(pkg, cols):
     assert bool((guard[..., :1] == 77.0).all()) and bool((guard[..., 1 + cols:] == 77.0).all())
     # a table of one row for all indices, as a broadcast view
     assert torch.equal(pkg.embedding(i, t[:1].expand(30, cols)), lookup(i * 0, t, 1.0, torch.float16))
+
+
+@pytest.mark.parametrize("cols", range(1, 9))
+@pytest.mark.parametrize("ids", list(IDS))
+@pytest.mark.parametrize("dst", list(KINDS))
+def test_short_rows(pkg, cols, ids, dst):
+    """Tables that fit on the SM and those that do not, indices inside and outside, packed and strided, whole and ragged ends."""
+    for rows, count in ((1, 40), (7, 2048 * 3), (255, 5000), (256, 300), (2000, 9001), (9000, 100)):
+        t = values((rows, cols + 1), torch.float32, cols)[:, 1:]
+        i = indices((count + 8,), 0 if ids == "u8" else -3, min(rows + 9, 256) if ids == "u8" else rows + 9, IDS[ids], rows)
+        for view in (i[:count], i[8:], i[3:3 + count], i[::2]):
+            assert torch.equal(pkg.embedding(view, t, 0.3, data_type=KINDS[dst]), lookup(view, t, 0.3, KINDS[dst])), (rows, count)
 
 
 def test_palette_of_a_label_map(pkg):
