@@ -617,13 +617,21 @@ __device__ __forceinline__ void store_pairs(uint8_t *row, int c, int step, int e
         }
         return;
     }
+    uint8_t *at = row + c * kElemBytes<DT>;
 #pragma unroll
     for (int v = 0; v < E / 2; ++v)
     {
-        if (c + v * step < end)
-            store_elem_as<DT>(row, c + v * step, f[2 * v]);
-        if (c + v * step + 1 < end)
-            store_elem_as<DT>(row, c + v * step + 1, f[2 * v + 1]);
+        // past the end for every thread of the row, or for none, but for one vector
+        if (c + v * step >= end)
+            break;
+        if (whole && c + v * step + 1 < end)
+            store_vec<DT, 2>(at, v * step, f + 2 * v);
+        else
+        {
+            store_elem_as<DT>(at, v * step, f[2 * v]);
+            if (c + v * step + 1 < end)
+                store_elem_as<DT>(at, v * step + 1, f[2 * v + 1]);
+        }
     }
 }
 
