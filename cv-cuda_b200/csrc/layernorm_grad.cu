@@ -1,20 +1,11 @@
 // Host side of LayerNorm's gradient: argument validation, kernel selection and launch.
-#include "layernorm_grad_kernels.cuh"
-#include "row_host.h"
+#include "layernorm_grad_launch.cuh"
 
 #include <algorithm>
 
 using namespace b200pp;
 
 namespace {
-
-// How the rows are dealt out. One-pass kernel: `threads` per row and CTA with `values` values each, `groups` rows per CTA, a cluster of
-// `ctas` CTAs with `span` columns each per row, one part per CTA or cluster; for longer rows (values = 0) the sums over the rows
-// are a kernel of their own.
-struct GradPlan
-{
-    int threads, groups, values, ctas, span, parts;
-};
 
 GradPlan plan_layernorm_grad(long long rows, long long cols, int elem)
 {
@@ -59,71 +50,21 @@ size_t grad_workspace(const GradPlan &g, long long cols)
     return static_cast<size_t>(g.parts) * 2 * cols * sizeof(float);
 }
 
-template<int SRC, int GRAD, int E, int W, bool WARP, bool FULL>
-int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
-{
-    typedef GradRing<SRC, GRAD, E, W>      Ring;
-    static std::atomic<unsigned long long> raised{0};
-    const int                              warps = g.threads * g.groups / 32, slots = WARP ? warps : g.groups;
-    const int                              columns = WARP ? p.cols : g.span;
-    const int ring = Ring::bytes(g.threads, g.groups) * Ring::kStages + g.threads * E * static_cast<int>(sizeof(float));
-    const int sums = p.partials && slots > 1 ? slots * 2 * columns * static_cast<int>(sizeof(float)) : 0;
-    const int smem = std::max(ring, sums);
-    if (smem > 32 * 1024) // a launch gets 48 KB unasked, static memory included
-        if (int st = raise_smem(layernorm_grad_kernel<SRC, GRAD, E, W, WARP, FULL>, 208 * 1024, raised))
-            return st;
-    Launch(dim3(p.parts * g.ctas), dim3(g.threads, g.groups), smem, stream, g.ctas, false)
-        .run(layernorm_grad_kernel<SRC, GRAD, E, W, WARP, FULL>, p, g.span);
-    return check_launch("LayerNormBackward");
-}
-
-template<int SRC, int GRAD, int W>
-int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream_t stream)
-{
-    if (g.threads > 32)
-        return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, false, true>(p, g, stream)
-                              : launch_one_pass<SRC, GRAD, 24, W, false, true>(p, g, stream);
-    if (g.values == 8)
-        return launch_one_pass<SRC, GRAD, 8, W, true, false>(p, g, stream);
-    if (g.threads == 32)
-        return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, true, true>(p, g, stream) : launch_one_pass<SRC, GRAD, 24, W, true, true>(p, g, stream);
-    return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, true, false>(p, g, stream) : launch_one_pass<SRC, GRAD, 24, W, true, false>(p, g, stream);
-}
-
-template<int SRC, int GRAD>
-int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, int width, cudaStream_t stream)
-{
-    // vectors of 16 bytes at most on the way through shared memory; of four elements at least, otherwise the rows' lines as they are
-    if constexpr (SRC != B200PP_F32 && GRAD != B200PP_F32)
-        if (width == 8)
-            return launch_one_pass<SRC, GRAD, 8>(p, g, stream);
-    if (width >= 4)
-        return launch_one_pass<SRC, GRAD, 4>(p, g, stream);
-    return launch_one_pass<SRC, GRAD, 0>(p, g, stream);
-}
-
-// The pairs of element types the one-pass kernel is built for: gradients of the source's type or float32, any for uint8.
-// -1: not this pair, or rows too long.
+// -1: not these types, or rows too long.
 int launch_one_pass(int srcType, const LayerNormGradKParams &p, const GradPlan &g, int width, cudaStream_t stream)
 {
     if (g.values == 0)
         return -1;
-    switch (srcType * 16 + p.gradType)
+    switch (srcType)
     {
-#define B200PP_PAIR(S, G) \
-    case S * 16 + G:      \
-        return launch_one_pass<S, G>(p, g, width, stream);
-        B200PP_PAIR(B200PP_U8, B200PP_F32)
-        B200PP_PAIR(B200PP_U8, B200PP_F16)
-        B200PP_PAIR(B200PP_U8, B200PP_BF16)
-        B200PP_PAIR(B200PP_F16, B200PP_F16)
-        B200PP_PAIR(B200PP_F16, B200PP_F32)
-        B200PP_PAIR(B200PP_BF16, B200PP_BF16)
-        B200PP_PAIR(B200PP_BF16, B200PP_F32)
-        B200PP_PAIR(B200PP_F32, B200PP_F32)
-#undef B200PP_PAIR
+    case B200PP_U8:
+        return layernorm_grad_u8(p, g, width, stream);
+    case B200PP_F16:
+        return layernorm_grad_f16(p, g, width, stream);
+    case B200PP_BF16:
+        return layernorm_grad_bf16(p, g, width, stream);
     }
-    return -1;
+    return layernorm_grad_f32(p, g, width, stream);
 }
 
 template<int SRC>

@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(256) layernorm_grad_columns_kernel(const Layer
 }
 
 // Adds up the parts: blockDim.y threads share a column, each takes every blockDim.y-th part, and the first joins them in order.
-__global__ void __launch_bounds__(1024) layernorm_grad_join_kernel(const LayerNormGradKParams p)
+static __global__ void __launch_bounds__(1024) layernorm_grad_join_kernel(const LayerNormGradKParams p)
 {
     __shared__ float sum[32][33];
     const long long  c = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, n = 2LL * p.cols; // column of dw, db

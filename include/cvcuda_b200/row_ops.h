@@ -47,8 +47,8 @@ typedef struct B200ppRows
  * of the row (variance: the mean of the squared distances to the mean). src: uint8, float16, bfloat16 or float32; dst:
  * float16, bfloat16 or float32. weight and bias: `cols` adjacent values of float16, bfloat16 or float32, each NULL for 1
  * and 0. mean and rstd: if not NULL, the float32 statistics of the rows, packed, in row order, for the backward pass.
- * Sums are float32 (the variance about the mean, not the difference of two sums). dst may be src if the types agree. Rows of
- * up to 8192 columns need no workspace. */
+ * Sums are float32 (the variance about the mean, not the difference of two sums). dst may be src if the types agree; apart from
+ * that no output may overlap an input or another output. Rows of up to 8192 columns need no workspace. */
 typedef struct B200ppLayerNormOp
 {
     const void *weight;
@@ -67,8 +67,9 @@ B200PP_PUBLIC int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, 
  *   dweight = the sum over the rows of grad * h
  *   dbias   = the sum over the rows of grad
  * grad: float16, bfloat16 or float32, the gradient of the forward pass's dst; src, mean, rstd, weight: as there. dsrc (NULL
- * where it is not wanted; float16, bfloat16 or float32) may be grad, or src, if the types agree. dweight and dbias: `cols`
- * adjacent values, NULL where not wanted. All sums are float32, rounded to the output's type once. No rows: zeros. */
+ * where it is not wanted; float16, bfloat16 or float32) may be grad, or src, if the types agree; other overlaps are not
+ * allowed. dweight and dbias: `cols` adjacent values, NULL where not wanted. All sums are float32, rounded to the output's
+ * type once. No rows: zeros. */
 typedef struct B200ppLayerNormGradOp
 {
     const float *mean, *rstd;

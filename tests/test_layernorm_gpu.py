@@ -73,6 +73,17 @@ def test_backward_row_lengths(pkg, cols, src, grad):
         verify_backward(pkg, g, x, m, r, w)
 
 
+# gradients of another type than the rows, above the row length one kernel holds too
+@pytest.mark.parametrize("cols", [20, 130, 760, 1030, 4096, 10001, 65536, 65537, 70001])
+@pytest.mark.parametrize("src,grad", [("f32", "f16"), ("f32", "bf16"), ("u8", "f16"), ("u8", "f32"), ("f16", "f32"), ("f16", "bf16"),
+                                      ("bf16", "f16"), ("bf16", "bf16")])
+def test_backward_of_mixed_types(pkg, cols, src, grad):
+    x, g = values((13, cols), KINDS[src], cols), values((13, cols), KINDS[grad], 3)
+    w = values((cols,), torch.float32, 1, 0.3, 1.0)
+    _, m, r = pkg.layernorm(x, stats=True)
+    verify_backward(pkg, g, x, m, r, w)
+
+
 @pytest.mark.parametrize("src", list(KINDS))
 @pytest.mark.parametrize("dst", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("wk,bk", [(None, None), ("f32", None), (None, "bf16"), ("f16", "f32"), ("bf16", "bf16")])
