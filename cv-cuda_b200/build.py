@@ -17,7 +17,7 @@ LIB = os.path.join(HERE, "libcvcuda_b200.so")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 SOURCES = ["library.cu", "layernorm.cu", "layernorm_grad.cu", "layernorm_grad_u8.cu", "layernorm_grad_f16.cu", "layernorm_grad_bf16.cu",
-           "layernorm_grad_f32.cu", "embedding.cu", "cvcuda_ops.cpp", "random_crop.cpp"]
+           "layernorm_grad_f32.cu", "embedding.cu", "embedding_grad_direct.cu", "cvcuda_ops.cpp", "random_crop.cpp"]
 
 
 def _stale() -> bool:

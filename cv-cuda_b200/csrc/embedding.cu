@@ -1,4 +1,5 @@
 // Host side of the embedding lookup and its gradient: argument validation, kernel selection and launch.
+#include "embedding_grad_direct.cuh"
 #include "embedding_kernels.cuh"
 #include "row_host.h"
 
@@ -236,19 +237,27 @@ int sort_ctas(long long count, size_t smem)
     return wide.load() & bit ? 16 : 8;
 }
 
+// Few indices: one kernel whose CTAs each read all of them. Tables of so many CTAs' columns and rows that the reading would take longer
+// than sorting are left to the others.
+bool goes_direct(long long count, long long rows, long long cols)
+{
+    return count <= kDirectCount && (cols + 31) / 32 * ((rows + kDirectRows - 1) / kDirectRows) <= 4096;
+}
+
 } // namespace
 
-extern "C" int b200ppEmbeddingBackwardWorkspace(const B200ppRows *grad, size_t *bytes)
+extern "C" int b200ppEmbeddingBackwardWorkspace(const B200ppRows *grad, const B200ppRows *dtable, size_t *bytes)
 {
-    if (!grad || !bytes)
+    if (!grad || !dtable || !bytes)
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
     RowMap     m;
-    long long  count = 0;
-    B200ppRows t     = *grad;
-    t.base           = reinterpret_cast<void *>(uintptr_t(256));
-    if (int st = take_rows(&t, "Gradient", false, m, count))
+    long long  count = 0, rows = 0;
+    B200ppRows g = *grad, t = *dtable;
+    g.base = t.base = reinterpret_cast<void *>(uintptr_t(256));
+    int st;
+    if ((st = take_rows(&g, "Gradient", false, m, count)) || (st = take_rows(&t, "Table gradient", true, m, rows)))
         return st;
-    *bytes = count > 0 ? plan_embedding_grad(count, t.cols).bytes : 0;
+    *bytes = count == 0 || goes_direct(count, rows, g.cols) ? 0 : plan_embedding_grad(count, g.cols).bytes;
     return B200PP_SUCCESS;
 }
 
@@ -274,6 +283,26 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
         return B200PP_SUCCESS;
     if (count == 0 && op->accumulate)
         return B200PP_SUCCESS;
+    const int padding = op->paddingIndex >= 0 && op->paddingIndex < rows ? static_cast<int>(op->paddingIndex) : -1;
+    if (goes_direct(count, rows, grad->cols))
+    {
+        EmbeddingDirectKParams d{};
+        d.grad       = p.grad;
+        d.indices    = p.indices;
+        d.dtable     = p.dtable;
+        d.gradType   = grad->dtype;
+        d.indexType  = indices->dtype;
+        d.dtableType = dtable->dtype;
+        d.count      = static_cast<unsigned>(count);
+        d.rows       = static_cast<int>(rows);
+        d.cols       = static_cast<int>(grad->cols);
+        d.scale      = op->scale;
+        d.accumulate = op->accumulate != 0;
+        VecWidth width(d.cols);
+        width.take(d.grad, row_elem_size(d.gradType));
+        width.take(d.dtable, row_elem_size(d.dtableType));
+        return embedding_grad_direct(d, width.width, padding, stream);
+    }
     const EmbeddingGradPlan w = plan_embedding_grad(count, grad->cols);
     if (count > 0 && (st = check_workspace(workspace, workspaceBytes, w.bytes)))
         return st;
@@ -286,7 +315,7 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     p.cols       = static_cast<int>(grad->cols);
     p.scale      = op->scale;
     p.accumulate = op->accumulate != 0;
-    p.padding    = op->paddingIndex >= 0 && op->paddingIndex < rows ? static_cast<int>(op->paddingIndex) : -1;
+    p.padding    = padding;
     p.units      = w.units;
     p.groups     = w.groups;
     for (int k = 0; k < 2; ++k) p.entries[k] = reinterpret_cast<uint2 *>(ws + w.entries[k]);

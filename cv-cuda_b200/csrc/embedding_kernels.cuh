@@ -244,9 +244,10 @@ struct EmbeddingGradKParams
 // A least-significant-digit radix sort by one CTA or one cluster. Each warp owns a contiguous range of the positions and counts its
 // digits in a table of its own; a prefix over the warps, the CTAs (through distributed shared memory) and the digits turns the
 // counts into the places each warp writes to. The arrays between the passes are in global memory (they stay in L2); the cluster
-// barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and most counts of indices are
-// small; clearing the table goes on at the same time. Few indices cost latency -- the trips to memory, the barriers, code that is
-// fetched to run once (8 us for 1000) -- many the scattered stores and the ballots (25 us for 65536 of 50000, 59 us for 262144 of
+// barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and clearing
+// the table goes on at the same time. Few indices (of tables so large that the one kernel in embedding_grad_direct.cuh is not for
+// them) cost latency -- the trips to memory, the barriers, code that is fetched to run once (8 us for 1000) -- many the scattered
+// stores and the ballots (25 us for 65536 of 50000, 59 us for 262144 of
 // 128000, sixteen CTAs). A match instruction instead of the ballots takes a turn for each different digit of a warp (43 us for the
 // 65536 with eight CTAs, where ballots take 34).
 constexpr int kSortThreads = 1024;

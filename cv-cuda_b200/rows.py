@@ -70,7 +70,7 @@ def _lib() -> C.CDLL:
                            ("LayerNormBackwardWorkspace", [R, S]),
                            ("LayerNormBackward", [R, R, R, O, C.c_void_p, C.c_size_t, C.c_void_p]),
                            ("Embedding", [R, R, R, C.c_float, C.c_void_p]),
-                           ("EmbeddingBackwardWorkspace", [R, S]),
+                           ("EmbeddingBackwardWorkspace", [R, R, S]),
                            ("EmbeddingBackward", [R, R, R, O, C.c_void_p, C.c_size_t, C.c_void_p])):
             f = getattr(L, "b200pp" + name)
             f.restype, f.argtypes = C.c_int, args
@@ -202,6 +202,14 @@ def _workspace_size(name: str, code: int, cols: int, rows: int) -> int:
     """What the library asks for; it depends on the shape alone."""
     n = C.c_size_t(0)
     _check(getattr(_lib(), name)(_pack_rows(256, code, cols, rows, 1, 1, cols * 8, 0, 0), C.byref(n)))
+    return n.value
+
+
+@lru_cache(maxsize=1024)
+def _embedding_workspace_size(code: int, cols: int, count: int, dcode: int, rows: int) -> int:
+    n = C.c_size_t(0)
+    _check(_lib().b200ppEmbeddingBackwardWorkspace(_pack_rows(256, code, cols, count, 1, 1, cols * 8, 0, 0),
+                                                   _pack_rows(256, dcode, cols, rows, 1, 1, cols * 8, 0, 0), C.byref(n)))
     return n.value
 
 
@@ -397,9 +405,10 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *,
 def _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate, device, handle):
     g, cols, count = _rows(grad, 1, "Gradient")
     op = _pack_emb_grad(scale, int(accumulate), -1 if padding_index is None else int(padding_index))
-    size = _workspace_size("b200ppEmbeddingBackwardWorkspace", _TYPES.get(grad.dtype, -1), cols, count)
-    ws = _scratch(size, device)
-    _check(_lib().b200ppEmbeddingBackward(g, _indices(indices), _rows(dtable, 1, "Table gradient")[0], op, ws.data_ptr(), size, handle))
+    t, _, rows = _rows(dtable, 1, "Table gradient")
+    size = _embedding_workspace_size(_TYPES.get(grad.dtype, -1), cols, count, _TYPES.get(dtable.dtype, -1), rows)
+    keep = _scratch(size, device) if size else None
+    _check(_lib().b200ppEmbeddingBackward(g, _indices(indices), t, op, keep.data_ptr() if size else None, size, handle))
 
 
 def embedding_backward_into(dtable: torch.Tensor, grad: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, *,
@@ -422,7 +431,8 @@ def embedding_backward(grad: torch.Tensor, indices: torch.Tensor, rows: int, sca
                        padding_index: Optional[int] = None, data_type: torch.dtype = torch.float32, stream=None) -> torch.Tensor:
     """The gradient of :func:`embedding` with respect to a table of ``rows`` rows: row v is ``scale`` times the sum of the rows
     of ``grad`` whose index is v, zero if there is none. Indices outside the table and those equal to ``padding_index`` take
-    no part. The sums are float32 in an order that depends on the indices alone, rounded to ``data_type`` once."""
+    no part. The sums are float32, in an order that the indices, the types and the tensors' layout settle, rounded to ``data_type``
+    once."""
     device = _device_of(grad, indices)
     if grad.dim() < 1 or grad.shape[:-1] != indices.shape:
         raise _invalid("The gradient must have the indices' shape followed by the table's number of columns")

@@ -92,7 +92,7 @@ B200PP_PUBLIC int b200ppEmbedding(const B200ppRows *indices, const B200ppRows *t
                                   cudaStream_t stream);
 
 /* Gradient of the embedding lookup: row v of dtable = scale * the sum of the rows i of grad with indices[i] = v, in float32,
- * in an order that depends on the indices alone; a row no index names is zero. With `accumulate`, the sum is added to what
+ * in an order that the indices, the types and the tensors' layout settle; a row no index names is zero. With `accumulate`, the sum is added to what
  * dtable holds, and rows no index names stay as they are. Indices outside the table, and those equal to paddingIndex (a value
  * outside the table: none), take no part. grad and dtable: float16, bfloat16 or float32. dtable must not overlap grad. */
 typedef struct B200ppEmbeddingGradOp
@@ -102,7 +102,7 @@ typedef struct B200ppEmbeddingGradOp
     int64_t paddingIndex;
 } B200ppEmbeddingGradOp;
 
-B200PP_PUBLIC int b200ppEmbeddingBackwardWorkspace(const B200ppRows *grad, size_t *bytes);
+B200PP_PUBLIC int b200ppEmbeddingBackwardWorkspace(const B200ppRows *grad, const B200ppRows *dtable, size_t *bytes);
 B200PP_PUBLIC int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows *indices, const B200ppRows *dtable,
                                           const B200ppEmbeddingGradOp *op, void *workspace, size_t workspaceBytes,
                                           cudaStream_t stream);

@@ -143,6 +143,44 @@ def test_gradient(pkg, cols, grad, dst, ids):
         check_grad(got, g, i, 0.7, what=f"{count} of {rows}")
 
 
+# more indices than one kernel takes at once
+@pytest.mark.parametrize("cols", [c for c in COLS if c <= 1024])
+@pytest.mark.parametrize("grad,dst", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+def test_gradient_of_many_indices(pkg, cols, grad, dst):
+    for count, rows in ((16384, 9000), (16385, 9000), (20011, 70)):
+        g, i = values((count, cols), KINDS[grad], cols), indices((count,), -3, rows + 3, torch.int64, cols)
+        check_grad(pkg.embedding_backward(g, i, rows, 0.7, data_type=KINDS[dst]), g, i, 0.7, what=f"{count} of {rows}")
+
+
+# runs around the lengths that groups of lanes, warps and whole blocks take; column counts of every vector width; indices in order
+# and in the opposite one
+@pytest.mark.parametrize("cols", [1, 2, 7, 12, 64, 65, 200])
+@pytest.mark.parametrize("grad", list(KINDS))
+def test_gradient_runs_of_every_length(pkg, cols, grad):
+    i = torch.repeat_interleave(torch.arange(12), torch.tensor([1, 2, 8, 9, 31, 32, 33, 511, 0, 512, 513, 2000])).cuda()
+    g = values((len(i), cols), KINDS[grad], cols)
+    shuffled = i[torch.randperm(len(i), generator=torch.Generator().manual_seed(cols)).cuda()]
+    for j in (i, 11 - i, shuffled, i * 2048, i * 2047, shuffled * 148 + 3):
+        check_grad(pkg.embedding_backward(g, j, 30000, 1.5), g, j, 1.5)
+        into = torch.ones((30000, cols), dtype=torch.float32, device="cuda")
+        pkg.embedding_backward_into(into, g, j, 1.5, accumulate=True)
+        check_grad(into, g, j, 1.5, before=torch.ones_like(into))
+
+
+# tables around the rows that a block keeps track of, and those left to the kernels for many indices (a wide table of many rows)
+@pytest.mark.parametrize("rows,cols", [(2047, 5000), (2048, 5000), (2049, 5000), (4096, 9480), (4097, 9480), (2097152, 33), (300000, 1000),
+                                       (1, 70000), (149, 8)])
+def test_gradient_of_tables_of_many_rows(pkg, rows, cols):
+    g, i = values((37, cols), torch.bfloat16, 1), indices((37,), 0, rows, torch.int64, rows)
+    i[5:9] = rows - 1
+    got = pkg.embedding_backward(g, i, rows, data_type=torch.bfloat16)
+    named = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    named[i] = True
+    assert not bool(got[~named].any())
+    at, inverse = torch.unique(i, return_inverse=True)
+    check_grad(got[at], g, inverse, 1.0)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 255, 256, 1023, 1024, 1025, 40000, 1 << 20, (1 << 20) + 1])
 @pytest.mark.parametrize("count", [31, 1024, 8193, 70001])
 def test_gradient_of_every_number_of_digits(pkg, rows, count):

@@ -117,7 +117,11 @@ def test_embedding_backward_refusals(pkg):
     R = lambda **k: _rows(pkg, **k)  # noqa: E731
     ids = R(dtype=S64, cols=1)
     need = C.c_size_t(0)
-    assert L.b200ppEmbeddingBackwardWorkspace(C.byref(R()), C.byref(need)) == 0 and need.value > 0
+    assert L.b200ppEmbeddingBackwardWorkspace(C.byref(R()), C.byref(R()), C.byref(need)) == 0 and need.value == 0
+    # many indices are sorted in a workspace
+    many, many_ids = R(count=(40000, 1, 1)), R(dtype=S64, cols=1, count=(40000, 1, 1))
+    assert L.b200ppEmbeddingBackwardWorkspace(C.byref(many), C.byref(R()), C.byref(need)) == 0 and need.value > 0
+    assert L.b200ppEmbeddingBackwardWorkspace(C.byref(many), None, C.byref(need)) == INVALID
 
     def call(g, i, t, ws=65536, size=1 << 30):
         op = pkg.rows._EmbeddingGradOp(1.0, 0, -1)
@@ -130,9 +134,9 @@ def test_embedding_backward_refusals(pkg):
     assert call(R(cols=4), ids, R()) == INVALID
     assert call(R(count=(3, 1, 1)), ids, R()) == INVALID
     assert call(R(), ids, R(stride=(0, 0, 0))) == INVALID
-    assert call(R(), ids, R(), size=need.value - 1) == INVALID
-    assert call(R(), ids, R(), ws=None) == INVALID
-    assert call(R(), ids, R(), ws=65537) == INVALID
+    assert call(many, many_ids, R(), size=need.value - 1) == INVALID
+    assert call(many, many_ids, R(), ws=None) == INVALID
+    assert call(many, many_ids, R(), ws=65537) == INVALID
     assert call(R(), ids, R(count=(0, 1, 1))) == 0  # a table without rows
 
 
