@@ -7,12 +7,22 @@ using namespace b200pp;
 
 namespace {
 
-GradPlan plan_layernorm_grad(long long rows, long long cols, int elem)
+// The rows of the CTAs of a plan start like one another if row `step` rows on does, and so do those of a warp, which are `warps` apart.
+bool rows_start_alike(const GradPlan &g, const RowShift &s)
 {
-    GradPlan g{};
-    if (cols <= 8 * 16 * kGradResident)
+    const bool warp = g.threads < 32;
+    return s.valid && g.parts * g.groups * s.step % s.width == 0 && (!warp || g.threads * g.groups / 32 * s.step % s.width == 0);
+}
+
+GradPlan plan_layernorm_grad(long long rows, long long length, int elem)
+{
+    GradPlan        g{};
+    if (length <= 8 * 16 * kGradResident)
     {
         g.ctas = 1;
+        // room for rows that start anywhere in a vector, unless that takes more CTAs
+        while (g.ctas * 16 * kGradResident < length) g.ctas *= 2;
+        const long long cols = length % 4 && length + 7 <= g.ctas * 16 * kGradResident ? length + 7 : length;
         if (cols <= 768)
         {
             // as few lanes per row as leave little idle
@@ -25,10 +35,11 @@ GradPlan plan_layernorm_grad(long long rows, long long cols, int elem)
         }
         else
         {
-            while (g.ctas * 16 * kGradResident < cols) g.ctas *= 2;
-            // sixteen values, or 24 where that lets two CTAs share an SM (shared memory is too small for two with float32 rows)
+            // sixteen values, or 24 where that lets two CTAs share an SM or leaves no more lanes idle (50030 rows of 2051 float16: 176 ->
+            // 157 us; 30000 of 1536: 67 -> 60 us). With float32 rows shared memory is too small for two CTAs
             const long long part = (cols + g.ctas - 1) / g.ctas;
-            g.values             = elem < 4 && part > 16 * kGradResident / 2 && part <= 24 * kGradResident / 2 ? 24 : 16;
+            const bool      pair = part > 16 * kGradResident / 2 && part <= 24 * kGradResident / 2;
+            g.values             = elem < 4 && (pair || (part + 767) / 768 * 768 <= (part + 511) / 512 * 512) ? 24 : 16;
             g.threads            = static_cast<int>((part + 32 * g.values - 1) / (32 * g.values) * 32);
         }
         g.span = g.threads * g.values;
@@ -38,9 +49,18 @@ GradPlan plan_layernorm_grad(long long rows, long long cols, int elem)
         const long long turns = (rows + g.groups - 1) / g.groups;
         const int       most  = std::max(1, kSms * std::max(1, kGradResident / (g.threads * g.groups)) / g.ctas);
         g.parts               = static_cast<int>(std::max(1LL, std::min<long long>(turns, most)));
+        // every eighth row of packed ones starts at the boundary of a vector: as many CTAs that each of them has rows that start alike,
+        // unless it takes them another turn
+        int apart = 8;
+        while (apart > 1 && (length * g.groups * apart / 2) % 8 == 0) apart /= 2;
+        const int more = (g.parts + apart - 1) / apart * apart, less = g.parts / apart * apart;
+        if (cols != length && more <= most)
+            g.parts = more;
+        else if (cols != length && less > 0 && (turns + less - 1) / less <= (turns + g.parts - 1) / g.parts + turns / (16LL * g.parts))
+            g.parts = less;
         return g;
     }
-    const long long blocks = (cols + 31) / 32;
+    const long long blocks = (length + 31) / 32;
     g.parts = static_cast<int>(std::max(1LL, std::min({(rows + 31) / 32, (kSms * 8 + blocks - 1) / blocks, 65535LL})));
     return g;
 }
@@ -129,8 +149,8 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     if (rows > 0 && (!op->mean || !op->rstd))
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "The backward pass needs the forward pass's mean and rstd");
     p.cols  = static_cast<int>(src->cols);
-    const GradPlan plan = plan_layernorm_grad(rows, p.cols, row_elem_size(src->dtype));
-    p.parts             = plan.parts;
+    GradPlan plan = plan_layernorm_grad(rows, p.cols, row_elem_size(src->dtype));
+    p.parts       = plan.parts;
     if (op->dweight || op->dbias)
     {
         if ((st = check_workspace(workspace, workspaceBytes, grad_workspace(plan, p.cols))))
@@ -157,6 +177,21 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     width.take(p.grad, row_elem_size(p.gradType));
     width.take(p.dsrc, row_elem_size(p.dsrcType));
     width.take(p.weight, 0, row_elem_size(p.weightType));
+    const int wide = src->dtype == B200PP_F32 || p.gradType == B200PP_F32 ? 4 : 8;
+    RowShift  shift(wide);
+    shift.take(p.src, row_elem_size(src->dtype), rows);
+    shift.take(p.grad, row_elem_size(p.gradType), rows);
+    shift.take(p.dsrc, row_elem_size(p.dsrcType), rows);
+    // below four vectors per row, the first and the last one cost more than the pairs do
+    if (width.width < 4 && plan.values && p.cols >= 4 * wide && p.cols + wide - 1 <= plan.span * plan.ctas && rows_start_alike(plan, shift))
+    {
+        p.shift0     = shift.start;
+        p.shift      = shift.step;
+        p.ownWeights = shift.step != 0 && plan.groups > 1;
+        // copies of the weights that leave no room for a second CTA are not worth it
+        plan.ragged  = !(p.ownWeights && p.weight && wide == 4 && plan.values == 24);
+        p.ownWeights = p.ownWeights && plan.ragged;
+    }
     st = launch_one_pass(src->dtype, p, plan, width.width, stream);
     if (st >= 0)
         ; // done, or refused

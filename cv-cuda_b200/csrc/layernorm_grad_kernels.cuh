@@ -24,6 +24,8 @@ struct LayerNormGradKParams
     uint8_t       *dweight, *dbias;
     float         *partials; // [parts][2][cols]
     int            parts;
+    int            shift0, shift; // row r starts (shift0 + r * shift) % W elements after the boundary of a vector, in all tensors
+    int            ownWeights;    // a copy of the weights for each row group, whose rows start like one another
 };
 
 // All gradients in one pass over the data. WARP: blockDim.x lanes of a warp per row (a power of two) and blockDim.y rows per CTA at a
@@ -48,8 +50,12 @@ struct GradRing
     }
 };
 
-// FULL: rows have whole warps.
-template<int SRC, int GRAD, int E, int W, bool WARP, bool FULL>
+// FULL: rows have whole warps. RAGGED: rows that are no whole vectors of W, which start anywhere. Each thread then counts its columns
+// from the boundary of a vector at or before the row's start; all rows that a thread goes through start alike, and so do those of a
+// warp, so that the sums over the rows stay in registers: only the first and the last vector are not whole. (W = 0, pairs of
+// elements picked out of the rows' lines, is for rows that start differently in the tensors, and for few: 50030 rows of 2051 float16
+// take it 225 us instead of 157, 77821 of 257 66 instead of 44.)
+template<int SRC, int GRAD, int E, int W, bool WARP, bool FULL, bool RAGGED>
 __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) layernorm_grad_kernel(const LayerNormGradKParams p, int span)
 {
     namespace cg = cooperative_groups;
@@ -67,22 +73,25 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
     const int       xBytes = X::bytes(threads, groups), stageBytes = Ring::bytes(threads, groups);
     cg::cluster_group cluster = cg::this_cluster();
     const int       ctas = WARP ? 1 : cluster.num_blocks(), rank = WARP ? 0 : cluster.block_rank();
-    const int       from = rank * span, end = WARP ? p.cols : min(p.cols - from, span); // this CTA's columns
+    // RAGGED: the rows of a warp are as many apart as there are warps, so that they start alike
+    const unsigned  step = gridDim.x / ctas * groups, base = blockIdx.x / ctas * groups;
+    unsigned        r    = base + (WARP && RAGGED ? warp + k.g % (32 / threads) * (threads * groups / 32) : k.g);
+    // columns count from the boundary of a vector before the row's start: this CTA's begin with `from` and hold begin..end of the row
+    const int       before = RAGGED ? (p.shift0 + static_cast<int>(r % 8u) * p.shift) & (W - 1) : 0;
+    const int       from = rank * span, begin = rank ? 0 : before, end = WARP ? p.cols + before : min(p.cols + before - from, span);
     const unsigned  ring0 = static_cast<unsigned>(__cvta_generic_to_shared(ring));
     f32x2           dw[E / 2], db[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) dw[i] = db[i] = both(0.0f);
-    const unsigned step = gridDim.x / ctas * groups, base = blockIdx.x / ctas * groups;
-    unsigned       r    = base + k.g;
     int            half = 0, stage = 0;
     uint8_t       *ring8 = reinterpret_cast<uint8_t *>(ring);
-    auto xRow = [&](unsigned n) { return p.src.at(n) + static_cast<long long>(from) * kElemBytes<SRC>; };
-    auto gRow = [&](unsigned n) { return p.grad.at(n) + static_cast<long long>(from) * kElemBytes<GRAD>; };
+    auto xRow = [&](unsigned n) { return p.src.at(n) + static_cast<long long>(from - before) * kElemBytes<SRC>; };
+    auto gRow = [&](unsigned n) { return p.grad.at(n) + static_cast<long long>(from - before) * kElemBytes<GRAD>; };
     auto fetch = [&](int s, unsigned n) {
         if (n < p.rows)
         {
-            X::fetch(ring0 + s * stageBytes, k, xRow(n), end);
-            G::fetch(ring0 + s * stageBytes + xBytes, k, gRow(n), end);
+            X::template fetch<RAGGED>(ring0 + s * stageBytes, k, xRow(n), end);
+            G::template fetch<RAGGED>(ring0 + s * stageBytes + xBytes, k, gRow(n), end);
         }
         copies_commit();
     };
@@ -105,19 +114,26 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
     for (int s = 0; s < kStages - 1; ++s) fetch(s, r + s * step);
     // the weights as float32, one copy for the row groups: thread t's vectors of four are `threads` apart, which no two lanes clash on.
     // Registers would have to be shared with the sums (E = 24 has 48 of those), and from L1 they cost the conversion for each row.
-    f32x2 *weights = reinterpret_cast<f32x2 *>(ring8 + kStages * stageBytes);
+    f32x2    *weights = reinterpret_cast<f32x2 *>(ring8 + kStages * stageBytes);
+    const int copies = RAGGED && p.ownWeights ? threads * groups : threads, copy = RAGGED && p.ownWeights ? tid : k.t;
     if (p.weight && p.dsrc.base)
     {
-        if (k.g == 0)
+        if (k.g == 0 || (RAGGED && p.ownWeights))
         {
+            float f[RAGGED ? E : 8];
+            if constexpr (RAGGED)
+                load_scattered<E>(p.weight, p.weightType, p.cols, f, [&](int i) { return from - before + k.c + i / W * k.step + i % W; });
 #pragma unroll
             for (int j = 0; j < E / 8; ++j)
             {
                 f32x2 w[4];
-                load_param<W>(p.weight, p.weightType, from + k.c + j * (8 / kStep<W>) * k.step, k.step, from + end, w);
+                if constexpr (RAGGED)
+                    pairs<8>(f + 8 * j, w);
+                else
+                    load_param<W>(p.weight, p.weightType, from + k.c + j * (8 / kStep<W>) * k.step, k.step, from + end, w);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    *reinterpret_cast<ulonglong2 *>(weights + ((2 * j + i) * threads + k.t) * 2) = make_ulonglong2(w[2 * i], w[2 * i + 1]);
+                    *reinterpret_cast<ulonglong2 *>(weights + ((2 * j + i) * copies + copy) * 2) = make_ulonglong2(w[2 * i], w[2 * i + 1]);
             }
         }
         __syncthreads();
@@ -138,8 +154,8 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
         {
             const uint8_t *at = ring8 + stage * stageBytes;
             const unsigned n  = live ? r : 0;
-            X::take(at, k, W == 0 ? xRow(n) : nullptr, h);
-            G::take(at + xBytes, k, W == 0 ? gRow(n) : nullptr, gv);
+            X::take(at, k, W == 0 ? xRow(n) : nullptr, h, RAGGED ? begin : 0);
+            G::take(at + xBytes, k, W == 0 ? gRow(n) : nullptr, gv, RAGGED ? begin : 0);
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
 #pragma unroll
@@ -163,7 +179,7 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
 #pragma unroll
             for (int i = 0; i < E / 4; ++i)
             {
-                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(weights + (i * threads + k.t) * 2);
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(weights + (i * copies + copy) * 2);
                 gv[2 * i]     = mul2(gv[2 * i], w.x);
                 gv[2 * i + 1] = mul2(gv[2 * i + 1], w.y);
             }
@@ -215,7 +231,8 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
         const float c1 = t1 * p.invCols, c2 = t2 * p.invCols;
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) gv[i] = mul2(add2(fma2(h[i], both(-c2), gv[i]), both(-c1)), both(rstd));
-        store_row<E, W>(p.dsrc.at(r) + static_cast<long long>(from) * (p.dsrcType == B200PP_F32 ? 4 : 2), p.dsrcType, k, end, gv);
+        store_row<E, W, RAGGED>(p.dsrc.at(r) + static_cast<long long>(from - before) * (p.dsrcType == B200PP_F32 ? 4 : 2), p.dsrcType, k, end,
+                                gv, begin);
     }
     if (ctas > 1)
         cluster.sync(); // no CTA leaves while another may still write to it
@@ -236,36 +253,63 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
             }
     const int  slot = WARP ? warp : k.g, slots = WARP ? (threads * groups) >> 5 : groups;
     const bool holds = !WARP || (tid & 31) < threads;
-    const int  columns = WARP ? p.cols : span;
-    float     *sums = reinterpret_cast<float *>(ring);
-    float     *part = p.partials + static_cast<long long>(blockIdx.x / ctas) * 2 * p.cols + from;
+    float     *part = p.partials + static_cast<long long>(blockIdx.x / ctas) * 2 * p.cols + from + begin - before;
+    // vectors of up to four, wherever they go: single values, a vector apart, took 8 us of 28 for 300 rows of 5001 float16
+    constexpr int P = kStep<W> == 8 ? 4 : kStep<W>;
+    if (!RAGGED && slots == 1)
+    {
+        if (holds)
+#pragma unroll
+            for (int e = 0; e < E; e += P)
+            {
+                const int c = k.c + e / kStep<W> * k.step + e % kStep<W>;
+                if constexpr (W > 0)
+                {
+                    if (c < end)
+                    {
+                        store_vec<B200PP_F32, P>(reinterpret_cast<uint8_t *>(part), c, fw + e);
+                        store_vec<B200PP_F32, P>(reinterpret_cast<uint8_t *>(part + p.cols), c, fb + e);
+                    }
+                }
+                else
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        if (c + i < end)
+                        {
+                            part[c + i]          = fw[e + i];
+                            part[p.cols + c + i] = fb[e + i];
+                        }
+            }
+        return;
+    }
+    float *sums = reinterpret_cast<float *>(ring); // [slots][2][span]
     __syncthreads(); // the ring is not needed any more
     if (holds)
     {
-        float *to = slots > 1 ? sums + slot * 2 * columns : part;
-        const int next = slots > 1 ? columns : p.cols;
+        uint8_t *to = reinterpret_cast<uint8_t *>(sums + slot * 2 * span);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int e = 0; e < E; e += P)
         {
             const int c = k.c + e / kStep<W> * k.step + e % kStep<W>;
-            if (c < end)
-            {
-                to[c]        = fw[e];
-                to[next + c] = fb[e];
-            }
+            store_vec<B200PP_F32, P>(to, c, fw + e);
+            store_vec<B200PP_F32, P>(to, span + c, fb + e);
         }
     }
-    if (slots == 1)
-        return;
     __syncthreads();
-    for (int c = tid; c < 2 * columns; c += threads * groups)
-    {
-        float s = 0.0f;
-        for (int i = 0; i < slots; ++i) s += sums[i * 2 * columns + c];
-        const int col = c < columns ? c : c - columns;
-        if (col < end)
-            part[c < columns ? col : p.cols + col] = s;
-    }
+    // (in a cluster there is one row at a time, and one slot)
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which)
+#pragma unroll 4
+        for (int c = tid; c < end - begin; c += threads * groups)
+        {
+            float s = 0.0f;
+            for (int i = 0; i < slots; ++i)
+            {
+                const int first = RAGGED && !rank ? (p.shift0 + static_cast<int>((base + i) % 8u) * p.shift) & (W - 1) : 0;
+                s += sums[(2 * i + which) * span + first + c];
+            }
+            part[which * p.cols + c] = s;
+        }
 }
 
 // dx, one CTA per row, any row length.

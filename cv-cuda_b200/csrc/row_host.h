@@ -164,6 +164,32 @@ struct VecWidth
     }
 };
 
+// Rows that start anywhere, in vectors of W all the same: how many elements after the boundary of a vector row 0 starts, and how many
+// more each row does, modulo W -- if that is the same in all tensors.
+struct RowShift
+{
+    int  width, start = 0, step = 0;
+    bool valid = true, first = true;
+
+    explicit RowShift(int w)
+        : width(w)
+    {
+    }
+
+    void take(const RowMap &m, int elem, long long rows)
+    {
+        if (!m.base)
+            return;
+        const int a = static_cast<int>(reinterpret_cast<uintptr_t>(m.base) / elem % width);
+        const int s = rows > 1 ? static_cast<int>((m.s2 / elem % width + width) % width) : first ? 0 : step;
+        if (m.n2 != 0 || (rows > 1 && m.s2 % elem != 0) || (!first && (a != start || s != step)))
+            valid = false;
+        start = a;
+        step  = s;
+        first = false;
+    }
+};
+
 // Raises a kernel's dynamic shared-memory limit, once per device.
 template<typename K>
 int raise_smem(K kernel, int bytes, std::atomic<unsigned long long> &done)

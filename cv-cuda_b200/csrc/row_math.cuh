@@ -459,6 +459,8 @@ struct RowStage
                 store_raw<kVec>(stage + (v * all + tid) * kVec, zero_raw<kVec>());
     }
 
+    // RAGGED: the row may end inside a vector.
+    template<bool RAGGED = false>
     static __device__ __forceinline__ void fetch(unsigned stage, const RowThread &k, const uint8_t *row, int end)
     {
         const int      tid = k.g * k.threads + k.t, all = k.threads * k.groups;
@@ -466,11 +468,12 @@ struct RowStage
 #pragma unroll
         for (int v = 0; v < V; ++v)
             if (k.c + v * k.step < end)
-                copy_async<kVec>(stage + (v * all + tid) * kVec, at + v * k.step * kElemBytes<DT>, kVec);
+                copy_async<kVec>(stage + (v * all + tid) * kVec, at + v * k.step * kElemBytes<DT>,
+                                 RAGGED ? min(W, end - k.c - v * k.step) * kElemBytes<DT> : kVec);
     }
 
-    // The thread's values, zeros behind the row's end.
-    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *, f32x2 *out)
+    // The thread's values, zeros behind the row's end, and before `begin` (which lies in the first vector).
+    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *, f32x2 *out, int begin = 0)
     {
         const int  tid = k.g * k.threads + k.t, all = k.threads * k.groups;
         Vec<DT, W> raw[V];
@@ -479,6 +482,9 @@ struct RowStage
         for (int v = 0; v < V; ++v) raw[v] = load_raw<kVec>(stage + (v * all + tid) * kVec);
 #pragma unroll
         for (int v = 0; v < V; ++v) unpack<DT, W>(raw[v], f + v * W);
+        if (k.c < begin)
+#pragma unroll
+            for (int e = 0; e < W; ++e) f[e] = e < begin ? 0.0f : f[e];
         pairs<E>(f, out);
     }
 };
@@ -504,6 +510,7 @@ struct RowStage<DT, E, 0>
 
     static __device__ __forceinline__ void clear(uint8_t *, const RowThread &, int) {}
 
+    template<bool = false>
     static __device__ __forceinline__ void fetch(unsigned stage, const RowThread &k, const uint8_t *row, int end)
     {
         const int            off   = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
@@ -518,7 +525,7 @@ struct RowStage<DT, E, 0>
         }
     }
 
-    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *row, f32x2 *out)
+    static __device__ __forceinline__ void take(const uint8_t *stage, const RowThread &k, const uint8_t *row, f32x2 *out, int = 0)
     {
         // the thread's first pair starts `at` bytes into the lines
         const int       at    = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) + k.c * kSize;
@@ -593,6 +600,28 @@ __device__ __forceinline__ void load_param(const uint8_t *p, int dtype, int c, i
     pairs<8>(f, out);
 }
 
+// N elements of a parameter, all under way at once; where `at` points outside, the nearest one.
+template<int DT, int N, typename F>
+__device__ __forceinline__ void load_scattered(const uint8_t *p, int count, float *out, F at)
+{
+    Vec<DT, 1> raw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw[i] = load_raw<kElemBytes<DT>>(p + static_cast<long long>(min(max(at(i), 0), count - 1)) * kElemBytes<DT>);
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack<DT, 1>(raw[i], out + i);
+}
+
+template<int N, typename F>
+__device__ __forceinline__ void load_scattered(const uint8_t *p, int dtype, int count, float *out, F at)
+{
+    if (dtype == B200PP_F32)
+        load_scattered<B200PP_F32, N>(p, count, out, at);
+    else if (dtype == B200PP_BF16)
+        load_scattered<B200PP_BF16, N>(p, count, out, at);
+    else
+        load_scattered<B200PP_F16, N>(p, count, out, at);
+}
+
 // A thread's values to its row, which may start anywhere.
 template<int DT, int E>
 __device__ __forceinline__ void store_pairs(uint8_t *row, int c, int step, int end, const float *f)
@@ -635,12 +664,41 @@ __device__ __forceinline__ void store_pairs(uint8_t *row, int c, int step, int e
     }
 }
 
-template<int E, int W>
-__device__ __forceinline__ void store_row(uint8_t *row, int dtype, const RowThread &k, int end, const f32x2 *x)
+// A thread's values to its row from element `begin`, which lies in the first vector, to `end`, which may lie inside one.
+template<int DT, int E, int W>
+__device__ __forceinline__ void store_ragged(uint8_t *row, const RowThread &k, int begin, int end, const float *f)
+{
+#pragma unroll
+    for (int v = 0; v < E / W; ++v)
+    {
+        const int c = k.c + v * k.step;
+        if (c >= begin && c + W <= end)
+            store_vec<DT, W>(row, c, f + v * W);
+        else
+        {
+#pragma unroll
+            for (int e = 0; e < W; ++e)
+                if (c + e >= begin && c + e < end)
+                    store_elem_as<DT>(row, c + e, f[v * W + e]);
+        }
+    }
+}
+
+template<int E, int W, bool RAGGED = false>
+__device__ __forceinline__ void store_row(uint8_t *row, int dtype, const RowThread &k, int end, const f32x2 *x, int begin = 0)
 {
     float f[E];
     singles<E>(x, f);
-    if constexpr (W > 0)
+    if constexpr (W > 0 && RAGGED)
+    {
+        if (dtype == B200PP_F32)
+            store_ragged<B200PP_F32, E, W>(row, k, begin, end, f);
+        else if (dtype == B200PP_BF16)
+            store_ragged<B200PP_BF16, E, W>(row, k, begin, end, f);
+        else
+            store_ragged<B200PP_F16, E, W>(row, k, begin, end, f);
+    }
+    else if constexpr (W > 0)
         store_vecs<W, E / W>(row, dtype, k.c, k.step, end, f);
     else if (dtype == B200PP_F32)
         store_pairs<B200PP_F32, E>(row, k.c, k.step, end, f);

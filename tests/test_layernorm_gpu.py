@@ -73,6 +73,34 @@ def test_backward_row_lengths(pkg, cols, src, grad):
         verify_backward(pkg, g, x, m, r, w)
 
 
+# rows that are no whole vectors: all tensors packed; slices whose rows start alike, with other values around them; slices whose rows
+# do not; what lies around the rows is neither used nor written
+@pytest.mark.parametrize("cols", [17, 33, 77, 257, 385, 767, 1001, 2051, 4099, 5001, 9999])
+@pytest.mark.parametrize("src,grad", [("f16", "f16"), ("bf16", "f32"), ("f32", "f32"), ("u8", "bf16")])
+def test_backward_of_rows_that_start_anywhere(pkg, cols, src, grad):
+    out = KINDS[grad]
+    for rows in (1, 7, 150, 1203):
+        x, g = values((rows, cols), KINDS[src], cols), values((rows, cols), KINDS[grad], 3)
+        w = values((cols,), torch.float32, 1, 0.3, 1.0)
+        _, m, r = pkg.layernorm(x, stats=True)
+        verify_backward(pkg, g, x, m, r, w)
+        for width, starts in ((cols + 5, (3, 3, 3)), (cols + 8, (1, 9, 1)), (cols + 16, (8, 8, 8)), (cols + 5, (0, 3, 5))):
+            wide = [torch.full((rows, width + 9), 255 if k == torch.uint8 else float("nan"), device="cuda").to(k)
+                    for k in (KINDS[src], KINDS[grad], out)]
+            xs, gs, ds = (t[:, s:s + cols] for t, s in zip(wide, starts))
+            xs.copy_(x)
+            gs.copy_(g)
+            dw, db = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+            pkg.layernorm_backward_into(ds, dw, db, gs, xs, m, r, w)
+            want, bound = layernorm_backward64(g, x, m, r, w)
+            for got, y, e, what in zip((ds, dw, db), want, bound, ("dsrc", "dweight", "dbias")):
+                check(got, y, e, what)
+            ds.fill_(float("nan"))
+            assert bool(wide[2].isnan().all())
+            pkg.layernorm_backward_into(gs, None, None, gs, xs, m, r, w)  # in place
+            check(gs, want[0], bound[0], "dsrc in place")
+
+
 # gradients of another type than the rows, above the row length one kernel holds too
 @pytest.mark.parametrize("cols", [20, 130, 760, 1030, 4096, 10001, 65536, 65537, 70001])
 @pytest.mark.parametrize("src,grad", [("f32", "f16"), ("f32", "bf16"), ("u8", "f16"), ("u8", "f32"), ("f16", "f32"), ("f16", "bf16"),
