@@ -25,48 +25,66 @@ WarpPlan plan_warp(int cols)
     return {table[i][1], table[i][2]};
 }
 
+int chunk_of(long long cols)
+{
+    return cols % 8 ? kChunk - 8 : kChunk;
+}
+
 // Chunks of a row; 0 for those the other kernels take (no workspace up to 8192 columns, row_ops.h).
 long long layernorm_chunks(long long cols)
 {
-    return cols > kBlockCols ? (cols + kChunk - 1) / kChunk : 0;
+    return cols > kBlockCols ? (cols + chunk_of(cols) - 1) / chunk_of(cols) : 0;
 }
 
-template<int SRC, int E, int W, bool FULL>
+template<int SRC, int E, int W, bool RAGGED, bool FULL>
 int launch_warp(const LayerNormKParams &p, const WarpPlan &plan, cudaStream_t stream)
 {
     static std::atomic<unsigned long long> raised{0};
     const dim3                             block(plan.lanes, 256 / plan.lanes);
     const int                              ring = RowStage<SRC, E, W>::bytes(block.x, block.y) * kWarpStages;
     if (ring > 32 * 1024) // a launch gets 48 KB unasked, static memory included
-        if (int st = raise_smem(layernorm_warp_kernel<SRC, E, W, FULL>, 112 * 1024, raised))
+        if (int st = raise_smem(layernorm_warp_kernel<SRC, E, W, FULL, RAGGED>, 112 * 1024, raised))
             return st;
     const unsigned turns = (p.rows + block.y - 1) / block.y;
-    layernorm_warp_kernel<SRC, E, W, FULL><<<std::min(turns, static_cast<unsigned>(kSms * kWarpCtas<E>)), block, ring, stream>>>(p);
+    layernorm_warp_kernel<SRC, E, W, FULL, RAGGED><<<std::min(turns, static_cast<unsigned>(kSms * kWarpCtas<E>)), block, ring, stream>>>(p);
     return B200PP_SUCCESS;
 }
 
-template<int SRC, int W>
+// RAGGED: with room for rows that start anywhere in a vector.
+template<int SRC, int W, bool RAGGED>
 int launch_staged(const LayerNormKParams &p, cudaStream_t stream)
 {
-    if (p.cols > 1024)
+    const int cols = p.cols + (RAGGED ? W - 1 : 0);
+    if (cols > 1024)
     {
         static std::atomic<unsigned long long> raised{0};
-        const int                              threads = (p.cols + 511) / 512 * 32;
+        const int                              threads = (cols + 511) / 512 * 32;
         const int                              ring    = RowStage<SRC, 16, W>::bytes(threads, 1) * 3;
         if (ring > 32 * 1024)
-            if (int st = raise_smem(layernorm_block_kernel<SRC, W>, 112 * 1024, raised))
+            if (int st = raise_smem(layernorm_block_kernel<SRC, W, RAGGED>, 112 * 1024, raised))
                 return st;
-        layernorm_block_kernel<SRC, W><<<std::min(p.rows, static_cast<unsigned>(kSms * (kBlockResident / threads))), threads, ring, stream>>>(p);
+        unsigned ctas = kSms * (kBlockResident / threads);
+        if (RAGGED)
+            ctas -= ctas % 8; // the rows of a CTA start alike
+        layernorm_block_kernel<SRC, W, RAGGED><<<std::min(p.rows, ctas), threads, ring, stream>>>(p);
         return B200PP_SUCCESS;
     }
-    const WarpPlan plan = plan_warp(p.cols);
+    const WarpPlan plan = plan_warp(cols);
     if (plan.values == 8)
-        return launch_warp<SRC, 8, W, false>(p, plan, stream);
+        return launch_warp<SRC, 8, W, RAGGED, false>(p, plan, stream);
     if (plan.values == 32)
-        return launch_warp<SRC, 32, W, true>(p, plan, stream);
+        return launch_warp<SRC, 32, W, RAGGED, true>(p, plan, stream);
     if (plan.lanes == 32)
-        return plan.values == 16 ? launch_warp<SRC, 16, W, true>(p, plan, stream) : launch_warp<SRC, 24, W, true>(p, plan, stream);
-    return plan.values == 16 ? launch_warp<SRC, 16, W, false>(p, plan, stream) : launch_warp<SRC, 24, W, false>(p, plan, stream);
+        return plan.values == 16 ? launch_warp<SRC, 16, W, RAGGED, true>(p, plan, stream) : launch_warp<SRC, 24, W, RAGGED, true>(p, plan, stream);
+    return plan.values == 16 ? launch_warp<SRC, 16, W, RAGGED, false>(p, plan, stream) : launch_warp<SRC, 24, W, RAGGED, false>(p, plan, stream);
+}
+
+template<int SRC, int W, bool RAGGED>
+int launch_chunks(const LayerNormKParams &p, cudaStream_t stream)
+{
+    layernorm_chunk_stats_kernel<SRC, W, RAGGED><<<p.rows * p.chunks, kChunkThreads, 0, stream>>>(p);
+    Launch(dim3(p.rows * p.chunks), dim3(kChunkThreads), 0, stream, 1, true).run(layernorm_chunk_apply_kernel<SRC, W, RAGGED>, p);
+    return B200PP_SUCCESS;
 }
 
 template<int SRC, int W>
@@ -74,8 +92,7 @@ bool launch_direct(const LayerNormKParams &p, cudaStream_t stream)
 {
     if (p.chunks)
     {
-        layernorm_chunk_stats_kernel<SRC, W><<<p.rows * p.chunks, kChunkThreads, 0, stream>>>(p);
-        Launch(dim3(p.rows * p.chunks), dim3(kChunkThreads), 0, stream, 1, true).run(layernorm_chunk_apply_kernel<SRC, W>, p);
+        launch_chunks<SRC, W, false>(p, stream);
         return true;
     }
     if (p.cols > 256 && p.cols <= 4096 && p.rows <= static_cast<unsigned>(kSms))
@@ -87,18 +104,38 @@ bool launch_direct(const LayerNormKParams &p, cudaStream_t stream)
 }
 
 template<int SRC>
-int launch_layernorm(const LayerNormKParams &p, int width, cudaStream_t stream)
+int launch_layernorm(LayerNormKParams &p, int width, cudaStream_t stream)
 {
+    // rows that are no whole vectors of four, but start alike in both tensors
+    constexpr int kWide = SRC == B200PP_F32 ? 4 : 8; // of the staged kernels, as below
+    const int     wide  = p.chunks ? 8 : kWide;
+    RowShift      shift(wide);
+    shift.take(p.src, kElemBytes<SRC>, p.rows);
+    shift.take(p.dst, row_elem_size(p.dstType), p.rows);
+    if (width < 4 && shift.valid)
+    {
+        p.shift0 = shift.start;
+        p.shift  = shift.step;
+        if (p.chunks)
+        {
+            // float32 rows with weights, read eight values apart: 150 of 77777 49 us, value by value 38
+            if (p.chunk < kChunk && (SRC != B200PP_F32 || (!p.weight && !p.bias)))
+                return launch_chunks<SRC, 8, true>(p, stream);
+        }
+        // below four vectors per row, the first and the last one cost more than the pairs do
+        else if (p.cols >= 4 * wide && !(p.cols > 256 && p.cols <= 4096 && p.rows <= static_cast<unsigned>(kSms)))
+            return launch_staged<SRC, kWide, true>(p, stream);
+    }
     if (width == 8 ? launch_direct<SRC, 8>(p, stream)
                    : width == 4 ? launch_direct<SRC, 4>(p, stream) : width == 2 ? launch_direct<SRC, 2>(p, stream) : launch_direct<SRC, 1>(p, stream))
         return B200PP_SUCCESS;
     // vectors of 16 bytes at most on the way through shared memory; of four elements at least, otherwise the rows' lines as they are
     if constexpr (SRC != B200PP_F32)
         if (width == 8)
-            return launch_staged<SRC, 8>(p, stream);
+            return launch_staged<SRC, 8, false>(p, stream);
     if (width >= 4)
-        return launch_staged<SRC, 4>(p, stream);
-    return launch_staged<SRC, 0>(p, stream);
+        return launch_staged<SRC, 4, false>(p, stream);
+    return launch_staged<SRC, 0, false>(p, stream);
 }
 
 } // namespace
@@ -157,6 +194,7 @@ extern "C" int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, con
     p.mean       = op->mean;
     p.rstd       = op->rstd;
     p.chunks     = static_cast<unsigned>(chunks);
+    p.chunk      = chunk_of(p.cols);
     p.partials   = static_cast<float2 *>(workspace);
     VecWidth width(p.cols);
     width.take(p.src, row_elem_size(src->dtype));

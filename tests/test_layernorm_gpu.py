@@ -73,6 +73,31 @@ def test_backward_row_lengths(pkg, cols, src, grad):
         verify_backward(pkg, g, x, m, r, w)
 
 
+# the forward pass of the same, long rows in chunks too
+@pytest.mark.parametrize("cols", [17, 33, 77, 257, 385, 767, 1001, 1021, 2051, 5001, 8189, 8193, 16369, 24553, 50003])
+@pytest.mark.parametrize("src,dst", [("f16", "f16"), ("bf16", "f32"), ("f32", "f32"), ("u8", "bf16")])
+def test_rows_that_start_anywhere(pkg, cols, src, dst):
+    for rows in (1, 7, 150, 1203) if cols < 10000 else (1, 7, 40):
+        x = values((rows, cols), KINDS[src], cols, 1.0, 3.0)
+        w, b = values((cols,), torch.float32, 1, 0.3, 1.0), values((cols,), torch.bfloat16, 2, 0.3)
+        for wb in ((w, b), (None, None)):
+            verify(pkg, x, *wb, KINDS[dst])
+        (want, _, _), (bound, _, _) = layernorm64(x, w, b, EPS)
+        for width, starts in ((cols + 5, (3, 3)), (cols + 8, (1, 9)), (cols + 16, (8, 8)), (cols + 5, (0, 3))):
+            wide = [torch.full((rows, width + 9), 255 if k == torch.uint8 else float("nan"), device="cuda").to(k) for k in (KINDS[src], KINDS[dst])]
+            xs, ys = (t[:, s:s + cols] for t, s in zip(wide, starts))
+            xs.copy_(x)
+            pkg.layernorm_into(ys, xs, w, b, EPS)
+            check(ys, want, bound, "result")
+            ys.fill_(float("nan"))
+            assert bool(wide[1].isnan().all())
+            if src == dst:
+                pkg.layernorm_into(xs, xs, w, b, EPS)
+                check(xs, want, bound, "result in place")
+                xs.fill_(float("nan"))
+                assert bool(wide[0].isnan().all())
+
+
 # rows that are no whole vectors: all tensors packed; slices whose rows start alike, with other values around them; slices whose rows
 # do not; what lies around the rows is neither used nor written
 @pytest.mark.parametrize("cols", [17, 33, 77, 257, 385, 767, 1001, 2051, 4099, 5001, 9999])
