@@ -28,7 +28,8 @@ struct EmbeddingKParams
 // blockDim.x * U vectors of the row. All loads go out before the first is used, and none is conditional: past the row's end its last
 // vector is loaded again, for an index outside the table the first row. What bounds the kernel is how many bytes it has under way
 // and, for short rows, how many instructions a row takes (3.3 million rows of nine: 155 us with each lane of a row reading the
-// index), so a warp reads 32 indices at a time and hands them out. DST: the output's type, -1 for any.
+// index, now 81), so a warp reads 32 indices at a time and hands them out. 65536 rows of 1024 bfloat16: 29.3 us, 5.7 TB/s, 0.88 of a
+// copy's rate. DST: the output's type, -1 for any.
 template<int W>
 constexpr int kLookupVectors = W == 8 ? 4 : 8; // U * R
 
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingKParams p
 // lines. SHARED: the table's rows, times the scale and rounded to the output's type, are copied to shared memory first, with a row of
 // zeros for indices outside the table. Gathers bound this kernel: from L1 a warp's 32 addresses take a cycle for each 128-byte line
 // they touch (114 us for 16.6 million indices and a palette of 256 x 3 floats), from shared memory one for each clash of banks, which
-// 16-bit rows read whole (8 bytes for three) have half as many of as three floats read one by one (37 us).
+// 16-bit rows read whole (8 bytes for three) have half as many of as three floats read one by one (26 us, 4.4 TB/s, against 37).
 constexpr int kShortTable = 16384; // bytes of a table that is copied to shared memory
 
 // Elements a row takes there: 16-bit rows a power of two, float32 rows an odd number, so that they start in all banks.
@@ -244,12 +245,11 @@ struct EmbeddingGradKParams
 // A least-significant-digit radix sort by one CTA or one cluster. Each warp owns a contiguous range of the positions and counts its
 // digits in a table of its own; a prefix over the warps, the CTAs (through distributed shared memory) and the digits turns the
 // counts into the places each warp writes to. The arrays between the passes are in global memory (they stay in L2); the cluster
-// barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and clearing
-// the table goes on at the same time. Few indices (of tables so large that the one kernel in embedding_grad_direct.cuh is not for
-// them) cost latency -- the trips to memory, the barriers, code that is fetched to run once (8 us for 1000) -- many the scattered
-// stores and the ballots (25 us for 65536 of 50000, 59 us for 262144 of
-// 128000, sixteen CTAs). A match instruction instead of the ballots takes a turn for each different digit of a warp (43 us for the
-// 65536 with eight CTAs, where ballots take 34).
+// barrier orders the passes. One cluster, because a grid-wide sort takes three launches a pass, and clearing the table goes on at the
+// same time. Few indices (of tables so large that the one kernel in embedding_grad_direct.cuh is not for them) cost latency -- the
+// trips to memory, the barriers, code that is fetched to run once (8 us for 1000) -- many the scattered stores and the ballots (25 us
+// for 65536 of 50000, 59 us for 262144 of 128000, sixteen CTAs). A match instruction instead of the ballots takes a turn for each
+// different digit of a warp (43 us for the 65536 with eight CTAs, where ballots take 34).
 constexpr int kSortThreads = 1024;
 constexpr int kSortMaxBits = 10;
 constexpr int kSortMaxCtas = 16;
@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(kZeroThreads) embedding_clear_kernel(const Emb
 //    the rows of a unit in flight at once; larger units left the GPU with little more than one wave of long-lived warps.
 //  - Longer runs are summed by groups of kShortRun positions into `partials` -- slot 0 for the run that comes from the group before,
 //    slot 1 for the one that starts in the group, a job each -- and joined by the third kernel.
+// 16384 indices of 32000 x 1024, bfloat16 to float32: 20 of 52 us; the sort takes 15 and the clearing beside it 22, the join 6.
 constexpr int kGradUnit  = 8;
 constexpr int kShortRun  = 32;
 template<int W>

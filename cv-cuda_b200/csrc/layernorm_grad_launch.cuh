@@ -30,7 +30,8 @@ int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream
     typedef GradRing<SRC, GRAD, E, W>      Ring;
     static std::atomic<unsigned long long> raised{0};
     const int                              warps = g.threads * g.groups / 32, slots = WARP ? warps : g.groups;
-    const int ring = Ring::bytes(g.threads, g.groups) * Ring::kStages + g.threads * (p.ownWeights ? g.groups : 1) * E * static_cast<int>(sizeof(float));
+    const int copies = p.ownWeights ? g.groups : 1; // of the weights
+    const int ring   = Ring::bytes(g.threads, g.groups) * Ring::kStages + g.threads * copies * E * static_cast<int>(sizeof(float));
     const int sums = p.partials ? slots * 2 * g.span * static_cast<int>(sizeof(float)) : 0;
     const int smem = std::max(ring, sums);
     if (smem > 32 * 1024) // a launch gets 48 KB unasked, static memory included
@@ -50,8 +51,10 @@ int launch_one_pass(const LayerNormGradKParams &p, const GradPlan &g, cudaStream
     if (g.values == 8)
         return launch_one_pass<SRC, GRAD, 8, W, RAGGED, true, false>(p, g, stream);
     if (g.threads == 32)
-        return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, RAGGED, true, true>(p, g, stream) : launch_one_pass<SRC, GRAD, 24, W, RAGGED, true, true>(p, g, stream);
-    return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, RAGGED, true, false>(p, g, stream) : launch_one_pass<SRC, GRAD, 24, W, RAGGED, true, false>(p, g, stream);
+        return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, RAGGED, true, true>(p, g, stream)
+                              : launch_one_pass<SRC, GRAD, 24, W, RAGGED, true, true>(p, g, stream);
+    return g.values == 16 ? launch_one_pass<SRC, GRAD, 16, W, RAGGED, true, false>(p, g, stream)
+                          : launch_one_pass<SRC, GRAD, 24, W, RAGGED, true, false>(p, g, stream);
 }
 
 template<int SRC, int GRAD>

@@ -429,8 +429,8 @@ __device__ __forceinline__ void copies_wait()
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Who a thread is: thread t of the `threads` of a row (a power of two below 32, or whole warps), row group g of the CTA; a row's values are dealt out as vectors, the
-// thread's first at element c, `step` elements apart.
+// Who a thread is: thread t of the `threads` of a row (a power of two below 32, or whole warps), row group g of the CTA; a row's values
+// are dealt out as vectors, the thread's first at element c, `step` elements apart.
 struct RowThread
 {
     int t, threads, g, groups, c, step;
