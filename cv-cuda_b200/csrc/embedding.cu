@@ -250,6 +250,10 @@ extern "C" int b200ppEmbeddingBackwardWorkspace(const B200ppRows *grad, const B2
 {
     if (!grad || !dtable || !bytes)
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
+    if (!is_float(grad->dtype) || !is_float(dtable->dtype))
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Invalid DataType");
+    if (grad->cols != dtable->cols)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Gradient and table have different numbers of columns");
     RowMap     m;
     long long  count = 0, rows = 0;
     B200ppRows g = *grad, t = *dtable;

@@ -144,6 +144,8 @@ extern "C" int b200ppLayerNormWorkspace(const B200ppRows *src, size_t *bytes)
 {
     if (!src || !bytes)
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
+    if (!is_float(src->dtype) && src->dtype != B200PP_U8)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Invalid DataType");
     RowMap     m;
     long long  rows = 0;
     B200ppRows t    = *src;

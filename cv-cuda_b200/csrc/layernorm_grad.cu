@@ -16,7 +16,7 @@ bool rows_start_alike(const GradPlan &g, const RowShift &s)
 
 GradPlan plan_layernorm_grad(long long rows, long long length, int elem)
 {
-    GradPlan        g{};
+    GradPlan g{};
     if (length <= 8 * 16 * kGradResident)
     {
         g.ctas = 1;
@@ -112,6 +112,8 @@ extern "C" int b200ppLayerNormBackwardWorkspace(const B200ppRows *src, size_t *b
 {
     if (!src || !bytes)
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "Null argument");
+    if (!is_float(src->dtype) && src->dtype != B200PP_U8)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "Invalid DataType");
     RowMap    m;
     long long rows = 0;
     B200ppRows t   = *src;

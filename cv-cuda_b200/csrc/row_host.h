@@ -44,9 +44,10 @@ inline bool is_float(int dtype)
 // Checks a set of rows (its element type is checked by the caller) and works out the kernels' view of it.
 inline int take_rows(const B200ppRows *t, const char *what, bool written, RowMap &m, long long &rows)
 {
-    const long long limit = 0x7fffffffLL, elem = row_elem_size(t->dtype);
-    if (t->cols < 1 || t->cols > limit)
-        return fail(B200PP_ERROR_INVALID_ARGUMENT, "%s must have 1 to 2^31 - 1 columns", what);
+    // columns: room for the vectors behind the last one, whose numbers kernels compute before they leave them out
+    const long long limit = 0x7fffffffLL, widest = limit - 0xffff, elem = row_elem_size(t->dtype);
+    if (t->cols < 1 || t->cols > widest)
+        return fail(B200PP_ERROR_INVALID_ARGUMENT, "%s must have 1 to 2^31 - 2^16 columns", what);
     bool empty = false;
     for (int k = 0; k < 3; ++k)
     {
@@ -137,7 +138,6 @@ inline int check_workspace(const void *workspace, size_t have, size_t need)
         return fail(B200PP_ERROR_INVALID_ARGUMENT, "The workspace must start on a 16-byte boundary");
     return B200PP_SUCCESS;
 }
-
 
 // Largest number of elements (8, 4, 2, 1) that can be moved as one vector: it divides the row, and every row of every tensor starts
 // on its boundary.

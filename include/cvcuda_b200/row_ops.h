@@ -33,7 +33,7 @@ enum
 /* A set of rows of `cols` adjacent elements each. Row r = (r0 * count[1] + r1) * count[2] + r2 starts
  * r0 * stride[0] + r1 * stride[1] + r2 * stride[2] bytes after base, which expresses a matrix, the pixels of an NHWC tensor
  * with padded rows, or the images of a batch. Strides are multiples of the element size, of any sign; those of a tensor
- * that is written keep its rows apart. At most 2^31 - 1 rows, and at most 2^31 - 1 columns. */
+ * that is written keep its rows apart. At most 2^31 - 1 rows, and at most 2^31 - 2^16 columns. */
 typedef struct B200ppRows
 {
     void   *base;
@@ -92,9 +92,10 @@ B200PP_PUBLIC int b200ppEmbedding(const B200ppRows *indices, const B200ppRows *t
                                   cudaStream_t stream);
 
 /* Gradient of the embedding lookup: row v of dtable = scale * the sum of the rows i of grad with indices[i] = v, in float32,
- * in an order that the indices, the types and the tensors' layout settle; a row no index names is zero. With `accumulate`, the sum is added to what
- * dtable holds, and rows no index names stay as they are. Indices outside the table, and those equal to paddingIndex (a value
- * outside the table: none), take no part. grad and dtable: float16, bfloat16 or float32. dtable must not overlap grad. */
+ * in an order that the indices, the types and the tensors' layout settle; a row no index names is zero. With `accumulate`, the
+ * sum is added to what dtable holds, and rows no index names stay as they are. Indices outside the table, and those equal to
+ * paddingIndex (a value outside the table: none), take no part. grad and dtable: float16, bfloat16 or float32. dtable must not
+ * overlap grad or indices. Up to 8192 indices need no workspace, except with very large tables. */
 typedef struct B200ppEmbeddingGradOp
 {
     float   scale;

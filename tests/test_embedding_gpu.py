@@ -273,6 +273,29 @@ def test_equal_calls_give_equal_bits_on_any_stream(pkg):
         assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
+@pytest.mark.parametrize("count", [50, 8000])
+def test_equal_calls_of_few_indices_and_replays(pkg, count):
+    """Runs of every length, whose positions are put in order after an unordered step; a replay with other indices in place."""
+    i = (values((count,), torch.float32, 2) ** 4 * 3).long().clamp_(max=699)
+    g = values((count, 130), torch.bfloat16, 1)
+    first = pkg.embedding_backward(g, i, 700)
+    check_grad(first, g, i, 1.0)
+    for _ in range(5):
+        assert torch.equal(first, pkg.embedding_backward(g, i, 700))
+    ids, into = i.clone(), torch.zeros(700, 130, device="cuda")
+    pkg.embedding_backward_into(into, g, ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.embedding_backward_into(into, g, ids)
+    for shift in (0, 1, 350):
+        ids.copy_((i + shift) % 700)
+        into.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(into, torch.roll(first, shift, 0))
+
+
 def test_python_refusals(pkg):
     t, i = values((5, 8), torch.float32), indices((4,), 0, 5)
     g = values((4, 8), torch.float32)

@@ -31,6 +31,11 @@ def test_layernorm_refusals(pkg):
     assert _ln(pkg, R(), R(count=(5, 1, 1))) == INVALID
     assert _ln(pkg, R(cols=0), R(cols=0)) == INVALID
     assert _ln(pkg, R(cols=1 << 31), R(cols=1 << 31)) == INVALID
+    assert _ln(pkg, R(cols=(1 << 31) - 1), R(cols=(1 << 31) - 1)) == INVALID
+    L, size = pkg.rows._lib(), C.c_size_t(0)
+    for dtype in (S16, S32, S64, 12):
+        assert L.b200ppLayerNormWorkspace(C.byref(R(dtype=dtype)), C.byref(size)) == INVALID
+        assert L.b200ppLayerNormBackwardWorkspace(C.byref(R(dtype=dtype)), C.byref(size)) == INVALID
     assert _ln(pkg, R(count=(-1, 1, 1)), R(count=(-1, 1, 1))) == INVALID
     big = dict(count=(1 << 16, 1 << 16, 1), stride=(1 << 40, 32, 0))
     assert _ln(pkg, R(**big), R(**big)) == OVERFLOW
@@ -122,6 +127,8 @@ def test_embedding_backward_refusals(pkg):
     many, many_ids = R(count=(40000, 1, 1)), R(dtype=S64, cols=1, count=(40000, 1, 1))
     assert L.b200ppEmbeddingBackwardWorkspace(C.byref(many), C.byref(R()), C.byref(need)) == 0 and need.value > 0
     assert L.b200ppEmbeddingBackwardWorkspace(C.byref(many), None, C.byref(need)) == INVALID
+    for g, t in ((R(dtype=U8), R()), (R(), R(dtype=S32)), (R(cols=9), R())):
+        assert L.b200ppEmbeddingBackwardWorkspace(C.byref(g), C.byref(t), C.byref(C.c_size_t(0))) == INVALID
 
     def call(g, i, t, ws=65536, size=1 << 30):
         op = pkg.rows._EmbeddingGradOp(1.0, 0, -1)
