@@ -65,9 +65,14 @@ GradPlan plan_layernorm_grad(long long rows, long long length, int elem)
     return g;
 }
 
-size_t grad_workspace(const GradPlan &g, long long cols)
+bool are_few(long long rows, long long cols)
 {
-    return static_cast<size_t>(g.parts) * 2 * cols * sizeof(float);
+    return rows <= kFewRows && cols <= kFewCols;
+}
+
+size_t grad_workspace(const GradPlan &g, long long rows, long long cols)
+{
+    return are_few(rows, cols) ? 0 : static_cast<size_t>(g.parts) * 2 * cols * sizeof(float);
 }
 
 // -1: not these types, or rows too long.
@@ -85,6 +90,23 @@ int launch_one_pass(int srcType, const LayerNormGradKParams &p, const GradPlan &
         return layernorm_grad_bf16(p, g, width, stream);
     }
     return layernorm_grad_f32(p, g, width, stream);
+}
+
+template<int SRC>
+int launch_few(const LayerNormGradKParams &p, cudaStream_t stream)
+{
+    const unsigned rows = p.dsrc.base ? p.rows : 0, columns = p.dweight || p.dbias ? (p.cols + 31u) / 32u : 0;
+    // dsrc over grad or src: the sums over the rows first
+    if (rows && columns && (p.dsrc.base == p.grad.base || p.dsrc.base == p.src.base))
+    {
+        layernorm_grad_few_kernel<SRC><<<columns, kFewThreads, 0, stream>>>(p, 0);
+        if (int st = check_launch("LayerNormBackward"))
+            return st;
+        layernorm_grad_few_kernel<SRC><<<rows, kFewThreads, 0, stream>>>(p, rows);
+    }
+    else if (rows + columns > 0)
+        layernorm_grad_few_kernel<SRC><<<rows + columns, kFewThreads, 0, stream>>>(p, rows);
+    return check_launch("LayerNormBackward");
 }
 
 template<int SRC>
@@ -120,7 +142,7 @@ extern "C" int b200ppLayerNormBackwardWorkspace(const B200ppRows *src, size_t *b
     t.base         = reinterpret_cast<void *>(uintptr_t(256));
     if (int st = take_rows(&t, "Input", false, m, rows))
         return st;
-    *bytes = grad_workspace(plan_layernorm_grad(rows, t.cols, row_elem_size(t.dtype)), t.cols);
+    *bytes = grad_workspace(plan_layernorm_grad(rows, t.cols, row_elem_size(t.dtype)), rows, t.cols);
     return B200PP_SUCCESS;
 }
 
@@ -155,7 +177,7 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     p.parts       = plan.parts;
     if (op->dweight || op->dbias)
     {
-        if ((st = check_workspace(workspace, workspaceBytes, grad_workspace(plan, p.cols))))
+        if ((st = check_workspace(workspace, workspaceBytes, grad_workspace(plan, rows, p.cols))))
             return st;
         p.partials = static_cast<float *>(workspace);
     }
@@ -174,6 +196,16 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
     p.dbias       = static_cast<uint8_t *>(op->dbias);
     if (rows == 0)
         p.dsrc.base = nullptr;
+    if (are_few(rows, p.cols))
+    {
+        if (src->dtype == B200PP_U8)
+            return launch_few<B200PP_U8>(p, stream);
+        if (src->dtype == B200PP_F16)
+            return launch_few<B200PP_F16>(p, stream);
+        if (src->dtype == B200PP_BF16)
+            return launch_few<B200PP_BF16>(p, stream);
+        return launch_few<B200PP_F32>(p, stream);
+    }
     VecWidth width(p.cols);
     width.take(p.src, row_elem_size(src->dtype));
     width.take(p.grad, row_elem_size(p.gradType));

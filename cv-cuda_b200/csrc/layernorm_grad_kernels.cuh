@@ -314,6 +314,103 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
         }
 }
 
+// Few rows, where only latency counts: the first `rowCtas` CTAs take a row each for dx, the others 32 columns each for the sums over the
+// rows, which reads everything twice (from L2). One launch without a workspace instead of two with one (17 rows of 1000 floats: 5.1 ->
+// 3.1 us, and 4.4 of 20 us on the host; 256 of 2048 float16: 8.0 -> 6.4; at 512 rows there is nothing left of it).
+constexpr int kFewRows = 256, kFewCols = 4096, kFewThreads = 256;
+
+// Sums over the rows from, from + step ... of column c, eight rows under way at once.
+template<int SRC, int GRAD>
+__device__ __forceinline__ void layernorm_grad_few_columns(const LayerNormGradKParams &p, int c, unsigned from, unsigned step, float &dw, float &db)
+{
+    constexpr int N = 8;
+    for (unsigned r0 = from; r0 < p.rows; r0 += N * step)
+    {
+        Vec<SRC, 1>  x[N];
+        Vec<GRAD, 1> g[N];
+        float        mean[N], rstd[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+        {
+            const unsigned r = min(r0 + k * step, p.rows - 1);
+            x[k]             = load_raw<kElemBytes<SRC>>(p.src.at(r) + static_cast<long long>(c) * kElemBytes<SRC>);
+            g[k]             = load_raw<kElemBytes<GRAD>>(p.grad.at(r) + static_cast<long long>(c) * kElemBytes<GRAD>);
+            mean[k]          = p.mean[r];
+            rstd[k]          = p.rstd[r];
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+        {
+            float xv, gv;
+            unpack<SRC, 1>(x[k], &xv);
+            unpack<GRAD, 1>(g[k], &gv);
+            if (r0 + k * step < p.rows)
+            {
+                db += gv;
+                dw = fmaf(gv, (xv - mean[k]) * rstd[k], dw);
+            }
+        }
+    }
+}
+
+template<int SRC>
+__global__ void __launch_bounds__(kFewThreads) layernorm_grad_few_kernel(const LayerNormGradKParams p, unsigned rowCtas)
+{
+    constexpr int    kWarps = kFewThreads / 32, kEach = kFewCols / kFewThreads;
+    __shared__ float scratch[2][32], sum[2][kWarps][32];
+    const int        lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x < rowCtas)
+    {
+        const unsigned r = blockIdx.x;
+        float          x[kEach], g[kEach], w[kEach], s1 = 0.0f, s2 = 0.0f;
+        auto           at = [&](int i) { return static_cast<int>(threadIdx.x) + i * kFewThreads; };
+        load_scattered<SRC, kEach>(p.src.at(r), p.cols, x, at);
+        load_scattered<kEach>(p.grad.at(r), p.gradType, p.cols, g, at);
+        if (p.weight)
+            load_scattered<kEach>(p.weight, p.weightType, p.cols, w, at);
+        const float mean = p.mean[r], rstd = p.rstd[r];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+        {
+            if (p.weight)
+                g[i] *= w[i];
+            x[i] = (x[i] - mean) * rstd;
+            if (at(i) < p.cols)
+            {
+                s1 += g[i];
+                s2 = fmaf(g[i], x[i], s2);
+            }
+        }
+        const float c1 = block_sum(s1, scratch[0]) * p.invCols, c2 = block_sum(s2, scratch[1]) * p.invCols;
+        uint8_t    *dx = p.dsrc.at(r);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (at(i) < p.cols)
+                store_elem_as(dx, at(i), p.dsrcType, rstd * (fmaf(x[i], -c2, g[i]) - c1));
+        return;
+    }
+    const int c = static_cast<int>(blockIdx.x - rowCtas) * 32 + lane;
+    float     dw = 0.0f, db = 0.0f;
+    if (c < p.cols && p.gradType == B200PP_F32)
+        layernorm_grad_few_columns<SRC, B200PP_F32>(p, c, warp, kWarps, dw, db);
+    else if (c < p.cols && p.gradType == B200PP_BF16)
+        layernorm_grad_few_columns<SRC, B200PP_BF16>(p, c, warp, kWarps, dw, db);
+    else if (c < p.cols)
+        layernorm_grad_few_columns<SRC, B200PP_F16>(p, c, warp, kWarps, dw, db);
+    sum[0][warp][lane] = dw;
+    sum[1][warp][lane] = db;
+    __syncthreads();
+    if (warp > 1 || c >= p.cols)
+        return;
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) s += sum[warp][k][lane];
+    if (warp == 0 && p.dweight)
+        store_elem_as(p.dweight, c, p.dweightType, s);
+    if (warp == 1 && p.dbias)
+        store_elem_as(p.dbias, c, p.dbiasType, s);
+}
+
 // dx, one CTA per row, any row length.
 template<int SRC>
 __global__ void __launch_bounds__(256) layernorm_grad_row_kernel(const LayerNormGradKParams p)

@@ -302,8 +302,9 @@ def _layernorm_backward(d, dweight, dbias, grad, src, mean, rstd, weight, axes, 
     keep, ws, size = None, None, 0
     if dw or db:
         size = _workspace_size("b200ppLayerNormBackwardWorkspace", _TYPES.get(src.dtype, -1), cols, count)
-        keep = _scratch(size, device)
-        ws = keep.data_ptr()
+        if size:
+            keep = _scratch(size, device)
+            ws = keep.data_ptr()
     _check(_lib().b200ppLayerNormBackward(g, s, d, op, ws, size, handle))
 
 

@@ -69,7 +69,7 @@ B200PP_PUBLIC int b200ppLayerNorm(const B200ppRows *src, const B200ppRows *dst, 
  * grad: float16, bfloat16 or float32, the gradient of the forward pass's dst; src, mean, rstd, weight: as there. dsrc (NULL
  * where it is not wanted; float16, bfloat16 or float32) may be grad, or src, if the types agree; other overlaps are not
  * allowed. dweight and dbias: `cols` adjacent values, NULL where not wanted. All sums are float32, rounded to the output's
- * type once. No rows: zeros. */
+ * type once. No rows: zeros. Up to 256 rows of up to 4096 columns, and calls without dweight and dbias, need no workspace. */
 typedef struct B200ppLayerNormGradOp
 {
     const float *mean, *rstd;

@@ -65,7 +65,7 @@ def test_row_lengths(pkg, cols, src, dst):
 @pytest.mark.parametrize("cols", LENGTHS)
 @pytest.mark.parametrize("src,grad", [("f16", "f16"), ("bf16", "f32"), ("f32", "f32"), ("u8", "bf16")])
 def test_backward_row_lengths(pkg, cols, src, grad):
-    for rows in (1, 5, 67):
+    for rows in (1, 67, 301):
         x = values((rows, cols), KINDS[src], cols + rows)
         g = values((rows, cols), KINDS[grad], 3)
         w = values((cols,), torch.float32, 1, 0.3, 1.0)
@@ -131,10 +131,30 @@ def test_backward_of_rows_that_start_anywhere(pkg, cols, src, grad):
 @pytest.mark.parametrize("src,grad", [("f32", "f16"), ("f32", "bf16"), ("u8", "f16"), ("u8", "f32"), ("f16", "f32"), ("f16", "bf16"),
                                       ("bf16", "f16"), ("bf16", "bf16")])
 def test_backward_of_mixed_types(pkg, cols, src, grad):
-    x, g = values((13, cols), KINDS[src], cols), values((13, cols), KINDS[grad], 3)
+    x, g = values((301, cols), KINDS[src], cols), values((301, cols), KINDS[grad], 3)
     w = values((cols,), torch.float32, 1, 0.3, 1.0)
     _, m, r = pkg.layernorm(x, stats=True)
     verify_backward(pkg, g, x, m, r, w)
+
+
+# around the rows and columns that go in one launch
+@pytest.mark.parametrize("cols", [1, 31, 33, 255, 257, 2049, 4095, 4096, 4097])
+@pytest.mark.parametrize("src,grad", [("f32", "f32"), ("u8", "f16"), ("bf16", "bf16")])
+def test_backward_of_few_rows(pkg, cols, src, grad):
+    for rows in (1, 2, 8, 9, 64, 65, 255, 256, 257):
+        x, g = values((rows, cols), KINDS[src], cols), values((rows, cols), KINDS[grad], 3)
+        w = values((cols,), torch.bfloat16, 1, 0.3, 1.0)
+        _, m, r = pkg.layernorm(x, stats=True)
+        verify_backward(pkg, g, x, m, r, None)
+        full = verify_backward(pkg, g, x, m, r, w)
+        for want in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1)):
+            out = pkg.layernorm_backward(g, x, m, r, w, src_grad=bool(want[0]), weight_grad=bool(want[1]), bias_grad=bool(want[2]))
+            assert all(o is None or torch.equal(o, f) for o, f in zip(out, full)) and [o is not None for o in out] == [bool(k) for k in want]
+        into, dw, db = g.clone(), torch.empty_like(w), torch.empty_like(w)
+        pkg.layernorm_backward_into(into, dw, db, into, x, m, r, w)
+        want, bound = layernorm_backward64(g, x, m, r, w)
+        for got, y, e, what in zip((into, dw, db), want, bound, ("dsrc", "dweight", "dbias")):
+            check(got, y, e, what + " in place")
 
 
 @pytest.mark.parametrize("src", list(KINDS))
@@ -162,7 +182,7 @@ def test_many_rows(pkg, rows, cols):
 @pytest.mark.parametrize("want", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 0, 1), (1, 1, 0)])
 @pytest.mark.parametrize("cols", [100, 1024, 2500, 40000])
 def test_only_the_gradients_asked_for(pkg, want, cols):
-    x, g = values((37, cols), torch.float16, 1), values((37, cols), torch.float16, 2)
+    x, g = values((307, cols), torch.float16, 1), values((307, cols), torch.float16, 2)
     w = values((cols,), torch.float16, 3, 0.3, 1.0)
     _, m, r = pkg.layernorm(x, w, stats=True)
     out = verify_backward(pkg, g, x, m, r, w, src_grad=bool(want[0]), weight_grad=bool(want[1]), bias_grad=bool(want[2]))
@@ -211,23 +231,23 @@ def test_zero_epsilon_and_infinities_stay_in_their_rows(pkg):
 @pytest.mark.parametrize("cols", [5, 64, 250, 2000])
 def test_strided_rows(pkg, kind, cols):
     """Rows of a wider tensor, every second one, transposed, and with other strides on every side."""
-    wide = values((6, 10, 4, cols + 11), KINDS[kind], 1)
+    wide = values((12, 20, 4, cols + 11), KINDS[kind], 1)
     x = wide[:, ::2, :3, 5:5 + cols].permute(1, 0, 2, 3)
     w = values((cols + 3,), torch.float32, 2)[3:]  # off the vector boundary
     want = pkg.layernorm(x.contiguous(), w.clone(), data_type=torch.float32)
-    guard = torch.full((5, 6, 3, cols + 9), 77.0, device="cuda")
+    guard = torch.full((10, 12, 3, cols + 9), 77.0, device="cuda")
     out = guard[..., 2:2 + cols]
-    m, r = (torch.full((5 * 6 * 3 + 2,), 5.0, device="cuda") for _ in range(2))
-    pkg.layernorm_into(out, x, w, mean=m[1:-1].reshape(5, 6, 3), rstd=r[1:-1].reshape(5, 6, 3))
+    m, r = (torch.full((10 * 12 * 3 + 2,), 5.0, device="cuda") for _ in range(2))
+    pkg.layernorm_into(out, x, w, mean=m[1:-1].reshape(10, 12, 3), rstd=r[1:-1].reshape(10, 12, 3))
     (y64, m64, r64), (dy, dm, dr) = layernorm64(x.reshape(-1, cols), w, None, EPS)
     check(out.reshape(-1, cols), y64, dy, "result")
     check(m[1:-1], m64, dm, "mean")
     assert float(m[0]) == float(m[-1]) == float(r[0]) == float(r[-1]) == 5.0
     assert bool((guard[..., :2] == 77.0).all()) and bool((guard[..., 2 + cols:] == 77.0).all())
     check(want.reshape(-1, cols), y64, dy, "packed")
-    m, r = m[1:-1].reshape(5, 6, 3).clone(), r[1:-1].reshape(5, 6, 3).clone()
-    g = values((5, 6, 3, cols * 2), torch.float32, 4)[..., 1:1 + cols]
-    guard = torch.full((5, 6, 3, cols + 9), 77.0, device="cuda")
+    m, r = m[1:-1].reshape(10, 12, 3).clone(), r[1:-1].reshape(10, 12, 3).clone()
+    g = values((10, 12, 3, cols * 2), torch.float32, 4)[..., 1:1 + cols]
+    guard = torch.full((10, 12, 3, cols + 9), 77.0, device="cuda")
     dx = guard[..., 3:3 + cols]
     params = torch.full((2 * cols + 6,), 5.0, device="cuda")
     dw, db = params[1:1 + cols], params[cols + 5:2 * cols + 5]

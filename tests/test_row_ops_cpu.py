@@ -91,10 +91,12 @@ def test_layernorm_backward_refusals(pkg):
     assert call(R(), R(), R(), dweight=4096, dweightType=S32) == INVALID
     assert call(R(), R(), R(), dbias=4098, dbiasType=F32) == INVALID
     need = C.c_size_t(0)
-    assert L.b200ppLayerNormBackwardWorkspace(C.byref(R()), C.byref(need)) == 0 and need.value > 0
-    assert call(R(), R(), R(), dweight=4096, dweightType=F32, size=need.value - 1) == INVALID
-    assert call(R(), R(), R(), dweight=4096, dweightType=F32, ws=None) == INVALID
-    assert call(R(), R(), R(), dweight=4096, dweightType=F32, ws=65544) == INVALID
+    assert L.b200ppLayerNormBackwardWorkspace(C.byref(R()), C.byref(need)) == 0 and need.value == 0  # few short rows
+    many = R(count=(400, 1, 1))
+    assert L.b200ppLayerNormBackwardWorkspace(C.byref(many), C.byref(need)) == 0 and need.value > 0
+    assert call(many, many, many, dweight=4096, dweightType=F32, size=need.value - 1) == INVALID
+    assert call(many, many, many, dweight=4096, dweightType=F32, ws=None) == INVALID
+    assert call(many, many, many, dweight=4096, dweightType=F32, ws=65544) == INVALID
 
 
 def test_embedding_refusals(pkg):
