@@ -75,6 +75,8 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
     const int       xBytes = X::bytes(threads, groups), stageBytes = Ring::bytes(threads, groups);
     cg::cluster_group cluster = cg::this_cluster();
     const int       ctas = WARP ? 1 : cluster.num_blocks(), rank = WARP ? 0 : cluster.block_rank();
+    if (ctas > 1)
+        cluster.barrier_arrive(); // waited for in front of the rows, when the copies of the first ones are under way
     // RAGGED: the rows of a warp are as many apart as there are warps, so that they start alike
     const unsigned  step = gridDim.x / ctas * groups, base = blockIdx.x / ctas * groups;
     unsigned        r    = base + (WARP && RAGGED ? warp + k.g % (32 / threads) * (threads * groups / 32) : k.g);
@@ -141,6 +143,8 @@ __global__ void __launch_bounds__(WARP ? 256 : kGradResident, WARP ? 2 : 1) laye
         __syncthreads();
     }
     float nextMean = r < p.rows ? p.mean[r] : 0.0f, nextRstd = r < p.rows ? p.rstd[r] : 0.0f;
+    if (ctas > 1)
+        cluster.barrier_wait(); // every CTA of the cluster has started, so that its shared memory may be written to
     // every thread of the CTA takes the same number of turns
     for (unsigned first = base; first < p.rows; first += step, r += step)
     {

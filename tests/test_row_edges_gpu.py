@@ -1,0 +1,36 @@
+"""The row operators where they could go wrong: clusters, infinite rows, long sums, wide tables, the sorted gradient."""
+import pytest
+import torch
+
+from row_bounds import check, layernorm64, layernorm_backward64
+
+pytestmark = pytest.mark.gpu
+
+KINDS = {"u8": torch.uint8, "f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def values(shape, kind, seed=0):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    if kind == torch.uint8:
+        return torch.randint(0, 256, shape, generator=gen, device="cuda", dtype=torch.uint8)
+    return torch.randn(shape, generator=gen, device="cuda").to(kind)
+
+
+# clusters of two, four and eight CTAs, with one row each, which is exchanged first thing, and with more
+@pytest.mark.parametrize("cols", [8193, 12288, 16385, 20000, 32769, 40003, 65536])
+@pytest.mark.parametrize("src,grad", [("f16", "f16"), ("f32", "f32"), ("u8", "bf16")])
+def test_backward_of_rows_split_over_clusters(pkg, cols, src, grad):
+    w = values((cols,), torch.float32, 1)
+    for rows in (1, 2, 19, 160):
+        x, g = values((rows, cols), KINDS[src], cols), values((rows, cols), KINDS[grad], 3)
+        (_, m, r), _ = layernorm64(x, None, None, 1e-5)
+        m, r = m.float(), r.float()
+        first = pkg.layernorm_backward(g, x, m, r, w)
+        want, bound = layernorm_backward64(g, x, m, r, w)
+        for got, y, e, what in zip(first, want, bound, ("dsrc", "dweight", "dbias")):
+            check(got, y, e, what)
+        # launched back to back: CTAs of a cluster start while those of the launch before end
+        again = [pkg.layernorm_backward(g, x, m, r, w) for _ in range(20)]
+        alone = [pkg.layernorm_backward(g, x, m, r, w, weight_grad=False, bias_grad=False)[0] for _ in range(20)]
+        assert all(torch.equal(a, f) for call in again for a, f in zip(call, first)) and all(torch.equal(a, first[0]) for a in alone)
