@@ -72,17 +72,18 @@ class Format(enum.Enum):
 
 
 _TORCH = {np.dtype(np.uint8): torch.uint8, np.dtype(np.int8): torch.int8, np.dtype(np.int16): torch.int16,
-          np.dtype(np.int32): torch.int32, np.dtype(np.int64): torch.int64, np.dtype(np.float32): torch.float32, np.dtype(np.float16): torch.float16}
+          np.dtype(np.int32): torch.int32, np.dtype(np.float32): torch.float32, np.dtype(np.float16): torch.float16}
 if hasattr(torch, "uint16"):
     _TORCH[np.dtype(np.uint16)] = torch.uint16
-_NUMPY = {v: k for k, v in _TORCH.items()}
+_STORED = {**_TORCH, np.dtype(np.int64): torch.int64}  # in tensors: the row operators' indices too
+_NUMPY = {v: k for k, v in _STORED.items()}
 
 
-def _torch_dtype(dt) -> torch.dtype:
+def _torch_dtype(dt, kinds=_TORCH) -> torch.dtype:
     if isinstance(dt, torch.dtype):
         return dt
     try:
-        return _TORCH[np.dtype(dt)]
+        return kinds[np.dtype(dt)]
     except (KeyError, TypeError):
         raise Error(Status.ERROR_INVALID_ARGUMENT, f"Unsupported element type {dt!r}") from None
 
@@ -143,7 +144,7 @@ class Tensor:
         lay = str(lay or "")
         if lay and len(lay) != len(tuple(shape)):
             raise Error(Status.ERROR_INVALID_ARGUMENT, "Layout rank must match the shape's")
-        self._t = torch.zeros(tuple(int(v) for v in shape), dtype=_torch_dtype(dtype), device=_device())
+        self._t = torch.zeros(tuple(int(v) for v in shape), dtype=_torch_dtype(dtype, _STORED), device=_device())
         self._layout = lay
 
     @property
@@ -362,7 +363,7 @@ def crop_flip_normalize_reformat(src: ImageBatchVarShape, out_shape: Sequence[in
                                  flags: Optional[int] = None, border: Border = Border.CONSTANT, bvalue: float = 0.0, *,
                                  stream=None) -> Tensor:
     """cvcuda.crop_flip_normalize_reformat (python/mod_cvcuda/OpCropFlipNormalizeReformat.cpp:65-74,86-126)."""
-    out = Tensor(tuple(out_shape), out_dtype, str(out_layout))
+    out = Tensor(tuple(out_shape), _torch_dtype(out_dtype), str(out_layout))
     return crop_flip_normalize_reformat_into(out, src, rect, flip_code, base, scale, globalscale, globalshift, epsilon, flags,
                                              border, bvalue, stream=stream)
 

@@ -140,6 +140,13 @@ for _name, _code in (("uint16", 2), ("uint32", 4)):
         _DTYPE_CODE[getattr(torch, _name)] = _code
 
 
+def _type_code(dtype: torch.dtype) -> int:
+    try:
+        return _DTYPE_CODE[dtype]
+    except KeyError:
+        raise Error(Status.ERROR_INVALID_ARGUMENT, f"Unsupported element type {dtype}") from None
+
+
 # ------------------------------------------------------------------------------------------------ library
 
 _lib: Optional[C.CDLL] = None
@@ -348,7 +355,7 @@ def _source_of(src: Union[torch.Tensor, ImageBatchVarShape]):
         if len(src) == 0:
             raise Error(Status.ERROR_INVALID_ARGUMENT, "Input image batch is empty")
         table = src.descriptor_table()
-        s.dtype = _DTYPE_CODE[src.dtype]
+        s.dtype = _type_code(src.dtype)
         s.channels, s.planar, s.numSamples = src.channels, int(src.planar), len(src)
         s.imageList = table.data_ptr()
         s.maxWidth, s.maxHeight = src.max_size
@@ -362,7 +369,7 @@ def _source_of(src: Union[torch.Tensor, ImageBatchVarShape]):
     es = t.element_size()
     if t.stride(3) != 1 or t.stride(2) != c:
         raise Error(Status.ERROR_INVALID_ARGUMENT, "Input pixels must be contiguous within a row")
-    s.dtype = _DTYPE_CODE[t.dtype]
+    s.dtype = _type_code(t.dtype)
     s.channels, s.planar, s.numSamples = c, 0, n
     s.base = t.data_ptr()
     s.sampleStride, s.rowStride, s.planeStride = t.stride(0) * es, t.stride(1) * es, 0
@@ -382,7 +389,7 @@ def _dest_of(dst: torch.Tensor, layout: str):
     t = dst if dst.dim() == 4 else dst.unsqueeze(0)
     es = t.element_size()
     d = _Dest()
-    d.base, d.dtype = t.data_ptr(), _DTYPE_CODE[t.dtype]
+    d.base, d.dtype = t.data_ptr(), _type_code(t.dtype)
     if layout.endswith("HWC"):
         n, h, w, c = t.shape
         d.sampleStride, d.rowStride, d.pixStride, d.chanStride = (t.stride(i) * es for i in range(4))
