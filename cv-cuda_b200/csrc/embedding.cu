@@ -187,13 +187,21 @@ EmbeddingGradPlan plan_embedding_grad(long long count, long long cols)
     return w;
 }
 
+// The workspace query and the call refuse the same sizes, before anything is launched. The largest grid is that of the runs, eight jobs
+// per CTA; for vectors that a lane has four values of, blocks of columns are smallest.
+int check_grad_size(const EmbeddingGradPlan &w, long long cols)
+{
+    const unsigned long long jobs = (static_cast<unsigned long long>(w.units) + 2 * w.groups) * ((cols + kGradCols<1> - 1) / kGradCols<1>);
+    if ((jobs + 7) / 8 > 0x7fffffffull)
+        return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
+    return B200PP_SUCCESS;
+}
+
 template<int GRAD, int W>
 int launch_runs(EmbeddingGradKParams &p, cudaStream_t stream)
 {
     p.blocks                      = static_cast<unsigned>((static_cast<long long>(p.cols) + kGradCols<W> - 1) / kGradCols<W>);
     const unsigned long long jobs = (static_cast<unsigned long long>(p.units) + 2 * p.groups) * p.blocks;
-    if (jobs > 0x7fffffffull)
-        return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
     Launch(dim3(static_cast<unsigned>((jobs + 7) / 8)), dim3(256), 0, stream, 1, true).run(embedding_grad_runs_kernel<GRAD, W>, p);
     return check_launch("EmbeddingBackward");
 }
@@ -261,7 +269,13 @@ extern "C" int b200ppEmbeddingBackwardWorkspace(const B200ppRows *grad, const B2
     int st;
     if ((st = take_rows(&g, "Gradient", false, m, count)) || (st = take_rows(&t, "Table gradient", true, m, rows)))
         return st;
-    *bytes = count == 0 || goes_direct(count, rows, g.cols) ? 0 : plan_embedding_grad(count, g.cols).bytes;
+    *bytes = 0;
+    if (count == 0 || goes_direct(count, rows, g.cols))
+        return B200PP_SUCCESS;
+    const EmbeddingGradPlan w = plan_embedding_grad(count, g.cols);
+    if ((st = check_grad_size(w, g.cols)))
+        return st;
+    *bytes = w.bytes;
     return B200PP_SUCCESS;
 }
 
@@ -308,7 +322,7 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
         return embedding_grad_direct(d, width.width, padding, stream);
     }
     const EmbeddingGradPlan w = plan_embedding_grad(count, grad->cols);
-    if (count > 0 && (st = check_workspace(workspace, workspaceBytes, w.bytes)))
+    if (count > 0 && ((st = check_grad_size(w, grad->cols)) || (st = check_workspace(workspace, workspaceBytes, w.bytes))))
         return st;
     uint8_t *ws  = static_cast<uint8_t *>(workspace);
     p.gradType   = grad->dtype;
@@ -369,9 +383,8 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
         st = launch_runs<B200PP_F32>(p, width.width, stream);
     if (st || w.groups == 1)
         return st;
+    p.joins               = (w.groups - 1 + 7) / 8;
     const unsigned blocks = static_cast<unsigned>((static_cast<long long>(p.cols) + kJoinCols - 1) / kJoinCols);
-    if (blocks > 65535u)
-        return fail(B200PP_ERROR_OVERFLOW, "Gradient is too large");
-    Launch(dim3((w.groups - 1 + 7) / 8, blocks), dim3(256), 0, stream, 1, true).run(embedding_grad_join_kernel, p);
+    Launch(dim3(p.joins * blocks), dim3(256), 0, stream, 1, true).run(embedding_grad_join_kernel, p);
     return check_launch("EmbeddingBackward");
 }

@@ -34,3 +34,16 @@ def test_backward_of_rows_split_over_clusters(pkg, cols, src, grad):
         again = [pkg.layernorm_backward(g, x, m, r, w) for _ in range(20)]
         alone = [pkg.layernorm_backward(g, x, m, r, w, weight_grad=False, bias_grad=False)[0] for _ in range(20)]
         assert all(torch.equal(a, f) for call in again for a, f in zip(call, first)) and all(torch.equal(a, first[0]) for a in alone)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradient_of_a_table_of_many_columns(pkg, accumulate):
+    cols = 16_780_000
+    ids = torch.full((70,), 1, device="cuda")
+    ids[50:60] = 0
+    g = (torch.arange(70 * 256, device="cuda") % 251).reshape(70, 256).half().repeat(1, cols // 256 + 1)[:, :cols]
+    into = torch.ones((3, cols), device="cuda")
+    pkg.embedding_backward_into(into, g, ids, accumulate=accumulate)
+    for row in range(3):
+        want = g[:, :256].float()[ids == row].sum(0) + accumulate  # whole numbers: exact
+        assert torch.equal(into[row], want.repeat(cols // 256 + 1)[:cols])
