@@ -708,11 +708,12 @@ __device__ __forceinline__ void store_row(uint8_t *row, int dtype, const RowThre
         store_pairs<B200PP_F16, E>(row, k.c, k.step, end, f);
 }
 
-// s / n for a count n and inv = 1 / n rounded: one step of division by residual. A sum of n equal values gives the value itself.
+// s / n for a count n and inv = 1 / n rounded: one step of division by residual. A sum of n equal values gives the value itself. An
+// infinite s has no residual and stays infinite.
 __device__ __forceinline__ float divide_count(float s, float n, float inv)
 {
     const float q = s * inv;
-    return fmaf(fmaf(-q, n, s), inv, q);
+    return isinf(q) ? q : fmaf(fmaf(-q, n, s), inv, q);
 }
 
 template<int DT>

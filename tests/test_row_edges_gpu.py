@@ -47,3 +47,25 @@ def test_gradient_of_a_table_of_many_columns(pkg, accumulate):
     for row in range(3):
         want = g[:, :256].float()[ids == row].sum(0) + accumulate  # whole numbers: exact
         assert torch.equal(into[row], want.repeat(cols // 256 + 1)[:cols])
+
+
+# every kernel of the forward pass: groups of lanes, a CTA per row, few rows, chunks, rows that start anywhere
+@pytest.mark.parametrize("src", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(40, 1), (40, 24), (300, 768), (300, 77), (9, 1000), (300, 2048), (300, 2051), (9, 20000), (9, 20003)])
+def test_statistics_of_rows_with_infinities(pkg, src, rows, cols):
+    """The mean of a row that holds infinities of one sign is that infinity, of both NaN; the other rows do not notice."""
+    x = torch.randn((rows, cols), device="cuda").to(KINDS[src])
+    clean = pkg.layernorm(x, stats=True)
+    bad = x.clone()
+    inf = float("inf")
+    bad[1, cols - 1], bad[3, cols // 2], bad[4, :], bad[5, 0], bad[6, 0] = inf, -inf, inf, float("nan"), inf
+    bad[6, cols - 1] = -inf
+    _, mean, rstd = got = pkg.layernorm(bad, stats=True)
+    want = bad.double().mean(1)
+    hit = [1, 3, 4, 5, 6]
+    same = (mean[hit].double() == want[hit]) | (mean[hit].isnan() & want[hit].isnan())
+    assert bool(same.all()), (mean[hit], want[hit])
+    assert bool(rstd[hit].isnan().all()) and bool(got[0][hit].isnan().any(1).all())
+    keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+    keep[hit] = False
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, clean))
