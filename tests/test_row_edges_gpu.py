@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from row_bounds import check, layernorm64, layernorm_backward64
+from row_bounds import U, check, layernorm64, layernorm_backward64
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,19 @@ def test_statistics_of_rows_with_infinities(pkg, src, rows, cols):
     keep = torch.ones(rows, dtype=torch.bool, device="cuda")
     keep[hit] = False
     assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, clean))
+
+
+# clusters of eight and of four CTAs, and rows too long for those; broadcast rows, so that only their number is large
+@pytest.mark.parametrize("cols,big", [(40_000, 18), (20_000, 37), (65_537, 8)])
+def test_sums_over_many_long_rows(pkg, cols, big):
+    """No float32 sum over the rows is deeper than 48 + rows / 64 + 1300 additions (row_bounds.py): 1 is half a step of 2^24, so a
+    chain that begins with that loses every addend."""
+    rows = 300_000
+    one = torch.ones((1, cols), device="cuda").expand(rows, cols)
+    m, r = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    r[:big] = 2.0 ** 24  # h = (1 - 0) r
+    _, dw, db = pkg.layernorm_backward(one, one, m, r, src_grad=False)
+    k = 48 + rows / 64 + 1300
+    want = torch.full((cols,), float(r.double().sum()), dtype=torch.float64, device="cuda")
+    check(dw, want, U * (k + 4) * want, "dweight")
+    check(db, torch.full_like(want, rows), torch.full_like(want, U * (k + 2) * rows), "dbias")

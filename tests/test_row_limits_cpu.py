@@ -26,3 +26,11 @@ def test_a_gradient_that_is_too_large_is_refused_before_anything_happens(pkg, ac
     # wide tables and few indices are not too large
     g, t = _rows(pkg, cols=1 << 30, count=70), _rows(pkg, cols=1 << 30)
     assert L.b200ppEmbeddingBackwardWorkspace(C.byref(g), C.byref(t), C.byref(need)) == 0 and need.value > 0
+
+
+@pytest.mark.parametrize("rows,cols,chains", [(300_000, 65_537, 8), (300_000, 40_000, 1), (300_000, 20_000, 1), (10_000_000, 65_537, 8)])
+def test_sums_over_many_long_rows_have_parts(pkg, rows, cols, chains):
+    """Room for as many parts as leave each of their chains of additions 1024 rows."""
+    need = C.c_size_t(0)
+    assert pkg.rows._lib().b200ppLayerNormBackwardWorkspace(C.byref(_rows(pkg, cols=cols, count=rows)), C.byref(need)) == 0
+    assert need.value // (2 * 4 * cols) * chains * 1024 >= rows
