@@ -139,6 +139,7 @@ def _view(t: torch.Tensor, axes: int, what: str):
 # The C structures as bytes, which ctypes passes by address: a third of the time a ctypes.Structure takes to fill in.
 _pack_rows = struct.Struct("=Qi4xq3q3q").pack
 _pack_ln = struct.Struct("=QQiif4xQQ").pack
+_pack_float = struct.Struct("=f").pack
 _pack_ln_grad = struct.Struct("=QQQi4xQQii").pack
 _pack_emb_grad = struct.Struct("=fiq").pack
 assert struct.calcsize("=Qi4xq3q3q") == C.sizeof(_Rows) and struct.calcsize("=QQiif4xQQ") == C.sizeof(_LayerNormOp)
@@ -174,6 +175,15 @@ def _param(t: torch.Tensor, numel: int, what: str, kinds=_FLOATS) -> Tuple[int, 
     if t.numel() != numel or not t.is_contiguous():
         raise _invalid(f"The {what} must be packed and hold {numel} value(s)")
     return t.data_ptr(), _TYPES[t.dtype]
+
+
+def _number(v, what: str) -> float:
+    """A number that float32 holds."""
+    try:
+        _pack_float(v)
+    except (struct.error, OverflowError):
+        raise _invalid(f"The {what} must be a float32 number") from None
+    return v
 
 
 def _enter(device: int, stream):
@@ -236,7 +246,7 @@ def _layernorm(d, src, weight, bias, epsilon, axes, mean, rstd, device, handle):
         d = _pack_rows(d.data_ptr(), _TYPES.get(d.dtype, -1), cols, count, 1, 1, cols * d.element_size(), 0, 0)
     w, wt = _param(weight, cols, "weight") if weight is not None else (0, 0)
     b, bt = _param(bias, cols, "bias") if bias is not None else (0, 0)
-    op = _pack_ln(w, b, wt, bt, epsilon, _param(mean, count, "mean", (torch.float32,))[0] if mean is not None else 0,
+    op = _pack_ln(w, b, wt, bt, _number(epsilon, "epsilon"), _param(mean, count, "mean", (torch.float32,))[0] if mean is not None else 0,
                   _param(rstd, count, "rstd", (torch.float32,))[0] if rstd is not None else 0)
     keep, ws, size = None, None, 0
     if cols > _WHOLE_ROWS:
@@ -371,7 +381,8 @@ def embedding_into(dst: torch.Tensor, indices: torch.Tensor, table: torch.Tensor
         raise _invalid("The output must have the indices' shape followed by the table's number of columns")
     handle, leave = _enter(device, stream)
     try:
-        _check(_lib().b200ppEmbedding(_indices(indices), _rows(table, 1, "Table")[0], _rows(dst, 1, "Output")[0], scale, handle))
+        _check(_lib().b200ppEmbedding(_indices(indices), _rows(table, 1, "Table")[0], _rows(dst, 1, "Output")[0],
+                                      _number(scale, "scale"), handle))
     finally:
         if leave is not None:
             leave.close()
@@ -396,7 +407,7 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *,
         else:
             dst = torch.empty(shape, dtype=data_type or table.dtype, device=_cuda(device))
         d = _pack_rows(dst.data_ptr(), _TYPES.get(dst.dtype, -1), cols, count, 1, 1, cols * dst.element_size(), 0, 0)
-        _check(_lib().b200ppEmbedding(i, t, d, scale, handle))
+        _check(_lib().b200ppEmbedding(i, t, d, _number(scale, "scale"), handle))
     finally:
         if leave is not None:
             leave.close()
@@ -405,8 +416,10 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *,
 
 def _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate, device, handle):
     g, cols, count = _rows(grad, 1, "Gradient")
-    op = _pack_emb_grad(scale, int(accumulate), -1 if padding_index is None else int(padding_index))
     t, _, rows = _rows(dtable, 1, "Table gradient")
+    if padding_index is None or not 0 <= padding_index < rows:
+        padding_index = -1
+    op = _pack_emb_grad(_number(scale, "scale"), int(accumulate), int(padding_index))
     size = _embedding_workspace_size(_TYPES.get(grad.dtype, -1), cols, count, _TYPES.get(dtable.dtype, -1), rows)
     keep = _scratch(size, device) if size else None
     _check(_lib().b200ppEmbeddingBackward(g, _indices(indices), t, op, keep.data_ptr() if size else None, size, handle))
@@ -437,9 +450,12 @@ def embedding_backward(grad: torch.Tensor, indices: torch.Tensor, rows: int, sca
     device = _device_of(grad, indices)
     if grad.dim() < 1 or grad.shape[:-1] != indices.shape:
         raise _invalid("The gradient must have the indices' shape followed by the table's number of columns")
+    rows = int(rows)
+    if rows < 0:
+        raise _invalid("The table must not have a negative number of rows")
     handle, leave = _enter(device, stream)
     try:
-        dtable = torch.empty((int(rows), grad.shape[-1]), dtype=data_type, device=_cuda(device))
+        dtable = torch.empty((rows, grad.shape[-1]), dtype=data_type, device=_cuda(device))
         _embedding_backward(dtable, grad, indices, scale, padding_index, False, device, handle)
     finally:
         if leave is not None:

@@ -85,3 +85,16 @@ def test_sums_over_many_long_rows(pkg, cols, big):
     want = torch.full((cols,), float(r.double().sum()), dtype=torch.float64, device="cuda")
     check(dw, want, U * (k + 4) * want, "dweight")
     check(db, torch.full_like(want, rows), torch.full_like(want, U * (k + 2) * rows), "dbias")
+
+
+def test_arguments_out_of_range(pkg):
+    g, i = torch.ones((4, 8), device="cuda"), torch.arange(4, device="cuda")
+    want = pkg.embedding_backward(g, i, 5)
+    for padding in (5, -1, 2 ** 63, -2 ** 70, 2 ** 32):  # values outside the table: none
+        assert torch.equal(pkg.embedding_backward(g, i, 5, padding_index=padding), want)
+    Error = pkg.ops.Error
+    for call in (lambda: pkg.embedding_backward(g, i, -1), lambda: pkg.embedding_backward(g, i, 5, 1e39),
+                 lambda: pkg.embedding(i, g, 1e39), lambda: pkg.embedding_into(want[:4], i, g, -1e39), lambda: pkg.layernorm(g, epsilon=1e39),
+                 lambda: pkg.layernorm(g, epsilon=None), lambda: pkg.embedding(i, g, "2")):
+        with pytest.raises(Error):
+            call()
