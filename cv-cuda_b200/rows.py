@@ -139,9 +139,9 @@ def _view(t: torch.Tensor, axes: int, what: str):
 # The C structures as bytes, which ctypes passes by address: a third of the time a ctypes.Structure takes to fill in.
 _pack_rows = struct.Struct("=Qi4xq3q3q").pack
 _pack_ln = struct.Struct("=QQiif4xQQ").pack
-_pack_float = struct.Struct("=f").pack
 _pack_ln_grad = struct.Struct("=QQQi4xQQii").pack
 _pack_emb_grad = struct.Struct("=fiq").pack
+_pack_float = struct.Struct("=f").pack
 assert struct.calcsize("=Qi4xq3q3q") == C.sizeof(_Rows) and struct.calcsize("=QQiif4xQQ") == C.sizeof(_LayerNormOp)
 assert struct.calcsize("=QQQi4xQQii") == C.sizeof(_LayerNormGradOp) and struct.calcsize("=fiq") == C.sizeof(_EmbeddingGradOp)
 
@@ -177,13 +177,7 @@ def _param(t: torch.Tensor, numel: int, what: str, kinds=_FLOATS) -> Tuple[int, 
     return t.data_ptr(), _TYPES[t.dtype]
 
 
-def _number(v, what: str) -> float:
-    """A number that float32 holds."""
-    try:
-        _pack_float(v)
-    except (struct.error, OverflowError):
-        raise _invalid(f"The {what} must be a float32 number") from None
-    return v
+_NOT_FLOAT32 = (struct.error, OverflowError)  # what packing raises for anything but a number that float32 holds
 
 
 def _enter(device: int, stream):
@@ -246,8 +240,12 @@ def _layernorm(d, src, weight, bias, epsilon, axes, mean, rstd, device, handle):
         d = _pack_rows(d.data_ptr(), _TYPES.get(d.dtype, -1), cols, count, 1, 1, cols * d.element_size(), 0, 0)
     w, wt = _param(weight, cols, "weight") if weight is not None else (0, 0)
     b, bt = _param(bias, cols, "bias") if bias is not None else (0, 0)
-    op = _pack_ln(w, b, wt, bt, _number(epsilon, "epsilon"), _param(mean, count, "mean", (torch.float32,))[0] if mean is not None else 0,
-                  _param(rstd, count, "rstd", (torch.float32,))[0] if rstd is not None else 0)
+    m = _param(mean, count, "mean", (torch.float32,))[0] if mean is not None else 0
+    r = _param(rstd, count, "rstd", (torch.float32,))[0] if rstd is not None else 0
+    try:
+        op = _pack_ln(w, b, wt, bt, epsilon, m, r)
+    except _NOT_FLOAT32:
+        raise _invalid("epsilon must be a float32 number") from None
     keep, ws, size = None, None, 0
     if cols > _WHOLE_ROWS:
         size = _workspace_size("b200ppLayerNormWorkspace", _TYPES.get(src.dtype, -1), cols, count)
@@ -381,8 +379,10 @@ def embedding_into(dst: torch.Tensor, indices: torch.Tensor, table: torch.Tensor
         raise _invalid("The output must have the indices' shape followed by the table's number of columns")
     handle, leave = _enter(device, stream)
     try:
-        _check(_lib().b200ppEmbedding(_indices(indices), _rows(table, 1, "Table")[0], _rows(dst, 1, "Output")[0],
-                                      _number(scale, "scale"), handle))
+        _pack_float(scale)
+        _check(_lib().b200ppEmbedding(_indices(indices), _rows(table, 1, "Table")[0], _rows(dst, 1, "Output")[0], scale, handle))
+    except _NOT_FLOAT32:
+        raise _invalid("The scale must be a float32 number") from None
     finally:
         if leave is not None:
             leave.close()
@@ -407,7 +407,10 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0, *,
         else:
             dst = torch.empty(shape, dtype=data_type or table.dtype, device=_cuda(device))
         d = _pack_rows(dst.data_ptr(), _TYPES.get(dst.dtype, -1), cols, count, 1, 1, cols * dst.element_size(), 0, 0)
-        _check(_lib().b200ppEmbedding(i, t, d, _number(scale, "scale"), handle))
+        _pack_float(scale)
+        _check(_lib().b200ppEmbedding(i, t, d, scale, handle))
+    except _NOT_FLOAT32:
+        raise _invalid("The scale must be a float32 number") from None
     finally:
         if leave is not None:
             leave.close()
@@ -419,7 +422,10 @@ def _embedding_backward(dtable, grad, indices, scale, padding_index, accumulate,
     t, _, rows = _rows(dtable, 1, "Table gradient")
     if padding_index is None or not 0 <= padding_index < rows:
         padding_index = -1
-    op = _pack_emb_grad(_number(scale, "scale"), int(accumulate), int(padding_index))
+    try:
+        op = _pack_emb_grad(scale, int(accumulate), int(padding_index))
+    except _NOT_FLOAT32:
+        raise _invalid("The scale must be a float32 number") from None
     size = _embedding_workspace_size(_TYPES.get(grad.dtype, -1), cols, count, _TYPES.get(dtable.dtype, -1), rows)
     keep = _scratch(size, device) if size else None
     _check(_lib().b200ppEmbeddingBackward(g, _indices(indices), t, op, keep.data_ptr() if size else None, size, handle))
