@@ -98,3 +98,38 @@ def test_arguments_out_of_range(pkg):
                  lambda: pkg.layernorm(g, epsilon=None), lambda: pkg.embedding(i, g, "2")):
         with pytest.raises(Error):
             call()
+
+
+def test_more_elements_than_32_bits_count(pkg):
+    n = 2 ** 31 - 5
+    ids = torch.empty(n, dtype=torch.uint8, device="cuda").random_(0, 256)
+    table = values((256, 2), torch.float16)
+    out = pkg.embedding(ids, table)
+    for a in (0, n // 2 - 1000, n - 100_003):
+        assert torch.equal(out[a:a + 100_003], table[ids[a:a + 100_003].long()])
+    del out, ids
+    rows = 310_000_003
+    x = torch.empty((rows, 7), dtype=torch.float16, device="cuda").normal_()
+    y, m, r = pkg.layernorm(x, stats=True)
+    dx = pkg.layernorm_backward(y, x, m, r, weight_grad=False, bias_grad=False)[0]
+    for a in (0, 2 ** 28 - 50, rows - 1000):
+        b = a + 1000
+        (y64, m64, r64), (dy, dm, dr) = layernorm64(x[a:b], None, None, 1e-5)
+        for got, want, bound in ((y, y64, dy), (m, m64, dm), (r, r64, dr)):
+            check(got[a:b], want, bound)
+        (dx64, _, _), (ex, _, _) = layernorm_backward64(y[a:b], x[a:b], m[a:b], r[a:b], None)
+        check(dx[a:b], dx64, ex)
+
+
+@pytest.mark.parametrize("cols", [40, 77, 1000, 2051, 9001])
+def test_one_row_broadcast_to_many(pkg, cols):
+    """Inputs whose rows are one and the same in memory."""
+    x, g = (values((1, 1, cols), torch.float32, k).expand(30, 20, cols) for k in (1, 2))
+    y, m, r = pkg.layernorm(x, stats=True)
+    # (packed rows start elsewhere, which deals the values out differently: other bits, the same bounds)
+    for a, b, e in zip((y.reshape(600, cols), m.flatten(), r.flatten()), *layernorm64(x.reshape(600, cols), None, None, 1e-5)):
+        check(a, b, e)
+    got = pkg.layernorm_backward(g, x, m, r)
+    want, bound = layernorm_backward64(g.reshape(600, cols), x.reshape(600, cols), m, r, None)
+    for a, b, e in zip(got, want, bound):
+        check(a.reshape(b.shape), b, e)
