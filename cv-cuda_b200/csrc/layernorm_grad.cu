@@ -246,7 +246,8 @@ extern "C" int b200ppLayerNormBackward(const B200ppRows *grad, const B200ppRows 
         st = launch_two_pass<B200PP_F32>(p, stream);
     if (st || !p.partials)
         return st;
-    // as many threads share a column as there are parts for
+    // as many threads share a column as there are parts for (50176 rows of 768 bfloat16, 296 parts: all in all 44 us with 32 threads, 50 with
+    // eight, 107 with one; 600 of 40000 float16, 18 parts: 92, 85 and 91 us)
     const int  share = p.parts >= 64 ? 32 : p.parts >= 8 ? 8 : 1;
     const dim3 block(share == 1 ? 128 : 32, share);
     Launch(dim3((2u * p.cols + block.x - 1) / block.x), block, 0, stream, 1, true).run(layernorm_grad_join_kernel, p);

@@ -1,6 +1,7 @@
 // LayerNorm.
 //
-// Per row of D values: m = sum(x) / D, v = sum((x - m)^2) / D, r = 1 / sqrt(v + epsilon), y = (x - m) r w + b.
+// Per row of D values: m = sum(x) / D, v = sum((x - m)^2) / D, r = 1 / sqrt(v + epsilon), y = (x - m) r w + b. r comes from rsqrtf,
+// which is off by two units in the last place at most; a rounded root and a rounded division would leave one.
 // Bound: HBM (about one operation per byte moved).
 #ifndef CVCUDA_B200_LAYERNORM_KERNELS_CUH
 #define CVCUDA_B200_LAYERNORM_KERNELS_CUH

@@ -47,8 +47,10 @@ typedef struct B200ppRows
  * of the row (variance: the mean of the squared distances to the mean). src: uint8, float16, bfloat16 or float32; dst:
  * float16, bfloat16 or float32. weight and bias: `cols` adjacent values of float16, bfloat16 or float32, each NULL for 1
  * and 0. mean and rstd: if not NULL, the float32 statistics of the rows, packed, in row order, for the backward pass.
- * Sums are float32 (the variance about the mean, not the difference of two sums). dst may be src if the types agree; apart from
- * that no output may overlap an input or another output. Rows of up to 8192 columns need no workspace. */
+ * Sums are float32 (the variance about the mean, not the difference of two sums), rstd is an approximate reciprocal square
+ * root, off by two units in the last place at most. The mean of a row with infinities of one sign is that infinity; its rstd
+ * and result, and those of a row with NaN, are NaN. dst may be src if the types agree; apart from that no output may overlap
+ * an input or another output. Rows of up to 8192 columns need no workspace. */
 typedef struct B200ppLayerNormOp
 {
     const void *weight;
