@@ -219,6 +219,27 @@ int launch_runs(EmbeddingGradKParams &p, int width, cudaStream_t stream)
     return launch_runs<GRAD, 1>(p, stream);
 }
 
+// The sums of the runs of the sorted positions, and the join of the long ones.
+int launch_sums(EmbeddingGradKParams &p, cudaStream_t stream)
+{
+    VecWidth width(p.cols);
+    width.take(p.grad, row_elem_size(p.gradType));
+    width.take(p.dtable, row_elem_size(p.dtableType));
+    width.take(p.partials, p.cols * static_cast<long long>(sizeof(float)), sizeof(float));
+    int st;
+    if (p.gradType == B200PP_F16)
+        st = launch_runs<B200PP_F16>(p, width.width, stream);
+    else if (p.gradType == B200PP_BF16)
+        st = launch_runs<B200PP_BF16>(p, width.width, stream);
+    else
+        st = launch_runs<B200PP_F32>(p, width.width, stream);
+    if (st || p.groups == 1)
+        return st;
+    const dim3 grid((p.groups - 1 + 7) / 8, (p.cols + kJoinCols - 1) / kJoinCols);
+    Launch(grid, dim3(256), 0, stream, 1, true).run(embedding_grad_join_kernel, p);
+    return check_launch("EmbeddingBackward");
+}
+
 // CTAs of the cluster that sorts: one for few indices, then eight; sixteen, where the GPU has room for such a cluster, once the
 // indices take longer than the exchange between the CTAs (16384 indices: 18 us with eight, 14 us with sixteen; 5003: 10.3 us both).
 int sort_ctas(long long count, size_t smem)
@@ -372,20 +393,16 @@ extern "C" int b200ppEmbeddingBackward(const B200ppRows *grad, const B200ppRows 
     }
     if (count == 0)
         return st;
-    VecWidth width(p.cols);
-    width.take(p.grad, row_elem_size(p.gradType));
-    width.take(p.dtable, row_elem_size(p.dtableType));
-    width.take(p.partials, p.cols * static_cast<long long>(sizeof(float)), sizeof(float));
-    if (p.gradType == B200PP_F16)
-        st = launch_runs<B200PP_F16>(p, width.width, stream);
-    else if (p.gradType == B200PP_BF16)
-        st = launch_runs<B200PP_BF16>(p, width.width, stream);
-    else
-        st = launch_runs<B200PP_F32>(p, width.width, stream);
-    if (st || w.groups == 1)
-        return st;
-    p.joins               = (w.groups - 1 + 7) / 8;
-    const unsigned blocks = static_cast<unsigned>((static_cast<long long>(p.cols) + kJoinCols - 1) / kJoinCols);
-    Launch(dim3(p.joins * blocks), dim3(256), 0, stream, 1, true).run(embedding_grad_join_kernel, p);
-    return check_launch("EmbeddingBackward");
+    // as many columns at a time as the join's grid has blocks for (blocks in another dimension, or a first column, cost the join 1 us of
+    // the 52 for 16384 indices of 32000 x 1024)
+    constexpr int kMostCols = 65535 * kJoinCols;
+    const int     gradElem = row_elem_size(p.gradType), tableElem = row_elem_size(p.dtableType);
+    for (int left = p.cols; left > 0 && !st; left -= p.cols)
+    {
+        p.cols = std::min(left, kMostCols);
+        st     = launch_sums(p, stream);
+        p.grad.base += static_cast<long long>(p.cols) * gradElem;
+        p.dtable.base += static_cast<long long>(p.cols) * tableElem;
+    }
+    return st;
 }

@@ -239,7 +239,6 @@ struct EmbeddingGradKParams
     float    *partials;                       // [groups][2][cols]
     unsigned  units, groups;                  // of kGradUnit and kShortRun sorted positions
     unsigned  blocks;                         // column blocks of kGradCols<W>
-    unsigned  joins;                          // CTAs that join a block of kJoinCols columns
 };
 
 // ---- first kernel: sort the positions 0..count-1 by index, stable; indices that take no part get the key `rows` and end up last.
@@ -618,11 +617,10 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
     __shared__ unsigned keys[8], parts[8]; // of the runs left to the whole CTA
     constexpr unsigned  kAll = 0xffffffffu;
     const unsigned      none = static_cast<unsigned>(p.rows);
-    const int           lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x / p.joins * kJoinCols + lane;
-    const unsigned      u0 = blockIdx.x % p.joins * 8; // the first group
+    const int           lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.y * kJoinCols + lane;
     cudaGridDependencySynchronize();
     {
-        const unsigned u = u0 + warp;
+        const unsigned u = blockIdx.x * 8 + warp;
         unsigned       k = none, more = 0; // the run's key, the groups it goes on in
         if (u + 1 < p.groups) // not the last group, so it is full
         {
@@ -660,7 +658,7 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
             continue;
         const unsigned per = (parts[l] + 7) / 8, from = min(parts[l], warp * per), to = min(parts[l], from + per);
         float          s[8] = {};
-        embedding_add_parts(p, u0 + l, from, to, c0, s);
+        embedding_add_parts(p, blockIdx.x * 8 + l, from, to, c0, s);
         __syncthreads(); // the sums of the run before are taken
 #pragma unroll
         for (int j = 0; j < 8; ++j) sums[warp][lane + 32 * j] = s[j];
