@@ -594,8 +594,8 @@ __global__ void __launch_bounds__(256, GRAD == B200PP_F32 && W >= 4 ? 2 : 3) emb
 
 // ---- third kernel: the runs longer than kShortRun. A CTA looks after eight groups, a warp each: it finds out whether such a run
 // starts in its group and adds up the run's parts for kJoinCols columns. Runs of more than kJoinAlone groups are left to the whole CTA,
-// each warp a contiguous share of the groups, the warps one after another. (16384 indices of 32000 x 1024, all kernels: 53.5 us; left to
-// the CTA from five groups on 50.3, from 65 on 61.7. 65536 of 50 x 512: 43.2, 43.1 and 57.9 us.)
+// each warp a contiguous share of the groups, the warps one after another. (16384 indices of 32000 x 1024, all kernels: 54.1 us; left to
+// the CTA from six groups on 51.7, from 66 on 61.1. 65536 of 50 x 512: 43.1, 43.1 and 55.1 us.)
 constexpr int      kJoinCols  = 256;
 constexpr unsigned kJoinAlone = 16;
 
